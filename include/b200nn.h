@@ -388,6 +388,56 @@ int b200_op_policy_attention(const void* q, const void* k, const float* w4, int 
 #define B200_STATIC_POLICY_MAX_POSITIONS 256
 int b200_op_policy_attention_static(const void* q, const void* k, const float* w4, int dm, int n, float* policy,
                                     int precision, void* stream);
+/* b200_op_gemm_adapters: a layer that all requests of a batch share, with a low-rank adapter per request beside it (one network,
+ *   an adapter per player or style): C[m] = act(X[m] . W^T + bias + scales[a] * (X[m] . A[a]^T) . B[a]^T), a = ids[m / group].
+ *   - X [M][K], W [N][K], C [M][N] (leading dimensions of 0 mean dense), bias [N] or NULL, `activation` and `precision` as in
+ *     b200_op_gemm; out_f32 != 0: C holds float whatever the precision.
+ *   - A [n_adapters][rank][K] and B [n_adapters][N][rank], dense, in `precision`; rank 1 to B200_ADAPTERS_MAX_RANK (an adapter of
+ *     a lower rank is padded with zeros); scales [n_adapters] or NULL (1).
+ *   - ids [ceil(M / group)]: `group` consecutive rows are one request (64 in a network's body, 1 in its heads).  A request whose id is
+ *     below 0 or not below n_adapters has no adapter; its rows are those of the plain product.
+ *   - workspace: b200_op_gemm_adapters_workspace() bytes of device memory on a 256-byte boundary, for this call alone until it has
+ *     run (two captured graphs that may overlap need two); status: device int or NULL, set non-zero (and never cleared) if a
+ *     bounded device-side wait gave up, the result is then undefined.
+ *   Sums in fp32.  Allocates nothing, does not synchronise, may be captured.  C may not overlap an input.  The ids are read on the
+ *   device: a captured call follows what they hold when it is replayed. */
+#define B200_ADAPTERS_MAX_RANK 128
+typedef struct b200_adapters_desc {
+  const void* X; const void* W; const float* bias; void* C;
+  int M, N, K;
+  long long ldx, ldw, ldc;
+  int activation, precision, out_f32;
+  const void* A; const void* B; const float* scales;
+  int n_adapters, rank;
+  const int* ids; int group;
+  int* status;
+  void* workspace; size_t workspace_bytes;
+} b200_adapters_desc;
+/* Bytes of workspace of a call with this description (pointers need not be set, but those that are count with their alignment). */
+int b200_op_gemm_adapters_workspace(const b200_adapters_desc* d, size_t* bytes);
+int b200_op_gemm_adapters(const b200_adapters_desc* d, void* stream);
+/* b200_op_sample: one entry drawn from every row of logits, with given random numbers (play from the policy at a temperature; the
+ *   probabilities themselves are b200_comp_legal_policy's).
+ *   - logits: rows of `width` entries of type `precision`, ld apart (0: width).  With move_ids the entries of a row are
+ *     logits[move_ids[row][i]], i < n_moves[row] (at most ld_moves, the stride of move_ids; ids not below width are no entries), else all
+ *     columns.  NaN and -infinity are no entries either.
+ *   - per row, each NULL for "off": temperature T (NULL: 1; 0, negative or NaN: the largest logit, at the lowest index), top_k (below
+ *     1: off), top_p (1 and more or NaN: off), min_p (0, negative or NaN: off).  u: random numbers in [0, 1).
+ *   With w = exp((l - max) / T) (+infinity: 1 each, nothing beside them), in the order of falling logits, equal ones by index: top_k
+ *   keeps the first k; top_p those ahead of which the weights of what top_k kept sum to less than top_p of their total, and the
+ *   first; min_p those with w >= min_p.  choice: the first kept entry, by index, at which the sum of the kept weights passes
+ *   u times their total: its column, or its place in the list of moves.  prob (may be NULL): its weight over that total.
+ *   -1 and 0 for a row without entries.
+ *   The choice is the one that sums in 64 bits give.  Allocates nothing, does not synchronise, may be captured. */
+#define B200_SAMPLE_MAX_WIDTH 262144
+typedef struct b200_sample_desc {
+  const void* logits; long long ld;
+  int rows, width, precision;
+  const uint16_t* move_ids; const int* n_moves; int ld_moves;
+  const float* temperature; const int* top_k; const float* top_p; const float* min_p; const float* u;
+  int* choice; float* prob;
+} b200_sample_desc;
+int b200_op_sample(const b200_sample_desc* d, void* stream);
 int b200_op_layer_norm(void* out, const void* x, const void* skip, const float* gamma,
                        const float* beta, int rows, int C, float alpha, float eps, int precision,
                        void* stream);

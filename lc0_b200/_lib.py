@@ -56,6 +56,29 @@ class GemmDesc(ctypes.Structure):
                 ("whole_tiles", ctypes.c_int)]
 
 
+class AdaptersDesc(ctypes.Structure):
+    """b200_adapters_desc (include/b200nn.h)."""
+    _fields_ = [("X", ctypes.c_void_p), ("W", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("C", ctypes.c_void_p),
+                ("M", ctypes.c_int), ("N", ctypes.c_int), ("K", ctypes.c_int),
+                ("ldx", ctypes.c_longlong), ("ldw", ctypes.c_longlong), ("ldc", ctypes.c_longlong),
+                ("activation", ctypes.c_int), ("precision", ctypes.c_int), ("out_f32", ctypes.c_int),
+                ("A", ctypes.c_void_p), ("B", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("n_adapters", ctypes.c_int), ("rank", ctypes.c_int),
+                ("ids", ctypes.c_void_p), ("group", ctypes.c_int),
+                ("status", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class SampleDesc(ctypes.Structure):
+    """b200_sample_desc (include/b200nn.h)."""
+    _fields_ = [("logits", ctypes.c_void_p), ("ld", ctypes.c_longlong),
+                ("rows", ctypes.c_int), ("width", ctypes.c_int), ("precision", ctypes.c_int),
+                ("move_ids", ctypes.c_void_p), ("n_moves", ctypes.c_void_p), ("ld_moves", ctypes.c_int),
+                ("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p),
+                ("min_p", ctypes.c_void_p), ("u", ctypes.c_void_p),
+                ("choice", ctypes.c_void_p), ("prob", ctypes.c_void_p)]
+
+
 class NetInfo(ctypes.Structure):
     _fields_ = [("input_format", ctypes.c_int), ("output_format", ctypes.c_int),
                 ("moves_left_format", ctypes.c_int), ("wdl", ctypes.c_int), ("has_mlh", ctypes.c_int),
@@ -133,6 +156,9 @@ SIGNATURES = {
     "b200_op_gemm_timed": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, ctypes.POINTER(ctypes.c_float), _P]),
     "b200_op_policy_attention": (_I, [_P, _P, _P, _I, _I, _P, _P, _I, _P]),
     "b200_op_policy_attention_static": (_I, [_P, _P, _P, _I, _I, _P, _I, _P]),
+    "b200_op_gemm_adapters_workspace": (_I, [ctypes.POINTER(AdaptersDesc), ctypes.POINTER(ctypes.c_size_t)]),
+    "b200_op_gemm_adapters": (_I, [ctypes.POINTER(AdaptersDesc), _P]),
+    "b200_op_sample": (_I, [ctypes.POINTER(SampleDesc), _P]),
     "b200_op_layer_norm": (_I, [_P, _P, _P, _P, _P, _I, _I, _F, _F, _I, _P]),
 }
 
