@@ -1,23 +1,34 @@
 // A product that all requests of a batch share, with a low-rank adapter per request beside it:
 //   C[m] = act(X[m] W^T + bias + s_a (X[m] A_a^T) B_a^T),  a = ids[m / group].
-// The narrow product H[m] = s_a X[m] A_a^T [M][rank] comes first (fp32, in the caller's workspace), then the shared product, which
-// meets H and B in fp32.
+// Two launches: the narrow product H[m] = s_a X[m] A_a^T [M][rank], and the shared product, which takes H and B in.  The second is
+// made dependent on the first early: it loads and multiplies X and W while H is computed.
+//
+// H, 16-bit, requests of whole 64-row blocks (adapters_shrink_mma_kernel): a CTA takes 64 rows of one request, k-blocks of X and of the
+//   adapter's A arrive by TMA in a ring, four warps multiply 16 rows each by mma.sync: what counts is X's one pass through.
+// H otherwise (adapters_shrink_rows_kernel): a CTA per row, the row in shared memory, a warp per row of A.
+// The shared product, 16-bit: kernels of gemm_tc.cu (H and B as further k-blocks) and gemm_split.cu (added in the epilogue), see
+//   gemm_adapters_supported; operands that TMA cannot read and fp32: gemm_fma.cu into fp32 sums, to which
+//   adapters_expand_kernel adds.
 #include "../../include/b200nn.h"
 #include "kernels.cuh"
+#include "tma_mma.cuh"
 
 namespace b200 {
+cudaError_t gemm_tensor_map(const void* ptr, long long ld, int rows, int cols, int box_rows, int prec, CUtensorMap* out);  // gemm_tc.cu
+
 namespace {
 
 struct AdapterParams {
   const void* X; const void* A; const void* B;
   const float* scales; const int* ids;
-  const float* bias;
-  float* H;          // [M][rank]
+  float* H;      // [M][rank]
+  void* pieces;  // [M][2 * rp] or nullptr: H as two values of the type
   const float* acc;  // [M][N] sums of the shared product and the bias
   long long ldacc;
   void* C; long long ldc;
   long long ldx;
-  int M, N, K, rank, group, n_adapters, act, out_f32;
+  int M, N, K, rank, rp, group, n_adapters, act, out_f32;
+  int* status;
 };
 
 __device__ __forceinline__ int adapter_of(const AdapterParams& p, int m) {
@@ -25,25 +36,151 @@ __device__ __forceinline__ int adapter_of(const AdapterParams& p, int m) {
   return a >= 0 && a < p.n_adapters ? a : -1;
 }
 
-// H: a warp per row.
-template <typename T>
-__global__ void __launch_bounds__(256) adapters_shrink_kernel(const AdapterParams p) {
-  const int m = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (m >= p.M) return;
-  const int a = adapter_of(p, m);
-  if (a < 0) return;  // never read
-  const T* x = static_cast<const T*>(p.X) + (long long)m * p.ldx;
-  const T* w = static_cast<const T*>(p.A) + (long long)a * p.rank * p.K;
-  const float scale = p.scales ? p.scales[a] : 1.f;
-  for (int r = 0; r < p.rank; ++r) {
-    float s = 0.f;
-    for (int k = lane; k < p.K; k += 32) s = fmaf(to_f(x[k]), to_f(w[(long long)r * p.K + k]), s);
-    s = warp_sum(s);
-    if (lane == 0) p.H[(long long)m * p.rank + r] = scale * s;
+// ---- H by tensor cores ------------------------------------------------------------------------------------------
+constexpr int kShrinkThreads = 160;  // four warps of 16 rows, one that loads
+template <int NB> struct ShrinkCfg {  // NB: blocks of 16 ranks
+  static constexpr int kStageBytes = 64 * 128 + NB * 16 * 128;
+  static constexpr int kStages = NB <= 2 ? 6 : NB <= 4 ? 5 : 4;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 1024;
+};
+
+template <typename T, int NB>
+__global__ void __launch_bounds__(kShrinkThreads)
+adapters_shrink_mma_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const AdapterParams p) {
+  using Cfg = ShrinkCfg<NB>;
+  constexpr int S = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[S], empty[S];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int m0 = blockIdx.x * 64;
+  const int a = adapter_of(p, m0);
+  grid_launch_dependents();  // nothing of this launch's is read before its end; what it reads was written before it began
+  if (a < 0) return;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(smem_u32(&full[i]), 1);
+      mbar_init(smem_u32(&empty[i]), 4);
+    }
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  const int k_blocks = (p.K + 63) / 64;
+  float acc[2 * NB][4] = {};
+  if (warp == 4) {
+    if (elect_one()) {
+      tma_prefetch_map(&map_x);
+      tma_prefetch_map(&map_a);
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        const int s = kb % S;
+        if (kb >= S && !mbar_wait(smem_u32(&empty[s]), (kb / S - 1) & 1, abort_flag, 1)) break;
+        const uint32_t fb = smem_u32(&full[s]), dst = smem_u32(smem + s * Cfg::kStageBytes);
+        mbar_expect_tx(fb, 64 * 128 + p.rank * 128);
+        tma_load_2d(dst, &map_x, kb * 64, m0, fb);
+        tma_load_2d(dst + 64 * 128, &map_a, kb * 64, a * p.rank, fb);
+      }
+    }
+  } else {
+    const int mat = lane >> 3, row8 = lane & 7;
+    for (int kb = 0; kb < k_blocks; ++kb) {
+      const int s = kb % S;
+      if (!mbar_wait(smem_u32(&full[s]), (kb / S) & 1, abort_flag, 2)) break;
+      const uint8_t* xs = smem + s * Cfg::kStageBytes;
+      const uint8_t* as = xs + 64 * 128;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t fa[4], fb[4];
+        ldmatrix_x4(fa, xs + swz<128>(warp * 16 + (mat & 1) * 8 + row8, 2 * k + (mat >> 1)));
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          ldmatrix_x4(fb, as + swz<128>(n * 16 + (mat >> 1) * 8 + row8, 2 * k + (mat & 1)));
+          mma16816<T>(acc[2 * n], fa, fb[0], fb[1]);
+          mma16816<T>(acc[2 * n + 1], fa, fb[2], fb[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
+    }
+    const float scale = p.scales ? p.scales[a] : 1.f;
+#pragma unroll
+    for (int n = 0; n < 2 * NB; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int m = m0 + warp * 16 + (lane >> 2) + 8 * i, r = n * 8 + (lane & 3) * 2;
+        if (m >= p.M || r >= p.rp) continue;  // (the blocks of 16 that a kernel has may be more than rp)
+        // rows of A behind this adapter's, or nothing at all, were multiplied beyond its rank
+        const float h0 = r < p.rank ? scale * acc[n][2 * i] : 0.f, h1 = r + 1 < p.rank ? scale * acc[n][2 * i + 1] : 0.f;
+        float* h = p.H + (long long)m * p.rank + r;
+        if (r < p.rank) h[0] = h0;
+        if (r + 1 < p.rank) h[1] = h1;
+        if (p.pieces) {
+          // the second piece holds what the first one rounds off: fp16 22 bits, bf16 16 of the 24
+          const uint32_t hi = pack2<T>(h0, h1);
+          const float2 f = unpack2<T>(hi);
+          T* q = static_cast<T*>(p.pieces) + (long long)m * 2 * p.rp + r;
+          *reinterpret_cast<uint32_t*>(q) = hi;
+          *reinterpret_cast<uint32_t*>(q + p.rp) = pack2<T>(h0 - f.x, h1 - f.y);
+        }
+      }
+  }
+  __syncthreads();
+  if (abort_word) {
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);  // copies in flight land before the shared memory is released
+    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, 800 + abort_word);
   }
 }
 
-// C = act(acc + H B^T): a thread per output.
+// ---- H row by row -----------------------------------------------------------------------------------------------
+constexpr int kShrinkChunk = 2048;  // numbers of a row held at a time
+
+template <typename T>
+__global__ void __launch_bounds__(256) adapters_shrink_rows_kernel(const AdapterParams p, int vec) {
+  __shared__ __align__(16) T row[kShrinkChunk];
+  constexpr int kPer = 16 / sizeof(T);
+  grid_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int m = blockIdx.x; m < p.M; m += gridDim.x) {
+    const int a = adapter_of(p, m);
+    if (a < 0) continue;  // never read
+    const T* x = static_cast<const T*>(p.X) + (long long)m * p.ldx;
+    const T* w = static_cast<const T*>(p.A) + (long long)a * p.rank * p.K;
+    const float scale = p.scales ? p.scales[a] : 1.f;
+    for (int k0 = 0; k0 < p.K; k0 += kShrinkChunk) {
+      const int n = p.K - k0 < kShrinkChunk ? p.K - k0 : kShrinkChunk;
+      __syncthreads();
+      if (vec) {
+        for (int i = threadIdx.x; i < n / kPer; i += 256) reinterpret_cast<uint4*>(row)[i] = reinterpret_cast<const uint4*>(x + k0)[i];
+      } else {
+        for (int i = threadIdx.x; i < n; i += 256) row[i] = x[k0 + i];
+      }
+      __syncthreads();
+      for (int r = warp; r < p.rank; r += 8) {
+        const T* wr = w + (long long)r * p.K + k0;
+        float s = 0.f;
+        if (vec) {
+#pragma unroll 4
+          for (int i = lane; i < n / kPer; i += 32) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(wr) + i), v = reinterpret_cast<const uint4*>(row)[i];
+            const T* e = reinterpret_cast<const T*>(&u);
+            const T* f = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) s = fmaf(to_f(e[j]), to_f(f[j]), s);
+          }
+        } else {
+          for (int i = lane; i < n; i += 32) s = fmaf(to_f(wr[i]), to_f(row[i]), s);
+        }
+        s = scale * warp_sum(s);
+        float* h = p.H + (long long)m * p.rank + r;
+        if (lane == 0) *h = k0 ? *h + s : s;
+      }
+    }
+  }
+}
+
+// ---- fp32 sums + H B^T ------------------------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(256) adapters_expand_kernel(const AdapterParams p) {
   const int n = blockIdx.x * 256 + threadIdx.x;
@@ -64,52 +201,93 @@ __global__ void __launch_bounds__(256) adapters_expand_kernel(const AdapterParam
   }
 }
 
+// ---- host -------------------------------------------------------------------------------------------------------
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; }
 
+// What a description is computed by, and its workspace: H, its pieces, the fp32 sums.  Nothing here depends on the device.
 struct AdapterPlan {
-  size_t h_bytes, acc_bytes;
-  size_t bytes() const { return h_bytes + acc_bytes; }
+  GemmParams g;
+  bool tensor = false, mma = false;
+  size_t h_bytes = 0, piece_bytes = 0, acc_bytes = 0;
+  size_t bytes() const { return h_bytes + piece_bytes + acc_bytes; }
 };
 AdapterPlan plan_of(const b200_adapters_desc& d) {
-  AdapterPlan p;
-  p.h_bytes = round256((size_t)d.M * d.rank * 4);
+  AdapterPlan out;
+  GemmParams& g = out.g;
+  g.A = d.X; g.lda = d.ldx ? d.ldx : d.K; g.W = d.W; g.ldw = d.ldw ? d.ldw : d.K; g.bias = d.bias;
+  g.C = d.C; g.ldc = d.ldc ? d.ldc : d.N; g.out_f32 = d.out_f32 != 0 || d.precision == B200_PREC_FP32;
+  g.M = d.M; g.N = d.N; g.K = d.K; g.act = d.activation; g.w_const = true; g.split_k = true;
+  g.ad_ids = d.ids; g.ad_b = d.B; g.ad_group = d.group; g.ad_n = d.n_adapters; g.ad_rank = d.rank; g.ad_rp = (d.rank + 15) / 16 * 16;
+  out.tensor = d.precision != B200_PREC_FP32 && gemm_tc_supported(g);
+  out.mma = out.tensor && d.group % 64 == 0 && aligned16(d.A) && (long long)d.n_adapters * d.rank < 0x7fffff00;
+  out.h_bytes = round256((size_t)d.M * d.rank * 4);
+  if (out.mma && gemm_adapters_pieces(g)) out.piece_bytes = round256((size_t)d.M * 2 * g.ad_rp * 2);
   // sums of the shared product: in C itself where it holds floats
-  p.acc_bytes = d.out_f32 || d.precision == B200_PREC_FP32 ? 0 : round256((size_t)d.M * d.N * 4);
-  return p;
+  if (!out.tensor && !g.out_f32) out.acc_bytes = round256((size_t)d.M * d.N * 4);
+  return out;
+}
+
+template <typename T, int NB>
+cudaError_t launch_shrink_mma(const AdapterParams& p, cudaStream_t s) {
+  cudaError_t e = raise_smem_limit<adapters_shrink_mma_kernel<T, NB>>(ShrinkCfg<NB>::kSmemBytes);
+  CUtensorMap mx, ma;
+  if (e == cudaSuccess) e = gemm_tensor_map(p.X, p.ldx, p.M, p.K, 64, TypeTag<T>::prec, &mx);
+  if (e == cudaSuccess) e = gemm_tensor_map(p.A, p.K, p.n_adapters * p.rank, p.K, p.rank, TypeTag<T>::prec, &ma);
+  if (e != cudaSuccess) return e;
+  adapters_shrink_mma_kernel<T, NB><<<ceil_div(p.M, 64), kShrinkThreads, ShrinkCfg<NB>::kSmemBytes, s>>>(mx, ma, p);
+  return cudaGetLastError();
 }
 
 template <typename T>
+cudaError_t launch_shrink_rows(const AdapterParams& p, cudaStream_t s) {
+  const int per = 16 / (int)sizeof(T);
+  const int vec = p.K % per == 0 && p.ldx % per == 0 && aligned16(p.X) && aligned16(p.A);
+  adapters_shrink_rows_kernel<T><<<p.M < 65536 ? p.M : 65536, 256, 0, s>>>(p, vec);
+  return cudaGetLastError();
+}
+
+// The second launch made dependent on the first.
+struct DependentScope {
+  bool before;
+  DependentScope() : before(t_dependent_launch) { t_dependent_launch = true; }
+  ~DependentScope() { t_dependent_launch = before; }
+};
+
+template <typename T>
 int run_adapters(const b200_adapters_desc& d, cudaStream_t s) {
-  const AdapterPlan plan = plan_of(d);
-  AdapterParams p = {};
-  p.X = d.X; p.ldx = d.ldx ? d.ldx : d.K; p.A = d.A; p.B = d.B; p.scales = d.scales; p.ids = d.ids; p.bias = d.bias;
-  p.C = d.C; p.ldc = d.ldc ? d.ldc : d.N;
-  p.M = d.M; p.N = d.N; p.K = d.K; p.rank = d.rank; p.group = d.group; p.n_adapters = d.n_adapters; p.act = d.activation;
-  p.out_f32 = sizeof(T) == 4 || d.out_f32;
+  AdapterPlan plan = plan_of(d);
+  GemmParams& g = plan.g;
   char* ws = static_cast<char*>(d.workspace);
+  AdapterParams p = {};
+  p.X = d.X; p.ldx = g.lda; p.A = d.A; p.B = d.B; p.scales = d.scales; p.ids = d.ids;
   p.H = reinterpret_cast<float*>(ws);
-  float* acc = plan.acc_bytes ? reinterpret_cast<float*>(ws + plan.h_bytes) : static_cast<float*>(d.C);
-  p.acc = acc;
-  p.ldacc = plan.acc_bytes ? d.N : p.ldc;
-  GemmParams g;
-  g.A = d.X; g.lda = p.ldx; g.W = d.W; g.ldw = d.ldw ? d.ldw : d.K; g.bias = d.bias;
-  g.C = acc; g.ldc = p.ldacc; g.out_f32 = true;
-  g.M = d.M; g.N = d.N; g.K = d.K; g.act = ACT_NONE; g.w_const = true;
-  g.split_k = d.M < 64;
-  bool tc = false;
+  p.C = d.C; p.ldc = g.ldc; p.status = d.status;
+  p.M = d.M; p.N = d.N; p.K = d.K; p.rank = d.rank; p.rp = g.ad_rp; p.group = d.group; p.n_adapters = d.n_adapters; p.act = d.activation;
+  p.out_f32 = g.out_f32;
   if constexpr (sizeof(T) == 2) {
-    tc = gemm_tc_supported(g);
-    if (tc) {
+    if (plan.tensor) {
       B200_CUDA(gemm_tc_init());
       int dev = 0, sms = 0;
       B200_CUDA(cudaGetDevice(&dev));
       B200_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+      g.ad_h = p.H;
+      if (plan.piece_bytes && gemm_adapters_pair(g, sms)) g.ad_pieces = p.pieces = ws + plan.h_bytes;
+      if (!plan.mma) B200_CUDA(launch_shrink_rows<T>(p, s));
+      else if (p.rp <= 16) B200_CUDA((launch_shrink_mma<T, 1>(p, s)));
+      else if (p.rp <= 32) B200_CUDA((launch_shrink_mma<T, 2>(p, s)));
+      else if (p.rp <= 64) B200_CUDA((launch_shrink_mma<T, 4>(p, s)));
+      else B200_CUDA((launch_shrink_mma<T, 8>(p, s)));
+      DependentScope dependent;
       B200_CUDA(launch_gemm_tc<T>(g, d.status, sms, s));
+      return B200_OK;
     }
   }
-  if (!tc) B200_CUDA(launch_gemm_fma<T>(g, s));
-  adapters_shrink_kernel<T><<<ceil_div(d.M, 8), 256, 0, s>>>(p);
-  B200_CUDA(cudaGetLastError());
+  void* acc = plan.acc_bytes ? ws + plan.h_bytes : d.C;
+  g.C = acc; g.ldc = plan.acc_bytes ? d.N : g.ldc; g.out_f32 = true; g.act = ACT_NONE; g.ad_ids = nullptr;
+  p.acc = static_cast<const float*>(acc); p.ldacc = g.ldc;
+  B200_CUDA(launch_shrink_rows<T>(p, s));
+  B200_CUDA(launch_gemm_fma<T>(g, s));
   adapters_expand_kernel<T><<<dim3(ceil_div(d.N, 256), d.M < 32768 ? d.M : 32768), 256, 0, s>>>(p);
   B200_CUDA(cudaGetLastError());
   return B200_OK;

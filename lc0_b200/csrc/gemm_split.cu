@@ -23,6 +23,9 @@
 // beta arrive by bulk copy ahead of the grid dependency.  A LayerNorm vector may span several rows of A (smolgen's
 // second one: 32 heads x 256), as long as a tile holds whole vectors.  Every column tile repeats the LayerNorm: worth it
 // while a launch costs more than that (Net::gemm_with_ln has the line); beyond, ln_rows_kernel does it with the same results.
+// With adapters (kAd) the epilogue adds H[m] . B_a^T in fp32: a thread reads the B rows of its eight columns, which the requests of a
+// tile have or have not in common, so that one row per request costs no more code than 64.  The kernel before this one only
+// writes H, and A and W are loaded and multiplied while it runs.
 // Every wait is bounded by wall-clock time like those of gemm_tc.cu; the cluster barriers are reached by all threads
 // whatever happened before them.
 #include <atomic>
@@ -160,7 +163,42 @@ ln_rows_kernel(const T* x, T* out, const float* __restrict__ gamma, const float*
   }
 }
 
-template <typename T, int BN, bool kLN>
+// v[i] += H[m] . B_a[col + i]
+template <typename T>
+__device__ __forceinline__ void add_adapter(const TcParams& p, int m, int col, float (&v)[8]) {
+  const int a = adapter_of_row(p, m);
+  if (a < 0 || col >= p.N) return;
+  const int rank = p.ad_rank, cols = p.N - col < 8 ? p.N - col : 8;
+  const float* h = p.ad_h + (long long)m * rank;
+  const T* b = static_cast<const T*>(p.ad_b) + ((long long)a * p.N + col) * rank;
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[i] = 0.f;
+  if (rank % 8 == 0 && (reinterpret_cast<uintptr_t>(p.ad_b) & 15) == 0) {
+    for (int r = 0; r < rank; r += 8) {
+      const float4 h0 = *reinterpret_cast<const float4*>(h + r), h1 = *reinterpret_cast<const float4*>(h + r + 4);
+      const float hh[8] = {h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i >= cols) break;
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(b + i * rank + r));
+        const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[i] = fmaf(hh[j], to_f(e[j]), s[i]);
+      }
+    }
+  } else {
+    for (int r = 0; r < rank; ++r) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < cols) s[i] = fmaf(h[r], to_f(b[i * rank + r]), s[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] += s[i];
+}
+
+template <typename T, int BN, bool kLN, bool kAd>
 __global__ void __launch_bounds__(kSplitThreads)
 gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w, const TcParams p,
                   const SplitCfg cfg) {
@@ -225,7 +263,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     // ---------------- TMA producer ----------------
     if (elect_one()) {
       const int early = kbn < S ? kbn : S;
-      if (!p.w_const) grid_dependency_wait();
+      if (!p.w_const && !kAd) grid_dependency_wait();
       for (int i = 0; i < early; ++i) {
         const uint32_t fb = smem_u32(&full_bar[i]);
         mbar_expect_tx(fb, kLN ? BN * 128 : stage_bytes);
@@ -237,7 +275,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         bulk_load(smem_u32(ln_gb), cfg.gamma, bytes, gb);
         bulk_load(smem_u32(ln_gb) + bytes, cfg.beta, bytes, gb);
       }
-      grid_dependency_wait();
+      if (!kAd) grid_dependency_wait();
       int s = 0;
       uint32_t ph = 0;
       for (int i = 0; !kLN && i < kbn; ++i) {
@@ -376,7 +414,17 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += vb[i];
       }
-      apply_activation(v, p.act);
+      if constexpr (kAd) {
+        add_adapter<T>(p, m, col, v);
+        if (p.out_f32) {  // 16-bit results hide what the fast forms round, fp32 ones do not
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = activate<false>(v[i], p.act);
+        } else {
+          apply_activation(v, p.act);
+        }
+      } else {
+        apply_activation(v, p.act);
+      }
       if (p.res_mode) {
         const T* rs = reinterpret_cast<const T*>(p.res) + (long long)m * p.ldres + col;
         float s[8];
@@ -499,14 +547,14 @@ SplitPlan split_plan(const GemmParams& g, int sm_count) {
   return best;
 }
 
-template <typename T, int BN, bool kLN = false>
+template <typename T, int BN, bool kLN = false, bool kAd = false>
 cudaError_t launch_split_bn(const GemmParams& g, const SplitPlan& plan, int* status, cudaStream_t s) {
   static std::atomic<unsigned long long> attr_mask{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (!(attr_mask.load() >> (dev & 63) & 1ull)) {
-    e = cudaFuncSetAttribute(gemm_split_kernel<T, BN, kLN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(gemm_split_kernel<T, BN, kLN, kAd>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              kLN ? SplitTile<BN>::bytes(64, kLnK / BK) + SplitTile<BN>::ln_bytes(kLnMaxGroup) : 112 * 1024);
     if (e != cudaSuccess) return e;
     attr_mask.fetch_or(1ull << (dev & 63));
@@ -539,7 +587,7 @@ cudaError_t launch_split_bn(const GemmParams& g, const SplitPlan& plan, int* sta
   }
   lc.attrs = attr;
   lc.numAttrs = na;
-  return cudaLaunchKernelEx(&lc, gemm_split_kernel<T, BN, kLN>, ma, mw, p, cfg);
+  return cudaLaunchKernelEx(&lc, gemm_split_kernel<T, BN, kLN, kAd>, ma, mw, p, cfg);
 }
 
 }  // namespace
@@ -572,6 +620,11 @@ template cudaError_t launch_gemm_ln<__nv_bfloat16>(const GemmParams&, int*, cuda
 template <typename T>
 cudaError_t launch_gemm_split(const GemmParams& g, int* status, int sm_count, cudaStream_t s) {
   const SplitPlan plan = split_plan(g, sm_count);
+  if (g.ad_ids) {
+    if (plan.bn == 32) return launch_split_bn<T, 32, false, true>(g, plan, status, s);
+    if (plan.bn == 64) return launch_split_bn<T, 64, false, true>(g, plan, status, s);
+    return launch_split_bn<T, 128, false, true>(g, plan, status, s);
+  }
   if (plan.bn == 32) return launch_split_bn<T, 32>(g, plan, status, s);
   if (plan.bn == 64) return launch_split_bn<T, 64>(g, plan, status, s);
   return launch_split_bn<T, 128>(g, plan, status, s);

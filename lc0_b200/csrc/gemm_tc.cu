@@ -54,13 +54,15 @@ __device__ __forceinline__ void flush_row_ctx(const TcParams& p, int m, const Ro
 // their own: with every question asked at run time an epilogue thread of the four-group form spilled registers.
 enum EpilogueMode { kAny = 0, kPlain = 1 /*bias, activation*/, kNormIn = 2 /*folded LayerNorm of A, bias, activation*/,
                     kResidual = 3 /*bias, residual (normalised or not), row statistics; no activation*/,
-                    kConv = 4 /*convolution: bias, activation; or squeeze-excitation, residual, activation*/ };
+                    kConv = 4 /*convolution: bias, activation; or squeeze-excitation, residual, activation*/,
+                    kAdapters = 5 /*bias, activation; low-rank adapters as further k-blocks*/ };
 template <int kMode> struct Epilogue {
   static __device__ __forceinline__ bool a_stats(const TcParams& p) { return kMode == kAny ? p.a_stats != nullptr : kMode == kNormIn; }
   static __device__ __forceinline__ int res_mode(const TcParams& p) { return kMode == kAny || kMode == kResidual || kMode == kConv ? p.res_mode : 0; }
   static __device__ __forceinline__ bool out_stats(const TcParams& p) { return kMode == kAny ? p.out_stats != nullptr : kMode == kResidual; }
 };
 inline int epilogue_mode(const GemmParams& g) {
+  if (g.ad_ids) return kAdapters;
   if (g.batch_rows > 0 || g.scale != 1.0f) return kAny;
   if (g.conv_cin > 0) return g.a_stats || g.out_stats || g.res_stats || (g.res && g.se_k == 0) ? kAny : kConv;
   if (g.res) return g.out_stats && !g.a_stats && g.act == ACT_NONE ? kResidual : kAny;
@@ -82,6 +84,32 @@ __device__ __forceinline__ void use_row_stats(const TcParams& p, const RowStats&
   if (Epilogue<kMode>::a_stats(p)) mean_rstd(s.a, p.a_inv_c, p.a_eps, rc.mean_a, rc.rstd_a);
   if (Epilogue<kMode>::res_mode(p) == 2) mean_rstd(s.r, p.res_inv_c, p.res_eps, rc.mean_r, rc.rstd_r);
 }
+
+// One element of a product with adapters, in fp32 by the lanes of a warp: for the elements that the tensor core left not finite.
+template <typename T>
+__device__ __noinline__ float adapter_element(const T* x, const T* w, int K, const float* h, const T* b, int rank, int lane) {
+  float s = 0.f;
+  for (int k = lane; k < K; k += 32) s = fmaf(to_f(x[k]), to_f(w[k]), s);
+  for (int r = lane; r < rank; r += 32) s = fmaf(h[r], to_f(b[r]), s);
+  return warp_sum(s);
+}
+// The adapters of a 256-row tile, one further group of k-blocks for each: request by request (64 rows are one request's), each
+// adapter where it occurs first.
+struct TileAdapters {
+  int a[4];
+  __device__ __forceinline__ void fetch(const TcParams& p, int m) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = m + 64 * i < p.M ? adapter_of_row(p, m + 64 * i) : -1;
+  }
+  __device__ __forceinline__ bool first(int i) const {
+    bool f = a[i] >= 0;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) f = f && (j >= i || a[j] != a[i]);
+    return f;
+  }
+};
+// k-blocks of an adapter: H's two pieces side by side where both fit one, else each in blocks of 64.
+__device__ __forceinline__ int adapter_blocks(int rp) { return rp <= 32 ? 1 : 2 * ((rp + 63) / 64); }
 
 // One 64-column slab of the epilogue fast path, executed by one group of four warps: TMEM -> registers ->
 // scale / folded-LayerNorm correction / bias / activation / residual -> 128B-swizzled staging buffer, which the
@@ -114,7 +142,7 @@ __device__ __forceinline__ void epilogue_slab(const TcParams& p, uint8_t* buf, u
                                               uint32_t full_bar, uint32_t use, bool leader, uint32_t taddr, int row,
                                               int lane, int nb, int next_nb, ColRegs& cr, float* wvec, RowCtx& rc,
                                               volatile int* abort_flag, const float* se_arg = nullptr,
-                                              uint32_t res_use = 0) {
+                                              uint32_t res_use = 0, int m_row = 0) {
   using Ep = Epilogue<kMode>;
   const float* se = kSe ? se_arg : nullptr;  // compiled out of the kernels that never fuse squeeze-excitation
   // se != nullptr: gate (se[0..63]) and shift (se[256..319]) of this row's sample for the slab's 64 columns; the
@@ -144,6 +172,31 @@ __device__ __forceinline__ void epilogue_slab(const TcParams& p, uint8_t* buf, u
     } else {
 #pragma unroll
       for (int j = 0; j < kCols; ++j) v[j] = __uint_as_float(r[j]);
+    }
+    if constexpr (kMode == kAdapters) {
+      // Rows of other requests meet an adapter's B as zeros, and a zero times an infinity or NaN there is NaN; an H beyond the
+      // type's range is infinite as a piece.  What is not finite is computed again.
+      float z = 0.f;
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) z = fmaf(v[j], 0.f, z);
+      if (__any_sync(0xffffffffu, z != 0.f)) {
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) {
+          const int n = nb + kCols * h + j;
+          uint32_t bad = __ballot_sync(0xffffffffu, !(fabsf(v[j]) <= 3.402823466e38f) && m_row < p.M && n < p.N);
+          while (bad) {
+            const int src = __ffs(bad) - 1;
+            const long long m = __shfl_sync(0xffffffffu, m_row, src);
+            const int a = adapter_of_row(p, (int)m);
+            const float again = adapter_element<T>(static_cast<const T*>(p.a) + m * p.lda, static_cast<const T*>(p.w) + n * p.ldw, p.K,
+                                                   p.ad_h + m * p.ad_rank,
+                                                   static_cast<const T*>(p.ad_b) + ((long long)a * p.N + n) * p.ad_rank,
+                                                   a < 0 ? 0 : p.ad_rank, lane);
+            if (lane == src) v[j] = again;
+            bad &= bad - 1;
+          }
+        }
+      }
     }
     if (Ep::a_stats(p)) {
 #pragma unroll
@@ -1142,7 +1195,8 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     tma_prefetch_map(&tmap_w);
     tma_prefetch_map(&tmap_c);
     if (p.res_mode) tma_prefetch_map(&tmap_r);
-    if (p.n_split > 0) tma_prefetch_map(&tmap_c2);
+    if (p.n_split > 0 || kMode == kAdapters) tma_prefetch_map(&tmap_c2);  // kAdapters: B's map
+    if (kMode == kAdapters) tma_prefetch_map(&tmap_r);                      // kAdapters: the map of H's pieces
     if (p.split_from < p.tiles_v) tma_prefetch_map(&tmap_wh);
   }
   if (threadIdx.x == 0) {
@@ -1174,7 +1228,8 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   cluster_sync_all();  // the peer's barriers are initialised before anything arrives on them
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  grid_dependency_wait();  // everything above overlapped the kernel before this one
+  // Everything above overlapped the kernel before this one.  With adapters that kernel only writes H: the threads that read H wait there.
+  if (kMode != kAdapters) grid_dependency_wait();
   grid_launch_dependents();
 
   if (warp == 0) {
@@ -1183,6 +1238,9 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       int s = 0;         // stage and phase of the next k-block
       uint32_t ph = 0;
       bool ok = true;
+      TileAdapters ad, ad_next;
+      bool h_there = false;
+      if (kMode == kAdapters && pair < tiles) ad_next.fetch(p, (tile_of(pair) / n_tiles) * (2 * BM));
       for (int t = pair; t < tiles && ok; t += pairs) {
         const int m0 = (tile_of(t) / n_tiles) * (2 * BM) + (int)rank * BM;
         // a narrower tile is computed with a narrower MMA, of which each CTA supplies half the W rows
@@ -1207,7 +1265,33 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           }
           if (++s == S) { s = 0; ph ^= 1; }
         }
+        if constexpr (kMode == kAdapters) {
+          ad = ad_next;
+          if (t + pairs < tiles) ad_next.fetch(p, (tile_of(t + pairs) / n_tiles) * (2 * BM));
+          if (!h_there) { grid_dependency_wait(); h_there = true; }
+          const int blocks = adapter_blocks(p.ad_rp);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (!ad.first(i)) continue;
+            for (int b = 0; b < blocks && ok; ++b) {
+              if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 1)) { ok = false; break; }
+              const uint32_t fb_local = smem_u32(&full_bar[s]);
+              if (rank == 0) mbar_expect_tx(fb_local, half ? 2 * (BM + BN / 4) * BK * 2 : 2 * Cfg::kStageBytes);
+              const uint32_t fb = mapa(fb_local, 0);
+              const uint32_t sa = smem_u32(smem + s * Cfg::kStageBytes);
+              const int kb = blocks == 1 ? 0 : b % (blocks / 2), x = blocks == 1 ? 0 : b / (blocks / 2) * p.ad_rp + kb * BK;
+              // H of the rows with this adapter; for the others a box behind the last row, which TMA fills with zeros
+              tma_load_2d_pair(sa, &tmap_r, x, (rank ? ad.a[2] : ad.a[0]) == ad.a[i] ? m0 : p.M, fb);
+              tma_load_2d_pair(sa + 64 * 128, &tmap_r, x, (rank ? ad.a[3] : ad.a[1]) == ad.a[i] ? m0 + 64 : p.M, fb);
+              const int y = ad.a[i] * p.N + n0;  // a narrow tile's spare rows are another adapter's: columns that are not stored
+              tma_load_2d_pair(sa + BM * BK * 2, &tmap_c2, kb * BK, y, fb);
+              if (!half) tma_load_2d_pair(sa + BM * BK * 2 + 64 * 128, &tmap_c2, kb * BK, y + 64, fb);
+              if (++s == S) { s = 0; ph ^= 1; }
+            }
+          }
+        }
       }
+      if (kMode == kAdapters && !h_there) grid_dependency_wait();
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (even CTA only) ----------------
@@ -1232,6 +1316,8 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       int s = 0;         // stage and phase of the next k-block
       uint32_t ph = 0, tile_it = 0;
       bool ok = true;
+      TileAdapters ad_next;
+      if (kMode == kAdapters && pair < tiles) ad_next.fetch(p, (tile_of(pair) / n_tiles) * (2 * BM));
       for (int t = pair; t < tiles && ok; t += pairs, ++tile_it) {
         const uint32_t acc = tile_it & 1, aph = (tile_it >> 1) & 1;
         if (!mbar_wait(smem_u32(&tempty_bar[acc]), aph ^ 1, abort_flag, 2)) break;
@@ -1250,11 +1336,34 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           commit(smem_u32(&empty_bar[s]));  // frees the stage in both CTAs once the MMAs have read it
           if (++s == S) { s = 0; ph ^= 1; }
         }
+        if constexpr (kMode == kAdapters) {
+          const TileAdapters ad = ad_next;
+          if (t + pairs < tiles) ad_next.fetch(p, (tile_of(t + pairs) / n_tiles) * (2 * BM));
+          const int blocks = adapter_blocks(p.ad_rp), of_b = p.ad_rp / 16;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (!ad.first(i)) continue;
+            for (int b = 0; b < blocks && ok; ++b) {
+              if (!mbar_wait(smem_u32(&full_bar[s]), ph, abort_flag, 3)) { ok = false; break; }
+              tcgen05_fence_after();
+              const uint32_t sa = smem_u32(smem + s * Cfg::kStageBytes);
+              const uint64_t adesc = make_smem_desc(sa);
+              const uint64_t bdesc = make_smem_desc(sa + BM * BK * 2);
+              // both pieces of a narrow H meet the same columns of B
+              const int left = blocks == 1 ? 2 * of_b : of_b - b % (blocks / 2) * 4;
+              for (int k = 0; k < 4 && k < left; ++k)
+                tcgen05_mma_f16_pair(d_tmem, adesc + 2 * k, bdesc + 2 * (blocks == 1 && k >= of_b ? k - of_b : k), idesc, 1u);
+              commit(smem_u32(&empty_bar[s]));
+              if (++s == S) { s = 0; ph ^= 1; }
+            }
+          }
+        }
         if (ok) commit(smem_u32(&tfull_bar[acc]));
       }
     }
   } else if (warp == 2 || warp == 3) {
     // ---------------- store warps (both CTAs): TMA stores of the staged slabs, half of the groups each ----------
+    if (kMode == kAdapters) grid_dependency_wait();
     if (elect_one())
       store_warp_loop<kGroups, kBufs>(p, &tmap_c, &tmap_c2, &tmap_r, epi_mem, stg_full, stg_free, res_bar,
                                       (warp - 2) * (kGroups / 2), (warp - 1) * (kGroups / 2), pair, pairs, tiles, n_tiles,
@@ -1262,6 +1371,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   } else {
     // ---------------- epilogue (warps 4.. of both CTAs): group g handles the 64-column slabs g, g + kGroups, ... of
     // every tile ----------------
+    if (kMode == kAdapters) grid_dependency_wait();  // adapter_element reads H
     const int quarter = warp & 3;
     const int group = (warp - 4) >> 2;
     const bool leader = ((warp - 4) & 3) == 0 && lane == 0;
@@ -1327,7 +1437,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         epilogue_slab<T, kMode == kConv, false, kMode, kGroups == 2 && kMode != kAny && kMode != kConv ? 64 : 32>(
             p, epi_mem + idx * (BM * 128), smem_u32(&res_bar[idx]), smem_u32(&stg_free[idx]), smem_u32(&stg_full[idx]),
             slab_it / kBufs, leader, trow + c0, quarter * 32 + lane, lane, n0 + c0, next_nb, cr, wvec, rc, abort_flag,
-            se_row ? se_row + c0 : nullptr);
+            se_row ? se_row + c0 : nullptr, 0, m);
         ++slab_it;
       }
       if (Epilogue<kMode>::out_stats(p)) flush_row_ctx(p, m, rc);
@@ -1757,6 +1867,11 @@ cudaError_t launch_pair_mode(const GemmParams& g, int* status, int sm_count, cud
     e = get_map(g.C2, g.ldc2, g.M, g.N - g.n_split, BM, prec, &mc2);
     if (e != cudaSuccess) return e;
   }
+  if (kMode == kAdapters) {
+    e = get_map(g.ad_pieces, 2 * g.ad_rp, g.M, 2 * g.ad_rp, 64, prec, &mr);
+    if (e == cudaSuccess) e = get_map(g.ad_b, g.ad_rank, g.ad_n * g.N, g.ad_rank, 64, prec, &mc2);
+    if (e != cudaSuccess) return e;
+  }
   TcParams p;
   fill_tc_params(p, g, status);
   p.tma_store = 1;
@@ -1812,6 +1927,8 @@ cudaError_t launch_pair(const GemmParams& g, int* status, int sm_count, cudaStre
                             : launch_pair_mode<T, 2, true, kResidual>(g, status, sm_count, s);
     case kConv:
       return launch_pair_mode<T, 2, true, kConv>(g, status, sm_count, s);
+    case kAdapters:
+      return launch_pair_mode<T, 2, true, kAdapters>(g, status, sm_count, s);
     default:
       if (few || (g.conv_cin == 0 && g.K <= (g.res ? 12 : g.out_stats ? 9 : 8) * BK))
         return launch_pair_mode<T, 4, false, kAny>(g, status, sm_count, s);
@@ -1908,6 +2025,11 @@ bool pair_eligible(const GemmParams& p, int sm_count) {
          (long long)ceil_div(p.M, 2 * BM) * ceil_div(p.N, 256) >= sm_count / 4;
 }
 }  // namespace
+
+bool gemm_adapters_pieces(const GemmParams& p) {
+  return p.ad_group % 64 == 0 && p.ad_rank % 8 == 0 && (long long)p.ad_n * p.N < 0x7fffff00 && (reinterpret_cast<uintptr_t>(p.ad_b) & 15) == 0;
+}
+bool gemm_adapters_pair(const GemmParams& p, int sm_count) { return gemm_adapters_pieces(p) && pair_eligible(p, sm_count); }
 
 bool gemm_tc_split_supported(const GemmParams& p) {
   if (!gemm_tc_supported(p) || p.n_split <= 0 || p.N <= p.n_split || !p.C2 || (p.ldc2 % 8) != 0 ||
@@ -2033,6 +2155,11 @@ cudaError_t launch_gemm_tc(const GemmParams& p, int* status, int sm_count, cudaS
   if (!gemm_tc_supported(p) || p.skip) return cudaErrorInvalidValue;  // residuals go through `res`
   if (p.n_split > 0 && !gemm_tc_split_supported(p)) return cudaErrorInvalidValue;
   if (!epilogue_supported(p)) return cudaErrorInvalidValue;
+  if (p.ad_ids) {
+    if (p.conv_cin > 0 || p.batch_rows > 0 || p.a_stats || p.res || p.out_stats || p.n_split > 0 || p.scale != 1.0f || !p.ad_h)
+      return cudaErrorInvalidValue;
+    return p.ad_pieces ? launch_pair<T>(p, status, sm_count, s) : launch_gemm_split<T>(p, status, sm_count, s);
+  }
   if (pair_eligible(p, sm_count)) return launch_pair<T>(p, status, sm_count, s);
   if (p.se_k > 0) return launch_bn<T, 256>(p, status, sm_count, s);  // the tile must hold every channel of two boards
   // More 128x128 tiles than two per SM: the persistent kernel's wide tiles (256x32768x768, the dense positional encoding of 256

@@ -303,6 +303,10 @@ struct TcParams {
   int vec_c;                 // gemm_split.cu: C (and C2) may be written in 16-byte pieces
   int w_const;               // gemm_split.cu: W may be requested ahead of the grid dependency
   int batch_rows;  // > 0: stacked products, rows [b * batch_rows, (b + 1) * batch_rows) use W rows [b * N, (b + 1) * N)
+  // low-rank adapters (see GemmParams)
+  const int* ad_ids; const float* ad_h; const void* ad_b;
+  int ad_group, ad_n, ad_rank, ad_rp;
+  const void* a; long long lda; const void* w; long long ldw;  // operands, for the elements that are computed again
 };
 
 __device__ __forceinline__ void mean_rstd(const double2 st, float inv_c, float eps, float& mean, float& rstd) {
@@ -326,6 +330,12 @@ template <> __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float l
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Adapter of row m, -1 for none.
+__device__ __forceinline__ int adapter_of_row(const TcParams& p, int m) {
+  const int a = __ldg(p.ad_ids + m / p.ad_group);
+  return a >= 0 && a < p.ad_n ? a : -1;
+}
+
 // Epilogue parameters of a product that are the same for every kernel.
 inline void fill_tc_params(TcParams& p, const GemmParams& g, int* status) {
   p.bias = g.bias; p.C = g.C; p.ldc = g.ldc;
@@ -344,6 +354,9 @@ inline void fill_tc_params(TcParams& p, const GemmParams& g, int* status) {
   p.se_k = g.se_k;
   p.batch_rows = g.batch_rows;
   p.w_const = g.w_const ? 1 : 0;
+  p.ad_ids = g.ad_ids; p.ad_h = g.ad_h; p.ad_b = g.ad_b;
+  p.ad_group = g.ad_group; p.ad_n = g.ad_n; p.ad_rank = g.ad_rank; p.ad_rp = g.ad_rp;
+  p.a = g.A; p.lda = g.lda; p.w = g.W; p.ldw = g.ldw;
   auto al16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
   const int per16 = g.out_f32 ? 4 : 8;
   p.vec_c = al16(g.C) && (g.ldc % per16) == 0 && (g.n_split == 0 || (al16(g.C2) && (g.ldc2 % per16) == 0));

@@ -169,7 +169,8 @@ def test_requests_without_an_adapter(lib, prec, M, group):
 def test_values_that_are_not_finite_stay_with_their_rows(lib):
     for M, group in ((40, 1), (8192, 64)):
         c = Call(lib, M, 512, 256, 16, group, 8, 2, ids=torch.arange((M + group - 1) // group) % 8)
-        clean = c.run().clone()
+        c.run()
+        want, allowed = c.want()
         c.x[3, 5] = float("inf")
         c.b[5, 7, 2] = float("nan")
         c.a[6, 3] = float("inf")
@@ -179,7 +180,9 @@ def test_values_that_are_not_finite_stay_with_their_rows(lib):
         bad[3] = True
         bad[ids == 6] = True
         bad[ids == 5, 7] = True
-        assert torch.equal(got[~bad], clean[~bad])
+        # not the same bits: an element that the tensor core met as zero times NaN is summed again in another order, and each order is
+        # within the allowance of the exact sum
+        assert ((got.double() - want).abs() <= allowed)[~bad].all()
         assert not torch.isfinite(got[ids == 5, 7]).any() and not torch.isfinite(got[3]).any() and not torch.isfinite(got[ids == 6]).any()
 
 
