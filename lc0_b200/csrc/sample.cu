@@ -22,8 +22,8 @@ namespace b200 {
 namespace {
 
 constexpr int kMaxCluster = 8;
-constexpr int kWide = 1024;             // threads of the largest CTA
-constexpr int kMaxPieces = 13;          // 16-byte pieces per thread there: 208 KB
+constexpr int kWide = 512;              // threads of the largest CTA
+constexpr int kMaxPieces = 17;          // 16-byte pieces per thread there: 136 KB
 constexpr int kWarpRows = 4;            // rows of a CTA whose groups are warps
 static_assert(kMaxCluster * kWide * kMaxPieces * 4 >= B200_SAMPLE_MAX_WIDTH + 8, "the widest row fits a cluster");
 
@@ -122,36 +122,27 @@ template <int kThreads> struct Group {
   }
 };
 
-// Weights in fp32 or, kExact, in 64 bits.
-template <bool kExact> struct Weight;
-template <> struct Weight<false> {
-  using type = float;
+// Weights in fp32 or in 64 bits, of a row whose largest logit is finite.
+struct Weight {
   float half_max, c, c_lo, max;
+  double inv_t;
   __device__ Weight(float m, float t) : max(m) {
-    const double e = 1.4426950408889634 / (double)t;
+    inv_t = 1.0 / (double)t;
+    const double e = 2.8853900817779268 * inv_t;  // 2 log2(e) / T
     half_max = 0.5f * m;
-    c = (float)(2.0 * e);
-    c_lo = (float)(2.0 * e - (double)c);
+    c = (float)fmin(e, 1e37);
+    c_lo = (float)(fmin(e, 1e37) - (double)c);
   }
-  __device__ bool usable() const { return fabsf(c) < 1e37f; }
+  __device__ bool fp32_usable() const { return c < 1e37f; }
   // 2^((l - m) log2(e) / T) with the exponent in two pieces; halves, since l - m can overflow
-  __device__ __forceinline__ float operator()(float l) const {
+  __device__ __forceinline__ float get(float l, float) const {
     const float x = 0.5f * l - half_max;
-    const float z = x * c;
+    const float z = fmaxf(x * c, -200.f);
     const float lo = fmaf(x, c_lo, fmaf(x, c, -z));
     const float w = exp2f(z);
-    return l == max ? 1.0f : z < -140.f || max == INFINITY ? 0.0f : fmaf(w, lo * 0.69314718f, w);
+    return z <= -140.f ? 0.0f : fmaf(w, lo * 0.69314718f, w);
   }
-};
-template <> struct Weight<true> {
-  using type = double;
-  double t;
-  float max;
-  __device__ Weight(float m, float temp) : t((double)temp), max(m) {}
-  __device__ bool usable() const { return true; }
-  __device__ __forceinline__ double operator()(float l) const {
-    return l == max ? 1.0 : max == INFINITY ? 0.0 : exp(((double)l - (double)max) / t);
-  }
+  __device__ __forceinline__ double get(float l, double) const { return exp(((double)l - (double)max) * inv_t); }
 };
 
 template <typename T> struct Pieces;  // 16 bytes of logits as fp32
@@ -218,187 +209,578 @@ __device__ int load_row(const SampleParams& p, const Group<kThreads>& g, int row
   return first;
 }
 
-// The row in `mine` (this thread's entries, slot0 the first one's slot): cuts and draw.  False: a comparison was open.
-template <bool kExact, int kThreads>
-__device__ bool draw_row(const SampleParams& p, Group<kThreads>& g, int row, float* mine, int slot0, int first, float temp) {
-  const int count = 4 * p.pieces;
-  const double slack = kExact ? 0.0 : (double)p.slack;
-  auto each = [&](auto f) {
+// What stays of a row: entries above `l`, and those equal to it up to `slot`.
+struct Cut {
+  float l = -INFINITY;
+  int slot = -1;
+  __device__ __forceinline__ bool keeps(float x, int s) const { return x > l || (x == l && s <= slot); }
+};
+
+constexpr int kBins = 256;
+constexpr int kSort = 64;    // entries that a warp sorts
+constexpr int kGather = 256;  // entries that a warp gathers from its row
+
+template <int kThreads> struct Shared {
+  double slots[2 * Group<kThreads>::kSlots];
+  uint32_t bins[kBins], total[kBins];
+  float list_l[kThreads == 32 ? kGather : kSort];
+  int list_slot[kThreads == 32 ? kGather : kSort];
+  int count;
+  int solved;
+  uint64_t cut;
+};
+
+// Entries as 64-bit numbers whose order is the row's: by logit, of equal ones the lower slot is larger.  0: none.
+__device__ __forceinline__ uint64_t entry_of(float l, int slot) {
+  return l > -INFINITY ? (uint64_t)key_of(l) << 32 | (uint32_t)~slot : 0;
+}
+__device__ __forceinline__ Cut cut_of(uint64_t e) {
+  Cut c;
+  c.l = of_key((uint32_t)(e >> 32));
+  c.slot = (int)~(uint32_t)e;
+  return c;
+}
+// Sorts 32 (b = 0) or 64 entries of a warp, falling: a lane's `a` is number lane, its `b` number 32 + lane.
+__device__ __forceinline__ void sort_entries(uint64_t& a, uint64_t& b, bool two, int lane) {
+  auto step = [&](uint64_t v, int j, bool larger) {
+    const uint64_t o = __shfl_xor_sync(0xffffffffu, v, j);
+    return (v > o) == larger ? v : o;
+  };
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      a = step(a, j, ((lane & j) == 0) == ((lane & k) == 0));
+      // the upper half rises, so that both form one bitonic run of 64
+      if (two) b = step(b, j, ((lane & j) == 0) == (k == 32 ? false : (lane & k) == 0));
+    }
+  if (!two) return;
+  if (b > a) { const uint64_t t = a; a = b; b = t; }
+#pragma unroll
+  for (int j = 16; j > 0; j >>= 1) {
+    a = step(a, j, (lane & j) == 0);
+    b = step(b, j, (lane & j) == 0);
+  }
+}
+__device__ __forceinline__ double warp_before(double v, double& total, int lane) {
+  double in = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double up = __shfl_up_sync(0xffffffffu, in, o);
+    if (lane >= o) in += up;
+  }
+  total = __shfl_sync(0xffffffffu, in, 31);
+  const double ex = __shfl_up_sync(0xffffffffu, in, 1);
+  return lane == 0 ? 0.0 : ex;
+}
+
+// A row in shared memory, seen by one thread of its group.
+template <int kThreads> struct Row {
+  Group<kThreads>& g;
+  Shared<kThreads>& sh;
+  const SampleParams& p;
+  float* mine;   // this thread's entries
+  int slot0;     // slot of the first of them
+  int count;     // their number
+  int row, first;
+  Weight wt;
+
+  template <typename F> __device__ __forceinline__ void each(F f) const {
+#pragma unroll 4
     for (int i = 0; i < count; i += 4) {
       const float4 x = *reinterpret_cast<const float4*>(mine + i);
       f(i, x.x); f(i + 1, x.y); f(i + 2, x.z); f(i + 3, x.w);
     }
-  };
-  float m = -INFINITY;
-  each([&](int, float l) { m = fmaxf(m, l); });
-  m = g.max(m);
-  auto give = [&](int slot, float prob) {
-    p.choice[row] = slot < 0 ? -1 : slot - first;
-    if (p.prob) p.prob[row] = prob;
-  };
-  if (m == -INFINITY) {
-    if (g.thread() == 0) give(-1, 0.f);
-    return true;
   }
-  if (!(temp > 0.f)) {  // the first of the largest
-    int at = 0x7fffffff;
-    each([&](int i, float l) { if (l == m && at == 0x7fffffff) at = slot0 + i; });
-    const int best = -(int)g.max(at == 0x7fffffff ? -INFINITY : -(float)at);
-    if (g.thread() == 0) give(best, 1.f);
-    return true;
-  }
-  const Weight<kExact> weight(m, temp);
-  if (!weight.usable()) return false;
-  using W = typename Weight<kExact>::type;
-  auto mass = [&](auto keep) {
-    W a[4] = {};
+  // Sum of f over this thread's entries: pieces of four, groups of four pieces in W, the groups in 64 bits.
+  template <typename W, typename F> __device__ __forceinline__ double sum(F f) const {
+    double total = 0.0;
+    W run = 0;
+#pragma unroll 4
     for (int i = 0; i < count; i += 4) {
       const float4 x = *reinterpret_cast<const float4*>(mine + i);
-      if (keep(x.x)) a[0] += weight(x.x);
-      if (keep(x.y)) a[1] += weight(x.y);
-      if (keep(x.z)) a[2] += weight(x.z);
-      if (keep(x.w)) a[3] += weight(x.w);
+      const W a = f(i, x.x), b = f(i + 1, x.y), c = f(i + 2, x.z), d = f(i + 3, x.w);
+      run += (a + b) + (c + d);
+      if ((i & 12) == 12) { total += (double)run; run = 0; }
     }
-    return (double)((a[0] + a[1]) + (a[2] + a[3]));
-  };
-  // Keeps what is larger than `cut` and the first `ties` of the entries that equal it.
-  auto cut_at = [&](float cut, long long ties) {
+    return total + (double)run;
+  }
+  __device__ __forceinline__ void give(int slot, float prob) const {
+    p.choice[row] = slot < 0 ? -1 : slot - first;
+    if (p.prob) p.prob[row] = prob;
+  }
+  // Slot of the j-th (from 0) entry equal to l.
+  __device__ int nth_equal(float l, double j) {
     int same = 0;
-    each([&](int, float l) { same += l == cut; });
+    each([&](int, float x) { same += x == l; });
     double all;
-    long long left = ties - (long long)g.before((double)same, all);
-    for (int i = 0; i < count; ++i) {
-      const float l = mine[i];
-      if (l == cut) { if (left <= 0) mine[i] = -INFINITY; --left; }
-      else if (l < cut) mine[i] = -INFINITY;
-    }
-  };
-  const uint32_t top = key_of(m), bottom = key_of(-INFINITY);
-  const float p_top = p.top_p ? p.top_p[row] : 1.f;
-  const int k = p_top <= 0.f ? 1 : p.top_k ? p.top_k[row] : 0;
-  if (k > 0 && k < g.threads() * count) {
-    // the smallest key above which fewer than k entries lie
-    uint32_t lo = bottom, hi = top;  // k or more above lo (else every entry stays), fewer above hi
-    auto above = [&](float cut) {
-      int c = 0;
-      each([&](int, float l) { c += l > cut; });
-      return g.sum((double)c);
-    };
-    if (above(-INFINITY) > (double)k) {
-      double over = 0.0;  // above hi
-      while (hi - lo > 1) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        const double c = above(of_key(mid));
-        if (c >= (double)k) lo = mid;
-        else { hi = mid; over = c; }
-      }
-      cut_at(of_key(hi), k - (long long)over);
-    }
+    double left = j - g.before((double)same, all);
+    int at = -1;
+    if (left >= 0.0 && left < (double)same)
+      each([&](int i, float x) {
+        if (x == l) {
+          if (left == 0.0) at = slot0 + i;
+          left -= 1.0;
+        }
+      });
+    return (int)g.max((float)at);
   }
-  if (p_top > 0.f && p_top < 1.f) {
-    const double all = g.sum(mass([](float l) { return l > -INFINITY; }));
-    const double target = (double)p_top * all;
-    uint32_t lo = bottom, hi = top;  // mass above lo: the target or more; above hi: less
+
+  // The end of the front part of what `in` keeps: the first entry ahead of which the measure (kMass: weights, else 1 each) sums to the
+  // target or more is out, with all behind it; the first of all stays.  `all`: the measure of what `in` keeps.  Bins of a range of
+  // logits, the bin that the target falls in, the exact measure above it and its entries, until those are few enough to be sorted.
+  // False: a comparison was open.
+  template <typename W, bool kMass> __device__ bool select(const Cut in, double target, double all, float hi, float lo, double slack, Cut& out) {
+    constexpr bool kOpen = kMass && sizeof(W) == 4;
+    auto measure = [&](float l) -> W { if constexpr (kMass) return wt.get(l, W()); else return W(1); };
+    double above = 0.0;  // of entries above the range
+    double inside = all;
+    for (int round = 0; round < 8; ++round) {
+      const float scale = fminf((kBins - 0.01f) / fminf(hi - lo, 3.4e38f), 1e37f);
+      // the lowest bin of the first round takes what lies below the range
+      auto bin = [&](float l) { return (int)fminf((hi - l) * scale, kBins - 1.f); };
+      auto ranged = [&](float l) { return l <= hi && (l >= lo || round == 0); };
+      const double quantum = 1073741824.0 / inside;
+      const float fq = (float)quantum;
+      g.barrier();  // the others are done with what is cleared
+      const int tid = kThreads == 32 ? g.lane : (int)threadIdx.x;
+      for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
+      if (tid == 0) sh.count = 0;
+      if (kThreads == 32) __syncwarp(); else __syncthreads();
+      each([&](int i, float l) {
+        if (in.keeps(l, slot0 + i) && ranged(l)) {
+          const uint32_t q = kMass ? (uint32_t)((float)wt.get(l, 0.f) * fq) : 1u;
+          if (q) atomicAdd(&sh.bins[bin(l)], q);
+        }
+      });
+      g.barrier();
+      const uint32_t* total = sh.bins;
+      if (kThreads == kWide && g.cluster > 1) {
+        for (int i = tid; i < kBins; i += kThreads) {
+          uint32_t t = 0;
+          for (int c = 0; c < g.cluster; ++c) t += *cg::this_cluster().map_shared_rank(&sh.bins[i], c);
+          sh.total[i] = t;
+        }
+        total = sh.total;
+        __syncthreads();
+      }
+      // first bin at whose end the target is reached; behind the last full one where rounding leaves none
+      uint32_t part[kBins / 32], sum8 = 0;
+#pragma unroll
+      for (int i = 0; i < kBins / 32; ++i) {
+        part[i] = total[g.lane * (kBins / 32) + i];
+        sum8 += part[i];
+      }
+      uint32_t in8 = sum8;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, in8, o);
+        if (g.lane >= o) in8 += up;
+      }
+      const double goal = (target - above) * (kMass ? quantum : 1.0);
+      uint32_t run = in8 - sum8;
+      int b = kBins, last = -1;
+#pragma unroll
+      for (int i = 0; i < kBins / 32; ++i) {
+        run += part[i];
+        if (part[i]) last = g.lane * (kBins / 32) + i;
+        if (b == kBins && part[i] && (double)run >= goal) b = g.lane * (kBins / 32) + i;
+      }
+      b = __reduce_min_sync(0xffffffffu, b);
+      last = __reduce_max_sync(0xffffffffu, last);
+      if (b == kBins) b = last;
+      if (b < 0) break;
+      float least = INFINITY, most = -INFINITY;
+      double more = 0.0;
+      {
+        W run4 = 0;
+        int n = 0;
+        each([&](int i, float l) {
+          if (in.keeps(l, slot0 + i) && ranged(l)) {
+            const int at = bin(l);
+            if (at < b) {
+              run4 += measure(l);
+              if (++n == 8) { more += (double)run4; run4 = 0; n = 0; }
+            } else if (at == b) {
+              least = fminf(least, l);
+              most = fmaxf(most, l);
+              const int pos = atomicAdd(&sh.count, 1);
+              if (pos < kSort) { sh.list_l[pos] = l; sh.list_slot[pos] = slot0 + i; }
+            }
+          }
+        });
+        more += (double)run4;
+      }
+      above += g.sum(more);
+      int n = sh.count;
+      if (kThreads == kWide && g.cluster > 1) {
+        n = 0;
+        for (int c = 0; c < g.cluster; ++c) n += *cg::this_cluster().map_shared_rank(&sh.count, c);
+      }
+      if (n == 0) break;
+      if (n > kSort) {
+        hi = g.max(most);
+        lo = -g.max(-least);
+        if (hi == lo) {  // equal entries
+          const double w = (double)measure(hi), ties = (target - above) / w;
+          if (kOpen && (w < 1e-30 || fabs(ties - rint(ties)) <= slack * all / w + 1e-6 * fabs(ties) || ties <= 0.0 || ties > (double)n)) return false;
+          if (!(ties > 0.0) || ties > (double)n) break;
+          out.l = hi;
+          out.slot = nth_equal(hi, ceil(ties) - 1.0);
+          return true;
+        }
+        inside = kMass ? fmin(all, fmax((double)n * (double)measure(hi), 1e-28)) : (double)n;
+        continue;
+      }
+      if (kThreads == 32 || g.warp == 0) {
+        uint64_t e[2] = {0, 0};
+        if (kThreads == kWide && g.cluster > 1) {
+          int base = 0;
+          for (int c = 0; c < g.cluster; ++c) {
+            const int nc = *cg::this_cluster().map_shared_rank(&sh.count, c);
+            const float* ll = cg::this_cluster().map_shared_rank(sh.list_l, c);
+            const int* ls = cg::this_cluster().map_shared_rank(sh.list_slot, c);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int i = g.lane + 32 * h - base;
+              if (i >= 0 && i < nc) e[h] = entry_of(ll[i], ls[i]);
+            }
+            base += nc;
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (g.lane + 32 * h < n) e[h] = entry_of(sh.list_l[g.lane + 32 * h], sh.list_slot[g.lane + 32 * h]);
+        }
+        sort_entries(e[0], e[1], n > 32, g.lane);
+        double w[2], t0, t1;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[h] = e[h] ? (double)measure(of_key((uint32_t)(e[h] >> 32))) : 0.0;
+        double before[2];
+        before[0] = above + warp_before(w[0], t0, g.lane);
+        before[1] = above + t0 + warp_before(w[1], t1, g.lane);
+        const double end = above + t0 + t1;
+        // entries of the list that stay: those ahead of which less than the target lies
+        const uint32_t in0 = __ballot_sync(0xffffffffu, e[0] && before[0] < target), in1 = __ballot_sync(0xffffffffu, e[1] && before[1] < target);
+        const int stay = __popc(in0) + __popc(in1);
+        bool open = false;
+        if (kOpen) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) open |= e[h] && fabs(before[h] - target) <= slack * all;
+          open = __any_sync(0xffffffffu, open) || fabs(end - target) <= slack * all;
+        }
+        const uint64_t c0 = __shfl_sync(0xffffffffu, e[0], (stay - 1) & 31), c1 = __shfl_sync(0xffffffffu, e[1], (stay - 1) & 31);
+        if (g.lane == 0) {
+          sh.solved = open ? 2 : stay > 0 && (end >= target || !kMass) ? 1 : 0;
+          sh.cut = stay > 32 ? c1 : c0;
+        }
+      }
+      if (kThreads == 32) __syncwarp(); else __syncthreads();
+      if (sh.solved == 2) return false;
+      if (sh.solved == 0) break;
+      out = cut_of(sh.cut);
+      return true;
+    }
+    if (kOpen) return false;
+    // Bins did not find it (sums of theirs are rounded, ranges can hold a few values many decades apart): bisection.
+    uint32_t lo_key = key_of(-INFINITY), hi_key = key_of(wt.max);  // measure above lo_key: the target or more; above hi_key: less
     double over = 0.0;
-    while (hi - lo > 1) {
-      const uint32_t mid = lo + (hi - lo) / 2;
+    while (hi_key - lo_key > 1) {
+      const uint32_t mid = lo_key + (hi_key - lo_key) / 2;
       const float cut = of_key(mid);
-      const double above = g.sum(mass([&](float l) { return l > cut; }));
-      if (!kExact && fabs(above - target) <= slack * all) return false;
-      if (above >= target) lo = mid;
-      else { hi = mid; over = above; }
+      const double m = g.sum(sum<W>([&](int i, float l) { return l > cut && in.keeps(l, slot0 + i) ? measure(l) : W(0); }));
+      if (m >= target) lo_key = mid;
+      else { hi_key = mid; over = m; }
     }
-    // of entries equal to the cut the j-th (from 0) stays while over + j w < target; the first of all always does
-    const float cut = of_key(hi);
-    const double w = (double)weight(cut), ties = (target - over) / w;
-    if (!kExact && (w < 1e-30 || fabs(ties - rint(ties)) <= 2.0 * slack * all / w + 1e-6 * fabs(ties))) {
-      // open, unless there is a single one
-      int same = 0;
-      each([&](int, float l) { same += l == cut; });
-      if (g.sum((double)same) > 1.0) return false;
-    }
-    cut_at(cut, ties >= 1e9 ? 1000000000ll : ties <= 1.0 ? 1ll : (long long)ceil(ties));
-  }
-  const float p_min = p.min_p ? p.min_p[row] : 0.f;
-  if (p_min > 0.f) {
-    bool open = false;
-    const W limit = (W)fminf(p_min, 1.f);
-    for (int i = 0; i < count; ++i) {
-      const W w = weight(mine[i]);
-      if (!kExact && mine[i] > -INFINITY && fabs((double)w - (double)limit) <= slack * (double)limit) open = mine[i] != m;
-      if (w < limit) mine[i] = -INFINITY;
-    }
-    if (!kExact && g.sum(open ? 1.0 : 0.0) > 0.0) return false;
-  }
-  double total;
-  const double own = mass([](float l) { return l > -INFINITY; });
-  const double ahead = g.before(own, total);
-  float u = p.u[row];
-  u = u >= 0.f ? fminf(u, 1.f - 0x1p-24f) : 0.f;
-  const double target = (double)u * total;
-  // the thread whose entries the running sum passes the target in; the last with a weight where rounding leaves none
-  const bool here = ahead <= target && target < ahead + own;
-  bool open = false;
-  int at = -1;
-  if (here) {
-    double run = ahead;
-    for (int i = 0; i < count; ++i) {
-      const double w = mine[i] > -INFINITY ? (double)weight(mine[i]) : 0.0;
-      if (w > 0.0) {
-        at = i;
-        if (run + w > target) break;
-      }
-      run += w;
-    }
-    const double w = (double)weight(mine[at]);
-    open = !kExact && (target - run <= slack * total || run + w - target <= slack * total);
-  }
-  if (!kExact) {
-    if (g.sum(here ? (open ? 2.0 : 1.0) : 0.0) != 1.0) return false;
-    if (here) give(slot0 + at, (float)((double)Weight<true>(m, temp)(mine[at]) / total));
+    out.l = of_key(hi_key);
+    const double ties = (target - over) / (double)measure(out.l);
+    out.slot = nth_equal(out.l, ties <= 1.0 ? 0.0 : ceil(fmin(ties, 1e9)) - 1.0);
+    if (out.slot < 0) out.slot = 0x7fffffff;  // all of them
     return true;
   }
-  // 64 bits: neighbours' bounds can differ in their last bit, so that two threads claim the draw (the first has it) or none does (the
-  // last thread with a weight has it)
-  const float id = (float)g.thread();
-  float owner = -g.max(here ? -id : -INFINITY);
-  if (owner == INFINITY) {
-    owner = g.max(own > 0.0 ? id : -INFINITY);
-    for (int i = 0; i < count; ++i)
-      if (mine[i] > -INFINITY && weight(mine[i]) > (W)0) at = i;
+
+  // The draw among what `cut` keeps and min-p.  False: a comparison was open.
+  template <typename W> __device__ bool draw(const Cut cut, float p_min, float u, double slack) {
+    constexpr bool kOpen = sizeof(W) == 4;
+    const W limit = p_min > 0.f ? (W)fminf(p_min, 1.f) : W(0);
+    bool open = false;
+    auto weigh = [&](int i, float l) -> W {
+      if (!cut.keeps(l, slot0 + i)) return W(0);
+      const W w = wt.get(l, W());
+      if (kOpen && limit > W(0) && fabsf((float)w - (float)limit) <= 4.f * (float)slack * (float)limit && l != wt.max) open = true;
+      return w >= limit ? w : W(0);
+    };
+    const double own = sum<W>(weigh);
+    double total;
+    const double ahead = g.before(own, total), target = (double)u * total;
+    const bool here = ahead <= target && target < ahead + own;
+    // the warp of the thread whose entries the sum passes the target in looks for the entry together
+    const float id = (float)g.thread();
+    float owner = 0.f;
+    bool claims = here;
+    if (!kOpen) {  // neighbours' bounds can differ in their last bit: the first that claims it, else the last with a weight
+      owner = -g.max(here ? -id : -INFINITY);
+      if (owner == INFINITY) owner = g.max(own > 0.0 ? id : -INFINITY);
+      claims = id == owner;
+    }
+    const uint32_t ballot = __ballot_sync(0xffffffffu, claims);
+    int at = -1;
+    double w_at = 0.0;
+    if (ballot) {
+      const int o = __ffs(ballot) - 1;
+      const float* theirs = mine + (o - g.lane) * count;
+      const int their_slot = slot0 + (o - g.lane) * count;
+      double run = __shfl_sync(0xffffffffu, ahead, o);
+      bool found = false;
+      for (int base = 0; base < count; base += 32) {
+        double w = 0.0, sum32;
+        const int i = base + g.lane;
+        if (i < count && cut.keeps(theirs[i], their_slot + i)) {
+          const W x = wt.get(theirs[i], W());
+          w = x >= limit ? (double)x : 0.0;
+        }
+        const double before = run + warp_before(w, sum32, g.lane);
+        const uint32_t any = __ballot_sync(0xffffffffu, w > 0.0), hit = __ballot_sync(0xffffffffu, w > 0.0 && before + w > target);
+        if (any) {
+          const int j = hit ? __ffs(hit) - 1 : 31 - __clz(any);
+          at = their_slot + base + j;
+          const double b = __shfl_sync(0xffffffffu, before, j);
+          w_at = __shfl_sync(0xffffffffu, w, j);
+          if (hit) {
+            if (kOpen) open |= target - b <= slack * total || b + w_at - target <= slack * total;
+            found = true;
+            break;
+          }
+        }
+        run += sum32;
+      }
+      if (kOpen && !found) open = true;
+    }
+    if (kOpen) {
+      if (g.sum((open ? 1048576.0 : 0.0) + (claims ? 1.0 : 0.0)) != 1.0) return false;
+    }
+    if (claims) {
+      if (kOpen) w_at = wt.get(mine[at - slot0], 0.0);
+      give(at, (float)(w_at / total));
+    }
+    return true;
   }
-  if (id == owner) give(slot0 + at, (float)((double)weight(mine[at]) / total));
-  return true;
-}
+
+  // ---- rows whose kept entries are few: a warp has them all, in the order of their indices, and sums in 64 bits ----
+  // l, slot: n <= 64 entries.
+  __device__ void finish(const float* l, const int* slot, int base, int n, int k, float p_top, float p_min, float u) {
+    const int lane = g.lane;
+    auto at = [&](int i) { return i < n ? entry_of(l[i], slot ? slot[i] : base + i) : 0; };
+    auto weigh = [&](uint64_t e) { return e ? wt.get(of_key((uint32_t)(e >> 32)), 0.0) : 0.0; };
+    uint64_t cut = 1;
+    if ((k > 0 && k < n) || p_top < 1.f) {
+      uint64_t e[2] = {at(lane), at(32 + lane)};
+      sort_entries(e[0], e[1], n > 32, lane);
+      int stay = __popc(__ballot_sync(0xffffffffu, e[0])) + __popc(__ballot_sync(0xffffffffu, e[1]));
+      if (k > 0 && k < stay) stay = k;
+      if (p_top < 1.f) {
+        const double w0 = lane < stay ? weigh(e[0]) : 0.0, w1 = n > 32 && 32 + lane < stay ? weigh(e[1]) : 0.0;
+        double t0, t1 = 0.0;
+        const double b0 = warp_before(w0, t0, lane), b1 = n > 32 ? t0 + warp_before(w1, t1, lane) : 0.0;
+        const double target = (double)p_top * (t0 + t1);
+        const int in = __popc(__ballot_sync(0xffffffffu, lane < stay && b0 < target)) +
+                       __popc(__ballot_sync(0xffffffffu, 32 + lane < stay && b1 < target));
+        stay = in > 1 ? in : 1;
+      }
+      const uint64_t c0 = __shfl_sync(0xffffffffu, e[0], (stay - 1) & 31), c1 = __shfl_sync(0xffffffffu, e[1], (stay - 1) & 31);
+      cut = stay > 32 ? c1 : c0;
+    }
+    const double limit = p_min > 0.f ? (double)fminf(p_min, 1.f) : 0.0;
+    double run = 0.0, total, w[2], before[2];
+    uint64_t e[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      e[h] = h == 0 || n > 32 ? at(32 * h + lane) : 0;
+      w[h] = e[h] >= cut ? weigh(e[h]) : 0.0;
+      if (w[h] < limit) w[h] = 0.0;
+      before[h] = 0.0;
+      if (h == 0 || n > 32) {
+        before[h] = run + warp_before(w[h], total, lane);
+        run += total;
+      }
+    }
+    const double target = (double)u * run;
+    uint32_t hit0 = __ballot_sync(0xffffffffu, w[0] > 0.0 && before[0] + w[0] > target);
+    uint32_t hit1 = __ballot_sync(0xffffffffu, w[1] > 0.0 && before[1] + w[1] > target);
+    if (!hit0 && !hit1) {  // rounding: the last with a weight
+      hit1 = __ballot_sync(0xffffffffu, w[1] > 0.0);
+      if (hit1) hit1 = 1u << (31 - __clz(hit1));
+      else hit0 = 1u << (31 - __clz(__ballot_sync(0xffffffffu, w[0] > 0.0)));
+    }
+    const int half = hit0 ? 0 : 1, j = __ffs(hit0 ? hit0 : hit1) - 1;
+    if (lane == j) give((int)~(uint32_t)e[half], (float)(w[half] / run));
+  }
+  // The entries that top-k can keep, gathered: those not below a logit that k entries reach.  Maxima of the lanes' runs give one: the
+  // k-th of them for small k, the least of all else, from which a bisection over the gathered entries goes on.  Number of entries, 0 if
+  // that found none or too many.
+  __device__ int gather_top(int k, float lane_max) {
+    const int lane = g.lane;
+    float s = lane_max;
+#pragma unroll
+    for (int kk = 2; kk <= 32; kk <<= 1)
+#pragma unroll
+      for (int j = kk >> 1; j > 0; j >>= 1) {
+        const float o = __shfl_xor_sync(0xffffffffu, s, j);
+        s = ((lane & j) == 0) == ((lane & kk) == 0) ? fmaxf(s, o) : fminf(s, o);
+      }
+    const float floor_l = __shfl_sync(0xffffffffu, s, k <= 24 ? k - 1 : 31);
+    if (floor_l == -INFINITY) return 0;
+    uint64_t hits = 0;
+    each([&](int i, float l) { hits |= (uint64_t)(l >= floor_l) << i; });
+    const int own = __popcll(hits);
+    int in = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, in, o);
+      if (lane >= o) in += up;
+    }
+    int n = __shfl_sync(0xffffffffu, in, 31);
+    if (n > kGather || n < k) return 0;
+    for (int pos = in - own; hits; hits &= hits - 1, ++pos) {
+      const int i = __ffsll((long long)hits) - 1;
+      sh.list_l[pos] = mine[i];
+      sh.list_slot[pos] = slot0 + i;
+    }
+    __syncwarp();
+    if (n <= kSort) return n;
+    float l[kGather / 32];
+    int slot[kGather / 32];
+#pragma unroll
+    for (int i = 0; i < kGather / 32; ++i) {
+      l[i] = 32 * i + lane < n ? sh.list_l[32 * i + lane] : -INFINITY;
+      slot[i] = 32 * i + lane < n ? sh.list_slot[32 * i + lane] : 0;
+    }
+    uint32_t lo = key_of(floor_l), hi = key_of(wt.max) + 1;  // more than 64 reach lo, fewer than k reach hi
+    float at = 0.f;
+    bool found = false;
+    while (hi - lo > 1 && !found) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      at = of_key(mid);
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < kGather / 32; ++i) c += l[i] >= at;
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (c > kSort) lo = mid;
+      else if (c < k) hi = mid;
+      else found = true;
+    }
+    if (!found) return 0;  // equal entries
+    __syncwarp();
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < kGather / 32; ++i) {
+      const bool stays = l[i] >= at;
+      const uint32_t b = __ballot_sync(0xffffffffu, stays);
+      if (stays) {
+        const int pos = n + __popc(b & ((1u << lane) - 1));
+        sh.list_l[pos] = l[i];
+        sh.list_slot[pos] = slot[i];
+      }
+      n += __popc(b);
+    }
+    __syncwarp();
+    return n;
+  }
+};
 
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads == 32 ? 32 * kWarpRows : kThreads)
 sample_kernel(const SampleParams p) {
   extern __shared__ float4 smem[];
-  __shared__ double slots[2 * Group<kThreads>::kSlots];
+  __shared__ Shared<kThreads> shared[kThreads == 32 ? kWarpRows : 1];
+  const int part = kThreads == 32 ? threadIdx.x >> 5 : 0;
   const int cap = kThreads * 4 * p.pieces;
-  float* v = reinterpret_cast<float*>(smem) + (kThreads == 32 ? (threadIdx.x >> 5) * cap : 0);
-  Group<kThreads> g(slots, p.cluster);
-  const int row = kThreads == 32 ? blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x / p.cluster;
+  float* v = reinterpret_cast<float*>(smem) + part * cap;
+  Shared<kThreads>& sh = shared[part];
+  Group<kThreads> g(sh.slots, p.cluster);
+  const int row = kThreads == 32 ? blockIdx.x * kWarpRows + part : blockIdx.x / p.cluster;
   if (row >= p.rows) return;
-  const float temp = p.temperature ? p.temperature[row] : 1.f;
-  const int local = (kThreads == 32 ? g.lane : (int)threadIdx.x) * 4 * p.pieces;
+  float temp = p.temperature ? p.temperature[row] : 1.f;
+  const float p_top = p.top_p ? p.top_p[row] : 1.f, p_min = p.min_p ? p.min_p[row] : 0.f;
+  const int k = p_top <= 0.f ? 1 : p.top_k ? p.top_k[row] : 0;
+  float u = p.u[row];
+  u = u >= 0.f ? fminf(u, 1.f - 0x1p-24f) : 0.f;
   int n = 0;
-  int first = load_row<T, kThreads>(p, g, row, v, cap, n);
+  const int first = load_row<T, kThreads>(p, g, row, v, cap, n);
   g.barrier();
-  if (!draw_row<false, kThreads>(p, g, row, v + local, g.crank * cap + local, first, temp)) {
+  const int local = (kThreads == 32 ? g.lane : (int)threadIdx.x) * 4 * p.pieces;
+  Row<kThreads> r{g, sh, p, v + local, g.crank * cap + local, 4 * p.pieces, row, first, Weight(0.f, 1.f)};
+  float own_max = -INFINITY;
+  r.each([&](int, float l) { own_max = fmaxf(own_max, l); });
+  float m = g.max(own_max);
+  bool done = false;
+  if (m == -INFINITY) {
+    if (g.thread() == 0) r.give(-1, 0.f);
+    done = true;
+  } else if (!(temp > 0.f)) {  // the first of the largest
+    const int at = r.nth_equal(m, 0.0);
+    if (g.thread() == 0) r.give(at, 1.f);
+    done = true;
+  } else if (m == INFINITY) {  // infinities are equal, and nothing is beside them
+    for (int i = 0; i < r.count; ++i) r.mine[i] = r.mine[i] == INFINITY ? 0.f : -INFINITY;
+    own_max = own_max == INFINITY ? 0.f : -INFINITY;
+    m = 0.f;
+    temp = 1.f;
     g.barrier();
-    first = load_row<T, kThreads>(p, g, row, v, cap, n);
-    g.barrier();
-    draw_row<true, kThreads>(p, g, row, v + local, g.crank * cap + local, first, temp);
   }
-  if (kThreads == kWide && p.cluster > 1) g.barrier();  // no CTA leaves while another may write to its slots
+  if (!done) {
+    r.wt = Weight(m, temp);
+    const bool fp32 = r.wt.fp32_usable();
+    const float tp = p_top <= 0.f ? 1.f : p_top;
+    if constexpr (kThreads == 32) {
+      if (n <= kSort) {
+        r.finish(v + first, nullptr, first, n, k, tp, p_min, u);
+        done = true;
+      } else if (k > 0 && k <= kSort) {
+        const int few = r.gather_top(k, own_max);
+        if (few) {
+          r.finish(sh.list_l, sh.list_slot, 0, few, k, tp, p_min, u);
+          done = true;
+        }
+      }
+    }
+    if (!done) {
+      const double slack = (double)p.slack;
+      Cut cut;
+      if (k > 0 && k < n) {
+        double all = 0.0;
+        float least = INFINITY;
+        r.each([&](int, float l) { if (l > -INFINITY) { all += 1.0; least = fminf(least, l); } });
+        all = g.sum(all);
+        if ((double)k < all) {
+          least = -g.max(-least);
+          r.template select<float, false>(cut, (double)k, all, m, least, 0.0, cut);
+        }
+      }
+      if (tp < 1.f) {
+        // weights below e^-24 of the largest are in the lowest bin
+        const float lo = m - 24.f * temp;
+        bool ok = false;
+        const Cut in = cut;
+        if (fp32) {
+          const double all = g.sum(r.template sum<float>([&](int i, float l) { return in.keeps(l, r.slot0 + i) ? r.wt.get(l, 0.f) : 0.f; }));
+          ok = r.template select<float, true>(in, (double)tp * all, all, m, lo, slack, cut);
+        }
+        if (!ok) {
+          const double all = g.sum(r.template sum<double>([&](int i, float l) { return in.keeps(l, r.slot0 + i) ? r.wt.get(l, 0.0) : 0.0; }));
+          r.template select<double, true>(in, (double)tp * all, all, m, lo, 0.0, cut);
+        }
+      }
+      if (!fp32 || !r.template draw<float>(cut, p_min, u, slack)) r.template draw<double>(cut, p_min, u, 0.0);
+    }
+  }
+  if (kThreads == kWide && p.cluster > 1) g.barrier();  // no CTA leaves while another may still read its shared memory
 }
 
 template <typename T, int kThreads>
 cudaError_t launch_group(const SampleParams& p, cudaStream_t s) {
   const int groups = kThreads == 32 ? kWarpRows : 1;
-  cudaError_t e = raise_smem_limit<sample_kernel<T, kThreads>>(kThreads == 32 ? 64 * 1024 : kThreads == kWide ? kWide * kMaxPieces * 16 : 64 * 1024);
+  cudaError_t e = raise_smem_limit<sample_kernel<T, kThreads>>(kThreads == kWide ? kWide * kMaxPieces * 16 : 64 * 1024);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(kThreads == 32 ? ceil_div(p.rows, kWarpRows) : p.rows * p.cluster);
@@ -420,14 +802,14 @@ cudaError_t launch_sample(SampleParams p, cudaStream_t s) {
   const int n = p.ids ? p.ld_ids : p.width + Pieces<T>::n - 1;
   auto pieces = [&](int threads) { return ceil_div(ceil_div(n, 4), threads) | 1; };
   p.cluster = 1;
-  int threads = n <= 512 ? 32 : n <= 8192 ? 256 : kWide;
+  const int threads = pieces(32) <= 15 ? 32 : n <= 8192 ? 256 : kWide;
   if (threads == kWide)
-    while (pieces(kWide * p.cluster) > kMaxPieces) p.cluster *= 2;
+    while (p.cluster < kMaxCluster && pieces(kWide * p.cluster) > 5) p.cluster *= 2;
   p.pieces = pieces(threads * p.cluster);
   // Bound of a sum's error over the sum of all weights, in steps of 2^-24.  A weight: its exponent carries the rounding of l - m, at
-  // most |z| steps with z = (l - m) / T, and the sum of w |z| is at most ln(n) times the sum of w; exp2f and the factor 6.
-  // Sums: a thread's four chains.  Twice that, since a threshold and a sum are compared.
-  p.slack = 2.f * (13.f + 6.f + p.pieces + 2.f) * 0x1p-24f;
+  // most |z| steps with z = (l - m) / T, and the sum of w |z| is at most ln(n) times the sum of w; exp2f and the factor 5.
+  // Sums: a thread's chains 8, the total 1.  Twice that, since two sums are compared.
+  p.slack = 2.f * (13.f + 5.f + 9.f) * 0x1p-24f;
   if (threads == 32) return launch_group<T, 32>(p, s);
   if (threads == 256) return launch_group<T, 256>(p, s);
   return launch_group<T, kWide>(p, s);
