@@ -134,15 +134,18 @@ struct Weight {
     c_lo = (float)(fmin(e, 1e37) - (double)c);
   }
   __device__ bool fp32_usable() const { return c < 1e37f; }
-  // 2^((l - m) log2(e) / T) with the exponent in two pieces; halves, since l - m can overflow
+  // 2^((l - m) log2(e) / T) with the exponent in two pieces; halves, since l - m can overflow.  No branch: passes over a row live on
+  // several entries being in work at once.
   __device__ __forceinline__ float get(float l, float) const {
-    const float x = 0.5f * l - half_max;
-    const float z = fmaxf(x * c, -200.f);
+    const float x = fmaf(l, 0.5f, -half_max);
+    const float z = x * c;
     const float lo = fmaf(x, c_lo, fmaf(x, c, -z));
-    const float w = exp2f(z);
-    return z <= -140.f ? 0.0f : fmaf(w, lo * 0.69314718f, w);
+    float w;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(z));
+    w = fmaf(w, lo * 0.69314718f, w);
+    return z > -126.f ? w : 0.f;
   }
-  __device__ __forceinline__ double get(float l, double) const { return exp(((double)l - (double)max) * inv_t); }
+  __device__ __forceinline__ double get(float l, double) const { return l > -INFINITY ? exp(((double)l - (double)max) * inv_t) : 0.0; }
 };
 
 template <typename T> struct Pieces;  // 16 bytes of logits as fp32
@@ -209,11 +212,10 @@ __device__ int load_row(const SampleParams& p, const Group<kThreads>& g, int row
   return first;
 }
 
-// What stays of a row: entries above `l`, and those equal to it up to `slot`.
+// The end of what stays of a row: entries above `l`, and those equal to it up to `slot`.
 struct Cut {
-  float l = -INFINITY;
-  int slot = -1;
-  __device__ __forceinline__ bool keeps(float x, int s) const { return x > l || (x == l && s <= slot); }
+  float l;
+  int slot;
 };
 
 constexpr int kBins = 256;
@@ -222,9 +224,12 @@ constexpr int kGather = 256;  // entries that a warp gathers from its row
 
 template <int kThreads> struct Shared {
   double slots[2 * Group<kThreads>::kSlots];
-  uint32_t bins[kBins], total[kBins];
-  float list_l[kThreads == 32 ? kGather : kSort];
-  int list_slot[kThreads == 32 ? kGather : kSort];
+  union {
+    struct { uint32_t bins[kBins], total[kThreads == kWide ? kBins : 1]; };
+    struct { float gather_l[kThreads == 32 ? kGather : 1]; int gather_slot[kThreads == 32 ? kGather : 1]; };
+  };
+  float list_l[kSort];
+  int list_slot[kSort];
   int count;
   int solved;
   uint64_t cut;
@@ -292,18 +297,31 @@ template <int kThreads> struct Row {
       f(i, x.x); f(i + 1, x.y); f(i + 2, x.z); f(i + 3, x.w);
     }
   }
-  // Sum of f over this thread's entries: pieces of four, groups of four pieces in W, the groups in 64 bits.
+  // Sum of f over this thread's entries: 16 at a time in W, those sums in 64 bits.
   template <typename W, typename F> __device__ __forceinline__ double sum(F f) const {
     double total = 0.0;
-    W run = 0;
+    int i = 0;
+    auto quad = [&](int at) -> W {
+      const float4 x = *reinterpret_cast<const float4*>(mine + at);
+      const W a = f(at, x.x), b = f(at + 1, x.y), c = f(at + 2, x.z), d = f(at + 3, x.w);
+      return (a + b) + (c + d);
+    };
+    for (; i + 16 <= count; i += 16) {
+      const W a = quad(i), b = quad(i + 4), c = quad(i + 8), d = quad(i + 12);
+      total += (double)((a + b) + (c + d));
+    }
+    for (; i < count; i += 4) total += (double)quad(i);
+    return total;
+  }
+  __device__ __forceinline__ void keep(const Cut cut) const {
+    const int last = cut.slot - slot0;
 #pragma unroll 4
     for (int i = 0; i < count; i += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(mine + i);
-      const W a = f(i, x.x), b = f(i + 1, x.y), c = f(i + 2, x.z), d = f(i + 3, x.w);
-      run += (a + b) + (c + d);
-      if ((i & 12) == 12) { total += (double)run; run = 0; }
+      float4 x = *reinterpret_cast<const float4*>(mine + i);
+      auto stays = [&](float l, int j) { return ((l > cut.l) | ((l == cut.l) & (j <= last))) ? l : -INFINITY; };
+      x.x = stays(x.x, i); x.y = stays(x.y, i + 1); x.z = stays(x.z, i + 2); x.w = stays(x.w, i + 3);
+      *reinterpret_cast<float4*>(mine + i) = x;
     }
-    return total + (double)run;
   }
   __device__ __forceinline__ void give(int slot, float prob) const {
     p.choice[row] = slot < 0 ? -1 : slot - first;
@@ -326,34 +344,43 @@ template <int kThreads> struct Row {
     return (int)g.max((float)at);
   }
 
-  // The end of the front part of what `in` keeps: the first entry ahead of which the measure (kMass: weights, else 1 each) sums to the
-  // target or more is out, with all behind it; the first of all stays.  `all`: the measure of what `in` keeps.  Bins of a range of
-  // logits, the bin that the target falls in, the exact measure above it and its entries, until those are few enough to be sorted.
+  // The end of the front part: the first entry ahead of which the measure (kMass: weights, else 1 each) sums to the target or more is out,
+  // with all behind it; the first of all stays.  kMass: `target` is a share of the sum of all weights.  Bins of a range of logits
+  // [lo, hi], the bin that the target falls in, the exact measure above it and its entries, until those are few enough to be sorted.
   // False: a comparison was open.
-  template <typename W, bool kMass> __device__ bool select(const Cut in, double target, double all, float hi, float lo, double slack, Cut& out) {
+  template <typename W, bool kMass> __device__ bool select(double target, float hi, float lo, double slack, Cut& out) {
     constexpr bool kOpen = kMass && sizeof(W) == 4;
     auto measure = [&](float l) -> W { if constexpr (kMass) return wt.get(l, W()); else return W(1); };
     double above = 0.0;  // of entries above the range
-    double inside = all;
+    double all = 0.0;    // kMass
+    const int tid = kThreads == 32 ? g.lane : (int)threadIdx.x;
+    // weights in bins: whole numbers, whose sum of n weights of at most 1 stays below 2^31 (order does not matter to them)
+    double quantum = kMass ? 2147483000.0 / (double)(g.threads() * count) : 1.0;
     for (int round = 0; round < 8; ++round) {
-      const float scale = fminf((kBins - 0.01f) / fminf(hi - lo, 3.4e38f), 1e37f);
       // the lowest bin of the first round takes what lies below the range
-      auto bin = [&](float l) { return (int)fminf((hi - l) * scale, kBins - 1.f); };
-      auto ranged = [&](float l) { return l <= hi && (l >= lo || round == 0); };
-      const double quantum = 1073741824.0 / inside;
+      const float scale = fminf((kBins - 0.5f) / fminf(hi - lo, 3.4e38f), 1e37f);
+      const float least_in = round == 0 ? -3.402823466e38f : lo;
+      auto bin = [&](float l) { return __float_as_int(fminf((hi - l) * scale, kBins - 1.f) + 8388608.f) & (kBins - 1); };
       const float fq = (float)quantum;
       g.barrier();  // the others are done with what is cleared
-      const int tid = kThreads == 32 ? g.lane : (int)threadIdx.x;
       for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
       if (tid == 0) sh.count = 0;
       if (kThreads == 32) __syncwarp(); else __syncthreads();
-      each([&](int i, float l) {
-        if (in.keeps(l, slot0 + i) && ranged(l)) {
-          const uint32_t q = kMass ? (uint32_t)((float)wt.get(l, 0.f) * fq) : 1u;
+      if (kMass && round == 0) {
+        all = g.sum(sum<W>([&](int, float l) -> W {
+          const float w = wt.get(l, 0.f);
+          const uint32_t q = (uint32_t)fmaf(w, fq, 0.5f);
           if (q) atomicAdd(&sh.bins[bin(l)], q);
-        }
-      });
-      g.barrier();
+          if constexpr (sizeof(W) == 4) return w; else return wt.get(l, W());
+        }));
+        target *= all;
+      } else {
+        each([&](int, float l) {
+          const uint32_t q = kMass ? (uint32_t)fmaf(wt.get(l, 0.f), fq, 0.5f) : 1u;
+          if ((l <= hi) & (l >= least_in) & (q > 0)) atomicAdd(&sh.bins[bin(l)], q);
+        });
+        g.barrier();
+      }
       const uint32_t* total = sh.bins;
       if (kThreads == kWide && g.cluster > 1) {
         for (int i = tid; i < kBins; i += kThreads) {
@@ -364,7 +391,7 @@ template <int kThreads> struct Row {
         total = sh.total;
         __syncthreads();
       }
-      // first bin at whose end the target is reached; behind the last full one where rounding leaves none
+      // first bin at whose end the target is reached, the last full one where rounding leaves none
       uint32_t part[kBins / 32], sum8 = 0;
 #pragma unroll
       for (int i = 0; i < kBins / 32; ++i) {
@@ -377,7 +404,7 @@ template <int kThreads> struct Row {
         const uint32_t up = __shfl_up_sync(0xffffffffu, in8, o);
         if (g.lane >= o) in8 += up;
       }
-      const double goal = (target - above) * (kMass ? quantum : 1.0);
+      const double goal = (target - above) * quantum;
       uint32_t run = in8 - sum8;
       int b = kBins, last = -1;
 #pragma unroll
@@ -389,106 +416,122 @@ template <int kThreads> struct Row {
       b = __reduce_min_sync(0xffffffffu, b);
       last = __reduce_max_sync(0xffffffffu, last);
       if (b == kBins) b = last;
-      if (b < 0) break;
-      float least = INFINITY, most = -INFINITY;
-      double more = 0.0;
-      {
-        W run4 = 0;
-        int n = 0;
-        each([&](int i, float l) {
-          if (in.keeps(l, slot0 + i) && ranged(l)) {
-            const int at = bin(l);
-            if (at < b) {
-              run4 += measure(l);
-              if (++n == 8) { more += (double)run4; run4 = 0; n = 0; }
-            } else if (at == b) {
-              least = fminf(least, l);
-              most = fmaxf(most, l);
-              const int pos = atomicAdd(&sh.count, 1);
-              if (pos < kSort) { sh.list_l[pos] = l; sh.list_slot[pos] = slot0 + i; }
-            }
+      auto next_bin = [&](int from, bool up) {  // the next one that is not empty, -1 if there is none
+        int at = up ? kBins : -1;
+#pragma unroll
+        for (int i = 0; i < kBins / 32; ++i) {
+          const int j = g.lane * (kBins / 32) + i;
+          if (part[i] && (up ? j > from : j < from)) at = up ? min(at, j) : j;
+        }
+        at = up ? __reduce_min_sync(0xffffffffu, at) : __reduce_max_sync(0xffffffffu, at);
+        return at == kBins ? -1 : at;
+      };
+      bool narrower = false;
+      for (int tries = 0; tries < 3 && b >= 0; ++tries) {
+        if (tries > 0) {
+          g.barrier();
+          if (tid == 0) sh.count = 0;
+          g.barrier();
+        }
+        float least = INFINITY, most = -INFINITY;
+        const double more = sum<W>([&](int i, float l) -> W {
+          const int at = bin(l);
+          const bool in = (l <= hi) & (l >= least_in);
+          if (in & (at == b)) {
+            least = fminf(least, l);
+            most = fmaxf(most, l);
+            const int pos = atomicAdd(&sh.count, 1);
+            if (pos < kSort) { sh.list_l[pos] = l; sh.list_slot[pos] = slot0 + i; }
           }
+          return in & (at < b) ? measure(l) : W(0);
         });
-        more += (double)run4;
-      }
-      above += g.sum(more);
-      int n = sh.count;
-      if (kThreads == kWide && g.cluster > 1) {
-        n = 0;
-        for (int c = 0; c < g.cluster; ++c) n += *cg::this_cluster().map_shared_rank(&sh.count, c);
-      }
-      if (n == 0) break;
-      if (n > kSort) {
-        hi = g.max(most);
-        lo = -g.max(-least);
-        if (hi == lo) {  // equal entries
-          const double w = (double)measure(hi), ties = (target - above) / w;
-          if (kOpen && (w < 1e-30 || fabs(ties - rint(ties)) <= slack * all / w + 1e-6 * fabs(ties) || ties <= 0.0 || ties > (double)n)) return false;
-          if (!(ties > 0.0) || ties > (double)n) break;
-          out.l = hi;
-          out.slot = nth_equal(hi, ceil(ties) - 1.0);
+        const double front = above + g.sum(more);
+        if (kOpen && fabs(front - target) <= slack * all) return false;
+        int n = sh.count;
+        if (kThreads == kWide && g.cluster > 1) {
+          n = 0;
+          for (int c = 0; c < g.cluster; ++c) n += *cg::this_cluster().map_shared_rank(&sh.count, c);
+        }
+        if (front >= target) {  // bins of weights are rounded sums: the target lies in an earlier one
+          b = next_bin(b, false);
+          continue;
+        }
+        if (n > kSort) {
+          hi = g.max(most);
+          lo = -g.max(-least);
+          above = front;
+          if (hi == lo) {  // equal entries
+            const double w = (double)measure(hi), ties = (target - above) / w;
+            if (kOpen && (w < 1e-30 || fabs(ties - rint(ties)) <= slack * all / w + 1e-6 * fabs(ties) || ties > (double)n)) return false;
+            if (ties > (double)n) break;
+            out.l = hi;
+            out.slot = nth_equal(hi, ceil(ties) - 1.0);
+            return true;
+          }
+          if (kMass) quantum = 2147483000.0 / fmax((double)n * (double)wt.get(hi, 0.f), 1e-28);
+          narrower = true;
+          break;
+        }
+        if (kThreads == 32 || g.warp == 0) {
+          uint64_t e[2] = {0, 0};
+          if (kThreads == kWide && g.cluster > 1) {
+            int base = 0;
+            for (int c = 0; c < g.cluster; ++c) {
+              const int nc = *cg::this_cluster().map_shared_rank(&sh.count, c);
+              const float* ll = cg::this_cluster().map_shared_rank(sh.list_l, c);
+              const int* ls = cg::this_cluster().map_shared_rank(sh.list_slot, c);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int i = g.lane + 32 * h - base;
+                if (i >= 0 && i < nc) e[h] = entry_of(ll[i], ls[i]);
+              }
+              base += nc;
+            }
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (g.lane + 32 * h < n) e[h] = entry_of(sh.list_l[g.lane + 32 * h], sh.list_slot[g.lane + 32 * h]);
+          }
+          sort_entries(e[0], e[1], n > 32, g.lane);
+          double w[2], t0, t1, before[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) w[h] = e[h] ? (double)measure(of_key((uint32_t)(e[h] >> 32))) : 0.0;
+          before[0] = front + warp_before(w[0], t0, g.lane);
+          before[1] = front + t0 + warp_before(w[1], t1, g.lane);
+          const double end = front + t0 + t1;
+          // entries of the list that stay: those ahead of which less than the target lies
+          const int stay = __popc(__ballot_sync(0xffffffffu, e[0] && before[0] < target)) +
+                           __popc(__ballot_sync(0xffffffffu, e[1] && before[1] < target));
+          bool open = false;
+          if (kOpen) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) open |= e[h] && fabs(before[h] - target) <= slack * all;
+            open = __any_sync(0xffffffffu, open) || fabs(end - target) <= slack * all;
+          }
+          const uint64_t c0 = __shfl_sync(0xffffffffu, e[0], (stay - 1) & 31), c1 = __shfl_sync(0xffffffffu, e[1], (stay - 1) & 31);
+          if (g.lane == 0) {
+            sh.solved = open ? 2 : end >= target ? 1 : 0;
+            sh.cut = stay > 32 ? c1 : c0;
+          }
+        }
+        if (kThreads == 32) __syncwarp(); else __syncthreads();
+        if (sh.solved == 2) return false;
+        if (sh.solved == 1) {
+          out = cut_of(sh.cut);
           return true;
         }
-        inside = kMass ? fmin(all, fmax((double)n * (double)measure(hi), 1e-28)) : (double)n;
-        continue;
+        b = next_bin(b, true);  // ... or in a later one
       }
-      if (kThreads == 32 || g.warp == 0) {
-        uint64_t e[2] = {0, 0};
-        if (kThreads == kWide && g.cluster > 1) {
-          int base = 0;
-          for (int c = 0; c < g.cluster; ++c) {
-            const int nc = *cg::this_cluster().map_shared_rank(&sh.count, c);
-            const float* ll = cg::this_cluster().map_shared_rank(sh.list_l, c);
-            const int* ls = cg::this_cluster().map_shared_rank(sh.list_slot, c);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int i = g.lane + 32 * h - base;
-              if (i >= 0 && i < nc) e[h] = entry_of(ll[i], ls[i]);
-            }
-            base += nc;
-          }
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (g.lane + 32 * h < n) e[h] = entry_of(sh.list_l[g.lane + 32 * h], sh.list_slot[g.lane + 32 * h]);
-        }
-        sort_entries(e[0], e[1], n > 32, g.lane);
-        double w[2], t0, t1;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) w[h] = e[h] ? (double)measure(of_key((uint32_t)(e[h] >> 32))) : 0.0;
-        double before[2];
-        before[0] = above + warp_before(w[0], t0, g.lane);
-        before[1] = above + t0 + warp_before(w[1], t1, g.lane);
-        const double end = above + t0 + t1;
-        // entries of the list that stay: those ahead of which less than the target lies
-        const uint32_t in0 = __ballot_sync(0xffffffffu, e[0] && before[0] < target), in1 = __ballot_sync(0xffffffffu, e[1] && before[1] < target);
-        const int stay = __popc(in0) + __popc(in1);
-        bool open = false;
-        if (kOpen) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) open |= e[h] && fabs(before[h] - target) <= slack * all;
-          open = __any_sync(0xffffffffu, open) || fabs(end - target) <= slack * all;
-        }
-        const uint64_t c0 = __shfl_sync(0xffffffffu, e[0], (stay - 1) & 31), c1 = __shfl_sync(0xffffffffu, e[1], (stay - 1) & 31);
-        if (g.lane == 0) {
-          sh.solved = open ? 2 : stay > 0 && (end >= target || !kMass) ? 1 : 0;
-          sh.cut = stay > 32 ? c1 : c0;
-        }
-      }
-      if (kThreads == 32) __syncwarp(); else __syncthreads();
-      if (sh.solved == 2) return false;
-      if (sh.solved == 0) break;
-      out = cut_of(sh.cut);
-      return true;
+      if (!narrower) break;
     }
     if (kOpen) return false;
-    // Bins did not find it (sums of theirs are rounded, ranges can hold a few values many decades apart): bisection.
+    // Bins did not find it (theirs are rounded sums, ranges can hold a few values many decades apart): bisection.
     uint32_t lo_key = key_of(-INFINITY), hi_key = key_of(wt.max);  // measure above lo_key: the target or more; above hi_key: less
     double over = 0.0;
     while (hi_key - lo_key > 1) {
       const uint32_t mid = lo_key + (hi_key - lo_key) / 2;
       const float cut = of_key(mid);
-      const double m = g.sum(sum<W>([&](int i, float l) { return l > cut && in.keeps(l, slot0 + i) ? measure(l) : W(0); }));
+      const double m = g.sum(sum<W>([&](int, float l) { return l > cut ? measure(l) : W(0); }));
       if (m >= target) lo_key = mid;
       else { hi_key = mid; over = m; }
     }
@@ -499,18 +542,22 @@ template <int kThreads> struct Row {
     return true;
   }
 
-  // The draw among what `cut` keeps and min-p.  False: a comparison was open.
-  template <typename W> __device__ bool draw(const Cut cut, float p_min, float u, double slack) {
+  // The draw among what is left and what min-p keeps of it.  False: a comparison was open.
+  template <typename W> __device__ bool draw(float p_min, float u, double slack) {
     constexpr bool kOpen = sizeof(W) == 4;
     const W limit = p_min > 0.f ? (W)fminf(p_min, 1.f) : W(0);
     bool open = false;
-    auto weigh = [&](int i, float l) -> W {
-      if (!cut.keeps(l, slot0 + i)) return W(0);
-      const W w = wt.get(l, W());
-      if (kOpen && limit > W(0) && fabsf((float)w - (float)limit) <= 4.f * (float)slack * (float)limit && l != wt.max) open = true;
-      return w >= limit ? w : W(0);
-    };
-    const double own = sum<W>(weigh);
+    const float near = 4.f * (float)slack * (float)limit;
+    double own;
+    if (limit > W(0)) {
+      own = sum<W>([&](int, float l) -> W {
+        const W w = wt.get(l, W());
+        if (kOpen) open |= (fabsf((float)w - (float)limit) <= near) & (l != wt.max);
+        return w >= limit ? w : W(0);
+      });
+    } else {
+      own = sum<W>([&](int, float l) -> W { return wt.get(l, W()); });
+    }
     double total;
     const double ahead = g.before(own, total), target = (double)u * total;
     const bool here = ahead <= target && target < ahead + own;
@@ -535,7 +582,7 @@ template <int kThreads> struct Row {
       for (int base = 0; base < count; base += 32) {
         double w = 0.0, sum32;
         const int i = base + g.lane;
-        if (i < count && cut.keeps(theirs[i], their_slot + i)) {
+        if (i < count) {
           const W x = wt.get(theirs[i], W());
           w = x >= limit ? (double)x : 0.0;
         }
@@ -616,7 +663,8 @@ template <int kThreads> struct Row {
     if (lane == j) give((int)~(uint32_t)e[half], (float)(w[half] / run));
   }
   // The entries that top-k can keep, gathered: those not below a logit that k entries reach.  Maxima of the lanes' runs give one: the
-  // k-th of them for small k, the least of all else, from which a bisection over the gathered entries goes on.  Number of entries, 0 if
+  // k-th of them for small k, one of the least else, which more than k entries reach nearly always; from there a bisection over the
+  // gathered entries goes on.  Number of entries, 0 if
   // that found none or too many.
   __device__ int gather_top(int k, float lane_max) {
     const int lane = g.lane;
@@ -628,7 +676,7 @@ template <int kThreads> struct Row {
         const float o = __shfl_xor_sync(0xffffffffu, s, j);
         s = ((lane & j) == 0) == ((lane & kk) == 0) ? fmaxf(s, o) : fminf(s, o);
       }
-    const float floor_l = __shfl_sync(0xffffffffu, s, k <= 24 ? k - 1 : 31);
+    const float floor_l = __shfl_sync(0xffffffffu, s, k <= 24 ? k - 1 : k <= 40 ? 28 : 30);  // (the last run may be empty)
     if (floor_l == -INFINITY) return 0;
     uint64_t hits = 0;
     each([&](int i, float l) { hits |= (uint64_t)(l >= floor_l) << i; });
@@ -643,8 +691,8 @@ template <int kThreads> struct Row {
     if (n > kGather || n < k) return 0;
     for (int pos = in - own; hits; hits &= hits - 1, ++pos) {
       const int i = __ffsll((long long)hits) - 1;
-      sh.list_l[pos] = mine[i];
-      sh.list_slot[pos] = slot0 + i;
+      sh.gather_l[pos] = mine[i];
+      sh.gather_slot[pos] = slot0 + i;
     }
     __syncwarp();
     if (n <= kSort) return n;
@@ -652,8 +700,8 @@ template <int kThreads> struct Row {
     int slot[kGather / 32];
 #pragma unroll
     for (int i = 0; i < kGather / 32; ++i) {
-      l[i] = 32 * i + lane < n ? sh.list_l[32 * i + lane] : -INFINITY;
-      slot[i] = 32 * i + lane < n ? sh.list_slot[32 * i + lane] : 0;
+      l[i] = 32 * i + lane < n ? sh.gather_l[32 * i + lane] : -INFINITY;
+      slot[i] = 32 * i + lane < n ? sh.gather_slot[32 * i + lane] : 0;
     }
     uint32_t lo = key_of(floor_l), hi = key_of(wt.max) + 1;  // more than 64 reach lo, fewer than k reach hi
     float at = 0.f;
@@ -678,8 +726,8 @@ template <int kThreads> struct Row {
       const uint32_t b = __ballot_sync(0xffffffffu, stays);
       if (stays) {
         const int pos = n + __popc(b & ((1u << lane) - 1));
-        sh.list_l[pos] = l[i];
-        sh.list_slot[pos] = slot[i];
+        sh.gather_l[pos] = l[i];
+        sh.gather_slot[pos] = slot[i];
       }
       n += __popc(b);
     }
@@ -739,7 +787,7 @@ sample_kernel(const SampleParams p) {
       } else if (k > 0 && k <= kSort) {
         const int few = r.gather_top(k, own_max);
         if (few) {
-          r.finish(sh.list_l, sh.list_slot, 0, few, k, tp, p_min, u);
+          r.finish(sh.gather_l, sh.gather_slot, 0, few, k, tp, p_min, u);
           done = true;
         }
       }
@@ -748,30 +796,24 @@ sample_kernel(const SampleParams p) {
       const double slack = (double)p.slack;
       Cut cut;
       if (k > 0 && k < n) {
-        double all = 0.0;
         float least = INFINITY;
-        r.each([&](int, float l) { if (l > -INFINITY) { all += 1.0; least = fminf(least, l); } });
-        all = g.sum(all);
-        if ((double)k < all) {
+        int own = 0;
+        r.each([&](int, float l) {
+          own += l > -INFINITY;
+          least = fminf(least, l > -INFINITY ? l : INFINITY);
+        });
+        if ((double)k < g.sum((double)own)) {
           least = -g.max(-least);
-          r.template select<float, false>(cut, (double)k, all, m, least, 0.0, cut);
+          r.template select<float, false>((double)k, m, least, 0.0, cut);
+          r.keep(cut);
         }
       }
       if (tp < 1.f) {
-        // weights below e^-24 of the largest are in the lowest bin
-        const float lo = m - 24.f * temp;
-        bool ok = false;
-        const Cut in = cut;
-        if (fp32) {
-          const double all = g.sum(r.template sum<float>([&](int i, float l) { return in.keeps(l, r.slot0 + i) ? r.wt.get(l, 0.f) : 0.f; }));
-          ok = r.template select<float, true>(in, (double)tp * all, all, m, lo, slack, cut);
-        }
-        if (!ok) {
-          const double all = g.sum(r.template sum<double>([&](int i, float l) { return in.keeps(l, r.slot0 + i) ? r.wt.get(l, 0.0) : 0.0; }));
-          r.template select<double, true>(in, (double)tp * all, all, m, lo, 0.0, cut);
-        }
+        const float lo = m - 24.f * temp;  // what is below, weights of less than e^-24, is in the lowest bin
+        if (!fp32 || !r.template select<float, true>((double)tp, m, lo, slack, cut)) r.template select<double, true>((double)tp, m, lo, 0.0, cut);
+        r.keep(cut);
       }
-      if (!fp32 || !r.template draw<float>(cut, p_min, u, slack)) r.template draw<double>(cut, p_min, u, 0.0);
+      if (!fp32 || !r.template draw<float>(p_min, u, slack)) r.template draw<double>(p_min, u, 0.0);
     }
   }
   if (kThreads == kWide && p.cluster > 1) g.barrier();  // no CTA leaves while another may still read its shared memory
@@ -808,7 +850,7 @@ cudaError_t launch_sample(SampleParams p, cudaStream_t s) {
   p.pieces = pieces(threads * p.cluster);
   // Bound of a sum's error over the sum of all weights, in steps of 2^-24.  A weight: its exponent carries the rounding of l - m, at
   // most |z| steps with z = (l - m) / T, and the sum of w |z| is at most ln(n) times the sum of w; exp2f and the factor 5.
-  // Sums: a thread's chains 8, the total 1.  Twice that, since two sums are compared.
+  // Sums: a thread's chains 4 (8 where bins are summed up), the total 1.  Twice that, since two sums are compared.
   p.slack = 2.f * (13.f + 5.f + 9.f) * 0x1p-24f;
   if (threads == 32) return launch_group<T, 32>(p, s);
   if (threads == 256) return launch_group<T, 256>(p, s);
