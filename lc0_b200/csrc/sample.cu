@@ -22,9 +22,10 @@ namespace b200 {
 namespace {
 
 constexpr int kMaxCluster = 8;
-constexpr int kWide = 512;              // threads of the largest CTA
-constexpr int kMaxPieces = 17;          // 16-byte pieces per thread there: 136 KB
+constexpr int kWide = 256;              // threads of a CTA that has a row, or a part of one
+constexpr int kMaxPieces = 33;          // 16-byte pieces per thread there: 132 KB
 constexpr int kWarpRows = 4;            // rows of a CTA whose groups are warps
+constexpr int kFewRows = 444;           // three CTAs per SM
 static_assert(kMaxCluster * kWide * kMaxPieces * 4 >= B200_SAMPLE_MAX_WIDTH + 8, "the widest row fits a cluster");
 
 struct SampleParams {
@@ -50,9 +51,10 @@ template <int kThreads> struct Group {
   static constexpr int kWarps = kThreads / 32;
   static constexpr int kSlots = kThreads == kWide ? kMaxCluster * kWarps : kWarps;
   double* slots;  // [2][kSlots], kThreads > 32
+  float* wide;    // [2][kSlots][8]
   int cluster, crank, turn;
   int lane, warp;
-  __device__ Group(double* s, int cl) : slots(s), cluster(kThreads == kWide ? cl : 1), crank(0), turn(0) {
+  __device__ Group(double* s, float* s8, int cl) : slots(s), wide(s8), cluster(kThreads == kWide ? cl : 1), crank(0), turn(0) {
     lane = threadIdx.x & 31;
     warp = kThreads == 32 ? 0 : threadIdx.x >> 5;
     if (kThreads == kWide && cluster > 1) crank = (int)cg::this_cluster().block_rank();
@@ -96,6 +98,39 @@ template <int kThreads> struct Group {
     for (int i = lane; i < cluster * kWarps; i += 32) t = fmaxf(t, (float)s[i]);
     return warp_max(t);
   }
+  // Sums of eight values at once, in a fixed order, for places to look in.
+  __device__ __forceinline__ void sum8(float (&a)[8]) {
+    // halving exchange: a lane is left with value ((lane >> 4) & 1) * 4 + ((lane >> 3) & 1) * 2 + ((lane >> 2) & 1) of its warp
+    auto halve = [&](bool upper, int o, float& low, float high) {
+      const float send = upper ? low : high, keep = upper ? high : low;
+      low = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) halve((lane & 16) != 0, 16, a[i], a[i + 4]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) halve((lane & 8) != 0, 8, a[i], a[i + 2]);
+    halve((lane & 4) != 0, 4, a[0], a[1]);
+    float v = a[0];
+    v += __shfl_xor_sync(0xffffffffu, v, 2);
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    if (kThreads > 32) {
+      float* mine = wide + (turn & 1) * kSlots * 8;
+      ++turn;
+      const int at = (crank * kWarps + warp) * 8 + (lane >> 2);
+      if (kThreads == kWide && cluster > 1) {
+        for (int c = lane & 3; c < cluster; c += 4) *cg::this_cluster().map_shared_rank(mine + at, c) = v;
+      } else if ((lane & 3) == 0) {
+        mine[at] = v;
+      }
+      barrier();
+      v = 0.f;
+      for (int w = lane & 3; w < cluster * kWarps; w += 4) v += mine[w * 8 + (lane >> 2)];
+      v += __shfl_xor_sync(0xffffffffu, v, 2);
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = __shfl_sync(0xffffffffu, v, j * 4);
+  }
   // Sum over the threads before this one; `total` over all.
   __device__ __forceinline__ double before(double v, double& total) {
     double in = v;
@@ -112,21 +147,62 @@ template <int kThreads> struct Group {
       return ex;
     }
     const double* s = gather(warp_total);
-    double ahead = 0.0, all = 0.0;  // every thread adds the warps in the same order
-    for (int i = 0; i < cluster * kWarps; ++i) {
-      if (i == crank * kWarps + warp) ahead = all;
-      all += s[i];
+    // every warp scans the warps' sums in the same order, a few per lane
+    constexpr int kEach = (kSlots + 31) / 32;
+    const int mine = crank * kWarps + warp;
+    double part[kEach], sum = 0.0, ahead = 0.0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      part[i] = sum;
+      const int at = lane * kEach + i;
+      if (at < cluster * kWarps) sum += s[at];
     }
-    total = all;
-    return ahead + ex;
+    double run = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double up = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += up;
+    }
+    total = __shfl_sync(0xffffffffu, run, 31);
+    run = __shfl_up_sync(0xffffffffu, run, 1);
+    if (lane == 0) run = 0.0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (i == mine % kEach) ahead = run + part[i];
+    return __shfl_sync(0xffffffffu, ahead, mine / kEach) + ex;
   }
 };
 
+// e^x in 64 bits for kN values x <= 0, side by side and without a branch (one after the other each step waits for the last): x = k ln 2 + r
+// with ln 2 in two pieces (Cody and Waite), the Taylor series of e^r up to r^13 (|r| <= 0.35: the next term is 1e-17), times 2^k in
+// two halves, whose product may be subnormal.
+template <int kN> __device__ __forceinline__ void exp_below(double (&x)[kN]) {
+  double r[kN], s[kN];
+  int n[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    const double y = fmax(x[i], -760.0), k = rint(y * 1.4426950408889634);
+    r[i] = fma(k, -0x1.abc9e3b39803fp-56, fma(k, -0x1.62e42fefa39efp-1, y));
+    n[i] = (int)k;
+    s[i] = 1.0 / 6227020800.0;
+  }
+  constexpr double kInverse[13] = {1.0 / 479001600.0, 1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0,
+                                   1.0 / 120.0, 1.0 / 24.0, 1.0 / 6.0, 0.5, 1.0, 1.0};
+#pragma unroll
+  for (int c = 0; c < 13; ++c)
+#pragma unroll
+    for (int i = 0; i < kN; ++i) s[i] = fma(s[i], r[i], kInverse[c]);
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    const int half = n[i] >> 1;
+    x[i] = s[i] * __hiloint2double((half + 1023) << 20, 0) * __hiloint2double((n[i] - half + 1023) << 20, 0);
+  }
+}
 // Weights in fp32 or in 64 bits, of a row whose largest logit is finite.
 struct Weight {
-  float half_max, c, c_lo, max;
+  float half_max, c, c_lo, max, temp;
   double inv_t;
-  __device__ Weight(float m, float t) : max(m) {
+  __device__ Weight(float m, float t) : max(m), temp(t) {
     inv_t = 1.0 / (double)t;
     const double e = 2.8853900817779268 * inv_t;  // 2 log2(e) / T
     half_max = 0.5f * m;
@@ -134,18 +210,40 @@ struct Weight {
     c_lo = (float)(fmin(e, 1e37) - (double)c);
   }
   __device__ bool fp32_usable() const { return c < 1e37f; }
-  // 2^((l - m) log2(e) / T) with the exponent in two pieces; halves, since l - m can overflow.  No branch: passes over a row live on
-  // several entries being in work at once.
+  // 2^((l - m) log2(e) / T), the difference (of halves, since l - m can overflow) and the exponent each in two pieces.  No branch: passes
+  // over a row live on several entries being in work at once.
   __device__ __forceinline__ float get(float l, float) const {
-    const float x = fmaf(l, 0.5f, -half_max);
+    const float a = 0.5f * l, x = a - half_max, b = x - a;
+    const float x_lo = (a - (x - b)) - (half_max + b);
     const float z = x * c;
-    const float lo = fmaf(x, c_lo, fmaf(x, c, -z));
+    const float lo = fmaf(x_lo, c, fmaf(x, c_lo, fmaf(x, c, -z)));
     float w;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(z));
     w = fmaf(w, lo * 0.69314718f, w);
     return z > -126.f ? w : 0.f;
   }
-  __device__ __forceinline__ double get(float l, double) const { return l > -INFINITY ? exp(((double)l - (double)max) * inv_t) : 0.0; }
+  // within 1e-5 of it
+  __device__ __forceinline__ float quick(float l) const {
+    float w;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaf(l, 0.5f, -half_max) * c));
+    return l > -INFINITY ? w : 0.f;
+  }
+  __device__ __forceinline__ double exponent(float l) const { return l > -INFINITY ? ((double)l - (double)max) * inv_t : -1e9; }
+  __device__ __forceinline__ double get(float l, double) const {
+    double x[1] = {exponent(l)};
+    exp_below(x);
+    return x[0];
+  }
+  template <typename W> __device__ __forceinline__ void get4(const float (&l)[4], W (&w)[4]) const {
+    if constexpr (sizeof(W) == 4) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = get(l[j], 0.f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = exponent(l[j]);
+      exp_below(w);
+    }
+  }
 };
 
 template <typename T> struct Pieces;  // 16 bytes of logits as fp32
@@ -172,43 +270,60 @@ template <> struct Pieces<__nv_bfloat16> {
   }
 };
 
-// A row's entries into shared memory; slot `first` + i holds entry i, -inf where there is none (NaN counts as none).  Whole 16-byte
-// pieces of memory are read with one load, those that reach beyond the row entry by entry.
+// A row's entries into shared memory; slot `first` + i holds entry i, -inf where there is none.  Whole 16-byte pieces of memory are read
+// with one load, eight of a thread on their way at a time, those that reach beyond the row entry by entry.  (NaN stays: every
+// comparison that would take it in is false, and its weight is 0.)
 template <typename T, int kThreads>
 __device__ int load_row(const SampleParams& p, const Group<kThreads>& g, int row, float* v, int cap, int& n) {
   const T* src = static_cast<const T*>(p.logits) + (long long)row * p.ld;
   const int base = g.crank * cap;  // this CTA holds slots [base, base + cap)
   const int tid = kThreads == 32 ? g.lane : (int)threadIdx.x;
-  auto clean = [](float x) { return x == x ? x : -INFINITY; };
   if (p.ids) {
     n = p.counts[row];
     n = n < 0 ? 0 : n > p.ld_ids ? p.ld_ids : n;
     const unsigned short* ids = p.ids + (long long)row * p.ld_ids;
+#pragma unroll 2
     for (int i = tid; i < cap; i += kThreads) {
       const int e = base + i;
       const int id = e < n ? ids[e] : 65536;
-      v[i] = id < p.width ? clean(to_f(src[id])) : -INFINITY;
+      v[i] = id < p.width ? to_f(src[id]) : -INFINITY;
     }
     return 0;
   }
   n = p.width;
   constexpr int kPer = Pieces<T>::n;
   const int first = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));  // the row's place in its first piece
-  const uint4* pieces = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src) & ~uintptr_t(15));
-  for (int i = tid; i < cap / kPer; i += kThreads) {
-    const int e = base + i * kPer - first;  // first entry of the piece
-    float f[kPer];
-    if (e >= 0 && e + kPer <= n) {
-      Pieces<T>::get(__ldg(pieces + base / kPer + i), f);
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) f[j] = clean(f[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) f[j] = e + j >= 0 && e + j < n ? clean(to_f(src[e + j])) : -INFINITY;
-    }
+  const uint4* pieces = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src) & ~uintptr_t(15)) + base / kPer;
+  auto put = [&](int i, const float (&f)[kPer]) {
 #pragma unroll
     for (int j = 0; j < kPer; j += 4) *reinterpret_cast<float4*>(v + i * kPer + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+  };
+  // of this CTA's pieces: those whole inside the row
+  const int whole0 = base == 0 && first > 0 ? 1 : 0, held = cap / kPer;
+  int whole1 = (first + n) / kPer - base / kPer;
+  whole1 = whole1 < whole0 ? whole0 : whole1 > held ? held : whole1;
+  for (int i0 = whole0 + tid; i0 < whole1; i0 += 8 * kThreads) {
+    uint4 u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + j * kThreads < whole1) u[j] = __ldg(pieces + i0 + j * kThreads);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + j * kThreads < whole1) {
+        float f[kPer];
+        Pieces<T>::get(u[j], f);
+        put(i0 + j * kThreads, f);
+      }
   }
+  auto edge = [&](int i) {
+    const int e = base + i * kPer - first;
+    float f[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) f[j] = e + j >= 0 && e + j < n ? to_f(src[e + j]) : -INFINITY;
+    put(i, f);
+  };
+  if (tid < whole0) edge(tid);
+  for (int i = whole1 + tid; i < held; i += kThreads) edge(i);
   return first;
 }
 
@@ -218,18 +333,16 @@ struct Cut {
   int slot;
 };
 
-constexpr int kBins = 256;
 constexpr int kSort = 64;    // entries that a warp sorts
-constexpr int kGather = 256;  // entries that a warp gathers from its row
+constexpr int kList = 256;   // entries between two logits that are solved by a warp
 
 template <int kThreads> struct Shared {
   double slots[2 * Group<kThreads>::kSlots];
-  union {
-    struct { uint32_t bins[kBins], total[kThreads == kWide ? kBins : 1]; };
-    struct { float gather_l[kThreads == 32 ? kGather : 1]; int gather_slot[kThreads == 32 ? kGather : 1]; };
-  };
-  float list_l[kSort];
-  int list_slot[kSort];
+  float wide[kThreads == 32 ? 1 : 2 * Group<kThreads>::kSlots * 8];
+  float list_l[kList];
+  int list_slot[kList];
+  uint64_t sorted[32];
+  double ahead;
   int count;
   int solved;
   uint64_t cut;
@@ -291,35 +404,45 @@ template <int kThreads> struct Row {
   Weight wt;
 
   template <typename F> __device__ __forceinline__ void each(F f) const {
-#pragma unroll 4
+#pragma unroll 2
     for (int i = 0; i < count; i += 4) {
       const float4 x = *reinterpret_cast<const float4*>(mine + i);
       f(i, x.x); f(i + 1, x.y); f(i + 2, x.z); f(i + 3, x.w);
     }
   }
-  // Sum of f over this thread's entries: 16 at a time in W, those sums in 64 bits.
-  template <typename W, typename F> __device__ __forceinline__ double sum(F f) const {
-    double total = 0.0;
-    int i = 0;
+  // Sum of f(i, l, w) over this thread's entries, w their weights (not computed where kWeights is false): 8 at a time in W, those sums
+  // in 64 bits.  (Longer loop bodies ran slower: instructions that did not arrive in time were half of the warps' stalls.)
+  template <typename W, bool kWeights, typename F> __device__ __forceinline__ double sum(F f) const {
     auto quad = [&](int at) -> W {
       const float4 x = *reinterpret_cast<const float4*>(mine + at);
-      const W a = f(at, x.x), b = f(at + 1, x.y), c = f(at + 2, x.z), d = f(at + 3, x.w);
+      const float l[4] = {x.x, x.y, x.z, x.w};
+      W w[4] = {};
+      if (kWeights) wt.get4(l, w);
+      const W a = f(at, l[0], w[0]), b = f(at + 1, l[1], w[1]), c = f(at + 2, l[2], w[2]), d = f(at + 3, l[3], w[3]);
       return (a + b) + (c + d);
     };
-    for (; i + 16 <= count; i += 16) {
-      const W a = quad(i), b = quad(i + 4), c = quad(i + 8), d = quad(i + 12);
-      total += (double)((a + b) + (c + d));
+    double total = 0.0;
+    int i = 0;
+    if constexpr (sizeof(W) == 4) {
+#pragma unroll 1
+      for (; i + 8 <= count; i += 8) {
+        const W a = quad(i), b = quad(i + 4);
+        total += (double)(a + b);
+      }
     }
+#pragma unroll 1
     for (; i < count; i += 4) total += (double)quad(i);
     return total;
   }
+  __device__ __forceinline__ bool keeps(const Cut cut, int i, float l) const { return (l > cut.l) | ((l == cut.l) & (i <= cut.slot - slot0)); }
   __device__ __forceinline__ void keep(const Cut cut) const {
-    const int last = cut.slot - slot0;
-#pragma unroll 4
+#pragma unroll 2
     for (int i = 0; i < count; i += 4) {
       float4 x = *reinterpret_cast<const float4*>(mine + i);
-      auto stays = [&](float l, int j) { return ((l > cut.l) | ((l == cut.l) & (j <= last))) ? l : -INFINITY; };
-      x.x = stays(x.x, i); x.y = stays(x.y, i + 1); x.z = stays(x.z, i + 2); x.w = stays(x.w, i + 3);
+      x.x = keeps(cut, i, x.x) ? x.x : -INFINITY;
+      x.y = keeps(cut, i + 1, x.y) ? x.y : -INFINITY;
+      x.z = keeps(cut, i + 2, x.z) ? x.z : -INFINITY;
+      x.w = keeps(cut, i + 3, x.w) ? x.w : -INFINITY;
       *reinterpret_cast<float4*>(mine + i) = x;
     }
   }
@@ -344,219 +467,255 @@ template <int kThreads> struct Row {
     return (int)g.max((float)at);
   }
 
-  // The end of the front part: the first entry ahead of which the measure (kMass: weights, else 1 each) sums to the target or more is out,
-  // with all behind it; the first of all stays.  kMass: `target` is a share of the sum of all weights.  Bins of a range of logits
-  // [lo, hi], the bin that the target falls in, the exact measure above it and its entries, until those are few enough to be sorted.
-  // False: a comparison was open.
-  template <typename W, bool kMass> __device__ bool select(double target, float hi, float lo, double slack, Cut& out) {
+  // The end of the front part inside a run of equal entries, ahead of which `front` is found.
+  template <typename W, bool kMass> __device__ bool equal_entries(float l, double front, double target, double all, double slack, Cut& out) {
+    const double w = kMass ? (double)wt.get(l, W()) : 1.0, ties = (target - front) / w;
+    if (kMass && sizeof(W) == 4 && (w < 1e-30 || fabs(ties - rint(ties)) <= slack * all / w + 1e-6 * fabs(ties))) return false;
+    out.l = l;
+    out.slot = nth_equal(l, ties <= 1.0 ? 0.0 : ceil(fmin(ties, 1e9)) - 1.0);
+    if (out.slot < 0) out.slot = 0x7fffffff;  // all of them
+    return true;
+  }
+  // The end among the n <= kList entries that were gathered, by one warp: bisection by the measure until 32 are left, which are
+  // sorted.  1: sh.cut; 2: a comparison was open; 3: in a run of entries equal to sh.cut, ahead of which sh.ahead is found; 0: not here.
+  template <typename W, bool kMass> __device__ int solve_list(int n, double front, double target, double slack) {
     constexpr bool kOpen = kMass && sizeof(W) == 4;
-    auto measure = [&](float l) -> W { if constexpr (kMass) return wt.get(l, W()); else return W(1); };
-    double above = 0.0;  // of entries above the range
-    double all = 0.0;    // kMass
+    constexpr int kEach = kList / 32;
+    const int lane = g.lane;
+    float l[kEach];
+    int slot[kEach];
+    W w[kEach];
+    int base = 0, held = kThreads == kWide && g.cluster > 1 ? 0 : n;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      l[i] = -INFINITY;
+      slot[i] = 0;
+      if (32 * i + lane < held) { l[i] = sh.list_l[32 * i + lane]; slot[i] = sh.list_slot[32 * i + lane]; }
+    }
+    if (kThreads == kWide && g.cluster > 1) {
+      for (int c = 0; c < g.cluster; ++c) {
+        const int nc = *cg::this_cluster().map_shared_rank(&sh.count, c);
+        const float* ll = cg::this_cluster().map_shared_rank(sh.list_l, c);
+        const int* ls = cg::this_cluster().map_shared_rank(sh.list_slot, c);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          const int at = 32 * i + lane - base;
+          if (at >= 0 && at < nc) { l[i] = ll[at]; slot[i] = ls[at]; }
+        }
+        base += nc;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) w[i] = l[i] > -INFINITY ? kMass ? wt.get(l[i], W()) : W(1) : W(0);
+    auto total = [&](auto in) {
+      double t = 0.0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) t += in(l[i]) ? (double)w[i] : 0.0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      return t;
+    };
+    uint32_t lo = key_of(-INFINITY), hi = key_of(wt.max);  // above lo the target or more, above hi less
+    double ahead = 0.0;
+    int left = n;
+    bool open = false;
+    while (left > 32) {
+      // the middle of what is left, in logits, or where that is none between them in keys
+      float down = INFINITY, up = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (l[i] > of_key(lo) && l[i] <= of_key(hi)) { down = fminf(down, l[i]); up = fmaxf(up, l[i]); }
+      up = warp_max(up);
+      down = -warp_max(-down);
+      if (!(down < up)) {
+        if (lane == 0) { sh.cut = entry_of(up, 0); sh.ahead = front + ahead; }
+        return left > 0 ? 3 : 0;
+      }
+      float at = 0.5f * down + 0.5f * up;
+      if (!(at >= down && at < up)) at = down;
+      const double m = total([&](float x) { return x > at; });
+      if (kOpen) open |= fabs(front + m - target) <= slack;
+      if (front + m >= target) lo = key_of(at);
+      else { hi = key_of(at); ahead = m; }
+      left = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) left += l[i] > of_key(lo) && l[i] <= of_key(hi);
+      left = __reduce_add_sync(0xffffffffu, left);
+    }
+    if (open) return 2;
+    // those left side by side, through the gathered entries' place
+    __syncwarp();
+    int pos = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const bool in = l[i] > of_key(lo) && l[i] <= of_key(hi);
+      const uint32_t b = __ballot_sync(0xffffffffu, in);
+      if (in) sh.sorted[pos + __popc(b & ((1u << lane) - 1))] = entry_of(l[i], slot[i]);
+      pos += __popc(b);
+    }
+    __syncwarp();
+    uint64_t e = lane < pos ? sh.sorted[lane] : 0, none = 0;
+    sort_entries(e, none, false, lane);
+    const float mine_l = of_key((uint32_t)(e >> 32));
+    double t0;
+    const double before = front + ahead + warp_before(!e ? 0.0 : kMass ? (double)wt.get(mine_l, W()) : 1.0, t0, lane);
+    const double end = front + ahead + t0;
+    // entries that stay: those ahead of which less than the target lies
+    const int stay = __popc(__ballot_sync(0xffffffffu, e && before < target));
+    if (kOpen && (__any_sync(0xffffffffu, e && fabs(before - target) <= slack) || fabs(end - target) <= slack)) return 2;
+    const uint64_t cut = __shfl_sync(0xffffffffu, e, (stay - 1) & 31);
+    if (lane == 0) sh.cut = cut;
+    return stay > 0 && end >= target ? 1 : 0;
+  }
+
+  // The end of the front part: the first entry ahead of which the measure (kMass: weights, else 1 each) sums to the target or more is out,
+  // with all behind it; the first of all stays.  kMass: `target` is a share of the sum of all weights.  The end lies between two
+  // logits, above the upper of which less than the target is found, above the lower the target or more; seven pivots between them
+  // per pass, where the last pass makes the end expected, until the entries between them are few enough to be sorted.  What finds
+  // the place are sums of quick weights with a margin; what decides is the exact measure above and the sorted entries.  (Counting
+  // in bins instead: an addition to shared memory took 64 cycles per warp, twice what the pivots take.)
+  // False: a comparison was open.
+  template <typename W, bool kMass> __device__ bool select(double target, float hi, float least, double slack, Cut& out) {
+    constexpr bool kOpen = kMass && sizeof(W) == 4;
     const int tid = kThreads == 32 ? g.lane : (int)threadIdx.x;
-    // weights in bins: whole numbers, whose sum of n weights of at most 1 stays below 2^31 (order does not matter to them)
-    double quantum = kMass ? 2147483000.0 / (double)(g.threads() * count) : 1.0;
-    for (int round = 0; round < 8; ++round) {
-      // the lowest bin of the first round takes what lies below the range
-      const float scale = fminf((kBins - 0.5f) / fminf(hi - lo, 3.4e38f), 1e37f);
-      const float least_in = round == 0 ? -3.402823466e38f : lo;
-      auto bin = [&](float l) { return __float_as_int(fminf((hi - l) * scale, kBins - 1.f) + 8388608.f) & (kBins - 1); };
-      const float fq = (float)quantum;
-      g.barrier();  // the others are done with what is cleared
-      for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
-      if (tid == 0) sh.count = 0;
-      if (kThreads == 32) __syncwarp(); else __syncthreads();
+    float lo = -INFINITY, reach_lo = 0.f, reach_hi = 0.f;  // found above them (lo: all, where it is infinite)
+    double all = 0.0;
+    float x[7];
+    {
+      constexpr float kSteps[7] = {1.f, 2.f, 3.f, 4.5f, 6.f, 8.f, 11.f}, kShares[7] = {0.03125f, 0.0625f, 0.125f, 0.25f, 0.375f, 0.5f, 0.75f};
+#pragma unroll
+      for (int j = 0; j < 7; ++j) x[j] = kMass ? hi - kSteps[j] * wt.temp : hi - kShares[j] * fminf(hi - least, 3.4e38f);
+    }
+    for (int round = 0; round < 16; ++round) {
+      float a[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] = 0.f;
+      auto pivots = [&](float l, float w) {
+#pragma unroll
+        for (int j = 0; j < 7; ++j) a[j] += l > x[j] ? w : 0.f;
+        a[7] += l > -INFINITY ? w : 0.f;
+      };
       if (kMass && round == 0) {
-        all = g.sum(sum<W>([&](int, float l) -> W {
-          const float w = wt.get(l, 0.f);
-          const uint32_t q = (uint32_t)fmaf(w, fq, 0.5f);
-          if (q) atomicAdd(&sh.bins[bin(l)], q);
-          if constexpr (sizeof(W) == 4) return w; else return wt.get(l, W());
-        }));
+        all = sum<W, true>([&](int, float l, W w) -> W { pivots(l, (float)w); return w; });
+        all = g.sum(all);
         target *= all;
       } else {
-        each([&](int, float l) {
-          const uint32_t q = kMass ? (uint32_t)fmaf(wt.get(l, 0.f), fq, 0.5f) : 1u;
-          if ((l <= hi) & (l >= least_in) & (q > 0)) atomicAdd(&sh.bins[bin(l)], q);
-        });
-        g.barrier();
+        each([&](int, float l) { pivots(l, kMass ? wt.quick(l) : 1.f); });
       }
-      const uint32_t* total = sh.bins;
+      g.sum8(a);
+      if (round == 0) reach_lo = a[7];
+      const float goal = (float)target, margin = kMass ? 1e-5f * (float)all : 0.f;
+#pragma unroll
+      for (int j = 0; j < 7; ++j)
+        if (x[j] < hi && a[j] < goal - margin) { hi = x[j]; reach_hi = a[j]; }
+#pragma unroll
+      for (int j = 6; j >= 0; --j)
+        if (x[j] > lo && x[j] < hi && a[j] >= goal + margin) { lo = x[j]; reach_lo = a[j]; }
+      // entries between the two, as many as there would be if all were as light as the lower end
+      const float most_here = (reach_lo - reach_hi + margin) / (kMass ? fmaxf(wt.quick(lo), 1e-30f) : 1.f);
+      const float low = lo > -INFINITY ? lo : kMass ? fmaxf(hi - 16.f * wt.temp, -3.4e38f) : fminf(least, hi);
+      const float f = fminf(fmaxf((goal - reach_hi) / (reach_lo - reach_hi), 0.f), 1.f), width = fminf(hi - low, 3.4e38f);
+      const float parts[7] = {0.25f * f, 0.75f * f, 0.9375f * f, f, f + 0.0625f * (1.f - f), f + 0.25f * (1.f - f), f + 0.75f * (1.f - f)};
+#pragma unroll
+      for (int j = 0; j < 7; ++j) x[j] = hi - parts[j] * width;
+      if (!(most_here <= (float)kList) && round < 3) continue;
+      // the exact measure above them, and the entries between them, marked 32 at a time
+      g.barrier();  // the others are done with what is cleared
+      if (tid == 0) sh.count = 0;
+      if (kThreads == 32) __syncwarp(); else __syncthreads();
+      float down = INFINITY, up = -INFINITY;
+      double more = 0.0;
+#pragma unroll 1
+      for (int i0 = 0; i0 < count; i0 += 32) {
+        uint32_t hits = 0;
+        const int end = count - i0 < 32 ? count - i0 : 32;
+#pragma unroll 1
+        for (int i = 0; i < end; i += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(mine + i0 + i);
+          const float l4[4] = {v.x, v.y, v.z, v.w};
+          W w4[4] = {1, 1, 1, 1};
+          if constexpr (kMass) wt.get4(l4, w4);
+          uint32_t four = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            four |= (l4[j] <= hi) & (l4[j] > lo) ? 1u << j : 0u;
+            w4[j] = l4[j] > hi ? w4[j] : W(0);
+          }
+          more += (double)((w4[0] + w4[1]) + (w4[2] + w4[3]));
+          hits |= four << i;
+        }
+        const int own = __popc(hits);
+        int pos = own ? atomicAdd(&sh.count, own) : 0;
+        for (; hits; hits &= hits - 1, ++pos) {
+          const int i = i0 + __ffs((int)hits) - 1;
+          const float l = mine[i];
+          down = fminf(down, l);
+          up = fmaxf(up, l);
+          if (pos < kList) { sh.list_l[pos] = l; sh.list_slot[pos] = slot0 + i; }
+        }
+      }
+      const double front = g.sum(more);
+      int n = sh.count;
       if (kThreads == kWide && g.cluster > 1) {
-        for (int i = tid; i < kBins; i += kThreads) {
-          uint32_t t = 0;
-          for (int c = 0; c < g.cluster; ++c) t += *cg::this_cluster().map_shared_rank(&sh.bins[i], c);
-          sh.total[i] = t;
-        }
-        total = sh.total;
-        __syncthreads();
+        n = 0;
+        for (int c = 0; c < g.cluster; ++c) n += *cg::this_cluster().map_shared_rank(&sh.count, c);
       }
-      // first bin at whose end the target is reached, the last full one where rounding leaves none
-      uint32_t part[kBins / 32], sum8 = 0;
+      if (n == 0 || front >= target) break;
+      if (n > kList) {
+        hi = g.max(up);  // the entries' own ends
+        const float bottom = -g.max(-down);
+        reach_hi = (float)front;
+        if (hi == bottom) return equal_entries<W, kMass>(hi, front, target, all, slack, out);
+        // the largest of them is above every next pivot but not above `hi`
 #pragma unroll
-      for (int i = 0; i < kBins / 32; ++i) {
-        part[i] = total[g.lane * (kBins / 32) + i];
-        sum8 += part[i];
+        for (int j = 0; j < 7; ++j) x[j] = hi - (j + 1) * 0.125f * fminf(hi - bottom, 3.4e38f);
+        continue;
       }
-      uint32_t in8 = sum8;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, in8, o);
-        if (g.lane >= o) in8 += up;
+      if (kThreads == 32 || g.warp == 0) {
+        const int result = solve_list<W, kMass>(n, front, target, slack * all);
+        if (g.lane == 0) sh.solved = result;
       }
-      const double goal = (target - above) * quantum;
-      uint32_t run = in8 - sum8;
-      int b = kBins, last = -1;
-#pragma unroll
-      for (int i = 0; i < kBins / 32; ++i) {
-        run += part[i];
-        if (part[i]) last = g.lane * (kBins / 32) + i;
-        if (b == kBins && part[i] && (double)run >= goal) b = g.lane * (kBins / 32) + i;
-      }
-      b = __reduce_min_sync(0xffffffffu, b);
-      last = __reduce_max_sync(0xffffffffu, last);
-      if (b == kBins) b = last;
-      auto next_bin = [&](int from, bool up) {  // the next one that is not empty, -1 if there is none
-        int at = up ? kBins : -1;
-#pragma unroll
-        for (int i = 0; i < kBins / 32; ++i) {
-          const int j = g.lane * (kBins / 32) + i;
-          if (part[i] && (up ? j > from : j < from)) at = up ? min(at, j) : j;
-        }
-        at = up ? __reduce_min_sync(0xffffffffu, at) : __reduce_max_sync(0xffffffffu, at);
-        return at == kBins ? -1 : at;
-      };
-      bool narrower = false;
-      for (int tries = 0; tries < 3 && b >= 0; ++tries) {
-        if (tries > 0) {
-          g.barrier();
-          if (tid == 0) sh.count = 0;
-          g.barrier();
-        }
-        float least = INFINITY, most = -INFINITY;
-        const double more = sum<W>([&](int i, float l) -> W {
-          const int at = bin(l);
-          const bool in = (l <= hi) & (l >= least_in);
-          if (in & (at == b)) {
-            least = fminf(least, l);
-            most = fmaxf(most, l);
-            const int pos = atomicAdd(&sh.count, 1);
-            if (pos < kSort) { sh.list_l[pos] = l; sh.list_slot[pos] = slot0 + i; }
-          }
-          return in & (at < b) ? measure(l) : W(0);
-        });
-        const double front = above + g.sum(more);
-        if (kOpen && fabs(front - target) <= slack * all) return false;
-        int n = sh.count;
-        if (kThreads == kWide && g.cluster > 1) {
-          n = 0;
-          for (int c = 0; c < g.cluster; ++c) n += *cg::this_cluster().map_shared_rank(&sh.count, c);
-        }
-        if (front >= target) {  // bins of weights are rounded sums: the target lies in an earlier one
-          b = next_bin(b, false);
-          continue;
-        }
-        if (n > kSort) {
-          hi = g.max(most);
-          lo = -g.max(-least);
-          above = front;
-          if (hi == lo) {  // equal entries
-            const double w = (double)measure(hi), ties = (target - above) / w;
-            if (kOpen && (w < 1e-30 || fabs(ties - rint(ties)) <= slack * all / w + 1e-6 * fabs(ties) || ties > (double)n)) return false;
-            if (ties > (double)n) break;
-            out.l = hi;
-            out.slot = nth_equal(hi, ceil(ties) - 1.0);
-            return true;
-          }
-          if (kMass) quantum = 2147483000.0 / fmax((double)n * (double)wt.get(hi, 0.f), 1e-28);
-          narrower = true;
-          break;
-        }
-        if (kThreads == 32 || g.warp == 0) {
-          uint64_t e[2] = {0, 0};
-          if (kThreads == kWide && g.cluster > 1) {
-            int base = 0;
-            for (int c = 0; c < g.cluster; ++c) {
-              const int nc = *cg::this_cluster().map_shared_rank(&sh.count, c);
-              const float* ll = cg::this_cluster().map_shared_rank(sh.list_l, c);
-              const int* ls = cg::this_cluster().map_shared_rank(sh.list_slot, c);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int i = g.lane + 32 * h - base;
-                if (i >= 0 && i < nc) e[h] = entry_of(ll[i], ls[i]);
-              }
-              base += nc;
-            }
-          } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              if (g.lane + 32 * h < n) e[h] = entry_of(sh.list_l[g.lane + 32 * h], sh.list_slot[g.lane + 32 * h]);
-          }
-          sort_entries(e[0], e[1], n > 32, g.lane);
-          double w[2], t0, t1, before[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) w[h] = e[h] ? (double)measure(of_key((uint32_t)(e[h] >> 32))) : 0.0;
-          before[0] = front + warp_before(w[0], t0, g.lane);
-          before[1] = front + t0 + warp_before(w[1], t1, g.lane);
-          const double end = front + t0 + t1;
-          // entries of the list that stay: those ahead of which less than the target lies
-          const int stay = __popc(__ballot_sync(0xffffffffu, e[0] && before[0] < target)) +
-                           __popc(__ballot_sync(0xffffffffu, e[1] && before[1] < target));
-          bool open = false;
-          if (kOpen) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) open |= e[h] && fabs(before[h] - target) <= slack * all;
-            open = __any_sync(0xffffffffu, open) || fabs(end - target) <= slack * all;
-          }
-          const uint64_t c0 = __shfl_sync(0xffffffffu, e[0], (stay - 1) & 31), c1 = __shfl_sync(0xffffffffu, e[1], (stay - 1) & 31);
-          if (g.lane == 0) {
-            sh.solved = open ? 2 : end >= target ? 1 : 0;
-            sh.cut = stay > 32 ? c1 : c0;
-          }
-        }
-        if (kThreads == 32) __syncwarp(); else __syncthreads();
-        if (sh.solved == 2) return false;
-        if (sh.solved == 1) {
-          out = cut_of(sh.cut);
-          return true;
-        }
-        b = next_bin(b, true);  // ... or in a later one
-      }
-      if (!narrower) break;
+      if (kThreads == 32) __syncwarp(); else __syncthreads();
+      if (sh.solved == 2) return false;
+      if (sh.solved == 0) break;
+      out = cut_of(sh.cut);
+      if (sh.solved == 3) return equal_entries<W, kMass>(out.l, sh.ahead, target, all, slack, out);
+      return true;
     }
     if (kOpen) return false;
-    // Bins did not find it (theirs are rounded sums, ranges can hold a few values many decades apart): bisection.
+    // Not found so (a few values many decades apart, a target that rounding puts beyond all): bisection.
     uint32_t lo_key = key_of(-INFINITY), hi_key = key_of(wt.max);  // measure above lo_key: the target or more; above hi_key: less
     double over = 0.0;
     while (hi_key - lo_key > 1) {
       const uint32_t mid = lo_key + (hi_key - lo_key) / 2;
       const float cut = of_key(mid);
-      const double m = g.sum(sum<W>([&](int, float l) { return l > cut ? measure(l) : W(0); }));
+      const double m = g.sum(sum<W, kMass>([&](int, float l, W w) { return l > cut ? (kMass ? w : W(1)) : W(0); }));
       if (m >= target) lo_key = mid;
       else { hi_key = mid; over = m; }
     }
     out.l = of_key(hi_key);
-    const double ties = (target - over) / (double)measure(out.l);
+    const double ties = (target - over) / (kMass ? (double)wt.get(out.l, W()) : 1.0);
     out.slot = nth_equal(out.l, ties <= 1.0 ? 0.0 : ceil(fmin(ties, 1e9)) - 1.0);
     if (out.slot < 0) out.slot = 0x7fffffff;  // all of them
     return true;
   }
 
-  // The draw among what is left and what min-p keeps of it.  False: a comparison was open.
-  template <typename W> __device__ bool draw(float p_min, float u, double slack) {
+  // The draw among what the cut and min-p keep.  False: a comparison was open.
+  template <typename W> __device__ bool draw(const Cut cut, float p_min, float u, double slack) {
     constexpr bool kOpen = sizeof(W) == 4;
     const W limit = p_min > 0.f ? (W)fminf(p_min, 1.f) : W(0);
     bool open = false;
     const float near = 4.f * (float)slack * (float)limit;
     double own;
     if (limit > W(0)) {
-      own = sum<W>([&](int, float l) -> W {
-        const W w = wt.get(l, W());
+      own = sum<W, true>([&](int i, float l, W w) -> W {
         if (kOpen) open |= (fabsf((float)w - (float)limit) <= near) & (l != wt.max);
-        return w >= limit ? w : W(0);
+        return keeps(cut, i, l) & (w >= limit) ? w : W(0);
       });
+    } else if (cut.l > -INFINITY) {
+      own = sum<W, true>([&](int i, float l, W w) -> W { return keeps(cut, i, l) ? w : W(0); });
     } else {
-      own = sum<W>([&](int, float l) -> W { return wt.get(l, W()); });
+      own = sum<W, true>([&](int, float, W w) -> W { return w; });
     }
     double total;
     const double ahead = g.before(own, total), target = (double)u * total;
@@ -582,7 +741,7 @@ template <int kThreads> struct Row {
       for (int base = 0; base < count; base += 32) {
         double w = 0.0, sum32;
         const int i = base + g.lane;
-        if (i < count) {
+        if (i < count && (theirs[i] > cut.l || (theirs[i] == cut.l && their_slot + i <= cut.slot))) {
           const W x = wt.get(theirs[i], W());
           w = x >= limit ? (double)x : 0.0;
         }
@@ -660,7 +819,7 @@ template <int kThreads> struct Row {
       else hit0 = 1u << (31 - __clz(__ballot_sync(0xffffffffu, w[0] > 0.0)));
     }
     const int half = hit0 ? 0 : 1, j = __ffs(hit0 ? hit0 : hit1) - 1;
-    if (lane == j) give((int)~(uint32_t)e[half], (float)(w[half] / run));
+    if (lane == j) give((int)~(uint32_t)(half ? e[1] : e[0]), (float)((half ? w[1] : w[0]) / run));
   }
   // The entries that top-k can keep, gathered: those not below a logit that k entries reach.  Maxima of the lanes' runs give one: the
   // k-th of them for small k, one of the least else, which more than k entries reach nearly always; from there a bisection over the
@@ -678,8 +837,15 @@ template <int kThreads> struct Row {
       }
     const float floor_l = __shfl_sync(0xffffffffu, s, k <= 24 ? k - 1 : k <= 40 ? 28 : 30);  // (the last run may be empty)
     if (floor_l == -INFINITY) return 0;
-    uint64_t hits = 0;
-    each([&](int i, float l) { hits |= (uint64_t)(l >= floor_l) << i; });
+    uint32_t hits_lo = 0, hits_hi = 0;
+#pragma unroll 4
+    for (int i = 0; i < count; i += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(mine + i);
+      const uint32_t four = (x.x >= floor_l ? 1u : 0u) | (x.y >= floor_l ? 2u : 0u) | (x.z >= floor_l ? 4u : 0u) | (x.w >= floor_l ? 8u : 0u);
+      if (i < 32) hits_lo |= four << i;
+      else hits_hi |= four << (i - 32);
+    }
+    uint64_t hits = (uint64_t)hits_hi << 32 | hits_lo;
     const int own = __popcll(hits);
     int in = own;
 #pragma unroll
@@ -688,20 +854,20 @@ template <int kThreads> struct Row {
       if (lane >= o) in += up;
     }
     int n = __shfl_sync(0xffffffffu, in, 31);
-    if (n > kGather || n < k) return 0;
+    if (n > kList || n < k) return 0;
     for (int pos = in - own; hits; hits &= hits - 1, ++pos) {
       const int i = __ffsll((long long)hits) - 1;
-      sh.gather_l[pos] = mine[i];
-      sh.gather_slot[pos] = slot0 + i;
+      sh.list_l[pos] = mine[i];
+      sh.list_slot[pos] = slot0 + i;
     }
     __syncwarp();
     if (n <= kSort) return n;
-    float l[kGather / 32];
-    int slot[kGather / 32];
+    float l[kList / 32];
+    int slot[kList / 32];
 #pragma unroll
-    for (int i = 0; i < kGather / 32; ++i) {
-      l[i] = 32 * i + lane < n ? sh.gather_l[32 * i + lane] : -INFINITY;
-      slot[i] = 32 * i + lane < n ? sh.gather_slot[32 * i + lane] : 0;
+    for (int i = 0; i < kList / 32; ++i) {
+      l[i] = 32 * i + lane < n ? sh.list_l[32 * i + lane] : -INFINITY;
+      slot[i] = 32 * i + lane < n ? sh.list_slot[32 * i + lane] : 0;
     }
     uint32_t lo = key_of(floor_l), hi = key_of(wt.max) + 1;  // more than 64 reach lo, fewer than k reach hi
     float at = 0.f;
@@ -711,7 +877,7 @@ template <int kThreads> struct Row {
       at = of_key(mid);
       int c = 0;
 #pragma unroll
-      for (int i = 0; i < kGather / 32; ++i) c += l[i] >= at;
+      for (int i = 0; i < kList / 32; ++i) c += l[i] >= at;
       c = __reduce_add_sync(0xffffffffu, c);
       if (c > kSort) lo = mid;
       else if (c < k) hi = mid;
@@ -721,13 +887,13 @@ template <int kThreads> struct Row {
     __syncwarp();
     n = 0;
 #pragma unroll
-    for (int i = 0; i < kGather / 32; ++i) {
+    for (int i = 0; i < kList / 32; ++i) {
       const bool stays = l[i] >= at;
       const uint32_t b = __ballot_sync(0xffffffffu, stays);
       if (stays) {
         const int pos = n + __popc(b & ((1u << lane) - 1));
-        sh.gather_l[pos] = l[i];
-        sh.gather_slot[pos] = slot[i];
+        sh.list_l[pos] = l[i];
+        sh.list_slot[pos] = slot[i];
       }
       n += __popc(b);
     }
@@ -737,7 +903,7 @@ template <int kThreads> struct Row {
 };
 
 template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads == 32 ? 32 * kWarpRows : kThreads)
+__global__ void __launch_bounds__(kThreads == 32 ? 32 * kWarpRows : kThreads, kThreads == 32 ? 5 : 3)
 sample_kernel(const SampleParams p) {
   extern __shared__ float4 smem[];
   __shared__ Shared<kThreads> shared[kThreads == 32 ? kWarpRows : 1];
@@ -745,7 +911,7 @@ sample_kernel(const SampleParams p) {
   const int cap = kThreads * 4 * p.pieces;
   float* v = reinterpret_cast<float*>(smem) + part * cap;
   Shared<kThreads>& sh = shared[part];
-  Group<kThreads> g(sh.slots, p.cluster);
+  Group<kThreads> g(sh.slots, sh.wide, p.cluster);
   const int row = kThreads == 32 ? blockIdx.x * kWarpRows + part : blockIdx.x / p.cluster;
   if (row >= p.rows) return;
   float temp = p.temperature ? p.temperature[row] : 1.f;
@@ -787,14 +953,14 @@ sample_kernel(const SampleParams p) {
       } else if (k > 0 && k <= kSort) {
         const int few = r.gather_top(k, own_max);
         if (few) {
-          r.finish(sh.gather_l, sh.gather_slot, 0, few, k, tp, p_min, u);
+          r.finish(sh.list_l, sh.list_slot, 0, few, k, tp, p_min, u);
           done = true;
         }
       }
     }
     if (!done) {
       const double slack = (double)p.slack;
-      Cut cut;
+      Cut cut{-INFINITY, -1};
       if (k > 0 && k < n) {
         float least = INFINITY;
         int own = 0;
@@ -805,15 +971,13 @@ sample_kernel(const SampleParams p) {
         if ((double)k < g.sum((double)own)) {
           least = -g.max(-least);
           r.template select<float, false>((double)k, m, least, 0.0, cut);
-          r.keep(cut);
+          if (tp < 1.f) r.keep(cut);
         }
       }
       if (tp < 1.f) {
-        const float lo = m - 24.f * temp;  // what is below, weights of less than e^-24, is in the lowest bin
-        if (!fp32 || !r.template select<float, true>((double)tp, m, lo, slack, cut)) r.template select<double, true>((double)tp, m, lo, 0.0, cut);
-        r.keep(cut);
+        if (!fp32 || !r.template select<float, true>((double)tp, m, 0.f, slack, cut)) r.template select<double, true>((double)tp, m, 0.f, 0.0, cut);
       }
-      if (!fp32 || !r.template draw<float>(p_min, u, slack)) r.template draw<double>(p_min, u, 0.0);
+      if (!fp32 || !r.template draw<float>(cut, p_min, u, slack)) r.template draw<double>(cut, p_min, u, 0.0);
     }
   }
   if (kThreads == kWide && p.cluster > 1) g.barrier();  // no CTA leaves while another may still read its shared memory
@@ -844,16 +1008,16 @@ cudaError_t launch_sample(SampleParams p, cudaStream_t s) {
   const int n = p.ids ? p.ld_ids : p.width + Pieces<T>::n - 1;
   auto pieces = [&](int threads) { return ceil_div(ceil_div(n, 4), threads) | 1; };
   p.cluster = 1;
-  const int threads = pieces(32) <= 15 ? 32 : n <= 8192 ? 256 : kWide;
+  // A warp per row costs the fewest instructions, a CTA the least time: few rows whose cut is not found among a few gathered entries take CTAs.
+  const bool few = p.rows <= kFewRows && p.top_p && !p.top_k && n > 2 * kList;
+  const int threads = pieces(32) <= 15 && !few ? 32 : kWide;
   if (threads == kWide)
-    while (p.cluster < kMaxCluster && pieces(kWide * p.cluster) > 5) p.cluster *= 2;
+    while (p.cluster < kMaxCluster && pieces(kWide * p.cluster) > 9) p.cluster *= 2;
   p.pieces = pieces(threads * p.cluster);
-  // Bound of a sum's error over the sum of all weights, in steps of 2^-24.  A weight: its exponent carries the rounding of l - m, at
-  // most |z| steps with z = (l - m) / T, and the sum of w |z| is at most ln(n) times the sum of w; exp2f and the factor 5.
-  // Sums: a thread's chains 4 (8 where bins are summed up), the total 1.  Twice that, since two sums are compared.
-  p.slack = 2.f * (13.f + 5.f + 9.f) * 0x1p-24f;
+  // Bound of a sum's error over the sum of all weights, in steps of 2^-24.  A weight: ex2.approx 3, the factor and the second pieces 1.
+  // Sums: 8 at a time 3.  Twice that, since two sums are compared.
+  p.slack = 2.f * (3.f + 1.f + 3.f + 1.f) * 0x1p-24f;
   if (threads == 32) return launch_group<T, 32>(p, s);
-  if (threads == 256) return launch_group<T, 256>(p, s);
   return launch_group<T, kWide>(p, s);
 }
 
