@@ -51,7 +51,7 @@ template <int kThreads> struct Group {
   static constexpr int kWarps = kThreads / 32;
   static constexpr int kSlots = kThreads == kWide ? kMaxCluster * kWarps : kWarps;
   double* slots;  // [2][kSlots], kThreads > 32
-  float* wide;    // [2][kSlots][8]
+  float* wide;    // [2][kSlots][4]
   int cluster, crank, turn;
   int lane, warp;
   __device__ Group(double* s, float* s8, int cl) : slots(s), wide(s8), cluster(kThreads == kWide ? cl : 1), crank(0), turn(0) {
@@ -98,38 +98,36 @@ template <int kThreads> struct Group {
     for (int i = lane; i < cluster * kWarps; i += 32) t = fmaxf(t, (float)s[i]);
     return warp_max(t);
   }
-  // Sums of eight values at once, in a fixed order, for places to look in.
-  __device__ __forceinline__ void sum8(float (&a)[8]) {
-    // halving exchange: a lane is left with value ((lane >> 4) & 1) * 4 + ((lane >> 3) & 1) * 2 + ((lane >> 2) & 1) of its warp
+  // Sums of four values at once, in a fixed order, for places to look in.
+  __device__ __forceinline__ void sum4(float (&a)[4]) {
+    // halving exchange: a lane is left with value lane >> 3 of its warp
     auto halve = [&](bool upper, int o, float& low, float high) {
       const float send = upper ? low : high, keep = upper ? high : low;
       low = keep + __shfl_xor_sync(0xffffffffu, send, o);
     };
-#pragma unroll
-    for (int i = 0; i < 4; ++i) halve((lane & 16) != 0, 16, a[i], a[i + 4]);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) halve((lane & 8) != 0, 8, a[i], a[i + 2]);
-    halve((lane & 4) != 0, 4, a[0], a[1]);
+    halve((lane & 16) != 0, 16, a[0], a[2]);
+    halve((lane & 16) != 0, 16, a[1], a[3]);
+    halve((lane & 8) != 0, 8, a[0], a[1]);
     float v = a[0];
-    v += __shfl_xor_sync(0xffffffffu, v, 2);
-    v += __shfl_xor_sync(0xffffffffu, v, 1);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (kThreads > 32) {
-      float* mine = wide + (turn & 1) * kSlots * 8;
+      float* mine = wide + (turn & 1) * kSlots * 4;
       ++turn;
-      const int at = (crank * kWarps + warp) * 8 + (lane >> 2);
+      const int at = (crank * kWarps + warp) * 4 + (lane >> 3);
       if (kThreads == kWide && cluster > 1) {
-        for (int c = lane & 3; c < cluster; c += 4) *cg::this_cluster().map_shared_rank(mine + at, c) = v;
-      } else if ((lane & 3) == 0) {
+        if ((lane & 7) < cluster) *cg::this_cluster().map_shared_rank(mine + at, lane & 7) = v;
+      } else if ((lane & 7) == 0) {
         mine[at] = v;
       }
       barrier();
       v = 0.f;
-      for (int w = lane & 3; w < cluster * kWarps; w += 4) v += mine[w * 8 + (lane >> 2)];
-      v += __shfl_xor_sync(0xffffffffu, v, 2);
-      v += __shfl_xor_sync(0xffffffffu, v, 1);
+      for (int w = lane & 7; w < cluster * kWarps; w += 8) v += mine[w * 4 + (lane >> 3)];
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = __shfl_sync(0xffffffffu, v, j * 4);
+    for (int j = 0; j < 4; ++j) a[j] = __shfl_sync(0xffffffffu, v, j * 8);
   }
   // Sum over the threads before this one; `total` over all.
   __device__ __forceinline__ double before(double v, double& total) {
@@ -338,7 +336,7 @@ constexpr int kList = 256;   // entries between two logits that are solved by a 
 
 template <int kThreads> struct Shared {
   double slots[2 * Group<kThreads>::kSlots];
-  float wide[kThreads == 32 ? 1 : 2 * Group<kThreads>::kSlots * 8];
+  float wide[kThreads == 32 ? 1 : 2 * Group<kThreads>::kSlots * 4];
   float list_l[kList];
   int list_slot[kList];
   uint64_t sorted[32];
@@ -570,7 +568,7 @@ template <int kThreads> struct Row {
 
   // The end of the front part: the first entry ahead of which the measure (kMass: weights, else 1 each) sums to the target or more is out,
   // with all behind it; the first of all stays.  kMass: `target` is a share of the sum of all weights.  The end lies between two
-  // logits, above the upper of which less than the target is found, above the lower the target or more; seven pivots between them
+  // logits, above the upper of which less than the target is found, above the lower the target or more; three pivots between them
   // per pass, where the last pass makes the end expected, until the entries between them are few enough to be sorted.  What finds
   // the place are sums of quick weights with a margin; what decides is the exact measure above and the sorted entries.  (Counting
   // in bins instead: an addition to shared memory took 64 cycles per warp, twice what the pivots take.)
@@ -580,20 +578,20 @@ template <int kThreads> struct Row {
     const int tid = kThreads == 32 ? g.lane : (int)threadIdx.x;
     float lo = -INFINITY, reach_lo = 0.f, reach_hi = 0.f;  // found above them (lo: all, where it is infinite)
     double all = 0.0;
-    float x[7];
+    float x[3];
     {
-      constexpr float kSteps[7] = {1.f, 2.f, 3.f, 4.5f, 6.f, 8.f, 11.f}, kShares[7] = {0.03125f, 0.0625f, 0.125f, 0.25f, 0.375f, 0.5f, 0.75f};
+      constexpr float kSteps[3] = {2.f, 4.5f, 8.f}, kShares[3] = {0.0625f, 0.25f, 0.5f};
 #pragma unroll
-      for (int j = 0; j < 7; ++j) x[j] = kMass ? hi - kSteps[j] * wt.temp : hi - kShares[j] * fminf(hi - least, 3.4e38f);
+      for (int j = 0; j < 3; ++j) x[j] = kMass ? hi - kSteps[j] * wt.temp : hi - kShares[j] * fminf(hi - least, 3.4e38f);
     }
     for (int round = 0; round < 16; ++round) {
-      float a[8];
+      float a[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] = 0.f;
+      for (int j = 0; j < 4; ++j) a[j] = 0.f;
       auto pivots = [&](float l, float w) {
 #pragma unroll
-        for (int j = 0; j < 7; ++j) a[j] += l > x[j] ? w : 0.f;
-        a[7] += l > -INFINITY ? w : 0.f;
+        for (int j = 0; j < 3; ++j) a[j] += l > x[j] ? w : 0.f;
+        a[3] += l > -INFINITY ? w : 0.f;
       };
       if (kMass && round == 0) {
         all = sum<W, true>([&](int, float l, W w) -> W { pivots(l, (float)w); return w; });
@@ -602,23 +600,23 @@ template <int kThreads> struct Row {
       } else {
         each([&](int, float l) { pivots(l, kMass ? wt.quick(l) : 1.f); });
       }
-      g.sum8(a);
-      if (round == 0) reach_lo = a[7];
+      g.sum4(a);
+      if (round == 0) reach_lo = a[3];
       const float goal = (float)target, margin = kMass ? 1e-5f * (float)all : 0.f;
 #pragma unroll
-      for (int j = 0; j < 7; ++j)
+      for (int j = 0; j < 3; ++j)
         if (x[j] < hi && a[j] < goal - margin) { hi = x[j]; reach_hi = a[j]; }
 #pragma unroll
-      for (int j = 6; j >= 0; --j)
+      for (int j = 2; j >= 0; --j)
         if (x[j] > lo && x[j] < hi && a[j] >= goal + margin) { lo = x[j]; reach_lo = a[j]; }
       // entries between the two, as many as there would be if all were as light as the lower end
       const float most_here = (reach_lo - reach_hi + margin) / (kMass ? fmaxf(wt.quick(lo), 1e-30f) : 1.f);
       const float low = lo > -INFINITY ? lo : kMass ? fmaxf(hi - 16.f * wt.temp, -3.4e38f) : fminf(least, hi);
       const float f = fminf(fmaxf((goal - reach_hi) / (reach_lo - reach_hi), 0.f), 1.f), width = fminf(hi - low, 3.4e38f);
-      const float parts[7] = {0.25f * f, 0.75f * f, 0.9375f * f, f, f + 0.0625f * (1.f - f), f + 0.25f * (1.f - f), f + 0.75f * (1.f - f)};
+      const float parts[3] = {0.875f * f, f + 0.015625f * (1.f - f), f + 0.125f * (1.f - f)};
 #pragma unroll
-      for (int j = 0; j < 7; ++j) x[j] = hi - parts[j] * width;
-      if (!(most_here <= (float)kList) && round < 3) continue;
+      for (int j = 0; j < 3; ++j) x[j] = hi - parts[j] * width;
+      if (!(most_here <= (float)kList) && round < 5) continue;
       // the exact measure above them, and the entries between them, marked 32 at a time
       g.barrier();  // the others are done with what is cleared
       if (tid == 0) sh.count = 0;
@@ -668,7 +666,7 @@ template <int kThreads> struct Row {
         if (hi == bottom) return equal_entries<W, kMass>(hi, front, target, all, slack, out);
         // the largest of them is above every next pivot but not above `hi`
 #pragma unroll
-        for (int j = 0; j < 7; ++j) x[j] = hi - (j + 1) * 0.125f * fminf(hi - bottom, 3.4e38f);
+        for (int j = 0; j < 3; ++j) x[j] = hi - (j + 1) * 0.25f * fminf(hi - bottom, 3.4e38f);
         continue;
       }
       if (kThreads == 32 || g.warp == 0) {
