@@ -40,7 +40,7 @@ __device__ __forceinline__ int adapter_of(const AdapterParams& p, int m) {
 constexpr int kShrinkThreads = 160;  // four warps of 16 rows, one that loads
 template <int NB> struct ShrinkCfg {  // NB: blocks of 16 ranks
   static constexpr int kStageBytes = 64 * 128 + NB * 16 * 128;
-  static constexpr int kStages = NB <= 2 ? 6 : NB <= 4 ? 5 : 4;
+  static constexpr int kStages = 3;
   static constexpr int kSmemBytes = kStages * kStageBytes + 1024;
 };
 
@@ -148,6 +148,10 @@ __global__ void __launch_bounds__(256) adapters_shrink_rows_kernel(const Adapter
     const T* x = static_cast<const T*>(p.X) + (long long)m * p.ldx;
     const T* w = static_cast<const T*>(p.A) + (long long)a * p.rank * p.K;
     const float scale = p.scales ? p.scales[a] : 1.f;
+    if (p.pieces && (int)threadIdx.x < 2 * (p.rp - p.rank)) {  // zeros beyond the rank
+      const int half = threadIdx.x & 1, r = p.rank + (threadIdx.x >> 1);
+      static_cast<uint16_t*>(p.pieces)[(long long)m * 2 * p.rp + half * p.rp + r] = 0;
+    }
     for (int k0 = 0; k0 < p.K; k0 += kShrinkChunk) {
       const int n = p.K - k0 < kShrinkChunk ? p.K - k0 : kShrinkChunk;
       __syncthreads();
@@ -174,7 +178,19 @@ __global__ void __launch_bounds__(256) adapters_shrink_rows_kernel(const Adapter
         }
         s = scale * warp_sum(s);
         float* h = p.H + (long long)m * p.rank + r;
-        if (lane == 0) *h = k0 ? *h + s : s;
+        if (lane == 0) {
+          if (k0) s += *h;
+          *h = s;
+          if constexpr (sizeof(T) == 2) {
+            if (p.pieces && k0 + n == p.K) {
+              T* q = static_cast<T*>(p.pieces) + (long long)m * 2 * p.rp + r;
+              const uint32_t hi = pack2<T>(s, 0.f);
+              const uint32_t lo = pack2<T>(s - unpack2<T>(hi).x, 0.f);
+              q[0] = *reinterpret_cast<const T*>(&hi);
+              q[p.rp] = *reinterpret_cast<const T*>(&lo);
+            }
+          }
+        }
       }
     }
   }
@@ -228,6 +244,9 @@ AdapterPlan plan_of(const b200_adapters_desc& d) {
   return out;
 }
 
+// Few rows: a CTA for each of them spreads over more SMs than one for every 64 does, at the price of reading A once per row.
+bool shrink_by_rows(const b200_adapters_desc& d) { return (long long)d.M * d.rank * d.K <= 4 << 20; }
+
 template <typename T, int NB>
 cudaError_t launch_shrink_mma(const AdapterParams& p, cudaStream_t s) {
   cudaError_t e = raise_smem_limit<adapters_shrink_mma_kernel<T, NB>>(ShrinkCfg<NB>::kSmemBytes);
@@ -272,8 +291,8 @@ int run_adapters(const b200_adapters_desc& d, cudaStream_t s) {
       B200_CUDA(cudaGetDevice(&dev));
       B200_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
       g.ad_h = p.H;
-      if (plan.piece_bytes && gemm_adapters_pair(g, sms)) g.ad_pieces = p.pieces = ws + plan.h_bytes;
-      if (!plan.mma) B200_CUDA(launch_shrink_rows<T>(p, s));
+      if (plan.piece_bytes) g.ad_pieces = p.pieces = ws + plan.h_bytes;
+      if (!plan.mma || shrink_by_rows(d)) B200_CUDA(launch_shrink_rows<T>(p, s));
       else if (p.rp <= 16) B200_CUDA((launch_shrink_mma<T, 1>(p, s)));
       else if (p.rp <= 32) B200_CUDA((launch_shrink_mma<T, 2>(p, s)));
       else if (p.rp <= 64) B200_CUDA((launch_shrink_mma<T, 4>(p, s)));

@@ -23,9 +23,9 @@
 // beta arrive by bulk copy ahead of the grid dependency.  A LayerNorm vector may span several rows of A (smolgen's
 // second one: 32 heads x 256), as long as a tile holds whole vectors.  Every column tile repeats the LayerNorm: worth it
 // while a launch costs more than that (Net::gemm_with_ln has the line); beyond, ln_rows_kernel does it with the same results.
-// With adapters (kAd) the epilogue adds H[m] . B_a^T in fp32: a thread reads the B rows of its eight columns, which the requests of a
-// tile have or have not in common, so that one row per request costs no more code than 64.  The kernel before this one only
-// writes H, and A and W are loaded and multiplied while it runs.
+// With adapters (kAd) the product takes H . B^T in.  kAdBlocks: as further k-blocks of one CTA of the cluster, like gemm_tc.cu's pair kernel;
+// kAdAdd: a warp per row adds it in fp32 to the sums in shared memory, a lane per column, for requests of any number of rows and
+// operands that TMA cannot read.  The kernel before this one only writes H: A and W are loaded and multiplied while it runs.
 // Every wait is bounded by wall-clock time like those of gemm_tc.cu; the cluster barriers are reached by all threads
 // whatever happened before them.
 #include <atomic>
@@ -163,44 +163,42 @@ ln_rows_kernel(const T* x, T* out, const float* __restrict__ gamma, const float*
   }
 }
 
-// v[i] += H[m] . B_a[col + i]
+enum SplitAdapters { kAdNone = 0, kAdAdd = 1, kAdBlocks = 2 };
+
+// H[m] . B_a[n]
 template <typename T>
-__device__ __forceinline__ void add_adapter(const TcParams& p, int m, int col, float (&v)[8]) {
-  const int a = adapter_of_row(p, m);
-  if (a < 0 || col >= p.N) return;
-  const int rank = p.ad_rank, cols = p.N - col < 8 ? p.N - col : 8;
+__device__ __forceinline__ float adapter_dot(const TcParams& p, int m, int n, int a, bool vec) {
+  const int rank = p.ad_rank;
   const float* h = p.ad_h + (long long)m * rank;
-  const T* b = static_cast<const T*>(p.ad_b) + ((long long)a * p.N + col) * rank;
-  float s[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s[i] = 0.f;
-  if (rank % 8 == 0 && (reinterpret_cast<uintptr_t>(p.ad_b) & 15) == 0) {
+  const T* b = static_cast<const T*>(p.ad_b) + ((long long)a * p.N + n) * rank;
+  float s = 0.f;
+  if (vec) {
+#pragma unroll 2
     for (int r = 0; r < rank; r += 8) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(b + r));
       const float4 h0 = *reinterpret_cast<const float4*>(h + r), h1 = *reinterpret_cast<const float4*>(h + r + 4);
-      const float hh[8] = {h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i >= cols) break;
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(b + i * rank + r));
-        const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[i] = fmaf(hh[j], to_f(e[j]), s[i]);
-      }
+      const T* e = reinterpret_cast<const T*>(&u);
+      s = fmaf(h0.x, to_f(e[0]), fmaf(h0.y, to_f(e[1]), fmaf(h0.z, to_f(e[2]), fmaf(h0.w, to_f(e[3]), s))));
+      s = fmaf(h1.x, to_f(e[4]), fmaf(h1.y, to_f(e[5]), fmaf(h1.z, to_f(e[6]), fmaf(h1.w, to_f(e[7]), s))));
     }
   } else {
-    for (int r = 0; r < rank; ++r) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < cols) s[i] = fmaf(h[r], to_f(b[i * rank + r]), s[i]);
-    }
+    for (int r = 0; r < rank; ++r) s = fmaf(h[r], to_f(b[r]), s);
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] += s[i];
+  return s;
+}
+// One element of a product with adapters from its operands: for those that the tensor core left not finite (see gemm_tc.cu).
+template <typename T>
+__device__ __noinline__ float adapter_element(const T* x, const T* w, int K, const float* h, const T* b, int rank) {
+  float s = 0.f;
+  for (int k = 0; k < K; ++k) s = fmaf(to_f(x[k]), to_f(w[k]), s);
+  for (int r = 0; r < rank; ++r) s = fmaf(h[r], to_f(b[r]), s);
+  return s;
 }
 
-template <typename T, int BN, bool kLN, bool kAd>
+template <typename T, int BN, bool kLN, int kAd>
 __global__ void __launch_bounds__(kSplitThreads)
-gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w, const TcParams p,
+gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
+                  const __grid_constant__ CUtensorMap tmap_h, const __grid_constant__ CUtensorMap tmap_b, const TcParams p,
                   const SplitCfg cfg) {
   constexpr int kMaxStages = 12;
   extern __shared__ uint8_t smem_raw[];
@@ -224,10 +222,21 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   const int k_blocks = (p.K + BK - 1) / BK;
   const int kb0 = k_blocks * rank / ks, kbn = k_blocks * (rank + 1) / ks - kb0;
   const int S = cfg.stages;
+  // kAdBlocks: the adapters of the tile's (at most two) blocks of 64 rows; this CTA has their k-blocks if it is the cluster's first
+  int ad0 = -1, ad1 = -1, ad_blocks = 0;
+  if constexpr (kAd == kAdBlocks) {
+    ad0 = m0 < p.M ? adapter_of_row(p, m0) : -1;
+    ad1 = cfg.a_rows > 64 && m0 + 64 < p.M ? adapter_of_row(p, m0 + 64) : -1;
+    if (rank == 0) ad_blocks = adapter_blocks(p.ad_rp) * ((ad0 >= 0 ? 1 : 0) + (ad1 >= 0 && ad1 != ad0 ? 1 : 0));
+  }
 
   if (tid == 256) {
     tma_prefetch_map(&tmap_w);
     tma_prefetch_map(&tmap_a);
+    if (kAd == kAdBlocks) {
+      tma_prefetch_map(&tmap_h);
+      tma_prefetch_map(&tmap_b);
+    }
     for (int i = 0; i < S; ++i) {
       mbar_init(smem_u32(&full_bar[i]), 1);
       mbar_init(smem_u32(&empty_bar[i]), 1);
@@ -263,7 +272,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     // ---------------- TMA producer ----------------
     if (elect_one()) {
       const int early = kbn < S ? kbn : S;
-      if (!p.w_const && !kAd) grid_dependency_wait();
+      if (!p.w_const && kAd == kAdNone) grid_dependency_wait();
       for (int i = 0; i < early; ++i) {
         const uint32_t fb = smem_u32(&full_bar[i]);
         mbar_expect_tx(fb, kLN ? BN * 128 : stage_bytes);
@@ -275,7 +284,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         bulk_load(smem_u32(ln_gb), cfg.gamma, bytes, gb);
         bulk_load(smem_u32(ln_gb) + bytes, cfg.beta, bytes, gb);
       }
-      if (!kAd) grid_dependency_wait();
+      if (kAd == kAdNone) grid_dependency_wait();
       int s = 0;
       uint32_t ph = 0;
       for (int i = 0; !kLN && i < kbn; ++i) {
@@ -287,6 +296,22 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         }
         tma_load_2d(sa, &tmap_a, (kb0 + i) * BK, m0, fb);
         if (++s == S) { s = 0; ph ^= 1; }
+      }
+      if constexpr (kAd == kAdBlocks) {
+        grid_dependency_wait();
+        const int blocks = adapter_blocks(p.ad_rp);
+        for (int i = 0; i < ad_blocks; ++i) {
+          const int a = i < blocks && ad0 >= 0 ? ad0 : ad1, b = i % blocks;
+          const int kb = blocks == 1 ? 0 : b % (blocks / 2), x = blocks == 1 ? 0 : b / (blocks / 2) * p.ad_rp + kb * BK;
+          const uint32_t fb = smem_u32(&full_bar[s]), sa = smem_u32(smem + s * stage_bytes);
+          if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 1)) break;
+          mbar_expect_tx(fb, stage_bytes);
+          // H of the rows with this adapter; for the others a box behind the last row, which TMA fills with zeros
+          tma_load_2d(sa, &tmap_h, x, ad0 == a ? m0 : p.M, fb);
+          if (cfg.a_rows > 64) tma_load_2d(sa + 64 * 128, &tmap_h, x, ad1 == a ? m0 + 64 : p.M, fb);
+          tma_load_2d(sa + cfg.a_rows * 128, &tmap_b, kb * BK, a * p.N + n0, fb);
+          if (++s == S) { s = 0; ph ^= 1; }
+        }
       }
     }
     __syncwarp();
@@ -305,8 +330,23 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 #pragma unroll
         for (int k = 0; k < BK / 16; ++k)
           tcgen05_mma_f16(tmem, adesc + 2 * k, bdesc + 2 * k, idesc, (i > 0 || k > 0) ? 1u : 0u);
-        if (i + S < kbn) tcgen05_commit(smem_u32(&empty_bar[s]));
+        if (i + S < kbn + ad_blocks) tcgen05_commit(smem_u32(&empty_bar[s]));
         if (++s == S) { s = 0; ph ^= 1; }
+      }
+      if constexpr (kAd == kAdBlocks) {
+        const int blocks = adapter_blocks(p.ad_rp), of_b = p.ad_rp / 16;
+        for (int i = 0; ok && i < ad_blocks; ++i) {
+          if (!mbar_wait(smem_u32(&full_bar[s]), ph, abort_flag, 3)) { ok = false; break; }
+          tcgen05_fence_after();
+          const uint32_t sa = smem_u32(smem + s * stage_bytes);
+          const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + cfg.a_rows * 128);
+          // both pieces of a narrow H meet the same columns of B
+          const int left = blocks == 1 ? 2 * of_b : of_b - i % blocks % (blocks / 2) * 4;
+          for (int k = 0; k < 4 && k < left; ++k)
+            tcgen05_mma_f16(tmem, adesc + 2 * k, bdesc + 2 * (blocks == 1 && k >= of_b ? k - of_b : k), idesc, 1u);
+          if (kbn + i + S < kbn + ad_blocks) tcgen05_commit(smem_u32(&empty_bar[s]));
+          if (++s == S) { s = 0; ph ^= 1; }
+        }
       }
       if (ok) tcgen05_commit(smem_u32(tfull_bar));
     }
@@ -382,6 +422,23 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     tcgen05_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)BN) : "memory");
   }
+  if constexpr (kAd == kAdAdd) {
+    if (warp < 8) {
+      const bool vec = p.ad_rank % 8 == 0 && (reinterpret_cast<uintptr_t>(p.ad_b) & 15) == 0;
+      float* part = reinterpret_cast<float*>(smem);
+#pragma unroll 4
+      for (int r = warp; r < rp; r += 8) {
+        const int m = m0 + rank * rp + r, a = m < p.M ? adapter_of_row(p, m) : -1;
+        if (a < 0) continue;
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) {
+          const int n = c + lane;
+          if (n0 + n < p.N) part[r * BN + ((((n >> 2) ^ (r & 7)) << 2) | (n & 3))] += adapter_dot<T>(p, m, n0 + n, a, vec);
+        }
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+  }
   if (warp < 8) {
     // lanes of this warp that finish the same row; they go through the loop together
     const uint32_t row_lanes = (kGroups == 32 ? 0xffffffffu : ((1u << kGroups) - 1u)) << (lane & ~(kGroups - 1));
@@ -414,8 +471,28 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += vb[i];
       }
-      if constexpr (kAd) {
-        add_adapter<T>(p, m, col, v);
+      if constexpr (kAd != kAdNone) {
+        if constexpr (kAd == kAdBlocks) {
+          float z = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z = fmaf(v[i], 0.f, z);
+          if (z != 0.f) {
+            const int a = adapter_of_row(p, m);
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) {
+              const int n = col + i;
+              float again = 0.f;
+              if (n < p.N)
+                again = adapter_element<T>(static_cast<const T*>(p.a) + m * p.lda, static_cast<const T*>(p.w) + n * p.ldw, p.K,
+                                           p.ad_h + (long long)m * p.ad_rank,
+                                           static_cast<const T*>(p.ad_b) + ((long long)a * p.N + n) * p.ad_rank, a < 0 ? 0 : p.ad_rank) +
+                        (p.bias ? __ldg(p.bias + n) : 0.f);
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (j == i) v[j] = again;
+            }
+          }
+        }
         if (p.out_f32) {  // 16-bit results hide what the fast forms round, fp32 ones do not
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = activate<false>(v[i], p.act);
@@ -547,7 +624,7 @@ SplitPlan split_plan(const GemmParams& g, int sm_count) {
   return best;
 }
 
-template <typename T, int BN, bool kLN = false, bool kAd = false>
+template <typename T, int BN, bool kLN = false, int kAd = kAdNone>
 cudaError_t launch_split_bn(const GemmParams& g, const SplitPlan& plan, int* status, cudaStream_t s) {
   static std::atomic<unsigned long long> attr_mask{0};
   int dev = 0;
@@ -563,6 +640,11 @@ cudaError_t launch_split_bn(const GemmParams& g, const SplitPlan& plan, int* sta
   CUtensorMap ma, mw;
   if ((e = gemm_tensor_map(g.A, g.lda, g.M, g.K, plan.a_rows, prec, &ma)) != cudaSuccess) return e;
   if ((e = gemm_tensor_map(g.W, g.ldw, g.N, g.K, BN, prec, &mw)) != cudaSuccess) return e;
+  CUtensorMap mh = ma, mb = mw;
+  if (kAd == kAdBlocks) {
+    if ((e = gemm_tensor_map(g.ad_pieces, 2 * g.ad_rp, g.M, 2 * g.ad_rp, 64, prec, &mh)) != cudaSuccess) return e;
+    if ((e = gemm_tensor_map(g.ad_b, g.ad_rank, g.ad_n * g.N, g.ad_rank, BN, prec, &mb)) != cudaSuccess) return e;
+  }
   TcParams p;
   fill_tc_params(p, g, status);
   const SplitCfg cfg{plan.stages, plan.a_rows, plan.ks, g.A, g.ln_gamma, g.ln_beta, g.ln_group, g.ln_eps};
@@ -587,7 +669,7 @@ cudaError_t launch_split_bn(const GemmParams& g, const SplitPlan& plan, int* sta
   }
   lc.attrs = attr;
   lc.numAttrs = na;
-  return cudaLaunchKernelEx(&lc, gemm_split_kernel<T, BN, kLN, kAd>, ma, mw, p, cfg);
+  return cudaLaunchKernelEx(&lc, gemm_split_kernel<T, BN, kLN, kAd>, ma, mw, mh, mb, p, cfg);
 }
 
 }  // namespace
@@ -620,10 +702,19 @@ template cudaError_t launch_gemm_ln<__nv_bfloat16>(const GemmParams&, int*, cuda
 template <typename T>
 cudaError_t launch_gemm_split(const GemmParams& g, int* status, int sm_count, cudaStream_t s) {
   const SplitPlan plan = split_plan(g, sm_count);
+  if (g.ad_ids && g.ad_pieces) {
+    SplitPlan with = plan;  // stages for the adapters' k-blocks too, within the same ring
+    with.stages += (plan.a_rows / 64) * adapter_blocks(g.ad_rp);
+    const int cap = 96 * 1024 / ((plan.a_rows + plan.bn) * 128);
+    if (with.stages > cap) with.stages = cap;
+    if (plan.bn == 32) return launch_split_bn<T, 32, false, kAdBlocks>(g, with, status, s);
+    if (plan.bn == 64) return launch_split_bn<T, 64, false, kAdBlocks>(g, with, status, s);
+    return launch_split_bn<T, 128, false, kAdBlocks>(g, with, status, s);
+  }
   if (g.ad_ids) {
-    if (plan.bn == 32) return launch_split_bn<T, 32, false, true>(g, plan, status, s);
-    if (plan.bn == 64) return launch_split_bn<T, 64, false, true>(g, plan, status, s);
-    return launch_split_bn<T, 128, false, true>(g, plan, status, s);
+    if (plan.bn == 32) return launch_split_bn<T, 32, false, kAdAdd>(g, plan, status, s);
+    if (plan.bn == 64) return launch_split_bn<T, 64, false, kAdAdd>(g, plan, status, s);
+    return launch_split_bn<T, 128, false, kAdAdd>(g, plan, status, s);
   }
   if (plan.bn == 32) return launch_split_bn<T, 32>(g, plan, status, s);
   if (plan.bn == 64) return launch_split_bn<T, 64>(g, plan, status, s);

@@ -108,8 +108,6 @@ struct TileAdapters {
     return f;
   }
 };
-// k-blocks of an adapter: H's two pieces side by side where both fit one, else each in blocks of 64.
-__device__ __forceinline__ int adapter_blocks(int rp) { return rp <= 32 ? 1 : 2 * ((rp + 63) / 64); }
 
 // One 64-column slab of the epilogue fast path, executed by one group of four warps: TMEM -> registers ->
 // scale / folded-LayerNorm correction / bias / activation / residual -> 128B-swizzled staging buffer, which the
@@ -2029,7 +2027,6 @@ bool pair_eligible(const GemmParams& p, int sm_count) {
 bool gemm_adapters_pieces(const GemmParams& p) {
   return p.ad_group % 64 == 0 && p.ad_rank % 8 == 0 && (long long)p.ad_n * p.N < 0x7fffff00 && (reinterpret_cast<uintptr_t>(p.ad_b) & 15) == 0;
 }
-bool gemm_adapters_pair(const GemmParams& p, int sm_count) { return gemm_adapters_pieces(p) && pair_eligible(p, sm_count); }
 
 bool gemm_tc_split_supported(const GemmParams& p) {
   if (!gemm_tc_supported(p) || p.n_split <= 0 || p.N <= p.n_split || !p.C2 || (p.ldc2 % 8) != 0 ||
@@ -2158,7 +2155,7 @@ cudaError_t launch_gemm_tc(const GemmParams& p, int* status, int sm_count, cudaS
   if (p.ad_ids) {
     if (p.conv_cin > 0 || p.batch_rows > 0 || p.a_stats || p.res || p.out_stats || p.n_split > 0 || p.scale != 1.0f || !p.ad_h)
       return cudaErrorInvalidValue;
-    return p.ad_pieces ? launch_pair<T>(p, status, sm_count, s) : launch_gemm_split<T>(p, status, sm_count, s);
+    return p.ad_pieces && pair_eligible(p, sm_count) ? launch_pair<T>(p, status, sm_count, s) : launch_gemm_split<T>(p, status, sm_count, s);
   }
   if (pair_eligible(p, sm_count)) return launch_pair<T>(p, status, sm_count, s);
   if (p.se_k > 0) return launch_bn<T, 256>(p, status, sm_count, s);  // the tile must hold every channel of two boards

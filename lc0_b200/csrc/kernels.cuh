@@ -75,7 +75,7 @@ struct GemmParams {
   int ln_group = 1;
   float ln_eps = 0.f;
   // Low-rank adapters (tensor-core kernels): rows [i * ad_group, (i + 1) * ad_group) add H[m] . B[ids[i]]^T ahead of the
-  // activation, ad_h [M][ad_rank] fp32, ad_b [ad_n][N][ad_rank].  ad_pieces (CTA-pair kernel): H as two values of the storage type,
+  // activation, ad_h [M][ad_rank] fp32, ad_b [ad_n][N][ad_rank].  ad_pieces: H as two values of the storage type,
   // [M][2 * ad_rp] with the first in columns [0, ad_rp) and the second behind, zeros beyond ad_rank.  H is written by the launch just
   // before this one, A, W and the ids by launches before that.
   const int* ad_ids = nullptr;
@@ -92,10 +92,9 @@ template <typename T> cudaError_t launch_gemm_fma(const GemmParams& p, cudaStrea
 // `status` is a device int the kernel sets non-zero when a bounded wait gives up.
 template <typename T> cudaError_t launch_gemm_tc(const GemmParams& p, int* status, int sm_count, cudaStream_t s);
 bool gemm_tc_supported(const GemmParams& p);
-// Whether adapters can go into the CTA-pair kernel as further k-blocks, which needs ad_pieces (every 64 rows one request's, B as TMA
-// reads it), and whether it takes this product.  Without ad_pieces launch_gemm_tc adds them in the epilogue of gemm_split.cu's kernel.
+// Whether adapters can be further k-blocks, which needs ad_pieces: every 64 rows one request's, B as TMA reads it.  Without ad_pieces
+// launch_gemm_tc adds them in the epilogue of gemm_split.cu's kernel.
 bool gemm_adapters_pieces(const GemmParams& p);
-bool gemm_adapters_pair(const GemmParams& p, int sm_count);
 // Product with the LayerNorm of its input in front (gemm_split.cu), for few rows.
 bool gemm_ln_supported(const GemmParams& p);
 template <typename T> cudaError_t launch_gemm_ln(const GemmParams& p, int* status, cudaStream_t s);

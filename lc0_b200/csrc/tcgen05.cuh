@@ -336,6 +336,9 @@ __device__ __forceinline__ int adapter_of_row(const TcParams& p, int m) {
   return a >= 0 && a < p.ad_n ? a : -1;
 }
 
+// k-blocks of an adapter: H's two pieces side by side where both fit one, else each in blocks of 64.
+__host__ __device__ __forceinline__ int adapter_blocks(int rp) { return rp <= 32 ? 1 : 2 * ((rp + 63) / 64); }
+
 // Epilogue parameters of a product that are the same for every kernel.
 inline void fill_tc_params(TcParams& p, const GemmParams& g, int* status) {
   p.bias = g.bias; p.C = g.C; p.ldc = g.ldc;
