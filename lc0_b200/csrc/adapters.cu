@@ -197,23 +197,67 @@ __global__ void __launch_bounds__(256) adapters_shrink_rows_kernel(const Adapter
 }
 
 // ---- fp32 sums + H B^T ------------------------------------------------------------------------------------------
+// A warp has 32 columns of 8 rows: eight ranks of a lane's row of B stay in registers for as many rows as have that adapter, H is the
+// same for the whole warp.  Sums are read and results written as whole lines.
+constexpr int kExpandRows = 8;
+
 template <typename T>
-__global__ void __launch_bounds__(256) adapters_expand_kernel(const AdapterParams p) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= p.N) return;
-  for (int m = blockIdx.y; m < p.M; m += gridDim.y) {
-    float v = p.acc[(long long)m * p.ldacc + n];
-    const int a = adapter_of(p, m);
-    if (a >= 0) {
-      const T* b = static_cast<const T*>(p.B) + ((long long)a * p.N + n) * p.rank;
-      const float* h = p.H + (long long)m * p.rank;
-      float s = 0.f;
-      for (int r = 0; r < p.rank; ++r) s = fmaf(h[r], to_f(b[r]), s);
-      v += s;
+__global__ void __launch_bounds__(256) adapters_expand_kernel(const AdapterParams p, int vec) {
+  grid_dependency_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = blockIdx.x * 64 + (warp & 1) * 32 + lane;
+  const bool mine = n < p.N;
+  for (long long m0 = ((long long)blockIdx.y * 4 + (warp >> 1)) * kExpandRows; m0 < p.M; m0 += (long long)gridDim.y * 4 * kExpandRows) {
+    int a[kExpandRows];
+    float v[kExpandRows], d[kExpandRows];
+#pragma unroll
+    for (int i = 0; i < kExpandRows; ++i) {
+      const long long m = m0 + i;
+      a[i] = m < p.M ? adapter_of(p, (int)m) : -1;
+      v[i] = mine && m < p.M ? p.acc[m * p.ldacc + n] : 0.f;
+      d[i] = 0.f;
     }
-    v = p.out_f32 ? activate<false>(v, p.act) : activate<true>(v, p.act);
-    if (p.out_f32) static_cast<float*>(p.C)[(long long)m * p.ldc + n] = v;
-    else static_cast<T*>(p.C)[(long long)m * p.ldc + n] = from_f<T>(v);
+    for (int r0 = 0; r0 < p.rank; r0 += 8) {
+      float b[8];
+#pragma unroll
+      for (int i = 0; i < kExpandRows; ++i) {
+        if (a[i] < 0) continue;
+        if (i == 0 || a[i] != a[i - 1]) {
+          const T* src = static_cast<const T*>(p.B) + ((long long)a[i] * p.N + (mine ? n : 0)) * p.rank + r0;
+          if (vec) {  // a multiple of eight ranks on 16-byte boundaries
+            constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+            for (int j = 0; j < 8; j += kPer) {
+              const uint4 u = __ldg(reinterpret_cast<const uint4*>(src + j));
+              const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+              for (int q = 0; q < kPer; ++q) b[j + q] = to_f(e[q]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[j] = r0 + j < p.rank ? to_f(src[j]) : 0.f;
+          }
+        }
+        const float* h = p.H + (m0 + i) * p.rank + r0;
+        if (vec) {
+          const float4 h0 = *reinterpret_cast<const float4*>(h), h1 = *reinterpret_cast<const float4*>(h + 4);
+          d[i] = fmaf(h0.x, b[0], fmaf(h0.y, b[1], fmaf(h0.z, b[2], fmaf(h0.w, b[3], d[i]))));
+          d[i] = fmaf(h1.x, b[4], fmaf(h1.y, b[5], fmaf(h1.z, b[6], fmaf(h1.w, b[7], d[i]))));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (r0 + j < p.rank) d[i] = fmaf(h[j], b[j], d[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kExpandRows; ++i) {
+      const long long m = m0 + i;
+      if (!mine || m >= p.M) continue;
+      const float x = v[i] + d[i], y = p.out_f32 ? activate<false>(x, p.act) : activate<true>(x, p.act);
+      if (p.out_f32) static_cast<float*>(p.C)[m * p.ldc + n] = y;
+      else static_cast<T*>(p.C)[m * p.ldc + n] = from_f<T>(y);
+    }
   }
 }
 
@@ -306,9 +350,12 @@ int run_adapters(const b200_adapters_desc& d, cudaStream_t s) {
   g.C = acc; g.ldc = plan.acc_bytes ? d.N : g.ldc; g.out_f32 = true; g.act = ACT_NONE; g.ad_ids = nullptr;
   p.acc = static_cast<const float*>(acc); p.ldacc = g.ldc;
   B200_CUDA(launch_shrink_rows<T>(p, s));
+  DependentScope dependent;
   B200_CUDA(launch_gemm_fma<T>(g, s));
-  adapters_expand_kernel<T><<<dim3(ceil_div(d.N, 256), d.M < 32768 ? d.M : 32768), 256, 0, s>>>(p);
-  B200_CUDA(cudaGetLastError());
+  const int row_blocks = ceil_div(d.M, 4 * kExpandRows);
+  const int vec = d.rank % 8 == 0 && aligned16(d.B);
+  B200_CUDA(launch_dependent(adapters_expand_kernel<T>, dim3(ceil_div(d.N, 64), row_blocks < 65535 ? row_blocks : 65535), dim3(256), 0, s, p,
+                             vec));
   return B200_OK;
 }
 
