@@ -483,24 +483,22 @@ template <int kThreads> struct Row {
     float l[kEach];
     int slot[kEach];
     W w[kEach];
-    int base = 0, held = kThreads == kWide && g.cluster > 1 ? 0 : n;
+    const bool parts = kThreads == kWide && g.cluster > 1;  // a list in each CTA of the cluster, one behind the other
+    const int own = parts && lane < g.cluster ? *cg::this_cluster().map_shared_rank(&sh.count, lane) : 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
+      int at = 32 * i + lane, cta = 0;
+      const bool there = at < n;
+      if (parts)
+        for (int c = 0; c < g.cluster - 1; ++c) {
+          const int nc = __shfl_sync(0xffffffffu, own, c);
+          if (cta == c && at >= nc) { at -= nc; ++cta; }
+        }
       l[i] = -INFINITY;
       slot[i] = 0;
-      if (32 * i + lane < held) { l[i] = sh.list_l[32 * i + lane]; slot[i] = sh.list_slot[32 * i + lane]; }
-    }
-    if (kThreads == kWide && g.cluster > 1) {
-      for (int c = 0; c < g.cluster; ++c) {
-        const int nc = *cg::this_cluster().map_shared_rank(&sh.count, c);
-        const float* ll = cg::this_cluster().map_shared_rank(sh.list_l, c);
-        const int* ls = cg::this_cluster().map_shared_rank(sh.list_slot, c);
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-          const int at = 32 * i + lane - base;
-          if (at >= 0 && at < nc) { l[i] = ll[at]; slot[i] = ls[at]; }
-        }
-        base += nc;
+      if (there) {
+        l[i] = parts ? cg::this_cluster().map_shared_rank(sh.list_l, cta)[at] : sh.list_l[at];
+        slot[i] = parts ? cg::this_cluster().map_shared_rank(sh.list_slot, cta)[at] : sh.list_slot[at];
       }
     }
 #pragma unroll
@@ -573,7 +571,7 @@ template <int kThreads> struct Row {
   // the place are sums of quick weights with a margin; what decides is the exact measure above and the sorted entries.  (Counting
   // in bins instead: an addition to shared memory took 64 cycles per warp, twice what the pivots take.)
   // False: a comparison was open.
-  template <typename W, bool kMass> __device__ bool select(double target, float hi, float least, double slack, Cut& out) {
+  template <typename W, bool kMass> __device__ bool select(int n_row, double target, float hi, float least, double slack, Cut& out) {
     constexpr bool kOpen = kMass && sizeof(W) == 4;
     const int tid = kThreads == 32 ? g.lane : (int)threadIdx.x;
     float lo = -INFINITY, reach_lo = 0.f, reach_hi = 0.f;  // found above them (lo: all, where it is infinite)
@@ -616,7 +614,7 @@ template <int kThreads> struct Row {
       const float parts[3] = {0.875f * f, f + 0.015625f * (1.f - f), f + 0.125f * (1.f - f)};
 #pragma unroll
       for (int j = 0; j < 3; ++j) x[j] = hi - parts[j] * width;
-      if (!(most_here <= (float)kList) && round < 5) continue;
+      if (!(most_here <= (float)kList) && n_row > kList && round < 5) continue;
       // the exact measure above them, and the entries between them, marked 32 at a time
       g.barrier();  // the others are done with what is cleared
       if (tid == 0) sh.count = 0;
@@ -655,8 +653,8 @@ template <int kThreads> struct Row {
       const double front = g.sum(more);
       int n = sh.count;
       if (kThreads == kWide && g.cluster > 1) {
-        n = 0;
-        for (int c = 0; c < g.cluster; ++c) n += *cg::this_cluster().map_shared_rank(&sh.count, c);
+        n = g.lane < g.cluster ? *cg::this_cluster().map_shared_rank(&sh.count, g.lane) : 0;
+        n = __reduce_add_sync(0xffffffffu, n);
       }
       if (n == 0 || front >= target) break;
       if (n > kList) {
@@ -823,7 +821,7 @@ template <int kThreads> struct Row {
   // k-th of them for small k, one of the least else, which more than k entries reach nearly always; from there a bisection over the
   // gathered entries goes on.  Number of entries, 0 if
   // that found none or too many.
-  __device__ int gather_top(int k, float lane_max) {
+  __device__ int gather_top(int n_row, int k, float lane_max) {
     const int lane = g.lane;
     float s = lane_max;
 #pragma unroll
@@ -833,7 +831,8 @@ template <int kThreads> struct Row {
         const float o = __shfl_xor_sync(0xffffffffu, s, j);
         s = ((lane & j) == 0) == ((lane & kk) == 0) ? fmaxf(s, o) : fminf(s, o);
       }
-    const float floor_l = __shfl_sync(0xffffffffu, s, k <= 24 ? k - 1 : k <= 40 ? 28 : 30);  // (the last run may be empty)
+    float floor_l = __shfl_sync(0xffffffffu, s, k <= 24 ? k - 1 : k <= 40 ? 28 : 30);  // (the last run may be empty)
+    if (n_row <= kList) floor_l = -3.402823466e38f;
     if (floor_l == -INFINITY) return 0;
     uint32_t hits_lo = 0, hits_hi = 0;
 #pragma unroll 4
@@ -852,14 +851,15 @@ template <int kThreads> struct Row {
       if (lane >= o) in += up;
     }
     int n = __shfl_sync(0xffffffffu, in, 31);
-    if (n > kList || n < k) return 0;
+    if (n > kList || (n < k && n_row > kList)) return 0;
     for (int pos = in - own; hits; hits &= hits - 1, ++pos) {
       const int i = __ffsll((long long)hits) - 1;
       sh.list_l[pos] = mine[i];
       sh.list_slot[pos] = slot0 + i;
     }
     __syncwarp();
-    if (n <= kSort) return n;
+    const int room = k <= 32 ? 32 : kSort;  // half as many are sorted in less than half the steps
+    if (n <= room || (n <= kSort && n <= k)) return n;
     float l[kList / 32];
     int slot[kList / 32];
 #pragma unroll
@@ -867,7 +867,7 @@ template <int kThreads> struct Row {
       l[i] = 32 * i + lane < n ? sh.list_l[32 * i + lane] : -INFINITY;
       slot[i] = 32 * i + lane < n ? sh.list_slot[32 * i + lane] : 0;
     }
-    uint32_t lo = key_of(floor_l), hi = key_of(wt.max) + 1;  // more than 64 reach lo, fewer than k reach hi
+    uint32_t lo = key_of(floor_l), hi = key_of(wt.max) + 1;  // too many reach lo, fewer than k reach hi
     float at = 0.f;
     bool found = false;
     while (hi - lo > 1 && !found) {
@@ -877,11 +877,11 @@ template <int kThreads> struct Row {
 #pragma unroll
       for (int i = 0; i < kList / 32; ++i) c += l[i] >= at;
       c = __reduce_add_sync(0xffffffffu, c);
-      if (c > kSort) lo = mid;
+      if (c > room) lo = mid;
       else if (c < k) hi = mid;
       else found = true;
     }
-    if (!found) return 0;  // equal entries
+    if (!found) return n <= kSort ? n : 0;  // equal entries
     __syncwarp();
     n = 0;
 #pragma unroll
@@ -949,7 +949,7 @@ sample_kernel(const SampleParams p) {
         r.finish(v + first, nullptr, first, n, k, tp, p_min, u);
         done = true;
       } else if (k > 0 && k <= kSort) {
-        const int few = r.gather_top(k, own_max);
+        const int few = r.gather_top(n, k, own_max);
         if (few) {
           r.finish(sh.list_l, sh.list_slot, 0, few, k, tp, p_min, u);
           done = true;
@@ -968,12 +968,12 @@ sample_kernel(const SampleParams p) {
         });
         if ((double)k < g.sum((double)own)) {
           least = -g.max(-least);
-          r.template select<float, false>((double)k, m, least, 0.0, cut);
+          r.template select<float, false>(n, (double)k, m, least, 0.0, cut);
           if (tp < 1.f) r.keep(cut);
         }
       }
       if (tp < 1.f) {
-        if (!fp32 || !r.template select<float, true>((double)tp, m, 0.f, slack, cut)) r.template select<double, true>((double)tp, m, 0.f, 0.0, cut);
+        if (!fp32 || !r.template select<float, true>(n, (double)tp, m, 0.f, slack, cut)) r.template select<double, true>(n, (double)tp, m, 0.f, 0.0, cut);
       }
       if (!fp32 || !r.template draw<float>(cut, p_min, u, slack)) r.template draw<double>(cut, p_min, u, 0.0);
     }
