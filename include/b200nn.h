@@ -427,7 +427,7 @@ int b200_op_gemm_adapters(const b200_adapters_desc* d, void* stream);
  *   keeps the first k; top_p those ahead of which the weights of what top_k kept sum to less than top_p of their total, and the
  *   first; min_p those with w >= min_p.  choice: the first kept entry, by index, at which the sum of the kept weights passes
  *   u times their total: its column, or its place in the list of moves.  prob (may be NULL): its weight over that total.
- *   -1 and 0 for a row without entries.
+ *   -1 and 0 for a row without entries; -2 where a bounded device-side wait gave up (rows of more than 9000 entries, a defect).
  *   The choice is the one that sums in 64 bits give.  Allocates nothing, does not synchronise, may be captured. */
 #define B200_SAMPLE_MAX_WIDTH 262144
 typedef struct b200_sample_desc {

@@ -35,7 +35,7 @@ struct SampleParams {
   const float* temperature; const int* top_k; const float* top_p; const float* min_p; const float* u;
   int* choice; float* prob;
   int pieces;   // 16-byte pieces per thread, odd
-  int cluster;  // CTAs per row (kThreads == kWide)
+  int cluster;  // CTAs per row (kCluster)
   float slack;  // bound of a sum's error, relative to the sum of all weights
 };
 
@@ -47,36 +47,81 @@ __device__ __forceinline__ uint32_t key_of(float v) {
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 // The threads of a row: sums, maxima and prefix sums over them in a fixed order.
-template <int kThreads> struct Group {
+template <int kThreads, bool kCluster> struct Group {
   static constexpr int kWarps = kThreads / 32;
-  static constexpr int kSlots = kThreads == kWide ? kMaxCluster * kWarps : kWarps;
+  static constexpr int kSlots = kCluster ? kMaxCluster * kWarps : kWarps;
   double* slots;  // [2][kSlots], kThreads > 32
   float* wide;    // [2][kSlots][4]
+  uint64_t* bars;  // [2], kCluster
   int cluster, crank, turn;
+  bool gave_up;   // a wait for the other CTAs has ended without them
   int lane, warp;
-  __device__ Group(double* s, float* s8, int cl) : slots(s), wide(s8), cluster(kThreads == kWide ? cl : 1), crank(0), turn(0) {
+  __device__ Group(double* s, float* s4, uint64_t* b, int cl) : slots(s), wide(s4), bars(b), cluster(kCluster ? cl : 1), crank(0), turn(0), gave_up(false) {
     lane = threadIdx.x & 31;
     warp = kThreads == 32 ? 0 : threadIdx.x >> 5;
-    if (kThreads == kWide && cluster > 1) crank = (int)cg::this_cluster().block_rank();
+    if (kCluster) {
+      crank = (int)cg::this_cluster().block_rank();
+      if (threadIdx.x < 2) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(address(bars + threadIdx.x)) : "memory");
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");  // (the row is read, and a barrier passed, before their first use)
+    }
+  }
+  static __device__ __forceinline__ uint32_t address(const void* q) { return (uint32_t)__cvta_generic_to_shared(q); }
+  static __device__ __forceinline__ uint32_t address(const void* q, int cta) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(address(q)), "r"(cta));
+    return a;
+  }
+  // The CTAs of a cluster hand values around by stores that count themselves in at the receiver's barrier: 2 k cycles less per exchange
+  // than a cluster barrier, which waits for all the memory traffic of the threads that arrive.  `bytes`: what a CTA receives this turn.
+  __device__ __forceinline__ void expect(int bytes) const {
+    if (threadIdx.x == 0)
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(address(bars + (turn & 1))), "r"(bytes) : "memory");
+  }
+  __device__ __forceinline__ void await() {
+    const uint32_t bar = address(bars + (turn & 1)), parity = turn >> 1 & 1;
+    unsigned long long t0 = 0;
+    for (int it = 0; !gave_up; ++it) {
+      uint32_t ok;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(bar), "r"(parity), "r"(20000u)
+          : "memory");
+      if (ok) break;
+      if ((it & 63) == 63) {
+        unsigned long long now;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+        if (t0 == 0) t0 = now;
+        gave_up = now - t0 > 2000000000ull;  // 2 s
+      }
+    }
+    ++turn;
   }
   __device__ __forceinline__ int thread() const { return (crank * kWarps + warp) * 32 + lane; }
   __device__ __forceinline__ int threads() const { return cluster * kThreads; }
   __device__ __forceinline__ void barrier() const {
     if (kThreads == 32) __syncwarp();
-    else if (kThreads == kWide && cluster > 1) cg::this_cluster().sync();
+    else if (kCluster) cg::this_cluster().sync();
     else __syncthreads();
   }
   // One value per warp, seen by all threads of the group afterwards.  Two sets of slots in turn: the barrier of one exchange
   // lies between the reads of the last and the writes of the next.
   __device__ __forceinline__ const double* gather(double v) {
     double* mine = slots + (turn & 1) * kSlots;
-    ++turn;
-    if (kThreads == kWide && cluster > 1) {
-      if (lane < cluster) *cg::this_cluster().map_shared_rank(mine + crank * kWarps + warp, lane) = v;
-    } else if (lane == 0) {
-      mine[warp] = v;
+    if (kCluster) {
+      expect(cluster * kWarps * 8);
+      if (lane < cluster)
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(address(mine + crank * kWarps + warp, lane)),
+                     "l"(__double_as_longlong(v)), "r"(address(bars + (turn & 1), lane))
+                     : "memory");
+      await();
+      return mine;
     }
-    barrier();
+    ++turn;
+    if (lane == 0) mine[warp] = v;
+    __syncthreads();
     return mine;
   }
   __device__ __forceinline__ double sum(double v) {
@@ -113,14 +158,19 @@ template <int kThreads> struct Group {
     for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (kThreads > 32) {
       float* mine = wide + (turn & 1) * kSlots * 4;
-      ++turn;
       const int at = (crank * kWarps + warp) * 4 + (lane >> 3);
-      if (kThreads == kWide && cluster > 1) {
-        if ((lane & 7) < cluster) *cg::this_cluster().map_shared_rank(mine + at, lane & 7) = v;
-      } else if ((lane & 7) == 0) {
-        mine[at] = v;
+      if (kCluster) {
+        expect(cluster * kWarps * 16);
+        if ((lane & 7) < cluster)
+          asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(address(mine + at, lane & 7)),
+                       "r"(__float_as_uint(v)), "r"(address(bars + (turn & 1), lane & 7))
+                       : "memory");
+        await();
+      } else {
+        ++turn;
+        if ((lane & 7) == 0) mine[at] = v;
+        __syncthreads();
       }
-      barrier();
       v = 0.f;
       for (int w = lane & 7; w < cluster * kWarps; w += 8) v += mine[w * 4 + (lane >> 3)];
 #pragma unroll
@@ -271,8 +321,8 @@ template <> struct Pieces<__nv_bfloat16> {
 // A row's entries into shared memory; slot `first` + i holds entry i, -inf where there is none.  Whole 16-byte pieces of memory are read
 // with one load, eight of a thread on their way at a time, those that reach beyond the row entry by entry.  (NaN stays: every
 // comparison that would take it in is false, and its weight is 0.)
-template <typename T, int kThreads>
-__device__ int load_row(const SampleParams& p, const Group<kThreads>& g, int row, float* v, int cap, int& n) {
+template <typename T, int kThreads, bool kCluster>
+__device__ int load_row(const SampleParams& p, const Group<kThreads, kCluster>& g, int row, float* v, int cap, int& n) {
   const T* src = static_cast<const T*>(p.logits) + (long long)row * p.ld;
   const int base = g.crank * cap;  // this CTA holds slots [base, base + cap)
   const int tid = kThreads == 32 ? g.lane : (int)threadIdx.x;
@@ -334,12 +384,13 @@ struct Cut {
 constexpr int kSort = 64;    // entries that a warp sorts
 constexpr int kList = 256;   // entries between two logits that are solved by a warp
 
-template <int kThreads> struct Shared {
-  double slots[2 * Group<kThreads>::kSlots];
-  float wide[kThreads == 32 ? 1 : 2 * Group<kThreads>::kSlots * 4];
+template <int kThreads, bool kCluster> struct Shared {
+  double slots[2 * Group<kThreads, kCluster>::kSlots];
+  float wide[kThreads == 32 ? 1 : 2 * Group<kThreads, kCluster>::kSlots * 4];
   float list_l[kList];
   int list_slot[kList];
   uint64_t sorted[32];
+  uint64_t bars[2];
   double ahead;
   int count;
   int solved;
@@ -391,9 +442,9 @@ __device__ __forceinline__ double warp_before(double v, double& total, int lane)
 }
 
 // A row in shared memory, seen by one thread of its group.
-template <int kThreads> struct Row {
-  Group<kThreads>& g;
-  Shared<kThreads>& sh;
+template <int kThreads, bool kCluster> struct Row {
+  Group<kThreads, kCluster>& g;
+  Shared<kThreads, kCluster>& sh;
   const SampleParams& p;
   float* mine;   // this thread's entries
   int slot0;     // slot of the first of them
@@ -483,10 +534,13 @@ template <int kThreads> struct Row {
     float l[kEach];
     int slot[kEach];
     W w[kEach];
-    const bool parts = kThreads == kWide && g.cluster > 1;  // a list in each CTA of the cluster, one behind the other
+    const bool parts = kCluster;  // a list in each CTA of the cluster, one behind the other
     const int own = parts && lane < g.cluster ? *cg::this_cluster().map_shared_rank(&sh.count, lane) : 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
+      l[i] = -INFINITY;
+      slot[i] = 0;
+      if (32 * i >= n) continue;
       int at = 32 * i + lane, cta = 0;
       const bool there = at < n;
       if (parts)
@@ -494,8 +548,6 @@ template <int kThreads> struct Row {
           const int nc = __shfl_sync(0xffffffffu, own, c);
           if (cta == c && at >= nc) { at -= nc; ++cta; }
         }
-      l[i] = -INFINITY;
-      slot[i] = 0;
       if (there) {
         l[i] = parts ? cg::this_cluster().map_shared_rank(sh.list_l, cta)[at] : sh.list_l[at];
         slot[i] = parts ? cg::this_cluster().map_shared_rank(sh.list_slot, cta)[at] : sh.list_slot[at];
@@ -571,10 +623,14 @@ template <int kThreads> struct Row {
   // the place are sums of quick weights with a margin; what decides is the exact measure above and the sorted entries.  (Counting
   // in bins instead: an addition to shared memory took 64 cycles per warp, twice what the pivots take.)
   // False: a comparison was open.
-  template <typename W, bool kMass> __device__ bool select(int n_row, double target, float hi, float least, double slack, Cut& out) {
+  // `lo_at`, `hi_at`: the two logits, from a call that left a comparison open to one in 64 bits (hi_at = infinity: none yet).
+  template <typename W, bool kMass>
+  __device__ bool select(int n_row, double target, float hi, float least, double slack, float& lo_at, float& hi_at, Cut& out) {
     constexpr bool kOpen = kMass && sizeof(W) == 4;
     const int tid = kThreads == 32 ? g.lane : (int)threadIdx.x;
     float lo = -INFINITY, reach_lo = 0.f, reach_hi = 0.f;  // found above them (lo: all, where it is infinite)
+    const bool known = hi_at < INFINITY;
+    if (known) { lo = lo_at; hi = hi_at; }
     double all = 0.0;
     float x[3];
     {
@@ -592,21 +648,23 @@ template <int kThreads> struct Row {
         a[3] += l > -INFINITY ? w : 0.f;
       };
       if (kMass && round == 0) {
-        all = sum<W, true>([&](int, float l, W w) -> W { pivots(l, (float)w); return w; });
+        if (known) all = sum<W, true>([&](int, float, W w) -> W { return w; });
+        else all = sum<W, true>([&](int, float l, W w) -> W { pivots(l, (float)w); return w; });
         all = g.sum(all);
         target *= all;
       } else {
         each([&](int, float l) { pivots(l, kMass ? wt.quick(l) : 1.f); });
       }
-      g.sum4(a);
+      const bool looked = !(known && round == 0);
+      if (looked) g.sum4(a);
       if (round == 0) reach_lo = a[3];
       const float goal = (float)target, margin = kMass ? 1e-5f * (float)all : 0.f;
 #pragma unroll
       for (int j = 0; j < 3; ++j)
-        if (x[j] < hi && a[j] < goal - margin) { hi = x[j]; reach_hi = a[j]; }
+        if (looked && x[j] < hi && a[j] < goal - margin) { hi = x[j]; reach_hi = a[j]; }
 #pragma unroll
       for (int j = 2; j >= 0; --j)
-        if (x[j] > lo && x[j] < hi && a[j] >= goal + margin) { lo = x[j]; reach_lo = a[j]; }
+        if (looked && x[j] > lo && x[j] < hi && a[j] >= goal + margin) { lo = x[j]; reach_lo = a[j]; }
       // entries between the two, as many as there would be if all were as light as the lower end
       const float most_here = (reach_lo - reach_hi + margin) / (kMass ? fmaxf(wt.quick(lo), 1e-30f) : 1.f);
       const float low = lo > -INFINITY ? lo : kMass ? fmaxf(hi - 16.f * wt.temp, -3.4e38f) : fminf(least, hi);
@@ -614,7 +672,9 @@ template <int kThreads> struct Row {
       const float parts[3] = {0.875f * f, f + 0.015625f * (1.f - f), f + 0.125f * (1.f - f)};
 #pragma unroll
       for (int j = 0; j < 3; ++j) x[j] = hi - parts[j] * width;
-      if (!(most_here <= (float)kList) && n_row > kList && round < 5) continue;
+      if (!(most_here <= (float)kList) && n_row > kList && round < 5 && !(known && round == 0)) continue;
+      lo_at = lo;
+      hi_at = hi;
       // the exact measure above them, and the entries between them, marked 32 at a time
       g.barrier();  // the others are done with what is cleared
       if (tid == 0) sh.count = 0;
@@ -651,8 +711,9 @@ template <int kThreads> struct Row {
         }
       }
       const double front = g.sum(more);
+      if (kCluster) g.barrier();  // the lists are read across the cluster
       int n = sh.count;
-      if (kThreads == kWide && g.cluster > 1) {
+      if (kCluster) {
         n = g.lane < g.cluster ? *cg::this_cluster().map_shared_rank(&sh.count, g.lane) : 0;
         n = __reduce_add_sync(0xffffffffu, n);
       }
@@ -900,16 +961,16 @@ template <int kThreads> struct Row {
   }
 };
 
-template <typename T, int kThreads>
+template <typename T, int kThreads, bool kCluster>
 __global__ void __launch_bounds__(kThreads == 32 ? 32 * kWarpRows : kThreads, kThreads == 32 ? 5 : 3)
 sample_kernel(const SampleParams p) {
   extern __shared__ float4 smem[];
-  __shared__ Shared<kThreads> shared[kThreads == 32 ? kWarpRows : 1];
+  __shared__ Shared<kThreads, kCluster> shared[kThreads == 32 ? kWarpRows : 1];
   const int part = kThreads == 32 ? threadIdx.x >> 5 : 0;
   const int cap = kThreads * 4 * p.pieces;
   float* v = reinterpret_cast<float*>(smem) + part * cap;
-  Shared<kThreads>& sh = shared[part];
-  Group<kThreads> g(sh.slots, sh.wide, p.cluster);
+  Shared<kThreads, kCluster>& sh = shared[part];
+  Group<kThreads, kCluster> g(sh.slots, sh.wide, sh.bars, p.cluster);
   const int row = kThreads == 32 ? blockIdx.x * kWarpRows + part : blockIdx.x / p.cluster;
   if (row >= p.rows) return;
   float temp = p.temperature ? p.temperature[row] : 1.f;
@@ -918,10 +979,10 @@ sample_kernel(const SampleParams p) {
   float u = p.u[row];
   u = u >= 0.f ? fminf(u, 1.f - 0x1p-24f) : 0.f;
   int n = 0;
-  const int first = load_row<T, kThreads>(p, g, row, v, cap, n);
+  const int first = load_row<T, kThreads, kCluster>(p, g, row, v, cap, n);
   g.barrier();
   const int local = (kThreads == 32 ? g.lane : (int)threadIdx.x) * 4 * p.pieces;
-  Row<kThreads> r{g, sh, p, v + local, g.crank * cap + local, 4 * p.pieces, row, first, Weight(0.f, 1.f)};
+  Row<kThreads, kCluster> r{g, sh, p, v + local, g.crank * cap + local, 4 * p.pieces, row, first, Weight(0.f, 1.f)};
   float own_max = -INFINITY;
   r.each([&](int, float l) { own_max = fmaxf(own_max, l); });
   float m = g.max(own_max);
@@ -968,23 +1029,29 @@ sample_kernel(const SampleParams p) {
         });
         if ((double)k < g.sum((double)own)) {
           least = -g.max(-least);
-          r.template select<float, false>(n, (double)k, m, least, 0.0, cut);
+          float lo_at = 0.f, hi_at = INFINITY;
+          r.template select<float, false>(n, (double)k, m, least, 0.0, lo_at, hi_at, cut);
           if (tp < 1.f) r.keep(cut);
         }
       }
       if (tp < 1.f) {
-        if (!fp32 || !r.template select<float, true>(n, (double)tp, m, 0.f, slack, cut)) r.template select<double, true>(n, (double)tp, m, 0.f, 0.0, cut);
+        float lo_at = 0.f, hi_at = INFINITY;
+        if (!fp32 || !r.template select<float, true>(n, (double)tp, m, 0.f, slack, lo_at, hi_at, cut))
+          r.template select<double, true>(n, (double)tp, m, 0.f, 0.0, lo_at, hi_at, cut);
       }
       if (!fp32 || !r.template draw<float>(cut, p_min, u, slack)) r.template draw<double>(cut, p_min, u, 0.0);
     }
   }
-  if (kThreads == kWide && p.cluster > 1) g.barrier();  // no CTA leaves while another may still read its shared memory
+  if (kCluster) {
+    g.barrier();  // no CTA leaves while another may still reach into its shared memory
+    if (g.gave_up) p.choice[row] = -2;
+  }
 }
 
-template <typename T, int kThreads>
+template <typename T, int kThreads, bool kCluster>
 cudaError_t launch_group(const SampleParams& p, cudaStream_t s) {
   const int groups = kThreads == 32 ? kWarpRows : 1;
-  cudaError_t e = raise_smem_limit<sample_kernel<T, kThreads>>(kThreads == kWide ? kWide * kMaxPieces * 16 : 64 * 1024);
+  cudaError_t e = raise_smem_limit<sample_kernel<T, kThreads, kCluster>>(kThreads == kWide ? kWide * kMaxPieces * 16 : 64 * 1024);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(kThreads == 32 ? ceil_div(p.rows, kWarpRows) : p.rows * p.cluster);
@@ -996,8 +1063,8 @@ cudaError_t launch_group(const SampleParams& p, cudaStream_t s) {
   attr[0].val.clusterDim.x = p.cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<T, kThreads>, p);
+  cfg.numAttrs = kCluster ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T, kThreads, kCluster>, p);
 }
 
 template <typename T>
@@ -1015,8 +1082,8 @@ cudaError_t launch_sample(SampleParams p, cudaStream_t s) {
   // Bound of a sum's error over the sum of all weights, in steps of 2^-24.  A weight: ex2.approx 3, the factor and the second pieces 1.
   // Sums: 8 at a time 3.  Twice that, since two sums are compared.
   p.slack = 2.f * (3.f + 1.f + 3.f + 1.f) * 0x1p-24f;
-  if (threads == 32) return launch_group<T, 32>(p, s);
-  return launch_group<T, kWide>(p, s);
+  if (threads == 32) return launch_group<T, 32, false>(p, s);
+  return p.cluster == 1 ? launch_group<T, kWide, false>(p, s) : launch_group<T, kWide, true>(p, s);
 }
 
 }  // namespace
