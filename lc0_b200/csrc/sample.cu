@@ -531,74 +531,78 @@ template <int kThreads, bool kCluster> struct Row {
     constexpr bool kOpen = kMass && sizeof(W) == 4;
     constexpr int kEach = kList / 32;
     const int lane = g.lane;
-    float l[kEach];
+    uint32_t key[kEach];  // 0: none
     int slot[kEach];
     W w[kEach];
-    const bool parts = kCluster;  // a list in each CTA of the cluster, one behind the other
-    const int own = parts && lane < g.cluster ? *cg::this_cluster().map_shared_rank(&sh.count, lane) : 0;
+    const int own = kCluster && lane < g.cluster ? *cg::this_cluster().map_shared_rank(&sh.count, lane) : 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      l[i] = -INFINITY;
-      slot[i] = 0;
-      if (32 * i >= n) continue;
-      int at = 32 * i + lane, cta = 0;
-      const bool there = at < n;
-      if (parts)
-        for (int c = 0; c < g.cluster - 1; ++c) {
+      int at = 32 * i + lane < n ? 32 * i + lane : 0, cta = 0;
+      if (kCluster)  // a list in each CTA of the cluster, one behind the other
+        for (int c = 0; c < kMaxCluster - 1; ++c) {
           const int nc = __shfl_sync(0xffffffffu, own, c);
-          if (cta == c && at >= nc) { at -= nc; ++cta; }
+          const bool behind = cta == c && at >= nc && c < g.cluster - 1;
+          at -= behind ? nc : 0;
+          cta += behind;
         }
-      if (there) {
-        l[i] = parts ? cg::this_cluster().map_shared_rank(sh.list_l, cta)[at] : sh.list_l[at];
-        slot[i] = parts ? cg::this_cluster().map_shared_rank(sh.list_slot, cta)[at] : sh.list_slot[at];
-      }
+      const float l = kCluster ? cg::this_cluster().map_shared_rank(sh.list_l, cta)[at] : sh.list_l[at];
+      slot[i] = kCluster ? cg::this_cluster().map_shared_rank(sh.list_slot, cta)[at] : sh.list_slot[at];
+      key[i] = 32 * i + lane < n ? key_of(l) : 0;
     }
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) w[i] = l[i] > -INFINITY ? kMass ? wt.get(l[i], W()) : W(1) : W(0);
-    auto total = [&](auto in) {
-      double t = 0.0;
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) t += in(l[i]) ? (double)w[i] : 0.0;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-      return t;
-    };
-    uint32_t lo = key_of(-INFINITY), hi = key_of(wt.max);  // above lo the target or more, above hi less
-    double ahead = 0.0;
+    for (int i = 0; i < kEach; ++i) w[i] = key[i] ? kMass ? wt.get(of_key(key[i]), W()) : W(1) : W(0);
+    uint32_t lo = 0, hi = 0xffffffffu;  // above lo the target or more, above hi less
     int left = n;
     bool open = false;
     while (left > 32) {
-      // the middle of what is left, in logits, or where that is none between them in keys
-      float down = INFINITY, up = -INFINITY;
+      // the middle of what is left, in logits
+      uint32_t down = 0xffffffffu, up = 0;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i)
-        if (l[i] > of_key(lo) && l[i] <= of_key(hi)) { down = fminf(down, l[i]); up = fmaxf(up, l[i]); }
-      up = warp_max(up);
-      down = -warp_max(-down);
-      if (!(down < up)) {
-        if (lane == 0) { sh.cut = entry_of(up, 0); sh.ahead = front + ahead; }
-        return left > 0 ? 3 : 0;
+      for (int i = 0; i < kEach; ++i) {
+        const bool in = key[i] > lo && key[i] <= hi;
+        down = in ? min(down, key[i]) : down;
+        up = in ? max(up, key[i]) : up;
       }
-      float at = 0.5f * down + 0.5f * up;
-      if (!(at >= down && at < up)) at = down;
-      const double m = total([&](float x) { return x > at; });
-      if (kOpen) open |= fabs(front + m - target) <= slack;
-      if (front + m >= target) lo = key_of(at);
-      else { hi = key_of(at); ahead = m; }
+      down = __reduce_min_sync(0xffffffffu, down);
+      up = __reduce_max_sync(0xffffffffu, up);
+      if (down >= up) {  // equal entries
+        double m = 0.0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) m += key[i] > up ? (double)w[i] : 0.0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+        if (lane == 0) { sh.cut = (uint64_t)up << 32; sh.ahead = front + m; }
+        return open ? 2 : 3;
+      }
+      uint32_t at = key_of(0.5f * of_key(down) + 0.5f * of_key(up));
+      if (at < down || at >= up) at = down;
+      W m = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) m += key[i] > at ? w[i] : W(0);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+      if (kOpen) open |= fabs(front + (double)m - target) <= slack + 13.0 * 0x1p-24 * (double)m;  // (thirteen additions)
+      if (front + (double)m >= target) lo = at;
+      else hi = at;
       left = 0;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) left += l[i] > of_key(lo) && l[i] <= of_key(hi);
+      for (int i = 0; i < kEach; ++i) left += key[i] > lo && key[i] <= hi;
       left = __reduce_add_sync(0xffffffffu, left);
     }
     if (open) return 2;
+    double ahead = 0.0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) ahead += key[i] > hi ? (double)w[i] : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
     // those left side by side, through the gathered entries' place
     __syncwarp();
     int pos = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const bool in = l[i] > of_key(lo) && l[i] <= of_key(hi);
+      const bool in = key[i] > lo && key[i] <= hi;
       const uint32_t b = __ballot_sync(0xffffffffu, in);
-      if (in) sh.sorted[pos + __popc(b & ((1u << lane) - 1))] = entry_of(l[i], slot[i]);
+      if (in) sh.sorted[pos + __popc(b & ((1u << lane) - 1))] = (uint64_t)key[i] << 32 | (uint32_t)~slot[i];
       pos += __popc(b);
     }
     __syncwarp();
