@@ -246,8 +246,10 @@ template <int kN> __device__ __forceinline__ void exp_below(double (&x)[kN]) {
     x[i] = s[i] * __hiloint2double((half + 1023) << 20, 0) * __hiloint2double((n[i] - half + 1023) << 20, 0);
   }
 }
-// Weights in fp32 or in 64 bits, of a row whose largest logit is finite.
-struct Weight {
+// Weights in fp32 or in 64 bits, of a row whose largest logit is finite.  kFine: the rounding of l - m is made good.  The rows of a warp do
+// without: it is a tenth of a pass over them, and the wider bound of their sums sends 1 % of them into 64 bits; of wider rows,
+// with more comparisons, it would be every third.
+template <bool kFine> struct Weight {
   float half_max, c, c_lo, max, temp;
   double inv_t;
   __device__ Weight(float m, float t) : max(m), temp(t) {
@@ -261,10 +263,15 @@ struct Weight {
   // 2^((l - m) log2(e) / T), the difference (of halves, since l - m can overflow) and the exponent each in two pieces.  No branch: passes
   // over a row live on several entries being in work at once.
   __device__ __forceinline__ float get(float l, float) const {
-    const float a = 0.5f * l, x = a - half_max, b = x - a;
-    const float x_lo = (a - (x - b)) - (half_max + b);
+    const float a = 0.5f * l, x = a - half_max;
+    float x_lo = 0.f;
+    if constexpr (kFine) {
+      const float b = x - a;
+      x_lo = (a - (x - b)) - (half_max + b);
+    }
     const float z = x * c;
-    const float lo = fmaf(x_lo, c, fmaf(x, c_lo, fmaf(x, c, -z)));
+    float lo = fmaf(x, c_lo, fmaf(x, c, -z));
+    if constexpr (kFine) lo = fmaf(x_lo, c, lo);
     float w;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(z));
     w = fmaf(w, lo * 0.69314718f, w);
@@ -390,6 +397,7 @@ template <int kThreads, bool kCluster> struct Shared {
   float list_l[kList];
   int list_slot[kList];
   uint64_t sorted[32];
+  double weights[kThreads == 32 ? kSort : 1];
   uint64_t bars[2];
   double ahead;
   int count;
@@ -429,16 +437,16 @@ __device__ __forceinline__ void sort_entries(uint64_t& a, uint64_t& b, bool two,
     b = step(b, j, (lane & j) == 0);
   }
 }
-__device__ __forceinline__ double warp_before(double v, double& total, int lane) {
-  double in = v;
+template <typename W> __device__ __forceinline__ W warp_before(W v, W& total, int lane) {
+  W in = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const double up = __shfl_up_sync(0xffffffffu, in, o);
+    const W up = __shfl_up_sync(0xffffffffu, in, o);
     if (lane >= o) in += up;
   }
   total = __shfl_sync(0xffffffffu, in, 31);
-  const double ex = __shfl_up_sync(0xffffffffu, in, 1);
-  return lane == 0 ? 0.0 : ex;
+  const W ex = __shfl_up_sync(0xffffffffu, in, 1);
+  return lane == 0 ? W(0) : ex;
 }
 
 // A row in shared memory, seen by one thread of its group.
@@ -450,7 +458,7 @@ template <int kThreads, bool kCluster> struct Row {
   int slot0;     // slot of the first of them
   int count;     // their number
   int row, first;
-  Weight wt;
+  Weight<(kThreads > 32)> wt;
 
   template <typename F> __device__ __forceinline__ void each(F f) const {
 #pragma unroll 2
@@ -800,26 +808,26 @@ template <int kThreads, bool kCluster> struct Row {
       double run = __shfl_sync(0xffffffffu, ahead, o);
       bool found = false;
       for (int base = 0; base < count; base += 32) {
-        double w = 0.0, sum32;
+        W w = 0, sum32;
         const int i = base + g.lane;
         if (i < count && (theirs[i] > cut.l || (theirs[i] == cut.l && their_slot + i <= cut.slot))) {
           const W x = wt.get(theirs[i], W());
-          w = x >= limit ? (double)x : 0.0;
+          w = x >= limit ? x : W(0);
         }
-        const double before = run + warp_before(w, sum32, g.lane);
-        const uint32_t any = __ballot_sync(0xffffffffu, w > 0.0), hit = __ballot_sync(0xffffffffu, w > 0.0 && before + w > target);
+        const double before = run + (double)warp_before(w, sum32, g.lane);
+        const uint32_t any = __ballot_sync(0xffffffffu, w > W(0)), hit = __ballot_sync(0xffffffffu, w > W(0) && before + (double)w > target);
         if (any) {
           const int j = hit ? __ffs(hit) - 1 : 31 - __clz(any);
           at = their_slot + base + j;
           const double b = __shfl_sync(0xffffffffu, before, j);
-          w_at = __shfl_sync(0xffffffffu, w, j);
+          w_at = (double)__shfl_sync(0xffffffffu, w, j);
           if (hit) {
             if (kOpen) open |= target - b <= slack * total || b + w_at - target <= slack * total;
             found = true;
             break;
           }
         }
-        run += sum32;
+        run += (double)sum32;
       }
       if (kOpen && !found) open = true;
     }
@@ -834,21 +842,34 @@ template <int kThreads, bool kCluster> struct Row {
   }
 
   // ---- rows whose kept entries are few: a warp has them all, in the order of their indices, and sums in 64 bits ----
-  // l, slot: n <= 64 entries.
+  // l, slot (NULL: from `base` on): n <= 64 entries.
   __device__ void finish(const float* l, const int* slot, int base, int n, int k, float p_top, float p_min, float u) {
     const int lane = g.lane;
-    auto at = [&](int i) { return i < n ? entry_of(l[i], slot ? slot[i] : base + i) : 0; };
-    auto weigh = [&](uint64_t e) { return e ? wt.get(of_key((uint32_t)(e >> 32)), 0.0) : 0.0; };
+    uint64_t own[2];  // entries lane and 32 + lane, by their places here (which rise with the indices)
+    double w[2], x[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = 32 * h + lane;
+      const float v = i < n ? l[i] : -INFINITY;
+      own[h] = entry_of(v, i);
+      x[h] = wt.exponent(v);
+    }
+    exp_below(x);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) w[h] = own[h] ? x[h] : 0.0;
     uint64_t cut = 1;
     if ((k > 0 && k < n) || p_top < 1.f) {
-      uint64_t e[2] = {at(lane), at(32 + lane)};
+      uint64_t e[2] = {own[0], own[1]};
       sort_entries(e[0], e[1], n > 32, lane);
-      int stay = __popc(__ballot_sync(0xffffffffu, e[0])) + __popc(__ballot_sync(0xffffffffu, e[1]));
+      int stay = __popc(__ballot_sync(0xffffffffu, e[0] != 0)) + __popc(__ballot_sync(0xffffffffu, e[1] != 0));
       if (k > 0 && k < stay) stay = k;
       if (p_top < 1.f) {
-        const double w0 = lane < stay ? weigh(e[0]) : 0.0, w1 = n > 32 && 32 + lane < stay ? weigh(e[1]) : 0.0;
+        sh.weights[lane] = w[0];
+        sh.weights[32 + lane] = w[1];
+        __syncwarp();
+        const double w0 = lane < stay ? sh.weights[~(uint32_t)e[0]] : 0.0, w1 = 32 + lane < stay ? sh.weights[~(uint32_t)e[1]] : 0.0;
         double t0, t1 = 0.0;
-        const double b0 = warp_before(w0, t0, lane), b1 = n > 32 ? t0 + warp_before(w1, t1, lane) : 0.0;
+        const double b0 = warp_before(w0, t0, lane), b1 = stay > 32 ? t0 + warp_before(w1, t1, lane) : 0.0;
         const double target = (double)p_top * (t0 + t1);
         const int in = __popc(__ballot_sync(0xffffffffu, lane < stay && b0 < target)) +
                        __popc(__ballot_sync(0xffffffffu, 32 + lane < stay && b1 < target));
@@ -858,13 +879,10 @@ template <int kThreads, bool kCluster> struct Row {
       cut = stay > 32 ? c1 : c0;
     }
     const double limit = p_min > 0.f ? (double)fminf(p_min, 1.f) : 0.0;
-    double run = 0.0, total, w[2], before[2];
-    uint64_t e[2];
+    double run = 0.0, total, before[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      e[h] = h == 0 || n > 32 ? at(32 * h + lane) : 0;
-      w[h] = e[h] >= cut ? weigh(e[h]) : 0.0;
-      if (w[h] < limit) w[h] = 0.0;
+      if (own[h] < cut || w[h] < limit) w[h] = 0.0;
       before[h] = 0.0;
       if (h == 0 || n > 32) {
         before[h] = run + warp_before(w[h], total, lane);
@@ -880,7 +898,8 @@ template <int kThreads, bool kCluster> struct Row {
       else hit0 = 1u << (31 - __clz(__ballot_sync(0xffffffffu, w[0] > 0.0)));
     }
     const int half = hit0 ? 0 : 1, j = __ffs(hit0 ? hit0 : hit1) - 1;
-    if (lane == j) give((int)~(uint32_t)(half ? e[1] : e[0]), (float)((half ? w[1] : w[0]) / run));
+    const int i = 32 * half + lane;
+    if (lane == j) give(slot ? slot[i] : base + i, (float)((half ? w[1] : w[0]) / run));
   }
   // The entries that top-k can keep, gathered: those not below a logit that k entries reach.  Maxima of the lanes' runs give one: the
   // k-th of them for small k, one of the least else, which more than k entries reach nearly always; from there a bisection over the
@@ -986,7 +1005,7 @@ sample_kernel(const SampleParams p) {
   const int first = load_row<T, kThreads, kCluster>(p, g, row, v, cap, n);
   g.barrier();
   const int local = (kThreads == 32 ? g.lane : (int)threadIdx.x) * 4 * p.pieces;
-  Row<kThreads, kCluster> r{g, sh, p, v + local, g.crank * cap + local, 4 * p.pieces, row, first, Weight(0.f, 1.f)};
+  Row<kThreads, kCluster> r{g, sh, p, v + local, g.crank * cap + local, 4 * p.pieces, row, first, Weight<(kThreads > 32)>(0.f, 1.f)};
   float own_max = -INFINITY;
   r.each([&](int, float l) { own_max = fmaxf(own_max, l); });
   float m = g.max(own_max);
@@ -1006,7 +1025,7 @@ sample_kernel(const SampleParams p) {
     g.barrier();
   }
   if (!done) {
-    r.wt = Weight(m, temp);
+    r.wt = Weight<(kThreads > 32)>(m, temp);
     const bool fp32 = r.wt.fp32_usable();
     const float tp = p_top <= 0.f ? 1.f : p_top;
     if constexpr (kThreads == 32) {
@@ -1083,9 +1102,10 @@ cudaError_t launch_sample(SampleParams p, cudaStream_t s) {
   if (threads == kWide)
     while (p.cluster < kMaxCluster && pieces(kWide * p.cluster) > 9) p.cluster *= 2;
   p.pieces = pieces(threads * p.cluster);
-  // Bound of a sum's error over the sum of all weights, in steps of 2^-24.  A weight: ex2.approx 3, the factor and the second pieces 1.
-  // Sums: 8 at a time 3.  Twice that, since two sums are compared.
-  p.slack = 2.f * (3.f + 1.f + 3.f + 1.f) * 0x1p-24f;
+  // Bound of a sum's error over the sum of all weights, in steps of 2^-24.  A weight: ex2.approx 3, the factor and the second pieces 1;
+  // without the rounding of l - m made good |z| more, z = (l - m) / T, and the sum of w |z| is at most ln(n) < 8 times the sum of w
+  // (of a warp's rows).  Sums: 8 at a time 3; the prefix sums of a warp's entries 5.  Twice that, since two sums are compared.
+  p.slack = 2.f * (3.f + 1.f + (threads == 32 ? 8.f : 0.f) + 8.f) * 0x1p-24f;
   if (threads == 32) return launch_group<T, 32, false>(p, s);
   return p.cluster == 1 ? launch_group<T, kWide, false>(p, s) : launch_group<T, kWide, true>(p, s);
 }
