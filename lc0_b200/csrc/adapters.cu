@@ -7,7 +7,7 @@
 //   adapter's A arrive by TMA in a ring, four warps multiply 16 rows each by mma.sync: what counts is X's one pass through.
 // H otherwise (adapters_shrink_rows_kernel): a CTA per row, the row in shared memory, a warp per row of A.
 // The shared product, 16-bit: kernels of gemm_tc.cu (H and B as further k-blocks) and gemm_split.cu (added in the epilogue), see
-//   gemm_adapters_supported; operands that TMA cannot read and fp32: gemm_fma.cu into fp32 sums, to which
+//   launch_gemm_tc; operands that TMA cannot read: gemm_fma.cu, fp32: gemm_f32.cu or gemm_fma.cu, into fp32 sums, to which
 //   adapters_expand_kernel adds.
 #include "../../include/b200nn.h"
 #include "kernels.cuh"
@@ -265,12 +265,17 @@ __global__ void __launch_bounds__(256) adapters_expand_kernel(const AdapterParam
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; }
 
-// What a description is computed by, and its workspace: H, its pieces, the fp32 sums.  Nothing here depends on the device.
+// fp32: whether a product is worth cutting its weights into pieces for the tensor cores, which every call does.  us with rank 16, FMA /
+// tensor cores: 64x512x256 22.6 / 21.3, 256x512x256 26.5 / 22.2, 1024x512x256 28.8 / 25.1, 512x1024x1024 53 / 34.5,
+// 64x1536x1536 42.6 / 40, 1024x1536x1536 190 / 95.  Fewer rows than a tile's share W among less than the pieces cost.
+bool worth_pieces(const b200_adapters_desc& d) { return d.M >= 64 && (long long)d.M * d.N * d.K >= 1 << 23; }
+
+// What a description is computed by, and its workspace: H, its pieces, the fp32 sums, the pieces of fp32 weights.  Nothing here depends on the device.
 struct AdapterPlan {
   GemmParams g;
   bool tensor = false, mma = false;
-  size_t h_bytes = 0, piece_bytes = 0, acc_bytes = 0;
-  size_t bytes() const { return h_bytes + piece_bytes + acc_bytes; }
+  size_t h_bytes = 0, piece_bytes = 0, acc_bytes = 0, w_bytes = 0;
+  size_t bytes() const { return h_bytes + piece_bytes + acc_bytes + w_bytes; }
 };
 AdapterPlan plan_of(const b200_adapters_desc& d) {
   AdapterPlan out;
@@ -285,6 +290,10 @@ AdapterPlan plan_of(const b200_adapters_desc& d) {
   if (out.mma && gemm_adapters_pieces(g)) out.piece_bytes = round256((size_t)d.M * 2 * g.ad_rp * 2);
   // sums of the shared product: in C itself where it holds floats
   if (!out.tensor && !g.out_f32) out.acc_bytes = round256((size_t)d.M * d.N * 4);
+  // fp32 on tensor cores: W is cut into pieces by every call
+  g.W3 = d.precision == B200_PREC_FP32 ? d.X : nullptr;  // (any aligned address, for the question alone)
+  if (d.precision == B200_PREC_FP32 && worth_pieces(d) && gemm_f32_supported(g)) out.w_bytes = round256((size_t)d.N * d.K * 6);
+  g.W3 = nullptr;
   return out;
 }
 
@@ -349,9 +358,22 @@ int run_adapters(const b200_adapters_desc& d, cudaStream_t s) {
   void* acc = plan.acc_bytes ? ws + plan.h_bytes : d.C;
   g.C = acc; g.ldc = plan.acc_bytes ? d.N : g.ldc; g.out_f32 = true; g.act = ACT_NONE; g.ad_ids = nullptr;
   p.acc = static_cast<const float*>(acc); p.ldacc = g.ldc;
-  B200_CUDA(launch_shrink_rows<T>(p, s));
+  if (plan.w_bytes) {
+    // (the product fetches the pieces ahead of its dependency: it is not launched dependent on what writes them)
+    B200_CUDA(gemm_tc_init());
+    int dev = 0, sms = 0;
+    B200_CUDA(cudaGetDevice(&dev));
+    B200_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    g.W3 = ws + plan.h_bytes;
+    B200_CUDA(launch_split_weights(static_cast<const float*>(d.W), (long long)d.N * d.K, ws + plan.h_bytes, s));
+    B200_CUDA(launch_shrink_rows<T>(p, s));
+    B200_CUDA(launch_gemm_f32(g, d.status, sms, s));
+  } else {
+    B200_CUDA(launch_shrink_rows<T>(p, s));
+    DependentScope dependent;
+    B200_CUDA(launch_gemm_fma<T>(g, s));
+  }
   DependentScope dependent;
-  B200_CUDA(launch_gemm_fma<T>(g, s));
   const int row_blocks = ceil_div(d.M, 4 * kExpandRows);
   const int vec = d.rank % 8 == 0 && aligned16(d.B);
   B200_CUDA(launch_dependent(adapters_expand_kernel<T>, dim3(ceil_div(d.N, 64), row_blocks < 65535 ? row_blocks : 65535), dim3(256), 0, s, p,

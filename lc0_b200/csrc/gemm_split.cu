@@ -24,7 +24,7 @@
 // second one: 32 heads x 256), as long as a tile holds whole vectors.  Every column tile repeats the LayerNorm: worth it
 // while a launch costs more than that (Net::gemm_with_ln has the line); beyond, ln_rows_kernel does it with the same results.
 // With adapters (kAd) the product takes H . B^T in.  kAdBlocks: as further k-blocks of one CTA of the cluster, like gemm_tc.cu's pair kernel;
-// kAdAdd: a warp per row adds it in fp32 to the sums in shared memory, a lane per column, for requests of any number of rows and
+// kAdAdd: a warp per row adds it in fp32 to the sums in shared memory, for requests of any number of rows and
 // operands that TMA cannot read.  The kernel before this one only writes H: A and W are loaded and multiplied while it runs.
 // Every wait is bounded by wall-clock time like those of gemm_tc.cu; the cluster barriers are reached by all threads
 // whatever happened before them.
@@ -165,25 +165,14 @@ ln_rows_kernel(const T* x, T* out, const float* __restrict__ gamma, const float*
 
 enum SplitAdapters { kAdNone = 0, kAdAdd = 1, kAdBlocks = 2 };
 
-// H[m] . B_a[n]
+// H[m] . B_a[n] for any rank and alignment.
 template <typename T>
-__device__ __forceinline__ float adapter_dot(const TcParams& p, int m, int n, int a, bool vec) {
-  const int rank = p.ad_rank;
-  const float* h = p.ad_h + (long long)m * rank;
-  const T* b = static_cast<const T*>(p.ad_b) + ((long long)a * p.N + n) * rank;
+__device__ __forceinline__ float adapter_dot(const TcParams& p, int m, int n, int a) {
+  const float* h = p.ad_h + (long long)m * p.ad_rank;
+  const T* b = static_cast<const T*>(p.ad_b) + ((long long)a * p.N + n) * p.ad_rank;
   float s = 0.f;
-  if (vec) {
-#pragma unroll 2
-    for (int r = 0; r < rank; r += 8) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(b + r));
-      const float4 h0 = *reinterpret_cast<const float4*>(h + r), h1 = *reinterpret_cast<const float4*>(h + r + 4);
-      const T* e = reinterpret_cast<const T*>(&u);
-      s = fmaf(h0.x, to_f(e[0]), fmaf(h0.y, to_f(e[1]), fmaf(h0.z, to_f(e[2]), fmaf(h0.w, to_f(e[3]), s))));
-      s = fmaf(h1.x, to_f(e[4]), fmaf(h1.y, to_f(e[5]), fmaf(h1.z, to_f(e[6]), fmaf(h1.w, to_f(e[7]), s))));
-    }
-  } else {
-    for (int r = 0; r < rank; ++r) s = fmaf(h[r], to_f(b[r]), s);
-  }
+#pragma unroll 4
+  for (int r = 0; r < p.ad_rank; ++r) s = fmaf(h[r], to_f(b[r]), s);
   return s;
 }
 // One element of a product with adapters from its operands: for those that the tensor core left not finite (see gemm_tc.cu).
@@ -424,16 +413,41 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   }
   if constexpr (kAd == kAdAdd) {
     if (warp < 8) {
-      const bool vec = p.ad_rank % 8 == 0 && (reinterpret_cast<uintptr_t>(p.ad_b) & 15) == 0;
       float* part = reinterpret_cast<float*>(smem);
+      const int pieces = p.ad_rank / 8;  // of 16 bytes in a row of B
+      auto at = [&](int r, int n) { return part + r * BN + ((((n >> 2) ^ (r & 7)) << 2) | (n & 3)); };
+      if (p.ad_rank % 8 == 0 && (pieces & (pieces - 1)) == 0 && (reinterpret_cast<uintptr_t>(p.ad_b) & 15) == 0) {
+        // as many lanes per column as its row of B has 16-byte pieces: a warp's loads are consecutive
+        const int piece = lane & (pieces - 1), sub = lane / pieces, cols = 32 / pieces;
+#pragma unroll 2
+        for (int r = warp; r < rp; r += 8) {
+          const int m = m0 + rank * rp + r, a = m < p.M ? adapter_of_row(p, m) : -1;
+          if (a < 0) continue;
+          const float* h = p.ad_h + (long long)m * p.ad_rank + piece * 8;
+          const float4 h0 = *reinterpret_cast<const float4*>(h), h1 = *reinterpret_cast<const float4*>(h + 4);
+          const T* b = static_cast<const T*>(p.ad_b) + (long long)a * p.N * p.ad_rank + piece * 8;
 #pragma unroll 4
-      for (int r = warp; r < rp; r += 8) {
-        const int m = m0 + rank * rp + r, a = m < p.M ? adapter_of_row(p, m) : -1;
-        if (a < 0) continue;
+          for (int c = 0; c < BN; c += cols) {
+            const int n = c + sub;
+            float s = 0.f;
+            if (n0 + n < p.N) {
+              const uint4 u = __ldg(reinterpret_cast<const uint4*>(b + (long long)(n0 + n) * p.ad_rank));
+              const T* e = reinterpret_cast<const T*>(&u);
+              s = fmaf(h0.x, to_f(e[0]), fmaf(h0.y, to_f(e[1]), fmaf(h0.z, to_f(e[2]), h0.w * to_f(e[3]))));
+              s = fmaf(h1.x, to_f(e[4]), fmaf(h1.y, to_f(e[5]), fmaf(h1.z, to_f(e[6]), fmaf(h1.w, to_f(e[7]), s))));
+            }
+            for (int o = pieces >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            if (piece == 0 && n0 + n < p.N) *at(r, n) += s;
+          }
+        }
+      } else {
+#pragma unroll 2
+        for (int r = warp; r < rp; r += 8) {
+          const int m = m0 + rank * rp + r, a = m < p.M ? adapter_of_row(p, m) : -1;
+          if (a < 0) continue;
 #pragma unroll
-        for (int c = 0; c < BN; c += 32) {
-          const int n = c + lane;
-          if (n0 + n < p.N) part[r * BN + ((((n >> 2) ^ (r & 7)) << 2) | (n & 3))] += adapter_dot<T>(p, m, n0 + n, a, vec);
+          for (int c = 0; c < BN; c += 32)
+            if (n0 + c + lane < p.N) *at(r, c + lane) += adapter_dot<T>(p, m, n0 + c + lane, a);
         }
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");

@@ -36,6 +36,7 @@ struct SampleParams {
   int* choice; float* prob;
   int pieces;   // 16-byte pieces per thread, odd
   int cluster;  // CTAs per row (kCluster)
+  int ahead;    // rows of one round of CTAs
   float slack;  // bound of a sum's error, relative to the sum of all weights
 };
 
@@ -918,23 +919,34 @@ template <int kThreads, bool kCluster> struct Row {
     float floor_l = __shfl_sync(0xffffffffu, s, k <= 24 ? k - 1 : k <= 40 ? 28 : 30);  // (the last run may be empty)
     if (n_row <= kList) floor_l = -3.402823466e38f;
     if (floor_l == -INFINITY) return 0;
-    uint32_t hits_lo = 0, hits_hi = 0;
+    // one row in five hundred has too few or too many above it; another logit is tried there, a row done by all its entries takes
+    // twenty times as long and the others wait for it
+    uint64_t hits = 0;
+    int own = 0, in = 0, n = 0;
+    float few = wt.max, many = -INFINITY;
+    for (int tries = 0; tries < 6; ++tries) {
+      uint32_t hits_lo = 0, hits_hi = 0;
 #pragma unroll 4
-    for (int i = 0; i < count; i += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(mine + i);
-      const uint32_t four = (x.x >= floor_l ? 1u : 0u) | (x.y >= floor_l ? 2u : 0u) | (x.z >= floor_l ? 4u : 0u) | (x.w >= floor_l ? 8u : 0u);
-      if (i < 32) hits_lo |= four << i;
-      else hits_hi |= four << (i - 32);
+      for (int i = 0; i < count; i += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(mine + i);
+        const uint32_t four = (x.x >= floor_l ? 1u : 0u) | (x.y >= floor_l ? 2u : 0u) | (x.z >= floor_l ? 4u : 0u) | (x.w >= floor_l ? 8u : 0u);
+        if (i < 32) hits_lo |= four << i;
+        else hits_hi |= four << (i - 32);
+      }
+      hits = (uint64_t)hits_hi << 32 | hits_lo;
+      own = __popcll(hits);
+      n = __reduce_add_sync(0xffffffffu, own);
+      if (n_row <= kList || (n >= k && n <= kList)) break;
+      if (n < k) few = floor_l;
+      else many = floor_l;
+      floor_l = many == -INFINITY ? floor_l - 0.25f * (wt.max - floor_l) : 0.5f * few + 0.5f * many;
     }
-    uint64_t hits = (uint64_t)hits_hi << 32 | hits_lo;
-    const int own = __popcll(hits);
-    int in = own;
+    in = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, in, o);
       if (lane >= o) in += up;
     }
-    int n = __shfl_sync(0xffffffffu, in, 31);
     if (n > kList || (n < k && n_row > kList)) return 0;
     for (int pos = in - own; hits; hits &= hits - 1, ++pos) {
       const int i = __ffsll((long long)hits) - 1;
@@ -1001,6 +1013,10 @@ sample_kernel(const SampleParams p) {
   const int k = p_top <= 0.f ? 1 : p.top_k ? p.top_k[row] : 0;
   float u = p.u[row];
   u = u >= 0.f ? fminf(u, 1.f - 0x1p-24f) : 0.f;
+  if (kThreads == 32 && !p.ids && row + p.ahead < p.rows) {  // a row of the next round of CTAs into L2, while this one is worked on
+    const char* next = static_cast<const char*>(p.logits) + (long long)(row + p.ahead) * p.ld * sizeof(T);
+    for (int i = g.lane * 128; i < p.width * (int)sizeof(T); i += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(next + i));
+  }
   int n = 0;
   const int first = load_row<T, kThreads, kCluster>(p, g, row, v, cap, n);
   g.barrier();
@@ -1102,6 +1118,11 @@ cudaError_t launch_sample(SampleParams p, cudaStream_t s) {
   if (threads == kWide)
     while (p.cluster < kMaxCluster && pieces(kWide * p.cluster) > 9) p.cluster *= 2;
   p.pieces = pieces(threads * p.cluster);
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  p.ahead = sms * 5 * kWarpRows;
   // Bound of a sum's error over the sum of all weights, in steps of 2^-24.  A weight: ex2.approx 3, the factor and the second pieces 1;
   // without the rounding of l - m made good |z| more, z = (l - m) / T, and the sum of w |z| is at most ln(n) < 8 times the sum of w
   // (of a warp's rows).  Sums: 8 at a time 3; the prefix sums of a warp's entries 5.  Twice that, since two sums are compared.
