@@ -287,7 +287,8 @@ AdapterPlan plan_of(const b200_adapters_desc& d) {
   out.tensor = d.precision != B200_PREC_FP32 && gemm_tc_supported(g);
   out.mma = out.tensor && d.group % 64 == 0 && aligned16(d.A) && (long long)d.n_adapters * d.rank < 0x7fffff00;
   out.h_bytes = round256((size_t)d.M * d.rank * 4);
-  if (out.mma && gemm_adapters_pieces(g)) out.piece_bytes = round256((size_t)d.M * 2 * g.ad_rp * 2);
+  // (a result in fp32 would show what the two pieces of H leave out)
+  if (out.mma && !g.out_f32 && gemm_adapters_pieces(g)) out.piece_bytes = round256((size_t)d.M * 2 * g.ad_rp * 2);
   // sums of the shared product: in C itself where it holds floats
   if (!out.tensor && !g.out_f32) out.acc_bytes = round256((size_t)d.M * d.N * 4);
   // fp32 on tensor cores: W is cut into pieces by every call
@@ -297,8 +298,11 @@ AdapterPlan plan_of(const b200_adapters_desc& d) {
   return out;
 }
 
-// Few rows: a CTA for each of them spreads over more SMs than one for every 64 does, at the price of reading A once per row.
-bool shrink_by_rows(const b200_adapters_desc& d) { return (long long)d.M * d.rank * d.K <= 4 << 20; }
+// Few long rows: a CTA for each of them spreads over more SMs than one for every 64 does, which has K / 64 steps one after the other, at
+// the price of reading A once per row.  Whole call (512 columns), us, tensor cores / by rows: 64x1024 rank 16 9.7 / 7.3, 128x1024 rank 16
+// 9.6 / 8.5, 256x1024 rank 16 10.2 / 10.2, 512x1024 rank 16 11.8 / 11.6, 192x1536 rank 8 11.8 / 9.7; short rows: 512x256 rank 8
+// 6.2 / 7.2, 1024x256 rank 16 7.9 / 10.2.
+bool shrink_by_rows(const b200_adapters_desc& d) { return d.K >= 512 && (long long)d.M * d.rank * d.K <= 4 << 20; }
 
 template <typename T, int NB>
 cudaError_t launch_shrink_mma(const AdapterParams& p, cudaStream_t s) {
@@ -384,7 +388,7 @@ int run_adapters(const b200_adapters_desc& d, cudaStream_t s) {
 // What does not depend on the pointers.
 const char* check_shape(const b200_adapters_desc* d) {
   if (!d) return "no description";
-  if (d->M < 0 || d->N < 1 || d->K < 1) return "M >= 0, N >= 1 and K >= 1";
+  if (d->M < 0 || d->M > 64 * 65535 || d->N < 1 || d->K < 1) return "M of 0 to 4194240, N >= 1 and K >= 1";
   if (d->rank < 1 || d->rank > B200_ADAPTERS_MAX_RANK) return "rank 1 to 128";
   if (d->n_adapters < 1 || d->group < 1) return "n_adapters and group are at least 1";
   if (d->precision < B200_PREC_FP32 || d->precision > B200_PREC_BF16) return "unknown precision";

@@ -6,8 +6,8 @@
 // among the entries that equal it, an index.  The draw runs over the indices: the first kept i with sum_{j <= i, kept} w_j > u W.
 //
 // The answer is a whole number, so it has to be the one that exact sums give.  Sums of fp32 weights decide where they can: with an
-// error of at most e S (kSlack below) a comparison that is closer than e S is open, and a row with an open comparison is done
-// again with weights and sums in 64 bits (one row in a few thousand for policies).
+// error of at most e S (SampleParams::slack) a comparison that is closer than e S is open, and what it belongs to, the cut or the
+// draw, is done again with weights and sums in 64 bits (1858 logits of spread 1.5: 0.3 % of the draws, 1 % of the top-p cuts).
 //
 // A row is held in shared memory as fp32 by a group of threads: a warp, a CTA or a cluster of CTAs.  Thread t owns a run of consecutive
 // entries (an odd number of 16-byte pieces: no bank conflicts), so that sums over threads run in the order of the indices.
@@ -25,7 +25,6 @@ constexpr int kMaxCluster = 8;
 constexpr int kWide = 256;              // threads of a CTA that has a row, or a part of one
 constexpr int kMaxPieces = 33;          // 16-byte pieces per thread there: 132 KB
 constexpr int kWarpRows = 4;            // rows of a CTA whose groups are warps
-constexpr int kFewRows = 444;           // three CTAs per SM
 static_assert(kMaxCluster * kWide * kMaxPieces * 4 >= B200_SAMPLE_MAX_WIDTH + 8, "the widest row fits a cluster");
 
 struct SampleParams {
@@ -260,7 +259,8 @@ template <bool kFine> struct Weight {
     c = (float)fmin(e, 1e37);
     c_lo = (float)(fmin(e, 1e37) - (double)c);
   }
-  __device__ bool fp32_usable() const { return c < 1e37f; }
+  // (beyond, temperatures of 1e-37 or 1e+30, c or its second piece leaves the range of fp32)
+  __device__ bool fp32_usable() const { return c < 1e37f && c > 1e-30f; }
   // 2^((l - m) log2(e) / T), the difference (of halves, since l - m can overflow) and the exponent each in two pieces.  No branch: passes
   // over a row live on several entries being in work at once.
   __device__ __forceinline__ float get(float l, float) const {
@@ -341,7 +341,7 @@ __device__ int load_row(const SampleParams& p, const Group<kThreads, kCluster>& 
 #pragma unroll 2
     for (int i = tid; i < cap; i += kThreads) {
       const int e = base + i;
-      const int id = e < n ? ids[e] : 65536;
+      const int id = e < n ? ids[e] : 0x7fffffff;
       v[i] = id < p.width ? to_f(src[id]) : -INFINITY;
     }
     return 0;
@@ -525,14 +525,32 @@ template <int kThreads, bool kCluster> struct Row {
     return (int)g.max((float)at);
   }
 
-  // The end of the front part inside a run of equal entries, ahead of which `front` is found.
-  template <typename W, bool kMass> __device__ bool equal_entries(float l, double front, double target, double all, double slack, Cut& out) {
-    const double w = kMass ? (double)wt.get(l, W()) : 1.0, ties = (target - front) / w;
-    if (kMass && sizeof(W) == 4 && (w < 1e-30 || fabs(ties - rint(ties)) <= slack * all / w + 1e-6 * fabs(ties))) return false;
-    out.l = l;
-    out.slot = nth_equal(l, ties <= 1.0 ? 0.0 : ceil(fmin(ties, 1e9)) - 1.0);
+  // The end of the front part by bisection over all entries: for what the quicker ways do not find.
+  template <typename W, bool kMass> __device__ bool bisect(double target, Cut& out) {
+    uint32_t lo_key = key_of(-INFINITY), hi_key = key_of(wt.max);  // measure above lo_key: the target or more; above hi_key: less
+    double over = 0.0;
+    while (hi_key - lo_key > 1) {
+      const uint32_t mid = lo_key + (hi_key - lo_key) / 2;
+      const float cut = of_key(mid);
+      const double m = g.sum(sum<W, kMass>([&](int, float l, W w) { return l > cut ? (kMass ? w : W(1)) : W(0); }));
+      if (m >= target) lo_key = mid;
+      else { hi_key = mid; over = m; }
+    }
+    out.l = of_key(hi_key);
+    const double ties = (target - over) / (kMass ? (double)wt.get(out.l, W()) : 1.0);
+    out.slot = nth_equal(out.l, ties <= 1.0 ? 0.0 : ceil(fmin(ties, 1e9)) - 1.0);
     if (out.slot < 0) out.slot = 0x7fffffff;  // all of them
     return true;
+  }
+  // The end of the front part inside a run of equal entries, ahead of which `front` is found.
+  template <typename W, bool kMass> __device__ bool equal_entries(float l, double front, double target, double all, double slack, Cut& out) {
+    constexpr bool kOpen = kMass && sizeof(W) == 4;
+    const double w = kMass ? (double)wt.get(l, W()) : 1.0, ties = (target - front) / w;
+    if (kOpen && (w < 1e-30 || fabs(ties - rint(ties)) <= slack * all / w + 1e-6 * fabs(ties))) return false;
+    out.l = l;
+    out.slot = nth_equal(l, ties <= 1.0 ? 0.0 : ceil(fmin(ties, 1e9)) - 1.0);
+    if (out.slot >= 0) return true;
+    return kOpen ? false : bisect<W, kMass>(target, out);  // the run ends before it
   }
   // The end among the n <= kList entries that were gathered, by one warp: bisection by the measure until 32 are left, which are
   // sorted.  1: sh.cut; 2: a comparison was open; 3: in a run of entries equal to sh.cut, ahead of which sh.ahead is found; 0: not here.
@@ -671,7 +689,7 @@ template <int kThreads, bool kCluster> struct Row {
       const bool looked = !(known && round == 0);
       if (looked) g.sum4(a);
       if (round == 0) reach_lo = a[3];
-      const float goal = (float)target, margin = kMass ? 1e-5f * (float)all : 0.f;
+      const float goal = (float)target, margin = kMass ? 2e-5f * (float)all : 0.f;
 #pragma unroll
       for (int j = 0; j < 3; ++j)
         if (looked && x[j] < hi && a[j] < goal - margin) { hi = x[j]; reach_hi = a[j]; }
@@ -752,22 +770,8 @@ template <int kThreads, bool kCluster> struct Row {
       if (sh.solved == 3) return equal_entries<W, kMass>(out.l, sh.ahead, target, all, slack, out);
       return true;
     }
-    if (kOpen) return false;
-    // Not found so (a few values many decades apart, a target that rounding puts beyond all): bisection.
-    uint32_t lo_key = key_of(-INFINITY), hi_key = key_of(wt.max);  // measure above lo_key: the target or more; above hi_key: less
-    double over = 0.0;
-    while (hi_key - lo_key > 1) {
-      const uint32_t mid = lo_key + (hi_key - lo_key) / 2;
-      const float cut = of_key(mid);
-      const double m = g.sum(sum<W, kMass>([&](int, float l, W w) { return l > cut ? (kMass ? w : W(1)) : W(0); }));
-      if (m >= target) lo_key = mid;
-      else { hi_key = mid; over = m; }
-    }
-    out.l = of_key(hi_key);
-    const double ties = (target - over) / (kMass ? (double)wt.get(out.l, W()) : 1.0);
-    out.slot = nth_equal(out.l, ties <= 1.0 ? 0.0 : ceil(fmin(ties, 1e9)) - 1.0);
-    if (out.slot < 0) out.slot = 0x7fffffff;  // all of them
-    return true;
+    // (a few values many decades apart, a target that rounding puts beyond all)
+    return kOpen ? false : bisect<W, kMass>(target, out);
   }
 
   // The draw among what the cut and min-p keep.  False: a comparison was open.
@@ -1112,16 +1116,18 @@ cudaError_t launch_sample(SampleParams p, cudaStream_t s) {
   const int n = p.ids ? p.ld_ids : p.width + Pieces<T>::n - 1;
   auto pieces = [&](int threads) { return ceil_div(ceil_div(n, 4), threads) | 1; };
   p.cluster = 1;
-  // A warp per row costs the fewest instructions, a CTA the least time: few rows whose cut is not found among a few gathered entries take CTAs.
-  const bool few = p.rows <= kFewRows && p.top_p && !p.top_k && n > 2 * kList;
-  const int threads = pieces(32) <= 15 && !few ? 32 : kWide;
-  if (threads == kWide)
-    while (p.cluster < kMaxCluster && pieces(kWide * p.cluster) > 9) p.cluster *= 2;
-  p.pieces = pieces(threads * p.cluster);
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
+  // A warp per row costs the fewest instructions, a CTA the least time: as many rows as there are places for CTAs take these, where the
+  // end of top-p is looked for among all entries.  1858 entries with top-p, us, warps / CTAs: 24 rows 28 / 20, 300 29 / 23, 444 29 / 24,
+  // 600 29 / 33; 600 entries, 24 rows 9.8 / 9.4, 300 11.4 / 11.5.
+  const bool few = p.rows <= 3 * sms && p.top_p && !p.top_k && n > 2 * kList;
+  const int threads = pieces(32) <= 15 && !few ? 32 : kWide;
+  if (threads == kWide)
+    while (p.cluster < kMaxCluster && pieces(kWide * p.cluster) > 9) p.cluster *= 2;
+  p.pieces = pieces(threads * p.cluster);
   p.ahead = sms * 5 * kWarpRows;
   // Bound of a sum's error over the sum of all weights, in steps of 2^-24.  A weight: ex2.approx 3, the factor and the second pieces 1;
   // without the rounding of l - m made good |z| more, z = (l - m) / T, and the sum of w |z| is at most ln(n) < 8 times the sum of w
@@ -1149,8 +1155,10 @@ extern "C" int b200_op_sample(const b200_sample_desc* d, void* stream) {
   if (!d->move_ids && d->n_moves) return bad("lengths without lists of moves");
   if (d->rows == 0) return B200_OK;
   if (!d->logits || !d->u || !d->choice) return bad("logits, random numbers and choices are needed");
-  const int size = d->precision == B200_PREC_FP32 ? 4 : 2;
-  if (reinterpret_cast<uintptr_t>(d->logits) % size) return bad("logits are not aligned to their type");
+  auto off = [](const void* q, uintptr_t n) { return reinterpret_cast<uintptr_t>(q) % n != 0; };
+  if (off(d->logits, d->precision == B200_PREC_FP32 ? 4 : 2) || off(d->move_ids, 2) || off(d->n_moves, 4) || off(d->temperature, 4) ||
+      off(d->top_k, 4) || off(d->top_p, 4) || off(d->min_p, 4) || off(d->u, 4) || off(d->choice, 4) || off(d->prob, 4))
+    return bad("an operand is not aligned to its type");
   SampleParams p = {};
   p.logits = d->logits; p.ld = d->ld ? d->ld : d->width; p.rows = d->rows; p.width = d->width;
   p.ids = d->move_ids; p.counts = d->n_moves; p.ld_ids = d->ld_moves;

@@ -187,6 +187,19 @@ def test_values_that_are_not_finite_stay_with_their_rows(lib):
 
 
 @gpu
+@pytest.mark.parametrize("M,group", [(40, 1), (1536, 64), (8192, 64)])
+def test_narrow_products_beyond_the_range_of_fp16(lib, M, group):
+    """X A^T up to 1e6 met by a small B: results of order one."""
+    c = Call(lib, M, 512, 256, 16, group, 8, 1)
+    c.a *= 2e4
+    c.b *= 1e-5
+    c.a[3] *= 1e-3  # one adapter whose products fit
+    c.run()
+    assert (c.x.float() @ c.a[0].float().T).abs().max() > 65504
+    c.check()
+
+
+@gpu
 def test_captured_call_follows_the_ids(lib):
     c = Call(lib, 8192, 512, 256, 16, 64, 5, 1)
     s = torch.cuda.Stream()
@@ -254,7 +267,7 @@ def test_refusals():
     assert lib.b200_op_gemm_adapters(None, None) == lib.b200_op_gemm_adapters_workspace(None, ctypes.byref(need)) == _lib.ERR_INVALID
     d = _lib.AdaptersDesc(**ok)
     assert lib.b200_op_gemm_adapters_workspace(ctypes.byref(d), None) == _lib.ERR_INVALID
-    for change in (dict(M=-1), dict(N=0), dict(K=0), dict(rank=0), dict(rank=129), dict(n_adapters=0), dict(group=0), dict(precision=3),
+    for change in (dict(M=-1), dict(M=64 * 65535 + 1), dict(N=0), dict(K=0), dict(rank=0), dict(rank=129), dict(n_adapters=0), dict(group=0), dict(precision=3),
                    dict(activation=0), dict(activation=9), dict(ldx=63), dict(ldw=8), dict(ldc=63), dict(ldc=-64)):
         assert both(**change) == (_lib.ERR_INVALID, _lib.ERR_INVALID), change
         assert b"b200_op_gemm_adapters" in lib.b200_last_error()

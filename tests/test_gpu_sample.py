@@ -200,6 +200,29 @@ def test_lists_of_moves(lib, prec, rows, ld_moves):
 
 
 @gpu
+def test_lists_of_entries_of_wide_rows(lib):
+    """Indices are 16 bits: a list names entries among the first 65536 of a wider row and nothing else."""
+    rng = np.random.default_rng(9)
+    held = rng.standard_normal((5, 70000)).astype(np.float32)
+    held[:, 65536:] += 50  # never named
+    ids = rng.integers(0, 65536, (5, 300)).astype(np.uint16)
+    counts = np.array([300, 3, 70, 0, 256], np.int32)
+    u = rng.random(5, np.float32)
+    got = draw(lib, torch.from_numpy(held).cuda(), u, moves=torch.from_numpy(ids).cuda(), counts=torch.from_numpy(counts).cuda())
+    compare([held[i].astype(np.float64)[ids[i, :c]] if c else np.array([-INF]) for i, c in enumerate(counts)], got, u)
+
+
+@gpu
+@pytest.mark.parametrize("temperature", [1e-44, 1e-37, 1e-20, 1e29, 1e31, 3e38, INF])
+def test_temperatures_of_every_size(lib, temperature):
+    rng = np.random.default_rng(4)
+    held = (rng.standard_normal((20, 700)) * 1e3).astype(np.float32)
+    u, T, p = rng.random(20, np.float32), np.full(20, temperature, np.float32), np.full(20, 0.5, np.float32)
+    compare(held.astype(np.float64), draw(lib, torch.from_numpy(held).cuda(), u, temperature=T), u, T=T)
+    compare(held.astype(np.float64), draw(lib, torch.from_numpy(held).cuda(), u, temperature=T, top_p=p), u, T=T, p=p)
+
+
+@gpu
 def test_a_row_does_not_depend_on_its_batch_or_stream(lib):
     g = torch.Generator(device="cuda").manual_seed(1)
     logits, u = torch.randn(2000, 1858, device="cuda", generator=g) * 3, torch.rand(2000, generator=torch.Generator().manual_seed(2)).numpy()
@@ -239,7 +262,8 @@ def test_refusals():
 
     assert lib.b200_op_sample(None, None) == _lib.ERR_INVALID
     for change in (dict(rows=-1), dict(width=0), dict(width=262145), dict(precision=3), dict(precision=-1), dict(ld=9), dict(ld=-1),
-                   dict(logits=None), dict(u=None), dict(choice=None), dict(logits=4098), dict(precision=1, logits=4097),
+                   dict(logits=None), dict(u=None), dict(choice=None), dict(logits=4098), dict(precision=1, logits=4097), dict(u=4098), dict(prob=4097),
+                   dict(top_k=4098), dict(temperature=4099), dict(move_ids=4097, n_moves=4096, ld_moves=4),
                    dict(move_ids=x, ld_moves=4), dict(n_moves=x), dict(move_ids=x, n_moves=x, ld_moves=0),
                    dict(move_ids=x, n_moves=x, ld_moves=65537), dict(rows=1 << 30)):
         assert code(**change) == _lib.ERR_INVALID, change
