@@ -3,8 +3,7 @@
 // Two launches: the narrow product H[m] = s_a X[m] A_a^T [M][rank], and the shared product, which takes H and B in.  The second is
 // made dependent on the first early: it loads and multiplies X and W while H is computed.
 //
-// H, 16-bit, requests of whole 64-row blocks (adapters_shrink_mma_kernel): a CTA takes 64 rows of one request, k-blocks of X and of the
-//   adapter's A arrive by TMA in a ring, four warps multiply 16 rows each by mma.sync: what counts is X's one pass through.
+// H, 16-bit, requests of whole 64-row blocks: adapters_shrink.cu, on tensor cores.
 // H otherwise (adapters_shrink_rows_kernel): a CTA per row, the row in shared memory, a warp per row of A.
 // The shared product, 16-bit: kernels of gemm_tc.cu (H and B as further k-blocks) and gemm_split.cu (added in the epilogue), see
 //   launch_gemm_tc; operands that TMA cannot read: gemm_fma.cu, fp32: gemm_f32.cu or gemm_fma.cu, into fp32 sums, to which
@@ -14,8 +13,6 @@
 #include "tma_mma.cuh"
 
 namespace b200 {
-cudaError_t gemm_tensor_map(const void* ptr, long long ld, int rows, int cols, int box_rows, int prec, CUtensorMap* out);  // gemm_tc.cu
-
 namespace {
 
 struct AdapterParams {
@@ -34,103 +31,6 @@ struct AdapterParams {
 __device__ __forceinline__ int adapter_of(const AdapterParams& p, int m) {
   const int a = p.ids[m / p.group];
   return a >= 0 && a < p.n_adapters ? a : -1;
-}
-
-// ---- H by tensor cores ------------------------------------------------------------------------------------------
-constexpr int kShrinkThreads = 160;  // four warps of 16 rows, one that loads
-template <int NB> struct ShrinkCfg {  // NB: blocks of 16 ranks
-  static constexpr int kStageBytes = 64 * 128 + NB * 16 * 128;
-  static constexpr int kStages = 3;
-  static constexpr int kSmemBytes = kStages * kStageBytes + 1024;
-};
-
-template <typename T, int NB>
-__global__ void __launch_bounds__(kShrinkThreads)
-adapters_shrink_mma_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const AdapterParams p) {
-  using Cfg = ShrinkCfg<NB>;
-  constexpr int S = Cfg::kStages;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[S], empty[S];
-  __shared__ int abort_word;
-  volatile int* abort_flag = &abort_word;
-  const int warp = warp_index(), lane = threadIdx.x & 31;
-  const int m0 = blockIdx.x * 64;
-  const int a = adapter_of(p, m0);
-  grid_launch_dependents();  // nothing of this launch's is read before its end; what it reads was written before it began
-  if (a < 0) return;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < S; ++i) {
-      mbar_init(smem_u32(&full[i]), 1);
-      mbar_init(smem_u32(&empty[i]), 4);
-    }
-    abort_word = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  __syncthreads();
-  const int k_blocks = (p.K + 63) / 64;
-  float acc[2 * NB][4] = {};
-  if (warp == 4) {
-    if (elect_one()) {
-      tma_prefetch_map(&map_x);
-      tma_prefetch_map(&map_a);
-      for (int kb = 0; kb < k_blocks; ++kb) {
-        const int s = kb % S;
-        if (kb >= S && !mbar_wait(smem_u32(&empty[s]), (kb / S - 1) & 1, abort_flag, 1)) break;
-        const uint32_t fb = smem_u32(&full[s]), dst = smem_u32(smem + s * Cfg::kStageBytes);
-        mbar_expect_tx(fb, 64 * 128 + p.rank * 128);
-        tma_load_2d(dst, &map_x, kb * 64, m0, fb);
-        tma_load_2d(dst + 64 * 128, &map_a, kb * 64, a * p.rank, fb);
-      }
-    }
-  } else {
-    const int mat = lane >> 3, row8 = lane & 7;
-    for (int kb = 0; kb < k_blocks; ++kb) {
-      const int s = kb % S;
-      if (!mbar_wait(smem_u32(&full[s]), (kb / S) & 1, abort_flag, 2)) break;
-      const uint8_t* xs = smem + s * Cfg::kStageBytes;
-      const uint8_t* as = xs + 64 * 128;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t fa[4], fb[4];
-        ldmatrix_x4(fa, xs + swz<128>(warp * 16 + (mat & 1) * 8 + row8, 2 * k + (mat >> 1)));
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          ldmatrix_x4(fb, as + swz<128>(n * 16 + (mat >> 1) * 8 + row8, 2 * k + (mat & 1)));
-          mma16816<T>(acc[2 * n], fa, fb[0], fb[1]);
-          mma16816<T>(acc[2 * n + 1], fa, fb[2], fb[3]);
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
-    }
-    const float scale = p.scales ? p.scales[a] : 1.f;
-#pragma unroll
-    for (int n = 0; n < 2 * NB; ++n)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int m = m0 + warp * 16 + (lane >> 2) + 8 * i, r = n * 8 + (lane & 3) * 2;
-        if (m >= p.M || r >= p.rp) continue;  // (the blocks of 16 that a kernel has may be more than rp)
-        // rows of A behind this adapter's, or nothing at all, were multiplied beyond its rank
-        const float h0 = r < p.rank ? scale * acc[n][2 * i] : 0.f, h1 = r + 1 < p.rank ? scale * acc[n][2 * i + 1] : 0.f;
-        float* h = p.H + (long long)m * p.rank + r;
-        if (r < p.rank) h[0] = h0;
-        if (r + 1 < p.rank) h[1] = h1;
-        if (p.pieces) {
-          // the second piece holds what the first one rounds off: fp16 22 bits, bf16 16 of the 24
-          const uint32_t hi = pack2<T>(h0, h1);
-          const float2 f = unpack2<T>(hi);
-          T* q = static_cast<T*>(p.pieces) + (long long)m * 2 * p.rp + r;
-          *reinterpret_cast<uint32_t*>(q) = hi;
-          *reinterpret_cast<uint32_t*>(q + p.rp) = pack2<T>(h0 - f.x, h1 - f.y);
-        }
-      }
-  }
-  __syncthreads();
-  if (abort_word) {
-    for (int i = 0; i < 200; ++i) __nanosleep(1000);  // copies in flight land before the shared memory is released
-    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, 800 + abort_word);
-  }
 }
 
 // ---- H row by row -----------------------------------------------------------------------------------------------
@@ -304,17 +204,6 @@ AdapterPlan plan_of(const b200_adapters_desc& d) {
 // 6.2 / 7.2, 1024x256 rank 16 7.9 / 10.2.
 bool shrink_by_rows(const b200_adapters_desc& d) { return d.K >= 512 && (long long)d.M * d.rank * d.K <= 4 << 20; }
 
-template <typename T, int NB>
-cudaError_t launch_shrink_mma(const AdapterParams& p, cudaStream_t s) {
-  cudaError_t e = raise_smem_limit<adapters_shrink_mma_kernel<T, NB>>(ShrinkCfg<NB>::kSmemBytes);
-  CUtensorMap mx, ma;
-  if (e == cudaSuccess) e = gemm_tensor_map(p.X, p.ldx, p.M, p.K, 64, TypeTag<T>::prec, &mx);
-  if (e == cudaSuccess) e = gemm_tensor_map(p.A, p.K, p.n_adapters * p.rank, p.K, p.rank, TypeTag<T>::prec, &ma);
-  if (e != cudaSuccess) return e;
-  adapters_shrink_mma_kernel<T, NB><<<ceil_div(p.M, 64), kShrinkThreads, ShrinkCfg<NB>::kSmemBytes, s>>>(mx, ma, p);
-  return cudaGetLastError();
-}
-
 template <typename T>
 cudaError_t launch_shrink_rows(const AdapterParams& p, cudaStream_t s) {
   const int per = 16 / (int)sizeof(T);
@@ -350,10 +239,7 @@ int run_adapters(const b200_adapters_desc& d, cudaStream_t s) {
       g.ad_h = p.H;
       if (plan.piece_bytes) g.ad_pieces = p.pieces = ws + plan.h_bytes;
       if (!plan.mma || shrink_by_rows(d)) B200_CUDA(launch_shrink_rows<T>(p, s));
-      else if (p.rp <= 16) B200_CUDA((launch_shrink_mma<T, 1>(p, s)));
-      else if (p.rp <= 32) B200_CUDA((launch_shrink_mma<T, 2>(p, s)));
-      else if (p.rp <= 64) B200_CUDA((launch_shrink_mma<T, 4>(p, s)));
-      else B200_CUDA((launch_shrink_mma<T, 8>(p, s)));
+      else B200_CUDA(launch_adapters_shrink<T>(g, d.A, d.scales, p.H, p.pieces, d.status, s));
       DependentScope dependent;
       B200_CUDA(launch_gemm_tc<T>(g, d.status, sms, s));
       return B200_OK;

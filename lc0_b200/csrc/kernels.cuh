@@ -95,6 +95,9 @@ bool gemm_tc_supported(const GemmParams& p);
 // Whether adapters can be further k-blocks, which needs ad_pieces: every 64 rows one request's, B as TMA reads it.  Without ad_pieces
 // launch_gemm_tc adds them in the epilogue of gemm_split.cu's kernel.
 bool gemm_adapters_pieces(const GemmParams& p);
+// H of the adapters `a` [ad_n][ad_rank][K] (adapters_shrink.cu), 16-bit, requests of whole blocks of 64 rows; pieces may be nullptr.
+template <typename T>
+cudaError_t launch_adapters_shrink(const GemmParams& g, const void* a, const float* scales, float* h, void* pieces, int* status, cudaStream_t s);
 // Product with the LayerNorm of its input in front (gemm_split.cu), for few rows.
 bool gemm_ln_supported(const GemmParams& p);
 template <typename T> cudaError_t launch_gemm_ln(const GemmParams& p, int* status, cudaStream_t s);
