@@ -4,7 +4,7 @@
 // made dependent on the first early: it loads and multiplies X and W while H is computed.
 //
 // H, 16-bit, requests of whole 64-row blocks: adapters_shrink.cu, on tensor cores.
-// H otherwise (adapters_shrink_rows_kernel): a CTA per row, the row in shared memory, a warp per row of A.
+// H otherwise: adapters_shrink_rows_kernel.
 // The shared product, 16-bit: kernels of gemm_tc.cu (H and B as further k-blocks) and gemm_split.cu (added in the epilogue), see
 //   launch_gemm_tc; operands that TMA cannot read: gemm_fma.cu, fp32: gemm_f32.cu or gemm_fma.cu, into fp32 sums, to which
 //   adapters_expand_kernel adds.
@@ -34,62 +34,51 @@ __device__ __forceinline__ int adapter_of(const AdapterParams& p, int m) {
 }
 
 // ---- H row by row -----------------------------------------------------------------------------------------------
-constexpr int kShrinkChunk = 2048;  // numbers of a row held at a time
-
+// A warp per rank, eight of a row to a CTA: what a lane reads of the row and of A is on its way together, and the row's other readers find
+// it in L1 (the row in shared memory first: a second trip to memory, fp32 64x1536x1536 40 us for 37).  Bound by latency at few rows, by
+// what L2 delivers of A, which is read once per row, at many: rank 32 of 4096 rows of 2048, 540 MB.
 template <typename T>
 __global__ void __launch_bounds__(256) adapters_shrink_rows_kernel(const AdapterParams p, int vec) {
-  __shared__ __align__(16) T row[kShrinkChunk];
   constexpr int kPer = 16 / sizeof(T);
   grid_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (r >= p.rp) return;
   for (int m = blockIdx.x; m < p.M; m += gridDim.x) {
     const int a = adapter_of(p, m);
     if (a < 0) continue;  // never read
-    const T* x = static_cast<const T*>(p.X) + (long long)m * p.ldx;
-    const T* w = static_cast<const T*>(p.A) + (long long)a * p.rank * p.K;
-    const float scale = p.scales ? p.scales[a] : 1.f;
-    if (p.pieces && (int)threadIdx.x < 2 * (p.rp - p.rank)) {  // zeros beyond the rank
-      const int half = threadIdx.x & 1, r = p.rank + (threadIdx.x >> 1);
-      static_cast<uint16_t*>(p.pieces)[(long long)m * 2 * p.rp + half * p.rp + r] = 0;
+    T* q = p.pieces ? static_cast<T*>(p.pieces) + (long long)m * 2 * p.rp + r : nullptr;
+    if (r >= p.rank) {  // zeros beyond the rank
+      if (q && lane < 2) q[lane * p.rp] = from_f<T>(0.f);
+      continue;
     }
-    for (int k0 = 0; k0 < p.K; k0 += kShrinkChunk) {
-      const int n = p.K - k0 < kShrinkChunk ? p.K - k0 : kShrinkChunk;
-      __syncthreads();
-      if (vec) {
-        for (int i = threadIdx.x; i < n / kPer; i += 256) reinterpret_cast<uint4*>(row)[i] = reinterpret_cast<const uint4*>(x + k0)[i];
-      } else {
-        for (int i = threadIdx.x; i < n; i += 256) row[i] = x[k0 + i];
-      }
-      __syncthreads();
-      for (int r = warp; r < p.rank; r += 8) {
-        const T* wr = w + (long long)r * p.K + k0;
-        float s = 0.f;
-        if (vec) {
+    const T* x = static_cast<const T*>(p.X) + (long long)m * p.ldx;
+    const T* w = static_cast<const T*>(p.A) + ((long long)a * p.rank + r) * p.K;
+    float s = 0.f;
+    if (vec) {
+      const uint4* x4 = reinterpret_cast<const uint4*>(x);
+      const uint4* w4 = reinterpret_cast<const uint4*>(w);
+      const int n = p.K / kPer;
 #pragma unroll 4
-          for (int i = lane; i < n / kPer; i += 32) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(wr) + i), v = reinterpret_cast<const uint4*>(row)[i];
-            const T* e = reinterpret_cast<const T*>(&u);
-            const T* f = reinterpret_cast<const T*>(&v);
+      for (int i = lane; i < n; i += 32) {
+        const uint4 u = __ldg(w4 + i), v = __ldg(x4 + i);
+        const T* e = reinterpret_cast<const T*>(&u);
+        const T* f = reinterpret_cast<const T*>(&v);
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) s = fmaf(to_f(e[j]), to_f(f[j]), s);
-          }
-        } else {
-          for (int i = lane; i < n; i += 32) s = fmaf(to_f(wr[i]), to_f(row[i]), s);
-        }
-        s = scale * warp_sum(s);
-        float* h = p.H + (long long)m * p.rank + r;
-        if (lane == 0) {
-          if (k0) s += *h;
-          *h = s;
-          if constexpr (sizeof(T) == 2) {
-            if (p.pieces && k0 + n == p.K) {
-              T* q = static_cast<T*>(p.pieces) + (long long)m * 2 * p.rp + r;
-              const uint32_t hi = pack2<T>(s, 0.f);
-              const uint32_t lo = pack2<T>(s - unpack2<T>(hi).x, 0.f);
-              q[0] = *reinterpret_cast<const T*>(&hi);
-              q[p.rp] = *reinterpret_cast<const T*>(&lo);
-            }
-          }
+        for (int j = 0; j < kPer; ++j) s = fmaf(to_f(e[j]), to_f(f[j]), s);
+      }
+    } else {
+#pragma unroll 4
+      for (int i = lane; i < p.K; i += 32) s = fmaf(to_f(w[i]), to_f(x[i]), s);
+    }
+    s = warp_sum(s) * (p.scales ? p.scales[a] : 1.f);
+    if (lane == 0) {
+      p.H[(long long)m * p.rank + r] = s;
+      if constexpr (sizeof(T) == 2) {
+        if (q) {
+          const uint32_t hi = pack2<T>(s, 0.f);
+          const uint32_t lo = pack2<T>(s - unpack2<T>(hi).x, 0.f);
+          q[0] = *reinterpret_cast<const T*>(&hi);
+          q[p.rp] = *reinterpret_cast<const T*>(&lo);
         }
       }
     }
@@ -208,7 +197,7 @@ template <typename T>
 cudaError_t launch_shrink_rows(const AdapterParams& p, cudaStream_t s) {
   const int per = 16 / (int)sizeof(T);
   const int vec = p.K % per == 0 && p.ldx % per == 0 && aligned16(p.X) && aligned16(p.A);
-  adapters_shrink_rows_kernel<T><<<p.M < 65536 ? p.M : 65536, 256, 0, s>>>(p, vec);
+  adapters_shrink_rows_kernel<T><<<dim3(p.M < 65536 ? p.M : 65536, ceil_div(p.pieces ? p.rp : p.rank, 8)), 256, 0, s>>>(p, vec);
   return cudaGetLastError();
 }
 

@@ -811,6 +811,7 @@ template <int kThreads, bool kCluster> struct Row {
       const float* theirs = mine + (o - g.lane) * count;
       const int their_slot = slot0 + (o - g.lane) * count;
       double run = __shfl_sync(0xffffffffu, ahead, o);
+      const double own_sum = __shfl_sync(0xffffffffu, own, o);
       bool found = false;
       for (int base = 0; base < count; base += 32) {
         W w = 0, sum32;
@@ -827,7 +828,9 @@ template <int kThreads, bool kCluster> struct Row {
           const double b = __shfl_sync(0xffffffffu, before, j);
           w_at = (double)__shfl_sync(0xffffffffu, w, j);
           if (hit) {
-            if (kOpen) open |= target - b <= slack * total || b + w_at - target <= slack * total;
+            // the sums ahead of this run of entries, and the run's own five additions
+            const double near_at = slack * total + 12.0 * 0x1p-24 * own_sum;
+            if (kOpen) open |= target - b <= near_at || b + w_at - target <= near_at;
             found = true;
             break;
           }
@@ -1131,8 +1134,8 @@ cudaError_t launch_sample(SampleParams p, cudaStream_t s) {
   p.ahead = sms * 5 * kWarpRows;
   // Bound of a sum's error over the sum of all weights, in steps of 2^-24.  A weight: ex2.approx 3, the factor and the second pieces 1;
   // without the rounding of l - m made good |z| more, z = (l - m) / T, and the sum of w |z| is at most ln(n) < 8 times the sum of w
-  // (of a warp's rows).  Sums: 8 at a time 3; the prefix sums of a warp's entries 5.  Twice that, since two sums are compared.
-  p.slack = 2.f * (3.f + 1.f + (threads == 32 ? 8.f : 0.f) + 8.f) * 0x1p-24f;
+  // (of a warp's rows).  Sums: 8 at a time 3, a total 1.  Twice that, since two sums are compared.
+  p.slack = 2.f * (3.f + 1.f + (threads == 32 ? 8.f : 0.f) + 4.f) * 0x1p-24f;
   if (threads == 32) return launch_group<T, 32, false>(p, s);
   return p.cluster == 1 ? launch_group<T, kWide, false>(p, s) : launch_group<T, kWide, true>(p, s);
 }
