@@ -136,12 +136,12 @@ template <int kThreads, bool kCluster> struct Group {
     return t;
   }
   __device__ __forceinline__ float max(float v) {
-    v = warp_max(v);
+    v = of_key(__reduce_max_sync(0xffffffffu, key_of(v)));
     if (kThreads == 32) return v;
     const double* s = gather((double)v);
-    float t = -INFINITY;
-    for (int i = lane; i < cluster * kWarps; i += 32) t = fmaxf(t, (float)s[i]);
-    return warp_max(t);
+    uint32_t t = 0;
+    for (int i = lane; i < cluster * kWarps; i += 32) t = ::max(t, key_of((float)s[i]));
+    return of_key(__reduce_max_sync(0xffffffffu, t));
   }
   // Sums of four values at once, in a fixed order, for places to look in.
   __device__ __forceinline__ void sum4(float (&a)[4]) {
