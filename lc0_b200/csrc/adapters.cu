@@ -155,8 +155,8 @@ size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; }
 
 // fp32: whether a product is worth cutting its weights into pieces for the tensor cores, which every call does.  us with rank 16, FMA /
-// tensor cores: 64x512x256 22.6 / 21.3, 256x512x256 26.5 / 22.2, 1024x512x256 28.8 / 25.1, 512x1024x1024 53 / 34.5,
-// 64x1536x1536 42.6 / 40, 1024x1536x1536 190 / 95.  Fewer rows than a tile's share W among less than the pieces cost.
+// tensor cores: 64x512x256 20.7 / 20.2, 256x512x256 25.6 / 21.2, 1024x512x256 28.1 / 24.4, 512x1024x1024 51 / 33,
+// 64x1536x1536 40 / 37, 1024x1536x1536 187 / 92.  Fewer rows than a tile's share W among less than the pieces cost.
 bool worth_pieces(const b200_adapters_desc& d) { return d.M >= 64 && (long long)d.M * d.N * d.K >= 1 << 23; }
 
 // What a description is computed by, and its workspace: H, its pieces, the fp32 sums, the pieces of fp32 weights.  Nothing here depends on the device.

@@ -7,7 +7,8 @@
 //
 // The answer is a whole number, so it has to be the one that exact sums give.  Sums of fp32 weights decide where they can: with an
 // error of at most e S (SampleParams::slack) a comparison that is closer than e S is open, and what it belongs to, the cut or the
-// draw, is done again with weights and sums in 64 bits (1858 logits of spread 1.5: 0.3 % of the draws, 1 % of the top-p cuts).
+// draw, is done again with weights and sums in 64 bits (spread 1.5: of 1858 logits 0.7 % of the draws and 1.4 % of the top-p cuts, of
+// 50257 bf16 logits 7.7 % and 9.4 %).
 //
 // A row is held in shared memory as fp32 by a group of threads: a warp, a CTA or a cluster of CTAs.  Thread t owns a run of consecutive
 // entries (an odd number of 16-byte pieces: no bank conflicts), so that sums over threads run in the order of the indices.
@@ -247,8 +248,8 @@ template <int kN> __device__ __forceinline__ void exp_below(double (&x)[kN]) {
   }
 }
 // Weights in fp32 or in 64 bits, of a row whose largest logit is finite.  kFine: the rounding of l - m is made good.  The rows of a warp do
-// without: it is a tenth of a pass over them, and the wider bound of their sums sends 1 % of them into 64 bits; of wider rows,
-// with more comparisons, it would be every third.
+// without, at the price of a wider bound: 1.4 % of them have their top-p cut done again in 64 bits.  Wider rows, whose sums have more
+// terms, keep it.
 template <bool kFine> struct Weight {
   float half_max, c, c_lo, max, temp;
   double inv_t;
