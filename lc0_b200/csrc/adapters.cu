@@ -155,8 +155,8 @@ size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; }
 
 // fp32: whether a product is worth cutting its weights into pieces for the tensor cores, which every call does.  us with rank 16, FMA /
-// tensor cores: 64x512x256 20.7 / 20.2, 256x512x256 25.6 / 21.2, 1024x512x256 28.1 / 24.4, 512x1024x1024 51 / 33,
-// 64x1536x1536 40 / 37, 1024x1536x1536 187 / 92.  Fewer rows than a tile's share W among less than the pieces cost.
+// tensor cores: 64x512x256 20.7 / 19.0, 256x512x256 25.6 / 20.4, 1024x512x256 28.1 / 23.4, 512x1024x1024 51 / 32,
+// 64x1536x1536 40 / 36, 1024x1536x1536 187 / 91.  Fewer rows than a tile's share W among less than the pieces cost.
 bool worth_pieces(const b200_adapters_desc& d) { return d.M >= 64 && (long long)d.M * d.N * d.K >= 1 << 23; }
 
 // What a description is computed by, and its workspace: H, its pieces, the fp32 sums, the pieces of fp32 weights.  Nothing here depends on the device.
@@ -238,7 +238,7 @@ int run_adapters(const b200_adapters_desc& d, cudaStream_t s) {
   g.C = acc; g.ldc = plan.acc_bytes ? d.N : g.ldc; g.out_f32 = true; g.act = ACT_NONE; g.ad_ids = nullptr;
   p.acc = static_cast<const float*>(acc); p.ldacc = g.ldc;
   if (plan.w_bytes) {
-    // (the product fetches the pieces ahead of its dependency: it is not launched dependent on what writes them)
+    // (the product fetches the pieces ahead of its dependency: what it depends on is the launch after the one that writes them)
     B200_CUDA(gemm_tc_init());
     int dev = 0, sms = 0;
     B200_CUDA(cudaGetDevice(&dev));
@@ -246,6 +246,7 @@ int run_adapters(const b200_adapters_desc& d, cudaStream_t s) {
     g.W3 = ws + plan.h_bytes;
     B200_CUDA(launch_split_weights(static_cast<const float*>(d.W), (long long)d.N * d.K, ws + plan.h_bytes, s));
     B200_CUDA(launch_shrink_rows<T>(p, s));
+    DependentScope dependent;
     B200_CUDA(launch_gemm_f32(g, d.status, sms, s));
   } else {
     B200_CUDA(launch_shrink_rows<T>(p, s));
