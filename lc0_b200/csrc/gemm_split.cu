@@ -48,6 +48,8 @@ struct SplitCfg {
   const float* beta;
   int group;
   float eps;
+  // kAdAdd: chains of so many k-blocks each, side by side in tensor memory
+  int chains, chain_blocks, tmem_cols;
 };
 constexpr int kLnK = 256;  // row width of A with a LayerNorm: four k-blocks, all of them resident
 constexpr int kLnMaxGroup = 32;
@@ -240,7 +242,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"((uint32_t)BN)
+                 "r"(kAd == kAdAdd ? (uint32_t)cfg.tmem_cols : (uint32_t)BN)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -309,6 +311,8 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     if (elect_one()) {
       constexpr uint32_t idesc = make_idesc<T, BN>();
       bool ok = !kLN || mbar_wait(smem_u32(a_bar), 0, abort_flag, 5);
+      [[maybe_unused]] int in_chain = 0;
+      [[maybe_unused]] uint32_t sums = tmem;
       int s = 0;
       uint32_t ph = 0;
       for (int i = 0; ok && i < kbn; ++i) {
@@ -317,8 +321,12 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         const uint32_t sa = smem_u32(smem + s * stage_bytes);
         const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + cfg.a_rows * 128);
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k)
-          tcgen05_mma_f16(tmem, adesc + 2 * k, bdesc + 2 * k, idesc, (i > 0 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < BK / 16; ++k) {
+          if constexpr (kAd == kAdAdd) tcgen05_mma_f16(sums, adesc + 2 * k, bdesc + 2 * k, idesc, (in_chain > 0 || k > 0) ? 1u : 0u);
+          else tcgen05_mma_f16(tmem, adesc + 2 * k, bdesc + 2 * k, idesc, (i > 0 || k > 0) ? 1u : 0u);
+        }
+        if constexpr (kAd == kAdAdd)
+          if (++in_chain == cfg.chain_blocks) { in_chain = 0; sums += BN; }
         if (i + S < kbn + ad_blocks) tcgen05_commit(smem_u32(&empty_bar[s]));
         if (++s == S) { s = 0; ph ^= 1; }
       }
@@ -395,6 +403,19 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         const uint32_t ta = tmem + ((uint32_t)(quarter * 32) << 16) + half * kCols + c;
         if constexpr (kStep == 16) tmem_ld16(ta, r); else tmem_ld32(ta, r);
         tmem_ld_wait();
+        if constexpr (kAd == kAdAdd) {
+#pragma unroll 1
+          for (int chain = 1; chain < cfg.chains; ++chain) {
+#pragma unroll
+            for (int h = 0; h < kStep; h += 16) {
+              uint32_t more[16];
+              tmem_ld16(ta + chain * BN + h, more);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) r[h + j] = __float_as_uint(__uint_as_float(r[h + j]) + __uint_as_float(more[j]));
+            }
+          }
+        }
 #pragma unroll
         for (int j = 0; j < kStep; j += 4) {
           // 16-byte pieces swizzled by the row: the 32 rows of a warp write the same columns
@@ -409,7 +430,8 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   if (ks > 1) cluster_sync_all(); else __syncthreads();
   if (warp == 9) {
     tcgen05_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)BN) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kAd == kAdAdd ? (uint32_t)cfg.tmem_cols : (uint32_t)BN)
+                 : "memory");
   }
   if constexpr (kAd == kAdAdd) {
     if (warp < 8) {
@@ -607,16 +629,19 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 //   1x256x2048      32/1 15.2  32/4 7.1   32/8 5.9   64/4 7.2                  32x4096x256    32/1 4.6   64/1 4.7  128/1 5.5
 // A CTA's time grows with its tile's width and its k-blocks, not with a second CTA beside it on the SM: what is waited for is
 // the latency of loads and of the epilogue.  Beyond two CTAs per SM the rest runs in another round.
-struct SplitPlan { int bn, ks, a_rows, stages; };
+struct SplitPlan { int bn, ks, a_rows, stages, chains = 1; };
 
 SplitPlan split_plan(const GemmParams& g, int sm_count) {
   SplitPlan best{64, 1, 128, 1};
   double best_cost = 1e30;
   const int k_blocks = ceil_div(g.K, BK);
   // The tensor core truncates its sums, always towards zero: the error grows with the length of a chain, and fp32 results show it.  Of
-  // adapters' products in fp32 a chain is at most 256 long as far as eight pieces go; the pieces are added in fp32, rounded to nearest.
-  // Relative error (root mean square) of 4000 x 1858 x 2048 bf16, chains of 2048 / 1024 / 512 / 256: 2e-6, 9e-7, 4.4e-7, 2.2e-7.
-  const int longest = g.ad_ids && g.out_f32 ? 4 : k_blocks;
+  // adapters' products in fp32 a chain is at most 256 long, and chains are added in fp32, rounded to nearest.  Relative error (root mean
+  // square) of 4000 x 1858 x 2048 bf16, chains of 2048 / 1024 / 512 / 256: 2e-6, 9e-7, 4.4e-7, 2.2e-7.  They are the pieces of a cluster, up
+  // to eight, or lie side by side in the tensor memory of one CTA, up to 512 columns: not both, since the CTAs of two clusters
+  // that each hold tensor memory and wait for their own would wait for one another.
+  const bool chained = g.ad_ids && g.out_f32;
+  const int longest = 4;
   // of plans that cost the same the one with the taller tiles, which fetch W less often
   for (int a_rows = g.M <= 64 ? 64 : 128; a_rows >= 64; a_rows /= 2) {
     const int m_tiles = ceil_div(g.M, a_rows);
@@ -625,14 +650,15 @@ SplitPlan split_plan(const GemmParams& g, int sm_count) {
       for (int ks = 1; ks <= 8; ks *= 2) {
         if (ks > k_blocks || (ks > 1 && !g.split_k)) break;
         const int kb = ceil_div(k_blocks, ks);
-        if (kb > longest && ks < 8) continue;
+        const int chains = chained && ks == 1 ? ceil_div(kb, longest) : 1, held = bn * chains;
+        if (held > 512 || (chained && ks > 1 && ks < 8 && kb > longest)) continue;
         const long long ctas = (long long)n_tiles * m_tiles * ks;
-        const int rounds = ceil_div(ctas, 2 * sm_count);
+        const int rounds = ceil_div(ctas, held > 256 ? sm_count : 2 * sm_count);
         const double tile = 2.5 + a_rows * bn * (1.0 / 3300), exchange = ks == 1 ? 0.0 : (0.25 + 0.2 * ks) * (a_rows == 64 ? 1.0 : 1.6);
         const double cost = rounds * (tile + 0.39 * kb + exchange + (ctas > sm_count ? 0.5 : 0.0));
         if (cost < best_cost) {
           best_cost = cost;
-          best = SplitPlan{bn, ks, a_rows, kb};
+          best = SplitPlan{bn, ks, a_rows, kb, chains};
         }
       }
     }
@@ -666,7 +692,10 @@ cudaError_t launch_split_bn(const GemmParams& g, const SplitPlan& plan, int* sta
   }
   TcParams p;
   fill_tc_params(p, g, status);
-  const SplitCfg cfg{plan.stages, plan.a_rows, plan.ks, g.A, g.ln_gamma, g.ln_beta, g.ln_group, g.ln_eps};
+  int cols = BN;
+  while (cols < BN * plan.chains) cols *= 2;
+  const int in_chain = plan.chains > 1 ? 4 : 1 << 30;
+  const SplitCfg cfg{plan.stages, plan.a_rows, plan.ks, g.A, g.ln_gamma, g.ln_beta, g.ln_group, g.ln_eps, plan.chains, in_chain, cols};
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3(ceil_div(g.N, BN) * plan.ks, ceil_div(g.M, plan.a_rows));
   lc.blockDim = dim3(kSplitThreads);

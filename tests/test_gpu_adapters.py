@@ -155,6 +155,16 @@ def test_fp32_results_do_not_show_long_chains(lib, prec, M, N, K, rank, group):
 
 
 @gpu
+@pytest.mark.parametrize("prec", [1, 2])
+@pytest.mark.parametrize("M,N,group", [(500, 264, 1), (1500, 1000, 1), (1984, 520, 64)])
+@pytest.mark.parametrize("K,rank", [(264, 16), (328, 16), (576, 48), (2056, 8), (2112, 128), (4104, 16), (8200, 32)])
+def test_fp32_results_with_chains_that_end_early(lib, prec, M, N, group, K, rank):
+    c = Call(lib, M, N, K, rank, group, 9, prec, out_f32=1)
+    c.run()
+    c.check()
+
+
+@gpu
 @pytest.mark.parametrize("prec", [0, 1, 2])
 @pytest.mark.parametrize("pads,shift", [((8, 8, 8), 0), ((1, 3, 5), 0), ((8, 8, 8), 8), ((8, 8, 8), 1), ((0, 0, 1), 0), ((0, 8, 0), 3)])
 @pytest.mark.parametrize("M,N,K,group", [(70, 72, 96, 1), (6400, 512, 256, 64)])
