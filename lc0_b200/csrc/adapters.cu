@@ -180,8 +180,9 @@ AdapterPlan plan_of(const b200_adapters_desc& d) {
   if (out.mma && !g.out_f32 && gemm_adapters_pieces(g)) out.piece_bytes = round256((size_t)d.M * 2 * g.ad_rp * 2);
   // sums of the shared product: in C itself where it holds floats
   if (!out.tensor && !g.out_f32) out.acc_bytes = round256((size_t)d.M * d.N * 4);
-  // fp32 on tensor cores: W is cut into pieces by every call
-  g.W3 = d.precision == B200_PREC_FP32 ? d.X : nullptr;  // (any aligned address, for the question alone)
+  // fp32 on tensor cores: W is cut into pieces by every call.  The question needs the address of pieces, which are laid out after it is
+  // answered: any aligned one, none of the description's, which need not be set yet.
+  g.W3 = reinterpret_cast<const void*>(uintptr_t(256));
   if (d.precision == B200_PREC_FP32 && worth_pieces(d) && gemm_f32_supported(g)) out.w_bytes = round256((size_t)d.N * d.K * 6);
   g.W3 = nullptr;
   return out;

@@ -304,3 +304,19 @@ def test_refusals():
                    dict(ids=4098), dict(scales=4097), dict(status=4098)):
         assert both(**change) == (_lib.OK, _lib.ERR_INVALID), change
     assert both(M=0, X=None, W=None, C=None, A=None, B=None, ids=None, workspace=None) == (_lib.OK, _lib.OK)
+
+
+@pytest.mark.parametrize("prec", [0, 1, 2])
+@pytest.mark.parametrize("out_f32", [0, 1])
+@pytest.mark.parametrize("M,N,K,rank,group", [(1, 8, 8, 1, 1), (1024, 512, 256, 16, 1), (1024, 512, 256, 16, 64), (64, 512, 256, 16, 64), (63, 512, 256, 16, 1),
+                                              (1000, 500, 252, 13, 7), (8192, 1024, 1024, 64, 64), (4096, 1858, 2048, 32, 1)])
+def test_workspace_of_a_description_without_pointers(prec, out_f32, M, N, K, rank, group):
+    """The size asked for before the tensors exist is that of the call with them."""
+    lib = _lib.load()
+    sizes = []
+    for pointers in ({}, dict(X=4096, W=8192, C=12288, A=4096, B=4096, ids=4096, bias=4096, scales=4096)):
+        d = _lib.AdaptersDesc(M=M, N=N, K=K, activation=oracle.ACT_NONE, precision=prec, out_f32=out_f32, n_adapters=5, rank=rank, group=group, **pointers)
+        need = ctypes.c_size_t()
+        assert lib.b200_op_gemm_adapters_workspace(ctypes.byref(d), ctypes.byref(need)) == _lib.OK
+        sizes.append(need.value)
+    assert sizes[0] == sizes[1]
