@@ -743,7 +743,8 @@ template <int kThreads, bool kCluster> struct Row {
         }
       }
       const double front = g.sum(more);
-      if (kCluster) g.barrier();  // the lists are read across the cluster
+      // the lists are read across the warp (whose sum is shuffles alone, which order no memory), the CTA (the sum has a barrier) or the cluster
+      if (kThreads == 32 || kCluster) g.barrier();
       int n = sh.count;
       if (kCluster) {
         n = g.lane < g.cluster ? *cg::this_cluster().map_shared_rank(&sh.count, g.lane) : 0;

@@ -235,6 +235,25 @@ def test_a_row_does_not_depend_on_its_batch_or_stream(lib):
         assert np.allclose(part[1], whole[1][5:5 + n], rtol=80 * 2.0 ** -24, atol=0)
 
 
+
+@gpu
+@pytest.mark.parametrize("grid", [0, 8])
+def test_rows_of_warps_that_gather_unevenly(lib, grid):
+    """The end of top-p among entries that the lanes of a warp put side by side, some lanes many, most none: logits fall over the row,
+    so that the heavy ones are one lane's.  The same answer every time."""
+    rng = np.random.default_rng(grid)
+    rows, width = 2000, 1200
+    held = rng.standard_normal((rows, width)) - np.linspace(0, 12, width) * rng.uniform(0, 1, (rows, 1))
+    held = (np.round(held * grid) / grid if grid else held).astype(np.float32)
+    u, p = rng.random(rows, np.float32), rng.uniform(0.05, 0.99, rows).astype(np.float32)
+    logits = torch.from_numpy(held).cuda()
+    first = draw(lib, logits, u, top_p=p)
+    compare(held.astype(np.float64), first, u, p=p)
+    for _ in range(4):
+        again = draw(lib, logits, u, top_p=p)
+        assert np.array_equal(again[0], first[0]) and np.array_equal(again[1], first[1])
+
+
 @gpu
 def test_captured_and_replayed(lib):
     logits, u = torch.randn(64, 1858, device="cuda"), torch.rand(64, device="cuda")
