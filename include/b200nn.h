@@ -427,7 +427,8 @@ int b200_op_gemm_adapters(const b200_adapters_desc* d, void* stream);
  *   keeps the first k; top_p those ahead of which the weights of what top_k kept sum to less than top_p of their total, and the
  *   first; min_p those with w >= min_p.  choice: the first kept entry, by index, at which the sum of the kept weights passes
  *   u times their total: its column, or its place in the list of moves.  prob (may be NULL): its weight over that total.
- *   -1 and 0 for a row without entries; -2 where a bounded device-side wait gave up (rows of more than 9000 entries, a defect).
+ *   -1 and 0 for a row without entries; -2 and 0 where a bounded device-side wait gave up (rows of more than 9000 entries, which a
+ *   cluster of CTAs has, after 2 s; a defect).
  *   The choice is the one that sums in 64 bits give.  Allocates nothing, does not synchronise, may be captured. */
 #define B200_SAMPLE_MAX_WIDTH 262144
 typedef struct b200_sample_desc {
@@ -438,6 +439,9 @@ typedef struct b200_sample_desc {
   int* choice; float* prob;
 } b200_sample_desc;
 int b200_op_sample(const b200_sample_desc* d, void* stream);
+/* Failure-injection hook for tests of that exit, process-wide: in calls from now on CTA `cta` (from 0) of each cluster behaves at its wait
+ * number `wait` (from 0) as if it had run out, and all others run out after 1 ms.  A negative number: no longer. */
+void b200_op_sample_inject_give_up(int cta, int wait);
 int b200_op_layer_norm(void* out, const void* x, const void* skip, const float* gamma,
                        const float* beta, int rows, int C, float alpha, float eps, int precision,
                        void* stream);

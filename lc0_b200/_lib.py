@@ -159,6 +159,7 @@ SIGNATURES = {
     "b200_op_gemm_adapters_workspace": (_I, [ctypes.POINTER(AdaptersDesc), ctypes.POINTER(ctypes.c_size_t)]),
     "b200_op_gemm_adapters": (_I, [ctypes.POINTER(AdaptersDesc), _P]),
     "b200_op_sample": (_I, [ctypes.POINTER(SampleDesc), _P]),
+    "b200_op_sample_inject_give_up": (None, [_I, _I]),
     "b200_op_layer_norm": (_I, [_P, _P, _P, _P, _P, _I, _I, _F, _F, _I, _P]),
 }
 

@@ -14,6 +14,8 @@
 // entries (an odd number of 16-byte pieces: no bank conflicts), so that sums over threads run in the order of the indices.
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "../../include/b200nn.h"
 #include "kernels.cuh"
 
@@ -38,6 +40,8 @@ struct SampleParams {
   int cluster;  // CTAs per row (kCluster)
   int ahead;    // rows of one round of CTAs
   float slack;  // bound of a sum's error, relative to the sum of all weights
+  unsigned long long wait_ns;  // after which a wait for the other CTAs of a cluster gives up
+  int give_up_cta, give_up_at;  // for tests: this CTA of each cluster gives up at its wait of this number; -1: none
 };
 
 // Larger keys are larger logits; -0 and +0 have one key.
@@ -53,16 +57,24 @@ template <int kThreads, bool kCluster> struct Group {
   static constexpr int kSlots = kCluster ? kMaxCluster * kWarps : kWarps;
   double* slots;  // [2][kSlots], kThreads > 32
   float* wide;    // [2][kSlots][4]
-  uint64_t* bars;  // [2], kCluster
-  int cluster, crank, turn;
-  bool gave_up;   // a wait for the other CTAs has ended without them
+  uint64_t* bars;  // [2] for exchanges, one for meetings; kCluster
+  int cluster, crank, turn, meetings;
+  unsigned long long wait_ns;
+  int give_up_at;
+  // A wait for the other CTAs has ended without them: the same in all threads of a CTA, which then make no further exchange (sums are 0,
+  // maxima -infinity, whatever has arrived) and leave.  The others' waits end the same way, so that every thread gets to the
+  // two cluster barriers of the hardware, which have no limit: one before the first exchange, one before the end.
+  bool gave_up;
   int lane, warp;
-  __device__ Group(double* s, float* s4, uint64_t* b, int cl) : slots(s), wide(s4), bars(b), cluster(kCluster ? cl : 1), crank(0), turn(0), gave_up(false) {
+  __device__ Group(double* s, float* s4, uint64_t* b, const SampleParams& p)
+      : slots(s), wide(s4), bars(b), cluster(kCluster ? p.cluster : 1), crank(0), turn(0), meetings(0), wait_ns(p.wait_ns), give_up_at(-1), gave_up(false) {
     lane = threadIdx.x & 31;
     warp = kThreads == 32 ? 0 : threadIdx.x >> 5;
     if (kCluster) {
       crank = (int)cg::this_cluster().block_rank();
-      if (threadIdx.x < 2) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(address(bars + threadIdx.x)) : "memory");
+      if (crank == p.give_up_cta) give_up_at = p.give_up_at;
+      if (threadIdx.x < 3)
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(address(bars + threadIdx.x)), "r"(threadIdx.x < 2 ? 1 : cluster) : "memory");
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");  // (the row is read, and a barrier passed, before their first use)
     }
   }
@@ -78,9 +90,10 @@ template <int kThreads, bool kCluster> struct Group {
     if (threadIdx.x == 0)
       asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(address(bars + (turn & 1))), "r"(bytes) : "memory");
   }
-  __device__ __forceinline__ void await() {
-    const uint32_t bar = address(bars + (turn & 1)), parity = turn >> 1 & 1;
+  __device__ __forceinline__ void wait(const uint64_t* b, uint32_t parity) {
+    const uint32_t bar = address(b);
     unsigned long long t0 = 0;
+    gave_up = turn + meetings == give_up_at;
     for (int it = 0; !gave_up; ++it) {
       uint32_t ok;
       asm volatile(
@@ -95,16 +108,29 @@ template <int kThreads, bool kCluster> struct Group {
         unsigned long long now;
         asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
         if (t0 == 0) t0 = now;
-        gave_up = now - t0 > 2000000000ull;  // 2 s
+        gave_up = now - t0 > wait_ns;
       }
     }
+    gave_up = __syncthreads_or(gave_up) != 0;
+  }
+  __device__ __forceinline__ void await() {
+    wait(bars + (turn & 1), turn >> 1 & 1);
     ++turn;
+  }
+  // All threads of the cluster, and what they have written to shared memory: a barrier with a limit.
+  __device__ __forceinline__ void meet() {
+    __syncthreads();
+    if (gave_up) return;
+    if ((int)threadIdx.x < cluster)
+      asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(address(bars + 2, threadIdx.x)) : "memory");
+    wait(bars + 2, meetings & 1);
+    ++meetings;
   }
   __device__ __forceinline__ int thread() const { return (crank * kWarps + warp) * 32 + lane; }
   __device__ __forceinline__ int threads() const { return cluster * kThreads; }
-  __device__ __forceinline__ void barrier() const {
+  __device__ __forceinline__ void barrier() {
     if (kThreads == 32) __syncwarp();
-    else if (kCluster) cg::this_cluster().sync();
+    else if (kCluster) meet();
     else __syncthreads();
   }
   // One value per warp, seen by all threads of the group afterwards.  Two sets of slots in turn: the barrier of one exchange
@@ -112,6 +138,7 @@ template <int kThreads, bool kCluster> struct Group {
   __device__ __forceinline__ const double* gather(double v) {
     double* mine = slots + (turn & 1) * kSlots;
     if (kCluster) {
+      if (gave_up) return mine;
       expect(cluster * kWarps * 8);
       if (lane < cluster)
         asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(address(mine + crank * kWarps + warp, lane)),
@@ -130,6 +157,7 @@ template <int kThreads, bool kCluster> struct Group {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (kThreads == 32) return v;
     const double* s = gather(v);
+    if (kCluster && gave_up) return 0.0;
     double t = 0.0;
     for (int i = lane; i < cluster * kWarps; i += 32) t += s[i];
 #pragma unroll
@@ -140,6 +168,7 @@ template <int kThreads, bool kCluster> struct Group {
     v = of_key(__reduce_max_sync(0xffffffffu, key_of(v)));
     if (kThreads == 32) return v;
     const double* s = gather((double)v);
+    if (kCluster && gave_up) return -INFINITY;
     uint32_t t = 0;
     for (int i = lane; i < cluster * kWarps; i += 32) t = ::max(t, key_of((float)s[i]));
     return of_key(__reduce_max_sync(0xffffffffu, t));
@@ -161,12 +190,18 @@ template <int kThreads, bool kCluster> struct Group {
       float* mine = wide + (turn & 1) * kSlots * 4;
       const int at = (crank * kWarps + warp) * 4 + (lane >> 3);
       if (kCluster) {
-        expect(cluster * kWarps * 16);
-        if ((lane & 7) < cluster)
-          asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(address(mine + at, lane & 7)),
-                       "r"(__float_as_uint(v)), "r"(address(bars + (turn & 1), lane & 7))
-                       : "memory");
-        await();
+        if (!gave_up) {
+          expect(cluster * kWarps * 16);
+          if ((lane & 7) < cluster)
+            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(address(mine + at, lane & 7)),
+                         "r"(__float_as_uint(v)), "r"(address(bars + (turn & 1), lane & 7))
+                         : "memory");
+          await();
+        }
+        if (gave_up) {
+          a[0] = a[1] = a[2] = a[3] = 0.f;
+          return;
+        }
       } else {
         ++turn;
         if ((lane & 7) == 0) mine[at] = v;
@@ -196,6 +231,10 @@ template <int kThreads, bool kCluster> struct Group {
       return ex;
     }
     const double* s = gather(warp_total);
+    if (kCluster && gave_up) {
+      total = 0.0;
+      return 0.0;
+    }
     // every warp scans the warps' sums in the same order, a few per lane
     constexpr int kEach = (kSlots + 31) / 32;
     const int mine = crank * kWarps + warp;
@@ -400,7 +439,7 @@ template <int kThreads, bool kCluster> struct Shared {
   int list_slot[kList];
   uint64_t sorted[32];
   double weights[kThreads == 32 ? kSort : 1];
-  uint64_t bars[2];
+  uint64_t bars[3];
   double ahead;
   int count;
   int solved;
@@ -534,6 +573,7 @@ template <int kThreads, bool kCluster> struct Row {
       const uint32_t mid = lo_key + (hi_key - lo_key) / 2;
       const float cut = of_key(mid);
       const double m = g.sum(sum<W, kMass>([&](int, float l, W w) { return l > cut ? (kMass ? w : W(1)) : W(0); }));
+      if (kCluster && g.gave_up) return true;
       if (m >= target) lo_key = mid;
       else { hi_key = mid; over = m; }
     }
@@ -689,6 +729,7 @@ template <int kThreads, bool kCluster> struct Row {
       }
       const bool looked = !(known && round == 0);
       if (looked) g.sum4(a);
+      if (kCluster && g.gave_up) return true;
       if (round == 0) reach_lo = a[3];
       const float goal = (float)target, margin = kMass ? 2e-5f * (float)all : 0.f;
 #pragma unroll
@@ -709,6 +750,7 @@ template <int kThreads, bool kCluster> struct Row {
       hi_at = hi;
       // the exact measure above them, and the entries between them, marked 32 at a time
       g.barrier();  // the others are done with what is cleared
+      if (kCluster && g.gave_up) return true;
       if (tid == 0) sh.count = 0;
       if (kThreads == 32) __syncwarp(); else __syncthreads();
       float down = INFINITY, up = -INFINITY;
@@ -745,6 +787,7 @@ template <int kThreads, bool kCluster> struct Row {
       const double front = g.sum(more);
       // the lists are read across the warp (whose sum is shuffles alone, which order no memory), the CTA (the sum has a barrier) or the cluster
       if (kThreads == 32 || kCluster) g.barrier();
+      if (kCluster && g.gave_up) return true;
       int n = sh.count;
       if (kCluster) {
         n = g.lane < g.cluster ? *cg::this_cluster().map_shared_rank(&sh.count, g.lane) : 0;
@@ -754,6 +797,7 @@ template <int kThreads, bool kCluster> struct Row {
       if (n > kList) {
         hi = g.max(up);  // the entries' own ends
         const float bottom = -g.max(-down);
+        if (kCluster && g.gave_up) return true;
         reach_hi = (float)front;
         if (hi == bottom) return equal_entries<W, kMass>(hi, front, target, all, slack, out);
         // the largest of them is above every next pivot but not above `hi`
@@ -795,6 +839,7 @@ template <int kThreads, bool kCluster> struct Row {
     }
     double total;
     const double ahead = g.before(own, total), target = (double)u * total;
+    if (kCluster && g.gave_up) return true;
     const bool here = ahead <= target && target < ahead + own;
     // the warp of the thread whose entries the sum passes the target in looks for the entry together
     const float id = (float)g.thread();
@@ -803,6 +848,7 @@ template <int kThreads, bool kCluster> struct Row {
     if (!kOpen) {  // neighbours' bounds can differ in their last bit: the first that claims it, else the last with a weight
       owner = -g.max(here ? -id : -INFINITY);
       if (owner == INFINITY) owner = g.max(own > 0.0 ? id : -INFINITY);
+      if (kCluster && g.gave_up) return true;
       claims = id == owner;
     }
     const uint32_t ballot = __ballot_sync(0xffffffffu, claims);
@@ -842,7 +888,9 @@ template <int kThreads, bool kCluster> struct Row {
       if (kOpen && !found) open = true;
     }
     if (kOpen) {
-      if (g.sum((open ? 1048576.0 : 0.0) + (claims ? 1.0 : 0.0)) != 1.0) return false;
+      const double one = g.sum((open ? 1048576.0 : 0.0) + (claims ? 1.0 : 0.0));
+      if (kCluster && g.gave_up) return true;
+      if (one != 1.0) return false;
     }
     if (claims) {
       if (kOpen) w_at = wt.get(mine[at - slot0], 0.0);
@@ -1014,7 +1062,7 @@ sample_kernel(const SampleParams p) {
   const int cap = kThreads * 4 * p.pieces;
   float* v = reinterpret_cast<float*>(smem) + part * cap;
   Shared<kThreads, kCluster>& sh = shared[part];
-  Group<kThreads, kCluster> g(sh.slots, sh.wide, sh.bars, p.cluster);
+  Group<kThreads, kCluster> g(sh.slots, sh.wide, sh.bars, p);
   const int row = kThreads == 32 ? blockIdx.x * kWarpRows + part : blockIdx.x / p.cluster;
   if (row >= p.rows) return;
   float temp = p.temperature ? p.temperature[row] : 1.f;
@@ -1028,14 +1076,17 @@ sample_kernel(const SampleParams p) {
   }
   int n = 0;
   const int first = load_row<T, kThreads, kCluster>(p, g, row, v, cap, n);
-  g.barrier();
+  if (kCluster) cg::this_cluster().sync();  // the barriers of all CTAs are there
+  else g.barrier();
   const int local = (kThreads == 32 ? g.lane : (int)threadIdx.x) * 4 * p.pieces;
   Row<kThreads, kCluster> r{g, sh, p, v + local, g.crank * cap + local, 4 * p.pieces, row, first, Weight<(kThreads > 32)>(0.f, 1.f)};
   float own_max = -INFINITY;
   r.each([&](int, float l) { own_max = fmaxf(own_max, l); });
   float m = g.max(own_max);
   bool done = false;
-  if (m == -INFINITY) {
+  if (kCluster && g.gave_up) {
+    done = true;
+  } else if (m == -INFINITY) {
     if (g.thread() == 0) r.give(-1, 0.f);
     done = true;
   } else if (!(temp > 0.f)) {  // the first of the largest
@@ -1048,6 +1099,7 @@ sample_kernel(const SampleParams p) {
     m = 0.f;
     temp = 1.f;
     g.barrier();
+    done = g.gave_up;
   }
   if (!done) {
     r.wt = Weight<(kThreads > 32)>(m, temp);
@@ -1076,7 +1128,7 @@ sample_kernel(const SampleParams p) {
           least = fminf(least, l > -INFINITY ? l : INFINITY);
         });
         if ((double)k < g.sum((double)own)) {
-          least = -g.max(-least);
+          least = -g.max(-least);  // (without the others: infinity; select finds that out)
           float lo_at = 0.f, hi_at = INFINITY;
           r.template select<float, false>(n, (double)k, m, least, 0.0, lo_at, hi_at, cut);
           if (tp < 1.f) r.keep(cut);
@@ -1091,8 +1143,14 @@ sample_kernel(const SampleParams p) {
     }
   }
   if (kCluster) {
-    g.barrier();  // no CTA leaves while another may still reach into its shared memory
-    if (g.gave_up) p.choice[row] = -2;
+    cg::this_cluster().sync();  // no CTA leaves while another may still reach into its shared memory
+    if (g.gave_up) {
+      for (int i = 0; i < 200; ++i) __nanosleep(1000);  // what others have sent without being waited for lands before the shared memory is released
+      if (threadIdx.x == 0) {  // behind the barrier: over what another CTA may have answered
+        p.choice[row] = -2;
+        if (p.prob) p.prob[row] = 0.f;
+      }
+    }
   }
 }
 
@@ -1114,6 +1172,8 @@ cudaError_t launch_group(const SampleParams& p, cudaStream_t s) {
   cfg.numAttrs = kCluster ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, sample_kernel<T, kThreads, kCluster>, p);
 }
+
+std::atomic<long long> give_up{-1};  // CTA << 32 | wait, below 0: none (see b200_op_sample_inject_give_up)
 
 template <typename T>
 cudaError_t launch_sample(SampleParams p, cudaStream_t s) {
@@ -1169,9 +1229,17 @@ extern "C" int b200_op_sample(const b200_sample_desc* d, void* stream) {
   p.ids = d->move_ids; p.counts = d->n_moves; p.ld_ids = d->ld_moves;
   p.temperature = d->temperature; p.top_k = d->top_k; p.top_p = d->top_p; p.min_p = d->min_p; p.u = d->u;
   p.choice = d->choice; p.prob = d->prob;
+  const long long injected = give_up.load(std::memory_order_relaxed);
+  p.wait_ns = injected < 0 ? 2000000000ull : 1000000ull;  // 2 s; 1 ms where one is known not to come
+  p.give_up_cta = injected < 0 ? -1 : (int)(injected >> 32);
+  p.give_up_at = injected < 0 ? -1 : (int)(injected & 0x7fffffff);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (d->precision == B200_PREC_FP32) B200_CUDA(launch_sample<float>(p, s));
   else if (d->precision == B200_PREC_FP16) B200_CUDA(launch_sample<__half>(p, s));
   else B200_CUDA(launch_sample<__nv_bfloat16>(p, s));
   return B200_OK;
+}
+
+extern "C" void b200_op_sample_inject_give_up(int cta, int wait) {
+  b200::give_up.store(cta < 0 || wait < 0 ? -1 : (long long)cta << 32 | wait, std::memory_order_relaxed);
 }

@@ -254,6 +254,41 @@ def test_rows_of_warps_that_gather_unevenly(lib, grid):
         assert np.array_equal(again[0], first[0]) and np.array_equal(again[1], first[1])
 
 
+
+@gpu
+@pytest.mark.parametrize("kind", ["plain", "k", "p", "all"])
+@pytest.mark.parametrize("rows,width", [(1, 262144), (40, 20000), (150, 50257)])
+def test_waits_that_give_up(lib, kind, rows, width):
+    """One CTA of a cluster gives up at any of its waits, the others wait for it in vain: the launch ends, and a row has its answer (where
+    that CTA has fewer waits) or -2 and 0."""
+    rng = np.random.default_rng(rows)
+    held = torch.from_numpy((rng.standard_normal((rows, width)) * 2).astype(np.float32)).to(torch.bfloat16)
+    logits = held.cuda()
+    T, k, p, m = settings(rng, rows, kind)
+    if kind == "k":
+        k = rng.integers(1, width, rows).astype(np.int32)
+    u = rng.random(rows, np.float32)
+    call = lambda: draw(lib, logits, u, temperature=T, top_k=k, top_p=p, min_p=m)
+    right = call()
+    at = sorted(rng.choice(rows, min(rows, 5), replace=False))
+    one = lambda v: None if v is None else v[at]
+    compare(held[at].double().numpy(), (right[0][at], right[1][at]), u[at], one(T), one(k), one(p), one(m))
+    gave_up = []
+    try:
+        for wait in range(14):
+            lib.b200_op_sample_inject_give_up(wait * 5 % (2 if width < 50000 else 4), wait)
+            choice, prob = call()
+            out = choice == -2
+            gave_up.append(int(out.sum()))
+            assert (prob[out] == 0).all()
+            assert np.array_equal(choice[~out], right[0][~out]) and np.array_equal(prob[~out], right[1][~out]), wait
+    finally:
+        lib.b200_op_sample_inject_give_up(-1, -1)
+    assert gave_up[0] == rows and gave_up == sorted(gave_up, reverse=True), gave_up
+    again = call()
+    assert np.array_equal(again[0], right[0]) and np.array_equal(again[1], right[1])
+
+
 @gpu
 def test_captured_and_replayed(lib):
     logits, u = torch.randn(64, 1858, device="cuda"), torch.rand(64, device="cuda")
