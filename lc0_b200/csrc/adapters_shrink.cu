@@ -4,8 +4,10 @@
 // side: every row meets both and keeps its own.  That doubles multiplications which cost nothing (256 of a k-block's columns at most)
 // and needs no masks.  X's and A's k-blocks arrive by TMA in a ring of about 100 KB, two CTAs to an SM; one thread issues
 // tcgen05.mma (cta_group::1, 128 x 2 rank x 16), the accumulator is in tensor memory, and a thread of the epilogue has a row: H as
-// fp32 and, where the shared product takes it as k-blocks, as two values of the type: the second holds what the first rounds off
+// fp32 (for a product with fp32 results, which shows that the tensor core truncates its sums, from two accumulators in turn that leave
+// tensor memory after every k-block and are added in registers) and, where the shared product takes it as k-blocks, as two values of the type: the second holds what the first rounds off
 // (fp16 22 bits of the 24 in all, bf16 16).
+#include "../../include/b200nn.h"
 #include "kernels.cuh"
 #include "tcgen05.cuh"
 
@@ -19,7 +21,6 @@ struct ShrinkParams {
   const float* scales; const int* ids;
   float* H; void* pieces;
   int M, K, rank, rp, group, n_adapters, stages, tmem_cols;
-  int chains, chain_blocks;  // sums of so many k-blocks each, side by side in tensor memory
   int* status;
 };
 
@@ -30,13 +31,13 @@ template <typename T> __device__ __forceinline__ uint32_t both(T lo, T hi) {
   return (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
 }
 
-template <typename T>
+template <typename T, bool kRounded>
 __global__ void __launch_bounds__(kShrinkThreads, 2)
 adapters_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const ShrinkParams p) {
   constexpr int kMaxStages = 8;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done;
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], done[2], taken[2];  // kRounded: an accumulator each, else done[0]
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
@@ -60,7 +61,10 @@ adapters_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
       mbar_init(smem_u32(&full[i]), 1);
       mbar_init(smem_u32(&empty[i]), 1);
     }
-    mbar_init(smem_u32(&done), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&done[i]), 1);
+      mbar_init(smem_u32(&taken[i]), 4);
+    }
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -98,71 +102,102 @@ adapters_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
-      int in_chain = 0;
-      uint32_t sums = tmem;
       for (int kb = 0; kb < k_blocks; ++kb) {
+        if (kRounded && !mbar_wait(smem_u32(&taken[kb & 1]), (kb >> 1 & 1) ^ 1, abort_flag, 4)) { ok = false; break; }
         if (!mbar_wait(smem_u32(&full[s]), ph, abort_flag, 2)) { ok = false; break; }
         tcgen05_fence_after();
-        const uint32_t sa = smem_u32(smem + s * stage_bytes);
+        const uint32_t sa = smem_u32(smem + s * stage_bytes), sums = tmem + (kRounded ? (kb & 1) * 2 * p.rp : 0);
         const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + BM * 128);
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k) tcgen05_mma_f16(sums, adesc + 2 * k, bdesc + 2 * k, idesc, (in_chain > 0 || k > 0) ? 1u : 0u);
-        if (++in_chain == p.chain_blocks) { in_chain = 0; sums += 2 * p.rp; }
+        for (int k = 0; k < BK / 16; ++k) tcgen05_mma_f16(sums, adesc + 2 * k, bdesc + 2 * k, idesc, ((!kRounded && kb > 0) || k > 0) ? 1u : 0u);
         tcgen05_commit(smem_u32(&empty[s]));
+        if (kRounded) tcgen05_commit(smem_u32(&done[kb & 1]));
         if (++s == S) { s = 0; ph ^= 1; }
       }
-      if (ok) tcgen05_commit(smem_u32(&done));
+      if (ok && !kRounded) tcgen05_commit(smem_u32(&done[0]));
     }
     __syncwarp();
   } else {
     const int row = warp * 32 + lane, m = m0 + row;
     const int a = warp < 2 ? a0 : a1;  // the same in the whole warp
     const float scale = a >= 0 && p.scales ? p.scales[a] : 1.f;
-    const bool there = mbar_wait(smem_u32(&done), 0, abort_flag, 3);
-    tcgen05_fence_after();
-    if (there && a >= 0) {
-      const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + (two && a == a1 ? p.rp : 0);
-      float* h = p.H + (long long)m * p.rank;
-      T* q = static_cast<T*>(p.pieces) + (long long)m * 2 * p.rp;
-      for (int r0 = 0; r0 < p.rp; r0 += 16) {
-        uint32_t v[16];
-        tmem_ld16(from + r0, v);
-        tmem_ld_wait();
-        float x[16];
+    const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + (two && a == a1 ? p.rp : 0);
+    float* h = p.H + (long long)m * p.rank;
+    T* q = static_cast<T*>(p.pieces) + (long long)m * 2 * p.rp;
+    // sixteen ranks of the row, from r0 on
+    auto finish = [&](int r0, float (&x)[16]) {
+      // beyond the rank what lay behind A's rows was multiplied
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = r0 + j < p.rank ? scale * x[j] : 0.f;
+      if (m >= p.M) return;
+      if (p.rank % 4 == 0) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 4)
+          if (r0 + j < p.rank) *reinterpret_cast<float4*>(h + r0 + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (r0 + j < p.rank) h[r0 + j] = x[j];
+      }
+      if (!kRounded && p.pieces) {
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const T c0 = narrow(x[2 * j], T()), c1 = narrow(x[2 * j + 1], T());
+          hi[j] = both(c0, c1);
+          lo[j] = both(narrow(x[2 * j] - to_f(c0), T()), narrow(x[2 * j + 1] - to_f(c1), T()));
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          *reinterpret_cast<uint4*>(q + r0 + 2 * j) = make_uint4(hi[j], hi[j + 1], hi[j + 2], hi[j + 3]);
+          *reinterpret_cast<uint4*>(q + p.rp + r0 + 2 * j) = make_uint4(lo[j], lo[j + 1], lo[j + 2], lo[j + 3]);
+        }
+      }
+    };
+    if constexpr (kRounded) {
+      constexpr int kMost = (B200_ADAPTERS_MAX_RANK + 15) / 16;
+      float x[kMost][16];
+#pragma unroll
+      for (int i = 0; i < kMost; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[i][j] = 0.f;
+      bool there = true;
 #pragma unroll 1
-        for (int chain = 1; chain < p.chains; ++chain) {
-          uint32_t more[16];
-          tmem_ld16(from + chain * 2 * p.rp + r0, more);
+      for (int kb = 0; kb < k_blocks && there; ++kb) {
+        there = mbar_wait(smem_u32(&done[kb & 1]), kb >> 1 & 1, abort_flag, 3);
+        tcgen05_fence_after();
+        if (there && a >= 0) {
+#pragma unroll
+          for (int i = 0; i < kMost; ++i) {
+            if (i * 16 >= p.rp) break;
+            uint32_t v[16];
+            tmem_ld16(from + (kb & 1) * 2 * p.rp + i * 16, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[i][j] += __uint_as_float(v[j]);
+          }
+        }
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&taken[kb & 1]));
+      }
+      if (there && a >= 0) {
+#pragma unroll
+        for (int i = 0; i < kMost; ++i)
+          if (i * 16 < p.rp) finish(i * 16, x[i]);
+      }
+    } else {
+      const bool there = mbar_wait(smem_u32(&done[0]), 0, abort_flag, 3);
+      tcgen05_fence_after();
+      if (there && a >= 0) {
+        for (int r0 = 0; r0 < p.rp; r0 += 16) {
+          uint32_t v[16];
+          tmem_ld16(from + r0, v);
           tmem_ld_wait();
+          float x[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(more[j]));
-        }
-        // beyond the rank what lay behind A's rows was multiplied
-#pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = r0 + j < p.rank ? scale * __uint_as_float(v[j]) : 0.f;
-        if (m >= p.M) continue;
-        if (p.rank % 4 == 0) {
-#pragma unroll
-          for (int j = 0; j < 16; j += 4)
-            if (r0 + j < p.rank) *reinterpret_cast<float4*>(h + r0 + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (r0 + j < p.rank) h[r0 + j] = x[j];
-        }
-        if (p.pieces) {
-          uint32_t hi[8], lo[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const T c0 = narrow(x[2 * j], T()), c1 = narrow(x[2 * j + 1], T());
-            hi[j] = both(c0, c1);
-            lo[j] = both(narrow(x[2 * j] - to_f(c0), T()), narrow(x[2 * j + 1] - to_f(c1), T()));
-          }
-#pragma unroll
-          for (int j = 0; j < 8; j += 4) {
-            *reinterpret_cast<uint4*>(q + r0 + 2 * j) = make_uint4(hi[j], hi[j + 1], hi[j + 2], hi[j + 3]);
-            *reinterpret_cast<uint4*>(q + p.rp + r0 + 2 * j) = make_uint4(lo[j], lo[j + 1], lo[j + 2], lo[j + 3]);
-          }
+          for (int j = 0; j < 16; ++j) x[j] = __uint_as_float(v[j]);
+          finish(r0, x);
         }
       }
     }
@@ -190,22 +225,16 @@ cudaError_t launch_adapters_shrink(const GemmParams& g, const void* a, const flo
   p.stages = kShrinkRing / stage;
   if (p.stages > 8) p.stages = 8;
   if (p.stages > k_blocks) p.stages = k_blocks;
-  // A result in fp32 shows that the tensor core truncates its sums, the more the longer they are: chains of 256, as far as half of the
-  // tensor memory goes (two CTAs share it), are added in fp32.  K 2048, rank 16, squared ReLU, bf16: 1.1e-6 -> 4.3e-7.
-  p.chain_blocks = k_blocks;
-  if (g.out_f32) {
-    const int most = 128 / p.rp;
-    p.chain_blocks = ceil_div(k_blocks, most) > 4 ? ceil_div(k_blocks, most) : 4;
-  }
-  p.chains = ceil_div(k_blocks, p.chain_blocks);
   p.tmem_cols = 32;
-  while (p.tmem_cols < 2 * p.rp * p.chains) p.tmem_cols *= 2;
-  cudaError_t e = raise_smem_limit<adapters_shrink_kernel<T>>(kShrinkRing + 1024);
+  while (p.tmem_cols < (g.out_f32 ? 4 : 2) * p.rp) p.tmem_cols *= 2;
+  cudaError_t e = g.out_f32 ? raise_smem_limit<adapters_shrink_kernel<T, true>>(kShrinkRing + 1024)
+                            : raise_smem_limit<adapters_shrink_kernel<T, false>>(kShrinkRing + 1024);
   CUtensorMap mx, ma;
   if (e == cudaSuccess) e = gemm_tensor_map(g.A, g.lda, g.M, g.K, BM, TypeTag<T>::prec, &mx);
   if (e == cudaSuccess) e = gemm_tensor_map(a, g.K, g.ad_n * g.ad_rank, g.K, g.ad_rank, TypeTag<T>::prec, &ma);
   if (e != cudaSuccess) return e;
-  adapters_shrink_kernel<T><<<ceil_div(g.M, BM), kShrinkThreads, p.stages * stage + 1024, s>>>(mx, ma, p);
+  auto* kernel = g.out_f32 ? adapters_shrink_kernel<T, true> : adapters_shrink_kernel<T, false>;
+  kernel<<<ceil_div(g.M, BM), kShrinkThreads, p.stages * stage + 1024, s>>>(mx, ma, p);
   return cudaGetLastError();
 }
 template cudaError_t launch_adapters_shrink<__half>(const GemmParams&, const void*, const float*, float*, void*, int*, cudaStream_t);

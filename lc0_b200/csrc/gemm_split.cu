@@ -26,6 +26,9 @@
 // With adapters (kAd) the product takes H . B^T in.  kAdBlocks: as further k-blocks of one CTA of the cluster, like gemm_tc.cu's pair kernel;
 // kAdAdd: a warp per row adds it in fp32 to the sums in shared memory, for requests of any number of rows and
 // operands that TMA cannot read.  The kernel before this one only writes H: A and W are loaded and multiplied while it runs.
+// The tensor core truncates its sums, always towards zero, the more the longer they are.  Results of 16 bits hide it; for fp32
+// results (kAdRounded) there are two accumulators in turn, which leave tensor memory after a k-block each, to be added in registers,
+// rounded to nearest, while the next one is multiplied.
 // Every wait is bounded by wall-clock time like those of gemm_tc.cu; the cluster barriers are reached by all threads
 // whatever happened before them.
 #include <atomic>
@@ -48,8 +51,6 @@ struct SplitCfg {
   const float* beta;
   int group;
   float eps;
-  // kAdAdd: chains of so many k-blocks each, side by side in tensor memory
-  int chains, chain_blocks, tmem_cols;
 };
 constexpr int kLnK = 256;  // row width of A with a LayerNorm: four k-blocks, all of them resident
 constexpr int kLnMaxGroup = 32;
@@ -165,7 +166,7 @@ ln_rows_kernel(const T* x, T* out, const float* __restrict__ gamma, const float*
   }
 }
 
-enum SplitAdapters { kAdNone = 0, kAdAdd = 1, kAdBlocks = 2 };
+enum SplitAdapters { kAdNone = 0, kAdAdd = 1, kAdBlocks = 2, kAdRounded = 3 };
 
 // H[m] . B_a[n] for any rank and alignment.
 template <typename T>
@@ -187,7 +188,7 @@ __device__ __noinline__ float adapter_element(const T* x, const T* w, int K, con
 }
 
 template <typename T, int BN, bool kLN, int kAd>
-__global__ void __launch_bounds__(kSplitThreads)
+__global__ void __launch_bounds__(kSplitThreads, kAd == kAdRounded ? 2 : 0)
 gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                   const __grid_constant__ CUtensorMap tmap_h, const __grid_constant__ CUtensorMap tmap_b, const TcParams p,
                   const SplitCfg cfg) {
@@ -204,6 +205,8 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint64_t* gb_bar = reinterpret_cast<uint64_t*>(misc + 216);    // kLN: gamma and beta have landed
   uint64_t* a_bar = gb_bar + 1;                                  // kLN: the normalised rows are in place
+  uint64_t* tfull1_bar = reinterpret_cast<uint64_t*>(misc + 216);  // kAdRounded: the second accumulator complete
+  uint64_t* tempty_bar = tfull1_bar + 1;                           // kAdRounded: [2] accumulators read
   float4* rowv = reinterpret_cast<float4*>(misc + 256);          // [rows of this CTA's slice] mean_a, rstd_a, mean_r, rstd_r
   float* ln_gb = reinterpret_cast<float*>(misc + 256 + 128 * 16);  // kLN: gamma [group * 256], beta [group * 256]
 
@@ -237,12 +240,17 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       mbar_init(smem_u32(gb_bar), 1);
       mbar_init(smem_u32(a_bar), 256);
     }
+    if (kAd == kAdRounded) {
+      mbar_init(smem_u32(tfull1_bar), 1);
+      mbar_init(smem_u32(&tempty_bar[0]), 8);
+      mbar_init(smem_u32(&tempty_bar[1]), 8);
+    }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(kAd == kAdAdd ? (uint32_t)cfg.tmem_cols : (uint32_t)BN)
+                 "r"(kAd == kAdRounded ? 2u * BN : (uint32_t)BN)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -258,6 +266,9 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   const int rp = cfg.a_rows / ks;  // rows of the slice
   const int cg = tid % kGroups, r0 = tid / kGroups, col = n0 + cg * 8;
   float vb[8], vc[8], vg[8], ve[8];
+  constexpr bool kEncoder = kAd != kAdRounded;  // (statistics and residuals are the encoder's alone; without them there are registers for the sums)
+  constexpr int kCols = BN / 2;  // columns of an epilogue warp's half of the tile
+  [[maybe_unused]] float sums[kAd == kAdRounded ? kCols : 1];
 
   if (warp == 8) {
     // ---------------- TMA producer ----------------
@@ -311,23 +322,23 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     if (elect_one()) {
       constexpr uint32_t idesc = make_idesc<T, BN>();
       bool ok = !kLN || mbar_wait(smem_u32(a_bar), 0, abort_flag, 5);
-      [[maybe_unused]] int in_chain = 0;
-      [[maybe_unused]] uint32_t sums = tmem;
       int s = 0;
       uint32_t ph = 0;
       for (int i = 0; ok && i < kbn; ++i) {
+        if constexpr (kAd == kAdRounded)
+          if (!mbar_wait(smem_u32(&tempty_bar[i & 1]), (i >> 1 & 1) ^ 1, abort_flag, 7)) { ok = false; break; }
         if (!mbar_wait(smem_u32(&full_bar[s]), ph, abort_flag, 3)) { ok = false; break; }
         tcgen05_fence_after();
         const uint32_t sa = smem_u32(smem + s * stage_bytes);
         const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + cfg.a_rows * 128);
 #pragma unroll
         for (int k = 0; k < BK / 16; ++k) {
-          if constexpr (kAd == kAdAdd) tcgen05_mma_f16(sums, adesc + 2 * k, bdesc + 2 * k, idesc, (in_chain > 0 || k > 0) ? 1u : 0u);
+          if constexpr (kAd == kAdRounded)
+            tcgen05_mma_f16(tmem + (i & 1) * BN, adesc + 2 * k, bdesc + 2 * k, idesc, k > 0 ? 1u : 0u);
           else tcgen05_mma_f16(tmem, adesc + 2 * k, bdesc + 2 * k, idesc, (i > 0 || k > 0) ? 1u : 0u);
         }
-        if constexpr (kAd == kAdAdd)
-          if (++in_chain == cfg.chain_blocks) { in_chain = 0; sums += BN; }
         if (i + S < kbn + ad_blocks) tcgen05_commit(smem_u32(&empty_bar[s]));
+        if constexpr (kAd == kAdRounded) tcgen05_commit(smem_u32(i & 1 ? tfull1_bar : tfull_bar));
         if (++s == S) { s = 0; ph ^= 1; }
       }
       if constexpr (kAd == kAdBlocks) {
@@ -345,18 +356,18 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
           if (++s == S) { s = 0; ph ^= 1; }
         }
       }
-      if (ok) tcgen05_commit(smem_u32(tfull_bar));
+      if (ok && kAd != kAdRounded) tcgen05_commit(smem_u32(tfull_bar));
     }
     __syncwarp();
   } else {
     // per-column vectors (constants) and per-row vectors (written by the kernels before this one) while the tile is computed
     if (p.bias) load8(p.bias, col, p.N, vb);
-    if (p.a_stats) load8(p.colsum, col, p.N, vc);
-    if (p.res_mode == 2) {
+    if (kEncoder && p.a_stats) load8(p.colsum, col, p.N, vc);
+    if (kEncoder && p.res_mode == 2) {
       load8(p.res_gamma, col, p.N, vg);
       load8(p.res_beta, col, p.N, ve);
     }
-    grid_dependency_wait();
+    if (kAd != kAdRounded) grid_dependency_wait();
     if constexpr (kLN) {
       const int row = tid >> 2, q = tid & 3;  // piece c of a row is piece c % 8 of k-block c / 8
       uint4 u[8];
@@ -375,7 +386,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       fence_async_smem();  // the tensor core reads the rows through the asynchronous proxy
       mbar_arrive(smem_u32(a_bar));
     }
-    if (tid < rp && (p.a_stats || p.res_mode == 2)) {
+    if (kEncoder && tid < rp && (p.a_stats || p.res_mode == 2)) {
       const int m = m0 + rank * rp + tid;
       float4 v = make_float4(0.f, 1.f, 0.f, 1.f);
       if (m < p.M) {
@@ -384,37 +395,69 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       }
       rowv[tid] = v;
     }
-    mbar_wait(smem_u32(tfull_bar), 0, abort_flag, 4);
-    tcgen05_fence_after();
+    if constexpr (kAd == kAdRounded) {
+      const int quarter = warp & 3;
+      const uint32_t ta = tmem + ((uint32_t)(quarter * 32) << 16) + (warp >> 2) * kCols;
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) sums[j] = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < kbn; ++c) {
+        if (!mbar_wait(smem_u32(c & 1 ? tfull1_bar : tfull_bar), c >> 1 & 1, abort_flag, 4)) break;
+        tcgen05_fence_after();
+        if (quarter * 32 < cfg.a_rows) {
+#pragma unroll
+          for (int j0 = 0; j0 < kCols; j0 += 16) {
+            uint32_t r[16];
+            tmem_ld16(ta + (c & 1) * BN + j0, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sums[j0 + j] += __uint_as_float(r[j]);
+          }
+        }
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[c & 1]));
+      }
+      grid_dependency_wait();  // H; the product was none of its business
+    } else {
+      mbar_wait(smem_u32(tfull_bar), 0, abort_flag, 4);
+      tcgen05_fence_after();
+    }
   }
   // The partial tiles overwrite the ring of the CTA that owns them: its MMAs must have read their last stage.
-  if (ks > 1) cluster_sync_all();
+  if constexpr (kAd == kAdRounded) {
+    // Two accumulators are not held while the cluster waits: CTAs that each wait for tensor memory that another cluster holds would
+    // wait for ever.  The warp that gives it back has arrived at the cluster's barrier before, nobody waits for it.
+    if (warp == 9) {
+      if (ks > 1) cluster_arrive();
+      asm volatile("bar.sync 2, 288;" ::: "memory");
+      tcgen05_fence_after();
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2u * BN) : "memory");
+      if (ks > 1) cluster_wait();
+    } else {
+      if (warp < 8) asm volatile("bar.arrive 2, 288;" ::: "memory");
+      if (ks > 1) cluster_sync_all();
+    }
+  } else if (ks > 1) {
+    cluster_sync_all();
+  }
   if (warp < 8) {
     const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
     if (quarter * 32 < cfg.a_rows) {
-      constexpr int kCols = BN / 2;  // columns of this warp's half
-      constexpr int kStep = kCols < 32 ? 16 : 32;
+      constexpr int kStep = kCols < 32 || kAd == kAdRounded ? 16 : 32;
       const int owner = row / rp, rr = row - owner * rp;
       uint32_t dst = smem_u32(smem) + (uint32_t)((rank * rp + rr) * BN) * 4;
       if (ks > 1) dst = mapa(dst, (uint32_t)owner);
 #pragma unroll
       for (int c = 0; c < kCols; c += kStep) {
         uint32_t r[kStep];
-        const uint32_t ta = tmem + ((uint32_t)(quarter * 32) << 16) + half * kCols + c;
-        if constexpr (kStep == 16) tmem_ld16(ta, r); else tmem_ld32(ta, r);
-        tmem_ld_wait();
-        if constexpr (kAd == kAdAdd) {
-#pragma unroll 1
-          for (int chain = 1; chain < cfg.chains; ++chain) {
+        if constexpr (kAd == kAdRounded) {
 #pragma unroll
-            for (int h = 0; h < kStep; h += 16) {
-              uint32_t more[16];
-              tmem_ld16(ta + chain * BN + h, more);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 16; ++j) r[h + j] = __float_as_uint(__uint_as_float(r[h + j]) + __uint_as_float(more[j]));
-            }
-          }
+          for (int j = 0; j < kStep; ++j) r[j] = __float_as_uint(sums[c + j]);
+        } else {
+          const uint32_t ta = tmem + ((uint32_t)(quarter * 32) << 16) + half * kCols + c;
+          if constexpr (kStep == 16) tmem_ld16(ta, r); else tmem_ld32(ta, r);
+          tmem_ld_wait();
         }
 #pragma unroll
         for (int j = 0; j < kStep; j += 4) {
@@ -428,12 +471,11 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   }
   tcgen05_fence_before();
   if (ks > 1) cluster_sync_all(); else __syncthreads();
-  if (warp == 9) {
+  if (kAd != kAdRounded && warp == 9) {
     tcgen05_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kAd == kAdAdd ? (uint32_t)cfg.tmem_cols : (uint32_t)BN)
-                 : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)BN) : "memory");
   }
-  if constexpr (kAd == kAdAdd) {
+  if constexpr (kAd == kAdAdd || kAd == kAdRounded) {
     if (warp < 8) {
       float* part = reinterpret_cast<float*>(smem);
       const int pieces = p.ad_rank / 8;  // of 16 bytes in a row of B
@@ -480,7 +522,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     const uint32_t row_lanes = (kGroups == 32 ? 0xffffffffu : ((1u << kGroups) - 1u)) << (lane & ~(kGroups - 1));
     const float* part = reinterpret_cast<const float*>(smem);
     const bool whole = col + 8 <= p.N;
-    const bool second = p.n_split > 0 && col >= p.n_split;
+    const bool second = kEncoder && p.n_split > 0 && col >= p.n_split;
 #pragma unroll 1
     for (int r = r0; r < rp; r += kRowStep) {
       const int m = m0 + rank * rp + r;
@@ -494,12 +536,12 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         const float4 b = *reinterpret_cast<const float4*>(src + (((2 * cg + 1) ^ (r & 7)) << 2));
         v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w; v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
       }
-      const float4 rv = (p.a_stats || p.res_mode == 2) ? rowv[r] : make_float4(0.f, 1.f, 0.f, 1.f);
-      if (p.scale != 1.0f) {
+      const float4 rv = kEncoder && (p.a_stats || p.res_mode == 2) ? rowv[r] : make_float4(0.f, 1.f, 0.f, 1.f);
+      if (kEncoder && p.scale != 1.0f) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] *= p.scale;
       }
-      if (p.a_stats) {
+      if (kEncoder && p.a_stats) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = rv.y * (v[i] - rv.x * vc[i]);
       }
@@ -538,7 +580,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       } else {
         apply_activation(v, p.act);
       }
-      if (p.res_mode) {
+      if (kEncoder && p.res_mode) {
         const T* rs = reinterpret_cast<const T*>(p.res) + (long long)m * p.ldres + col;
         float s[8];
         if (whole) {
@@ -558,7 +600,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = fmaf(p.alpha, v[i], s[i]);
       }
-      if (p.out_stats) {
+      if (kEncoder && p.out_stats) {
         // Sums of 32 columns (four lanes, one after the other) in fp32, their totals in double: the order of gemm_tc.cu,
         // so that a row's statistics do not depend on which kernel took the product.
         float a = 0.f, q = 0.f;
@@ -629,19 +671,12 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 //   1x256x2048      32/1 15.2  32/4 7.1   32/8 5.9   64/4 7.2                  32x4096x256    32/1 4.6   64/1 4.7  128/1 5.5
 // A CTA's time grows with its tile's width and its k-blocks, not with a second CTA beside it on the SM: what is waited for is
 // the latency of loads and of the epilogue.  Beyond two CTAs per SM the rest runs in another round.
-struct SplitPlan { int bn, ks, a_rows, stages, chains = 1; };
+struct SplitPlan { int bn, ks, a_rows, stages; };
 
 SplitPlan split_plan(const GemmParams& g, int sm_count) {
   SplitPlan best{64, 1, 128, 1};
   double best_cost = 1e30;
   const int k_blocks = ceil_div(g.K, BK);
-  // The tensor core truncates its sums, always towards zero: the error grows with the length of a chain, and fp32 results show it.  Of
-  // adapters' products in fp32 a chain is at most 256 long, and chains are added in fp32, rounded to nearest.  Relative error (root mean
-  // square) of 4000 x 1858 x 2048 bf16, chains of 2048 / 1024 / 512 / 256: 2e-6, 9e-7, 4.4e-7, 2.2e-7.  They are the pieces of a cluster, up
-  // to eight, or lie side by side in the tensor memory of one CTA, up to 512 columns: not both, since the CTAs of two clusters
-  // that each hold tensor memory and wait for their own would wait for one another.
-  const bool chained = g.ad_ids && g.out_f32;
-  const int longest = 4;
   // of plans that cost the same the one with the taller tiles, which fetch W less often
   for (int a_rows = g.M <= 64 ? 64 : 128; a_rows >= 64; a_rows /= 2) {
     const int m_tiles = ceil_div(g.M, a_rows);
@@ -650,15 +685,13 @@ SplitPlan split_plan(const GemmParams& g, int sm_count) {
       for (int ks = 1; ks <= 8; ks *= 2) {
         if (ks > k_blocks || (ks > 1 && !g.split_k)) break;
         const int kb = ceil_div(k_blocks, ks);
-        const int chains = chained && ks == 1 ? ceil_div(kb, longest) : 1, held = bn * chains;
-        if (held > 512 || (chained && ks > 1 && ks < 8 && kb > longest)) continue;
         const long long ctas = (long long)n_tiles * m_tiles * ks;
-        const int rounds = ceil_div(ctas, held > 256 ? sm_count : 2 * sm_count);
+        const int rounds = ceil_div(ctas, 2 * sm_count);
         const double tile = 2.5 + a_rows * bn * (1.0 / 3300), exchange = ks == 1 ? 0.0 : (0.25 + 0.2 * ks) * (a_rows == 64 ? 1.0 : 1.6);
         const double cost = rounds * (tile + 0.39 * kb + exchange + (ctas > sm_count ? 0.5 : 0.0));
         if (cost < best_cost) {
           best_cost = cost;
-          best = SplitPlan{bn, ks, a_rows, kb, chains};
+          best = SplitPlan{bn, ks, a_rows, kb};
         }
       }
     }
@@ -692,10 +725,7 @@ cudaError_t launch_split_bn(const GemmParams& g, const SplitPlan& plan, int* sta
   }
   TcParams p;
   fill_tc_params(p, g, status);
-  int cols = BN;
-  while (cols < BN * plan.chains) cols *= 2;
-  const int in_chain = plan.chains > 1 ? 4 : 1 << 30;
-  const SplitCfg cfg{plan.stages, plan.a_rows, plan.ks, g.A, g.ln_gamma, g.ln_beta, g.ln_group, g.ln_eps, plan.chains, in_chain, cols};
+  const SplitCfg cfg{plan.stages, plan.a_rows, plan.ks, g.A, g.ln_gamma, g.ln_beta, g.ln_group, g.ln_eps};
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3(ceil_div(g.N, BN) * plan.ks, ceil_div(g.M, plan.a_rows));
   lc.blockDim = dim3(kSplitThreads);
@@ -758,6 +788,11 @@ cudaError_t launch_gemm_split(const GemmParams& g, int* status, int sm_count, cu
     if (plan.bn == 32) return launch_split_bn<T, 32, false, kAdBlocks>(g, with, status, s);
     if (plan.bn == 64) return launch_split_bn<T, 64, false, kAdBlocks>(g, with, status, s);
     return launch_split_bn<T, 128, false, kAdBlocks>(g, with, status, s);
+  }
+  if (g.ad_ids && g.out_f32) {
+    if (plan.bn == 32) return launch_split_bn<T, 32, false, kAdRounded>(g, plan, status, s);
+    if (plan.bn == 64) return launch_split_bn<T, 64, false, kAdRounded>(g, plan, status, s);
+    return launch_split_bn<T, 128, false, kAdRounded>(g, plan, status, s);
   }
   if (g.ad_ids) {
     if (plan.bn == 32) return launch_split_bn<T, 32, false, kAdAdd>(g, plan, status, s);

@@ -154,6 +154,60 @@ def test_fp32_results_do_not_show_long_chains(lib, prec, M, N, K, rank, group):
     assert off <= (16 * 2 / 3 * 2 + 7) * 2.0 ** -24, off
 
 
+
+def rounded(K, rank=0):
+    """Relative error, root mean square, of sums whose every 64 terms are four truncated additions and whose further ones are rounded.  A
+    truncation takes half a step of 2^-23 on average, 0.72 of that in relation to the sum, which grows like the root of its
+    place: 0.36 (0.5 + 0.71 + 0.87 + 1) = 1.1 steps, always towards zero, so that all chains together are off by as much.  A rounding is off
+    by 1 / sqrt(12) of a step, 0.43 of 2^-24 in relation to the sum; K / 64 of them, of sums that grow, and those over the ranks.  A tenth for chance."""
+    return 1.1 * (2.2 ** 2 + 0.43 ** 2 * (K / 128 + rank / 2)) ** 0.5 * 2.0 ** -24
+
+
+@gpu
+@pytest.mark.parametrize("prec", [1, 2])
+@pytest.mark.parametrize("M,N,K,group", [(37, 1858, 256, 1), (4000, 1858, 256, 1), (4000, 520, 512, 1), (1000, 1000, 1000, 1), (37, 1858, 2048, 1), (500, 1858, 4096, 1),
+                                         (4000, 256, 2560, 1), (4000, 1858, 8192, 1), (2048, 1024, 256, 64), (8192, 512, 1024, 64)])
+def test_fp32_results_are_as_exact_as_a_plain_product(lib, prec, M, N, K, group):
+    """Of the rows without an adapter: within the error derived above or that of a product in fp32 of the same numbers (of fp16 the
+    products themselves have 22 bits, and any sum of them rounds more often)."""
+    c = Call(lib, M, N, K, 16, group, 20, prec, out_f32=1, bias=False, ids=torch.arange((M + group - 1) // group) % 3 - 1)
+    c.run()
+    c.check()
+    alone = (c.ids < 0).repeat_interleave(group)[:M]
+    want = c.want()[0][alone]
+    plain = c.x[alone].float() @ c.w.float().T
+    rms = lambda v: ((v.double() - want).norm() / want.norm()).item()
+    assert rms(c.out[alone]) <= max(rounded(K), 1.05 * rms(plain)), (rms(c.out[alone]), rms(plain))
+
+
+@gpu
+@pytest.mark.parametrize("prec", [1, 2])
+@pytest.mark.parametrize("M,N,K,rank,group", [(2048, 256, 256, 16, 64), (2048, 256, 2048, 16, 64), (4096, 264, 2048, 128, 64), (4160, 256, 8192, 40, 192),
+                                              (50, 256, 2048, 16, 1)])
+def test_fp32_results_of_adapters_alone(lib, prec, M, N, K, rank, group):
+    """A shared product of zeros: what is left shows how X A^T was summed."""
+    c = Call(lib, M, N, K, rank, group, 20, prec, out_f32=1, bias=False, ids=torch.arange((M + group - 1) // group) % 20)
+    c.w.zero_()
+    c.run()
+    want = c.want()[0]
+    x, ids = c.x.float(), c.ids.long().repeat_interleave(group)[:M]
+    plain = torch.cat([c.scales[j] * (x[i:i + 1] @ c.a[j].float().T @ c.b[j].float().T) for i, j in enumerate(ids.tolist()[:200])])
+    off = ((c.out.double() - want).norm() / want.norm()).item()
+    of_plain = ((plain.double() - want[:200]).norm() / want[:200].norm()).item()
+    assert off <= max(rounded(K, rank), 1.05 * of_plain), (off, of_plain)
+
+
+@gpu
+@pytest.mark.parametrize("prec", [1, 2])
+@pytest.mark.parametrize("K", [256, 2048])
+def test_fp32_results_are_not_biased_towards_zero(lib, prec, K):
+    """Squared ReLU doubles what truncation takes from every sum."""
+    c = Call(lib, 2000, 1858, K, 16, 1, 20, prec, act=oracle.ACT_RELU_2, out_f32=1, bias=False, ids=torch.full((2000,), -1))
+    c.run()
+    want = c.want()[0]
+    assert abs(((c.out.double() - want).sum() / want.sum()).item()) <= 2 * rounded(0)
+
+
 @gpu
 @pytest.mark.parametrize("prec", [1, 2])
 @pytest.mark.parametrize("M,N,group", [(500, 264, 1), (1500, 1000, 1), (1984, 520, 64)])
