@@ -399,7 +399,9 @@ int b200_op_policy_attention_static(const void* q, const void* k, const float* w
  *   - workspace: b200_op_gemm_adapters_workspace() bytes of device memory on a 256-byte boundary, for this call alone until it has
  *     run (two captured graphs that may overlap need two); status: device int or NULL, set non-zero (and never cleared) if a
  *     bounded device-side wait gave up, the result is then undefined.
- *   Sums in fp32.  Allocates nothing, does not synchronise, may be captured.  C may not overlap an input.  The ids are read on the
+ *   Sums in fp32; results in fp32 are as exact as a plain fp32 product.  For results of 16 bits scales[a] X . A[a]^T is held as two values of
+ *   the type where it goes through the tensor cores: to 2^-22 of itself or 2^-36 (fp16), to 2^-16 (bf16), well below the result's rounding.
+ *   Allocates nothing, does not synchronise, may be captured.  C may not overlap an input.  The ids are read on the
  *   device: a captured call follows what they hold when it is replayed. */
 #define B200_ADAPTERS_MAX_RANK 128
 typedef struct b200_adapters_desc {

@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(256) adapters_shrink_rows_kernel(const Adapter
       if constexpr (sizeof(T) == 2) {
         if (q) {
           const uint32_t hi = pack2<T>(s, 0.f);
-          const uint32_t lo = pack2<T>(s - unpack2<T>(hi).x, 0.f);
+          const uint32_t lo = pack2<T>((s - unpack2<T>(hi).x) * (1 << LowPiece<T>::shift), 0.f);
           q[0] = *reinterpret_cast<const T*>(&hi);
           q[p.rp] = *reinterpret_cast<const T*>(&lo);
         }

@@ -6,7 +6,7 @@
 // tcgen05.mma (cta_group::1, 128 x 2 rank x 16), the accumulator is in tensor memory, and a thread of the epilogue has a row: H as
 // fp32 (for a product with fp32 results, which shows that the tensor core truncates its sums, from two accumulators in turn that leave
 // tensor memory after every k-block and are added in registers) and, where the shared product takes it as k-blocks, as two values of the type: the second holds what the first rounds off
-// (fp16 22 bits of the 24 in all, bf16 16).
+// (fp16, where it is scaled by 2^11, 22 bits of the 24 in all, down to 2^-36; bf16 16).
 #include "../../include/b200nn.h"
 #include "kernels.cuh"
 #include "tcgen05.cuh"
@@ -145,7 +145,8 @@ adapters_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         for (int j = 0; j < 8; ++j) {
           const T c0 = narrow(x[2 * j], T()), c1 = narrow(x[2 * j + 1], T());
           hi[j] = both(c0, c1);
-          lo[j] = both(narrow(x[2 * j] - to_f(c0), T()), narrow(x[2 * j + 1] - to_f(c1), T()));
+          constexpr float kUp = 1 << LowPiece<T>::shift;
+          lo[j] = both(narrow((x[2 * j] - to_f(c0)) * kUp, T()), narrow((x[2 * j + 1] - to_f(c1)) * kUp, T()));
         }
 #pragma unroll
         for (int j = 0; j < 8; j += 4) {

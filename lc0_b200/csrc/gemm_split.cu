@@ -23,7 +23,8 @@
 // beta arrive by bulk copy ahead of the grid dependency.  A LayerNorm vector may span several rows of A (smolgen's
 // second one: 32 heads x 256), as long as a tile holds whole vectors.  Every column tile repeats the LayerNorm: worth it
 // while a launch costs more than that (Net::gemm_with_ln has the line); beyond, ln_rows_kernel does it with the same results.
-// With adapters (kAd) the product takes H . B^T in.  kAdBlocks: as further k-blocks of one CTA of the cluster, like gemm_tc.cu's pair kernel;
+// With adapters (kAd) the product takes H . B^T in.  kAdBlocks: as further k-blocks of one CTA of the cluster, like gemm_tc.cu's pair kernel, H's
+// second pieces, where they are scaled, into an accumulator of their own, which the epilogue adds;
 // kAdAdd: a warp per row adds it in fp32 to the sums in shared memory, for requests of any number of rows and
 // operands that TMA cannot read.  The kernel before this one only writes H: A and W are loaded and multiplied while it runs.
 // The tensor core truncates its sums, always towards zero, the more the longer they are.  Results of 16 bits hide it; for fp32
@@ -210,6 +211,8 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   float4* rowv = reinterpret_cast<float4*>(misc + 256);          // [rows of this CTA's slice] mean_a, rstd_a, mean_r, rstd_r
   float* ln_gb = reinterpret_cast<float*>(misc + 256 + 128 * 16);  // kLN: gamma [group * 256], beta [group * 256]
 
+  // kAdBlocks: columns of tensor memory of the products with H's second, scaled pieces, if those are scaled
+  constexpr int kLow = kAd == kAdBlocks && LowPiece<T>::shift > 0 ? BN : 0;
   const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
   const int ks = cfg.ks, rank = ks > 1 ? (int)cluster_ctarank() : 0;
   const int n0 = ((int)blockIdx.x / ks) * BN, m0 = (int)blockIdx.y * cfg.a_rows;
@@ -250,7 +253,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(kAd == kAdRounded ? 2u * BN : (uint32_t)BN)
+                 "r"(kAd == kAdRounded ? 2u * BN : (uint32_t)(BN + kLow))
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -343,6 +346,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       }
       if constexpr (kAd == kAdBlocks) {
         const int blocks = adapter_blocks(p.ad_rp), of_b = p.ad_rp / 16;
+        bool low = false;
         for (int i = 0; ok && i < ad_blocks; ++i) {
           if (!mbar_wait(smem_u32(&full_bar[s]), ph, abort_flag, 3)) { ok = false; break; }
           tcgen05_fence_after();
@@ -350,8 +354,12 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
           const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + cfg.a_rows * 128);
           // both pieces of a narrow H meet the same columns of B
           const int left = blocks == 1 ? 2 * of_b : of_b - i % blocks % (blocks / 2) * 4;
-          for (int k = 0; k < 4 && k < left; ++k)
-            tcgen05_mma_f16(tmem, adesc + 2 * k, bdesc + 2 * (blocks == 1 && k >= of_b ? k - of_b : k), idesc, 1u);
+          for (int k = 0; k < 4 && k < left; ++k) {
+            const bool second = blocks == 1 ? k >= of_b : i % blocks >= blocks / 2;
+            const bool first_low = kLow > 0 && second && !low;
+            low |= second;
+            tcgen05_mma_f16(tmem + (second ? kLow : 0), adesc + 2 * k, bdesc + 2 * (blocks == 1 && second ? k - of_b : k), idesc, first_low ? 0u : 1u);
+          }
           if (kbn + i + S < kbn + ad_blocks) tcgen05_commit(smem_u32(&empty_bar[s]));
           if (++s == S) { s = 0; ph ^= 1; }
         }
@@ -458,6 +466,17 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
           const uint32_t ta = tmem + ((uint32_t)(quarter * 32) << 16) + half * kCols + c;
           if constexpr (kStep == 16) tmem_ld16(ta, r); else tmem_ld32(ta, r);
           tmem_ld_wait();
+          if (kLow > 0 && ad_blocks > 0) {
+#pragma unroll
+            for (int h = 0; h < kStep; h += 16) {
+              uint32_t low[16];
+              tmem_ld16(ta + kLow + h, low);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                r[h + j] = __float_as_uint(fmaf(__uint_as_float(low[j]), 1.f / (1 << LowPiece<T>::shift), __uint_as_float(r[h + j])));
+            }
+          }
         }
 #pragma unroll
         for (int j = 0; j < kStep; j += 4) {
@@ -473,7 +492,7 @@ gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
   if (ks > 1) cluster_sync_all(); else __syncthreads();
   if (kAd != kAdRounded && warp == 9) {
     tcgen05_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)BN) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(BN + kLow)) : "memory");
   }
   if constexpr (kAd == kAdAdd || kAd == kAdRounded) {
     if (warp < 8) {

@@ -140,7 +140,7 @@ __device__ __forceinline__ void epilogue_slab(const TcParams& p, uint8_t* buf, u
                                               uint32_t full_bar, uint32_t use, bool leader, uint32_t taddr, int row,
                                               int lane, int nb, int next_nb, ColRegs& cr, float* wvec, RowCtx& rc,
                                               volatile int* abort_flag, const float* se_arg = nullptr,
-                                              uint32_t res_use = 0, int m_row = 0) {
+                                              uint32_t res_use = 0, int m_row = 0, uint32_t low_addr = 0) {
   using Ep = Epilogue<kMode>;
   const float* se = kSe ? se_arg : nullptr;  // compiled out of the kernels that never fuse squeeze-excitation
   // se != nullptr: gate (se[0..63]) and shift (se[256..319]) of this row's sample for the slab's 64 columns; the
@@ -172,6 +172,16 @@ __device__ __forceinline__ void epilogue_slab(const TcParams& p, uint8_t* buf, u
       for (int j = 0; j < kCols; ++j) v[j] = __uint_as_float(r[j]);
     }
     if constexpr (kMode == kAdapters) {
+      if (LowPiece<T>::shift > 0 && low_addr) {  // the products with H's second, scaled pieces
+#pragma unroll
+        for (int c = 0; c < kCols; c += 16) {
+          uint32_t low[16];
+          tmem_ld16(low_addr + kCols * h + c, low);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[c + j] = fmaf(__uint_as_float(low[j]), 1.f / (1 << LowPiece<T>::shift), v[c + j]);
+        }
+      }
       // Rows of other requests meet an adapter's B as zeros, and a zero times an infinity or NaN there is NaN; an H beyond the
       // type's range is infinite as a piece.  What is not finite is computed again.
       float z = 0.f;
@@ -1153,6 +1163,14 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   constexpr int kBufs = Cfg::kBufs;
   constexpr int S = Cfg::kStages;
   constexpr int BN = Cfg::BN;
+  // kAdapters, H's second pieces scaled (see LowPiece).  Their products are scaled back by an MMA that scales its accumulator, i.e. stand ahead
+  // of everything else of their rows, and the first tile waits for H.  A pair with a single tile does not: X's k-blocks are first, the
+  // second pieces meet in the other accumulator, which nothing else needs, and the epilogue adds them.  us with unscaled second pieces behind
+  // X / now: 65536x1024x1024 rank 16 160 / 161, 16384x1024x1024 rank 64 56.7 / 57.3, 8192x1024x512 rank 64 30.5 / 31.0, 32768x1024x256 rank 24
+  // 46.4 / 50.4, a tile per pair 2048x1536x1024 rank 16 18.4 / 19.4.  (That order for the first tile of several, its second pieces in the
+  // accumulator of the second: 65536x1024x1024 4 us more.  All adapters' second pieces first, without rows left out: their k-blocks hold
+  // four of five stages, 32768x1024x256 54.)
+  constexpr bool kScaled = kMode == kAdapters && LowPiece<T>::shift > 0;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* epi_mem = smem + S * Cfg::kStageBytes;
@@ -1187,6 +1205,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   // N of the MMA that computes virtual tile t: the tile's width, or what is left of N rounded up to 32
   auto mma_n_of = [&](int t) { return pair_mma_n(p.N - col_of(t), width_of(t)); };
   const int k_blocks = p.conv_cblocks > 0 ? 9 * p.conv_cblocks : (p.K + BK - 1) / BK;
+  const bool ahead = kScaled && pair + pairs < tiles;
 
   if (threadIdx.x == 64) {
     tma_prefetch_map(&tmap_a);
@@ -1236,15 +1255,43 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       int s = 0;         // stage and phase of the next k-block
       uint32_t ph = 0;
       bool ok = true;
-      TileAdapters ad, ad_next;
-      bool h_there = false;
+      TileAdapters ad = {}, ad_next;
       if (kMode == kAdapters && pair < tiles) ad_next.fetch(p, (tile_of(pair) / n_tiles) * (2 * BM));
+      // k-blocks of a tile's adapters: one each, or those of the first piece and those of the second, which is first where they are ahead
+      auto load_adapters = [&](int m0, int n0, bool half) {
+        const int blocks = adapter_blocks(p.ad_rp);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (!ad.first(i)) continue;
+          for (int b = 0; b < blocks && ok; ++b) {
+            if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 1)) { ok = false; break; }
+            const uint32_t fb_local = smem_u32(&full_bar[s]);
+            if (rank == 0) mbar_expect_tx(fb_local, half ? 2 * (BM + BN / 4) * BK * 2 : 2 * Cfg::kStageBytes);
+            const uint32_t fb = mapa(fb_local, 0);
+            const uint32_t sa = smem_u32(smem + s * Cfg::kStageBytes);
+            const int kb = blocks == 1 ? 0 : b % (blocks / 2), x = kb * BK + (blocks > 1 && (b >= blocks / 2) != ahead ? p.ad_rp : 0);
+            // H of the rows with this adapter; for the others a box behind the last row, which TMA fills with zeros
+            tma_load_2d_pair(sa, &tmap_r, x, (rank ? ad.a[2] : ad.a[0]) == ad.a[i] ? m0 : p.M, fb);
+            tma_load_2d_pair(sa + 64 * 128, &tmap_r, x, (rank ? ad.a[3] : ad.a[1]) == ad.a[i] ? m0 + 64 : p.M, fb);
+            const int y = ad.a[i] * p.N + n0;  // a narrow tile's spare rows are another adapter's: columns that are not stored
+            tma_load_2d_pair(sa + BM * BK * 2, &tmap_c2, kb * BK, y, fb);
+            if (!half) tma_load_2d_pair(sa + BM * BK * 2 + 64 * 128, &tmap_c2, kb * BK, y + 64, fb);
+            if (++s == S) { s = 0; ph ^= 1; }
+          }
+        }
+      };
+      if (ahead) grid_dependency_wait();
       for (int t = pair; t < tiles && ok; t += pairs) {
         const int m0 = (tile_of(t) / n_tiles) * (2 * BM) + (int)rank * BM;
         // a narrower tile is computed with a narrower MMA, of which each CTA supplies half the W rows
         const int n0 = col_of(t) + (int)rank * (mma_n_of(t) / 2) + (p.batch_rows > 0 ? (m0 / p.batch_rows) * p.N : 0);
         const bool half = t >= split_from;
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        if constexpr (kMode == kAdapters) {
+          ad = ad_next;
+          if (t + pairs < tiles) ad_next.fetch(p, (tile_of(t + pairs) / n_tiles) * (2 * BM));
+          if (ahead) load_adapters(m0, n0, half);
+        }
+        for (int kb = 0; kb < k_blocks && ok; ++kb) {
           if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 1)) { ok = false; break; }
           const uint32_t fb_local = smem_u32(&full_bar[s]);
           // both CTAs' bytes land on this barrier; a half-width tile takes 64 W rows per CTA instead of 128
@@ -1263,33 +1310,11 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           }
           if (++s == S) { s = 0; ph ^= 1; }
         }
-        if constexpr (kMode == kAdapters) {
-          ad = ad_next;
-          if (t + pairs < tiles) ad_next.fetch(p, (tile_of(t + pairs) / n_tiles) * (2 * BM));
-          if (!h_there) { grid_dependency_wait(); h_there = true; }
-          const int blocks = adapter_blocks(p.ad_rp);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (!ad.first(i)) continue;
-            for (int b = 0; b < blocks && ok; ++b) {
-              if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 1)) { ok = false; break; }
-              const uint32_t fb_local = smem_u32(&full_bar[s]);
-              if (rank == 0) mbar_expect_tx(fb_local, half ? 2 * (BM + BN / 4) * BK * 2 : 2 * Cfg::kStageBytes);
-              const uint32_t fb = mapa(fb_local, 0);
-              const uint32_t sa = smem_u32(smem + s * Cfg::kStageBytes);
-              const int kb = blocks == 1 ? 0 : b % (blocks / 2), x = blocks == 1 ? 0 : b / (blocks / 2) * p.ad_rp + kb * BK;
-              // H of the rows with this adapter; for the others a box behind the last row, which TMA fills with zeros
-              tma_load_2d_pair(sa, &tmap_r, x, (rank ? ad.a[2] : ad.a[0]) == ad.a[i] ? m0 : p.M, fb);
-              tma_load_2d_pair(sa + 64 * 128, &tmap_r, x, (rank ? ad.a[3] : ad.a[1]) == ad.a[i] ? m0 + 64 : p.M, fb);
-              const int y = ad.a[i] * p.N + n0;  // a narrow tile's spare rows are another adapter's: columns that are not stored
-              tma_load_2d_pair(sa + BM * BK * 2, &tmap_c2, kb * BK, y, fb);
-              if (!half) tma_load_2d_pair(sa + BM * BK * 2 + 64 * 128, &tmap_c2, kb * BK, y + 64, fb);
-              if (++s == S) { s = 0; ph ^= 1; }
-            }
-          }
+        if (kMode == kAdapters && !ahead) {
+          if (t == pair) grid_dependency_wait();
+          load_adapters(m0, n0, half);
         }
       }
-      if (kMode == kAdapters && !h_there) grid_dependency_wait();
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (even CTA only) ----------------
@@ -1314,15 +1339,96 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       int s = 0;         // stage and phase of the next k-block
       uint32_t ph = 0, tile_it = 0;
       bool ok = true;
-      TileAdapters ad_next;
+      TileAdapters ad = {}, ad_next;
       if (kMode == kAdapters && pair < tiles) ad_next.fetch(p, (tile_of(pair) / n_tiles) * (2 * BM));
+      // A tile's adapters behind X's k-blocks: second pieces into `low`, which is the tile's accumulator where they are not scaled.
+      auto issue_behind = [&](uint32_t d, uint32_t low, uint32_t idesc) {
+        const int blocks = adapter_blocks(p.ad_rp), of_b = p.ad_rp / 16;
+        uint32_t low_begun = kScaled ? 0u : 1u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (!ad.first(i)) continue;
+          for (int b = 0; b < blocks && ok; ++b) {
+            if (!mbar_wait(smem_u32(&full_bar[s]), ph, abort_flag, 3)) { ok = false; break; }
+            tcgen05_fence_after();
+            const uint32_t sa = smem_u32(smem + s * Cfg::kStageBytes);
+            const uint64_t adesc = make_smem_desc(sa);
+            const uint64_t bdesc = make_smem_desc(sa + BM * BK * 2);
+            // both pieces of a narrow H meet the same columns of B
+            const int left = blocks == 1 ? 2 * of_b : of_b - b % (blocks / 2) * 4;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (k >= left) continue;
+              const bool second = kScaled && (blocks == 1 ? k >= of_b : b >= blocks / 2);
+              tcgen05_mma_f16_pair(second ? low : d, adesc + 2 * k, bdesc + 2 * (blocks == 1 && k >= of_b ? k - of_b : k), idesc, second ? low_begun : 1u);
+              if (second) low_begun = 1u;
+            }
+            commit(smem_u32(&empty_bar[s]));
+            if (++s == S) { s = 0; ph ^= 1; }
+          }
+        }
+      };
+      // Ahead of X's k-blocks: an adapter's second pieces, then its first ones, of which the first MMA scales what the second ones left; in its
+      // own rows alone, but for the tile's first adapter, whose first MMA leaves zeros in all others.
+      auto issue_ahead = [&](uint32_t d, uint32_t idesc) {
+        const int of_b = p.ad_rp / 16, boxes = (of_b + 3) / 4;
+        uint32_t begun = 0;
+        auto scaled = [&](int i, bool first, uint64_t adesc, uint64_t bdesc) {
+          if (first) {
+            tcgen05_mma_f16_pair_scaled<LowPiece<T>::shift>(d, adesc, bdesc, idesc);
+          } else {
+            uint32_t off[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) off[w] = ad.a[w] == ad.a[i] ? 0u : 0xffffffffu;
+            tcgen05_mma_f16_pair_scaled<LowPiece<T>::shift>(d, adesc, bdesc, idesc, off);
+          }
+        };
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (!ad.first(i)) continue;
+          const bool first = begun == 0;
+          for (int b = 0; b < (of_b <= 2 ? 1 : 2 * boxes) && ok; ++b) {
+            if (!mbar_wait(smem_u32(&full_bar[s]), ph, abort_flag, 3)) { ok = false; break; }
+            tcgen05_fence_after();
+            const uint32_t sa = smem_u32(smem + s * Cfg::kStageBytes);
+            const uint64_t adesc = make_smem_desc(sa);
+            const uint64_t bdesc = make_smem_desc(sa + BM * BK * 2);
+            if (of_b == 1) {  // both pieces in one box
+              tcgen05_mma_f16_pair(d, adesc + 2, bdesc, idesc, begun);
+              scaled(i, first, adesc, bdesc);
+            } else if (of_b == 2) {
+              tcgen05_mma_f16_pair(d, adesc + 4, bdesc, idesc, begun);
+              tcgen05_mma_f16_pair(d, adesc + 6, bdesc + 2, idesc, 1u);
+              scaled(i, first, adesc, bdesc);
+              tcgen05_mma_f16_pair(d, adesc + 2, bdesc + 2, idesc, 1u);
+            } else {
+              if (b == boxes) scaled(i, first, adesc, bdesc);
+              else tcgen05_mma_f16_pair(d, adesc, bdesc, idesc, begun);
+              const int steps = of_b - (b < boxes ? b : b - boxes) * 4;
+#pragma unroll
+              for (int k = 1; k < 4; ++k)
+                if (k < steps) tcgen05_mma_f16_pair(d, adesc + 2 * k, bdesc + 2 * k, idesc, 1u);
+            }
+            begun = 1;
+            commit(smem_u32(&empty_bar[s]));
+            if (++s == S) { s = 0; ph ^= 1; }
+          }
+        }
+        return begun;
+      };
       for (int t = pair; t < tiles && ok; t += pairs, ++tile_it) {
         const uint32_t acc = tile_it & 1, aph = (tile_it >> 1) & 1;
         if (!mbar_wait(smem_u32(&tempty_bar[acc]), aph ^ 1, abort_flag, 2)) break;
         tcgen05_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
         const uint32_t idesc = idesc_base | ((uint32_t)(mma_n_of(t) >> 3) << 17);
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        uint32_t begun = 0;  // the accumulator holds something of this tile's
+        if constexpr (kMode == kAdapters) {
+          ad = ad_next;
+          if (t + pairs < tiles) ad_next.fetch(p, (tile_of(t + pairs) / n_tiles) * (2 * BM));
+          if (ahead) begun = issue_ahead(d_tmem, idesc);
+        }
+        for (int kb = 0; kb < k_blocks && ok; ++kb) {
           if (!mbar_wait(smem_u32(&full_bar[s]), ph, abort_flag, 3)) { ok = false; break; }
           tcgen05_fence_after();
           const uint32_t sa = smem_u32(smem + s * Cfg::kStageBytes);
@@ -1330,32 +1436,11 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           const uint64_t bdesc = make_smem_desc(sa + BM * BK * 2);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            tcgen05_mma_f16_pair(d_tmem, adesc + 2 * k, bdesc + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+            tcgen05_mma_f16_pair(d_tmem, adesc + 2 * k, bdesc + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : begun);
           commit(smem_u32(&empty_bar[s]));  // frees the stage in both CTAs once the MMAs have read it
           if (++s == S) { s = 0; ph ^= 1; }
         }
-        if constexpr (kMode == kAdapters) {
-          const TileAdapters ad = ad_next;
-          if (t + pairs < tiles) ad_next.fetch(p, (tile_of(t + pairs) / n_tiles) * (2 * BM));
-          const int blocks = adapter_blocks(p.ad_rp), of_b = p.ad_rp / 16;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (!ad.first(i)) continue;
-            for (int b = 0; b < blocks && ok; ++b) {
-              if (!mbar_wait(smem_u32(&full_bar[s]), ph, abort_flag, 3)) { ok = false; break; }
-              tcgen05_fence_after();
-              const uint32_t sa = smem_u32(smem + s * Cfg::kStageBytes);
-              const uint64_t adesc = make_smem_desc(sa);
-              const uint64_t bdesc = make_smem_desc(sa + BM * BK * 2);
-              // both pieces of a narrow H meet the same columns of B
-              const int left = blocks == 1 ? 2 * of_b : of_b - b % (blocks / 2) * 4;
-              for (int k = 0; k < 4 && k < left; ++k)
-                tcgen05_mma_f16_pair(d_tmem, adesc + 2 * k, bdesc + 2 * (blocks == 1 && k >= of_b ? k - of_b : k), idesc, 1u);
-              commit(smem_u32(&empty_bar[s]));
-              if (++s == S) { s = 0; ph ^= 1; }
-            }
-          }
-        }
+        if (kMode == kAdapters && !ahead) issue_behind(d_tmem, kScaled ? d_tmem + BN : d_tmem, idesc);
         if (ok) commit(smem_u32(&tfull_bar[acc]));
       }
     }
@@ -1410,6 +1495,8 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       tcgen05_fence_after();
       const uint32_t trow = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN;
       if constexpr (!kAhead) load_row_ctx(p, m, rc);
+      // 32 rows are one request's; without an adapter nothing was added to theirs (and without any in the tile nothing was written there)
+      const uint32_t low_row = kScaled && !ahead && m - lane < p.M && adapter_of_row(p, m - lane) >= 0 ? trow + BN : 0;
       const float* se_row = nullptr;
       if constexpr (kMode == kConv) {
         if (p.se_k > 0) {  // this CTA's 128 rows are two boards with all their channels
@@ -1435,7 +1522,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         epilogue_slab<T, kMode == kConv, false, kMode, kGroups == 2 && kMode != kAny && kMode != kConv ? 64 : 32>(
             p, epi_mem + idx * (BM * 128), smem_u32(&res_bar[idx]), smem_u32(&stg_free[idx]), smem_u32(&stg_full[idx]),
             slab_it / kBufs, leader, trow + c0, quarter * 32 + lane, lane, n0 + c0, next_nb, cr, wvec, rc, abort_flag,
-            se_row ? se_row + c0 : nullptr, 0, m);
+            se_row ? se_row + c0 : nullptr, 0, m, low_row ? low_row + c0 : 0);
         ++slab_it;
       }
       if (Epilogue<kMode>::out_stats(p)) flush_row_ctx(p, m, rc);

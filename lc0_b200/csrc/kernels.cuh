@@ -75,7 +75,7 @@ struct GemmParams {
   int ln_group = 1;
   float ln_eps = 0.f;
   // Low-rank adapters (tensor-core kernels): rows [i * ad_group, (i + 1) * ad_group) add H[m] . B[ids[i]]^T ahead of the
-  // activation, ad_h [M][ad_rank] fp32, ad_b [ad_n][N][ad_rank].  ad_pieces: H as two values of the storage type,
+  // activation, ad_h [M][ad_rank] fp32, ad_b [ad_n][N][ad_rank].  ad_pieces: H as two values of the storage type (see LowPiece),
   // [M][2 * ad_rp] with the first in columns [0, ad_rp) and the second behind, zeros beyond ad_rank.  H is written by the launch just
   // before this one, A, W and the ids by launches before that.
   const int* ad_ids = nullptr;
@@ -84,6 +84,11 @@ struct GemmParams {
   const void* ad_b = nullptr;
   int ad_group = 0, ad_n = 0, ad_rank = 0, ad_rp = 0;
 };
+
+// H = first + second 2^-shift.  fp16 ends at 2^-24: unscaled, the second would hold H to within 2^-25, which a large B shows beside
+// results of order one; scaled it is off by 2^-23 of H or 2^-36.  bf16 has the exponents of fp32.
+template <typename T> struct LowPiece { static constexpr int shift = sizeof(T) == 2 ? 11 : 0; };
+template <> struct LowPiece<__nv_bfloat16> { static constexpr int shift = 0; };
 
 // FMA kernel (gemm_fma.cu): any shape and alignment, batched products; no folded LayerNorm, residual or statistics.  A row's
 // result is the same whatever the number of rows.

@@ -223,6 +223,27 @@ __device__ __forceinline__ void tcgen05_mma_f16_pair(uint32_t tmem_d, uint64_t a
       : "memory");
 }
 
+// D = A B + D 2^-kShift.
+template <int kShift>
+__device__ __forceinline__ void tcgen05_mma_f16_pair_scaled(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.eq.b32 p, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p, %4;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "n"(kShift)
+      : "memory");
+}
+// The same, but for the blocks of 64 rows whose word in `off` is all ones, which stay as they are.
+template <int kShift>
+__device__ __forceinline__ void tcgen05_mma_f16_pair_scaled(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, const uint32_t (&off)[4]) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.eq.b32 p, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %4, %5, %5, %6, %6, %7, %7}, p, %8;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "n"(kShift)
+      : "memory");
+}
+
 // Shared-memory matrix descriptor of a K-major operand tile stored as rows of 128 bytes with the 128-byte
 // swizzle (what a TMA box of 64 16-bit elements x R rows with CU_TENSOR_MAP_SWIZZLE_128B produces):
 // start address >> 4 in bits [0,14), stride between 8-row groups (1024 B) >> 4 in bits [32,46),

@@ -281,6 +281,79 @@ def test_narrow_products_beyond_the_range_of_fp16(lib, M, group):
     c.check()
 
 
+
+BODIES = [(1536, 512, 256, 16, 64), (64, 256, 1024, 16, 64), (320, 512, 640, 40, 64),  # cut over clusters, X A^T row by row among them
+          (8192, 512, 256, 16, 64), (32768, 1024, 128, 16, 64), (32768, 1024, 128, 32, 128), (24000, 1096, 192, 48, 64), (32768, 768, 128, 128, 192)]
+
+
+@gpu
+@pytest.mark.parametrize("a,b", [(1.0, 1.0), (1e-4, 1e4), (1e-5, 2e4), (3e-3, 300.0)])
+@pytest.mark.parametrize("M,N,K,rank,group", BODIES)
+def test_small_narrow_products_met_by_a_large_b(lib, M, N, K, rank, group, a, b):
+    """X A^T far below what one fp16 value resolves, results of order one: as exact as the exact results rounded to fp16.  Sums in fp32
+    (K / 8 truncated additions at most: 2^-20 here) add less than a hundredth to the rounding's 2^-12."""
+    c = Call(lib, M, N, K, rank, group, 9, 1, ids=torch.randint(-1, 9, ((M + group - 1) // group,), generator=torch.Generator().manual_seed(M)))
+    c.scales *= a  # the scale is in X A^T
+    c.b *= b
+    c.run()
+    want, _ = c.want()
+    with_one = (c.ids.repeat_interleave(group)[:M] >= 0)
+    rms = lambda v: ((v.double() - want)[with_one].norm() / want[with_one].norm()).item()
+    assert rms(c.out) <= 1.02 * rms(want.half()), (rms(c.out), rms(want.half()))
+    # every element: half a step of the type, sums in fp32, of X A^T 22 bits or 2^-36 through B
+    ids = c.ids.long().repeat_interleave(group)[:M]
+    x, w = c.x.double(), c.w.double()
+    err = x.abs() @ w.abs().T + c.bias.double().abs() + want.abs()
+    err *= (K / 8 + 24) * 2.0 ** -24
+    for j in range(9):
+        r = (ids == j).nonzero()[:, 0]
+        h, hmag = c.scales[j].double() * (x[r] @ c.a[j].double().T), c.scales[j].double() * (x[r].abs() @ c.a[j].double().abs().T)
+        err[r] += (2.0 ** -22 * h.abs() + (K / 8 + 24) * 2.0 ** -24 * hmag + 2.0 ** -36) @ c.b[j].double().abs().T
+    assert ((c.out.double() - want).abs() <= 2.0 ** -11 * want.abs() + (1 + 2.0 ** -11) * err + 2.0 ** -25).all()
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K,rank,group", BODIES)
+def test_large_narrow_products_met_by_a_small_b(lib, M, N, K, rank, group):
+    """X A^T beyond fp16 in every kernel that makes or takes its two values."""
+    c = Call(lib, M, N, K, rank, group, 8, 1)
+    c.a *= 2e4
+    c.b *= 1e-5
+    c.a[3] *= 1e-3  # one adapter whose products fit
+    c.run()
+    if M > 64:  # (the one request of 64 rows may have none, or one whose products fit)
+        assert max((c.x.float() @ c.a[j].float().T).abs().max() * c.scales[j] for j in set(c.ids.tolist()) - {-1}) > 65504
+    c.check()
+    c.ids[:] = -1
+    plain = c.run().clone()
+    c.ids[0] = 4  # rows beside a request whose pieces are infinite
+    assert torch.equal(c.run()[group:], plain[group:])
+    c.check()
+
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K,rank,group", [(1536, 512, 256, 16, 64), (8192, 512, 256, 16, 64), (32768, 1024, 128, 16, 64), (32768, 768, 128, 32, 64),
+                                              (24000, 1096, 192, 48, 64)])
+def test_fp16_values_that_are_not_finite_stay_with_their_rows(lib, M, N, K, rank, group):
+    c = Call(lib, M, N, K, rank, group, 8, 1, ids=torch.arange((M + group - 1) // group) % 9 - 1)
+    c.run()
+    want, allowed = c.want()
+    c.x[3, 5] = float("inf")
+    c.x[700, 1] = float("nan")
+    c.b[5, 7, 2] = float("nan")
+    c.b[2, 300, 1] = float("inf")
+    c.a[6, 3] = float("inf")
+    got = c.run()
+    ids = c.ids.repeat_interleave(group)[:M]
+    bad = torch.zeros(M, N, dtype=torch.bool, device="cuda")
+    bad[3], bad[700], bad[ids == 6] = True, True, True
+    bad[ids == 5, 7] = True
+    bad[ids == 2, 300] = True
+    assert ((got.double() - want).abs() <= allowed)[~bad].all()  # (in another order of sums: each is within the allowance)
+    assert not (got[bad].abs() < 65504).any()  # (an infinite result of fp16 is its largest number, as in b200_op_gemm)
+
+
 @gpu
 def test_captured_call_follows_the_ids(lib):
     c = Call(lib, 8192, 512, 256, 16, 64, 5, 1)
