@@ -431,7 +431,8 @@ int b200_op_gemm_adapters(const b200_adapters_desc* d, void* stream);
  *   u times their total: its column, or its place in the list of moves.  prob (may be NULL): its weight over that total.
  *   -1 and 0 for a row without entries; -2 and 0 where a bounded device-side wait gave up (rows of more than 9000 entries, which a
  *   cluster of CTAs has, after 2 s; a defect).
- *   The choice is the one that sums in 64 bits give.  Allocates nothing, does not synchronise, may be captured. */
+ *   The choice is the one that sums in 64 bits give; prob is within 2^-20 of itself of what they give (its total may be one of fp32 weights).
+ *   Allocates nothing, does not synchronise, may be captured. */
 #define B200_SAMPLE_MAX_WIDTH 262144
 typedef struct b200_sample_desc {
   const void* logits; long long ld;

@@ -386,6 +386,24 @@ def test_two_calls_at_once(lib):
     b.check()
 
 
+
+@gpu
+def test_calls_of_every_kind_at_once(lib):
+    """A stream and a workspace each: the kernels of one call hold tensor memory, form clusters and wait for their H beside those of the others."""
+    kinds = [(16384, 1024, 512, 16, 64, 1, 0), (2048, 1536, 512, 32, 64, 1, 0), (320, 512, 1024, 16, 64, 1, 0), (37, 1858, 2048, 16, 1, 2, 1),
+             (1000, 264, 2048, 13, 1, 1, 0), (4096, 512, 1024, 128, 64, 2, 1), (1024, 512, 1536, 16, 64, 0, 0), (64, 256, 2048, 8, 64, 2, 0)]
+    calls = [Call(lib, M, N, K, rank, group, 20, prec, out_f32=f32, seed=i) for i, (M, N, K, rank, group, prec, f32) in enumerate(kinds)]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for c, s in zip(calls, streams):
+            _lib.check(lib.b200_op_gemm_adapters(ctypes.byref(c.d), s.cuda_stream))
+    torch.cuda.synchronize()
+    for c in calls:
+        assert c.status.item() == 0
+        c.check()
+
+
 @gpu
 def test_a_move_per_game_from_its_own_adapter(lib):
     """As a server of many games runs them: a shared policy head with an adapter per game, then a legal move from its logits."""

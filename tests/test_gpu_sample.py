@@ -289,6 +289,55 @@ def test_waits_that_give_up(lib, kind, rows, width):
     assert np.array_equal(again[0], right[0]) and np.array_equal(again[1], right[1])
 
 
+
+@gpu
+def test_a_move_from_the_policy_that_a_network_leaves_on_the_device(lib):
+    """b200_net_enqueue_device, then the draw on b200_net_stream: nothing in between goes over the host."""
+    from conftest import load_case
+    from lc0_b200 import network
+    net, pos, n, _ = load_case("cfg4_mini")
+    n = min(n, 16)
+    nw = network.Network(net, "precision=fp16,max_batch=16")
+    masks = torch.from_numpy(pos["masks"][:n].astype(np.int64)).cuda()
+    values = torch.from_numpy(pos["values"][:n].astype(np.float32)).cuda()
+    policy, qdm = torch.zeros(n, 1858, device="cuda"), torch.zeros(n, 3, device="cuda")
+    rng = np.random.default_rng(6)
+    moves = np.stack([rng.permutation(1858)[:256] for _ in range(n)]).astype(np.uint16)
+    counts = rng.integers(1, 60, n).astype(np.int32)
+    u, T = rng.random(n, np.float32), rng.uniform(0.3, 1.5, n).astype(np.float32)
+    held = [torch.from_numpy(v).cuda() for v in (u, T, counts)]
+    ids = torch.from_numpy(moves).cuda()
+    choice, prob = torch.full((n,), -7, dtype=torch.int32, device="cuda"), torch.zeros(n, device="cuda")
+    d = _lib.SampleDesc(logits=policy.data_ptr(), rows=n, width=1858, u=held[0].data_ptr(), temperature=held[1].data_ptr(), move_ids=ids.data_ptr(),
+                        n_moves=held[2].data_ptr(), ld_moves=256, choice=choice.data_ptr(), prob=prob.data_ptr())
+    torch.cuda.synchronize()
+    nw.enqueue_device(masks.data_ptr(), values.data_ptr(), n, policy.data_ptr(), qdm.data_ptr())
+    _lib.check(lib.b200_op_sample(ctypes.byref(d), nw.stream()))
+    nw.sync()
+    logits = policy.double().cpu().numpy()
+    assert (logits != 0).any()
+    compare([logits[i][moves[i, :c].astype(np.int64)] for i, c in enumerate(counts)], (choice.cpu().numpy(), prob.cpu().numpy()), u, T=T)
+    nw.close()
+
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["plain", "k", "p", "min", "all"])
+@pytest.mark.parametrize("rows,width", [(40, 60), (500, 1858), (20, 1858), (20, 50257)])
+def test_probabilities_are_as_near_as_documented(lib, kind, rows, width):
+    """2^-20 of themselves: weights of fp32 are off by 3 (ex2), 1 (its factor) and |z|, on average at most ln n < 8, steps of 2^-24, their
+    sums by 4; twice that is the bound of two sums compared, one of them is the total here."""
+    rng = np.random.default_rng(rows + width)
+    held = (rng.standard_normal((rows, width)) * 1.5).astype(np.float32)
+    T, k, p, m = settings(rng, rows, kind)
+    u = rng.random(rows, np.float32)
+    choice, prob = draw(lib, torch.from_numpy(held).cuda(), u, temperature=T, top_k=k, top_p=p, min_p=m)
+    at = lambda v, i, off: off if v is None else v[i]
+    for i in range(rows):
+        want = reference(held[i].astype(np.float64), at(T, i, 1.0), at(k, i, 0), at(p, i, 1.0), at(m, i, 0.0), u[i])
+        assert choice[i] == want[0] and abs(prob[i] - want[1]) <= 2.0 ** -20 * want[1], (i, choice[i], prob[i], want)
+
+
 @gpu
 def test_captured_and_replayed(lib):
     logits, u = torch.randn(64, 1858, device="cuda"), torch.rand(64, device="cuda")
