@@ -29,7 +29,8 @@
 // operands that TMA cannot read.  The kernel before this one only writes H: A and W are loaded and multiplied while it runs.
 // The tensor core truncates its sums, always towards zero, the more the longer they are.  Results of 16 bits hide it; for fp32
 // results (kAdRounded) there are two accumulators in turn, which leave tensor memory after a k-block each, to be added in registers,
-// rounded to nearest, while the next one is multiplied.
+// rounded to nearest, while the next one is multiplied.  us, bf16, chains of 256 side by side in tensor memory / now: 37x1858x2048 13.5 / 13.5,
+// 500x1858x2048 37.0 / 36.3, 2000x1858x1024 93.9 / 83.3, 4096x1858x2048 rank 32 355 / 308.
 // Every wait is bounded by wall-clock time like those of gemm_tc.cu; the cluster barriers are reached by all threads
 // whatever happened before them.
 #include <atomic>

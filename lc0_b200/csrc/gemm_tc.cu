@@ -1168,8 +1168,8 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   // second pieces meet in the other accumulator, which nothing else needs, and the epilogue adds them.  us with unscaled second pieces behind
   // X / now: 65536x1024x1024 rank 16 160 / 161, 16384x1024x1024 rank 64 56.7 / 57.3, 8192x1024x512 rank 64 30.5 / 31.0, 32768x1024x256 rank 24
   // 46.4 / 50.4, a tile per pair 2048x1536x1024 rank 16 18.4 / 19.4.  (That order for the first tile of several, its second pieces in the
-  // accumulator of the second: 65536x1024x1024 4 us more.  All adapters' second pieces first, without rows left out: their k-blocks hold
-  // four of five stages, 32768x1024x256 54.)
+  // accumulator of the second: 65536x1024x1024 4 us more.  With that, all adapters' second pieces first, without rows left out: their k-blocks
+  // hold four of five stages, 32768x1024x256 57.)
   constexpr bool kScaled = kMode == kAdapters && LowPiece<T>::shift > 0;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
