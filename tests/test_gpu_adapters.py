@@ -354,6 +354,29 @@ def test_fp16_values_that_are_not_finite_stay_with_their_rows(lib, M, N, K, rank
     assert not (got[bad].abs() < 65504).any()  # (an infinite result of fp16 is its largest number, as in b200_op_gemm)
 
 
+
+@gpu
+@pytest.mark.parametrize("prec", [1, 2])
+@pytest.mark.parametrize("M,N,K,rank,group", [(1, 8, 8, 1, 1), (1, 1858, 64, 8, 1), (3, 130, 72, 5, 1), (64, 8, 128, 16, 64), (65, 136, 192, 24, 64),
+                                              (129, 33, 8, 128, 64), (700, 40, 520, 12, 64), (10, 24, 4096, 16, 1), (2000, 72, 1000, 7, 30)])
+def test_fp32_results_of_small_and_odd_shapes(lib, prec, M, N, K, rank, group):
+    c = Call(lib, M, N, K, rank, group, 3, prec, out_f32=1, pads=(8, 0, 3))
+    c.run()
+    c.check()
+
+
+@gpu
+@pytest.mark.parametrize("prec", [1, 2])
+@pytest.mark.parametrize("M,N,K,rank,group", [(32700, 1024, 128, 16, 64), (32513, 1024, 64, 32, 64), (19010, 1536, 72, 72, 64), (25001, 776, 136, 16, 192),
+                                              (32768 + 64, 2048, 64, 8, 64), (600, 4872, 64, 16, 64)])
+def test_bodies_whose_last_request_is_not_whole(lib, prec, M, N, K, rank, group):
+    """Several tiles to a pair of CTAs, the last one with rows that are not there; one tile to a pair."""
+    for adapters in (2, 40):  # requests of a tile that share an adapter, and not
+        c = Call(lib, M, N, K, rank, group, adapters, prec)
+        c.run()
+        c.check()
+
+
 @gpu
 def test_captured_call_follows_the_ids(lib):
     c = Call(lib, 8192, 512, 256, 16, 64, 5, 1)
