@@ -279,36 +279,40 @@ const char* check_shape(const b200_adapters_desc* d) {
 
 extern "C" int b200_op_gemm_adapters_workspace(const b200_adapters_desc* d, size_t* bytes) {
   using namespace b200;
-  const char* wrong = check_shape(d);
-  if (!wrong && !bytes) wrong = "nowhere to put the size";
-  if (wrong) {
-    set_error(std::string("b200_op_gemm_adapters_workspace: ") + wrong);
-    return B200_ERR_INVALID;
-  }
-  *bytes = plan_of(*d).bytes();
-  return B200_OK;
+  return at_c_entry([&]() -> int {
+    const char* wrong = check_shape(d);
+    if (!wrong && !bytes) wrong = "nowhere to put the size";
+    if (wrong) {
+      set_error(std::string("b200_op_gemm_adapters_workspace: ") + wrong);
+      return B200_ERR_INVALID;
+    }
+    *bytes = plan_of(*d).bytes();
+    return B200_OK;
+  });
 }
 
 extern "C" int b200_op_gemm_adapters(const b200_adapters_desc* d, void* stream) {
   using namespace b200;
-  const char* wrong = check_shape(d);
-  if (!wrong && d->M > 0) {
-    const uintptr_t size = d->precision == B200_PREC_FP32 ? 4 : 2, csize = d->out_f32 ? 4 : size;
-    auto off = [](const void* q, uintptr_t n) { return reinterpret_cast<uintptr_t>(q) % n != 0; };
-    if (!d->X || !d->W || !d->C || !d->A || !d->B || !d->ids) wrong = "X, W, C, A, B and ids are needed";
-    else if (off(d->X, size) || off(d->W, size) || off(d->A, size) || off(d->B, size) || off(d->C, csize) || off(d->bias, 4) ||
-             off(d->scales, 4) || off(d->ids, 4) || off(d->status, 4))
-      wrong = "an operand is not aligned to its type";
-    else if (!d->workspace || off(d->workspace, 256) || d->workspace_bytes < plan_of(*d).bytes())
-      wrong = "the workspace is missing, too small or not on a 256-byte boundary";
-  }
-  if (wrong) {
-    set_error(std::string("b200_op_gemm_adapters: ") + wrong);
-    return B200_ERR_INVALID;
-  }
-  if (d->M == 0) return B200_OK;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (d->precision == B200_PREC_FP32) return run_adapters<float>(*d, s);
-  if (d->precision == B200_PREC_FP16) return run_adapters<__half>(*d, s);
-  return run_adapters<__nv_bfloat16>(*d, s);
+  return at_c_entry([&]() -> int {
+    const char* wrong = check_shape(d);
+    if (!wrong && d->M > 0) {
+      const uintptr_t size = d->precision == B200_PREC_FP32 ? 4 : 2, csize = d->out_f32 ? 4 : size;
+      auto off = [](const void* q, uintptr_t n) { return reinterpret_cast<uintptr_t>(q) % n != 0; };
+      if (!d->X || !d->W || !d->C || !d->A || !d->B || !d->ids) wrong = "X, W, C, A, B and ids are needed";
+      else if (off(d->X, size) || off(d->W, size) || off(d->A, size) || off(d->B, size) || off(d->C, csize) || off(d->bias, 4) ||
+               off(d->scales, 4) || off(d->ids, 4) || off(d->status, 4))
+        wrong = "an operand is not aligned to its type";
+      else if (!d->workspace || off(d->workspace, 256) || d->workspace_bytes < plan_of(*d).bytes())
+        wrong = "the workspace is missing, too small or not on a 256-byte boundary";
+    }
+    if (wrong) {
+      set_error(std::string("b200_op_gemm_adapters: ") + wrong);
+      return B200_ERR_INVALID;
+    }
+    if (d->M == 0) return B200_OK;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (d->precision == B200_PREC_FP32) return run_adapters<float>(*d, s);
+    if (d->precision == B200_PREC_FP16) return run_adapters<__half>(*d, s);
+    return run_adapters<__nv_bfloat16>(*d, s);
+  });
 }

@@ -8,6 +8,8 @@
 #include <atomic>
 #include <string>
 
+#include "../../include/b200nn.h"
+
 namespace b200 {
 
 // lczero::ActivationFunction values (src/neural/tables/activation_function.h:24-35).
@@ -19,6 +21,19 @@ enum Act : int {
 // Thread-local last-error string behind b200_last_error().
 void set_error(const std::string& msg);
 int cuda_fail(cudaError_t e, const char* what, const char* file, int line);
+
+// The body of a C entry point: what running out of host memory throws ends here, not in a caller that knows no exceptions.
+template <typename F> int at_c_entry(F&& f) noexcept {
+  try {
+    return f();
+  } catch (...) {
+    try {
+      set_error("out of host memory");
+    } catch (...) {  // (the message is one more allocation)
+    }
+    return B200_ERR_NOMEM;
+  }
+}
 
 #define B200_CUDA(call)                                                        \
   do {                                                                         \

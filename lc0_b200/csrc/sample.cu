@@ -1207,37 +1207,39 @@ cudaError_t launch_sample(SampleParams p, cudaStream_t s) {
 
 extern "C" int b200_op_sample(const b200_sample_desc* d, void* stream) {
   using namespace b200;
-  auto bad = [](const char* what) {
-    set_error(std::string("b200_op_sample: ") + what);
-    return B200_ERR_INVALID;
-  };
-  if (!d) return bad("no description");
-  if (d->rows < 0 || d->width < 1 || d->width > B200_SAMPLE_MAX_WIDTH) return bad("rows >= 0 and a width of 1 to 262144");
-  if (d->precision < B200_PREC_FP32 || d->precision > B200_PREC_BF16) return bad("unknown precision");
-  if (d->ld != 0 && d->ld < d->width) return bad("rows overlap");
-  if (d->rows > 0x7fffffff / kMaxCluster) return bad("too many rows");
-  if (d->move_ids && (!d->n_moves || d->ld_moves < 1 || d->ld_moves > 65536)) return bad("lists of moves need their lengths and a stride of 1 to 65536");
-  if (!d->move_ids && d->n_moves) return bad("lengths without lists of moves");
-  if (d->rows == 0) return B200_OK;
-  if (!d->logits || !d->u || !d->choice) return bad("logits, random numbers and choices are needed");
-  auto off = [](const void* q, uintptr_t n) { return reinterpret_cast<uintptr_t>(q) % n != 0; };
-  if (off(d->logits, d->precision == B200_PREC_FP32 ? 4 : 2) || off(d->move_ids, 2) || off(d->n_moves, 4) || off(d->temperature, 4) ||
-      off(d->top_k, 4) || off(d->top_p, 4) || off(d->min_p, 4) || off(d->u, 4) || off(d->choice, 4) || off(d->prob, 4))
-    return bad("an operand is not aligned to its type");
-  SampleParams p = {};
-  p.logits = d->logits; p.ld = d->ld ? d->ld : d->width; p.rows = d->rows; p.width = d->width;
-  p.ids = d->move_ids; p.counts = d->n_moves; p.ld_ids = d->ld_moves;
-  p.temperature = d->temperature; p.top_k = d->top_k; p.top_p = d->top_p; p.min_p = d->min_p; p.u = d->u;
-  p.choice = d->choice; p.prob = d->prob;
-  const long long injected = give_up.load(std::memory_order_relaxed);
-  p.wait_ns = injected < 0 ? 2000000000ull : 1000000ull;  // 2 s; 1 ms where one is known not to come
-  p.give_up_cta = injected < 0 ? -1 : (int)(injected >> 32);
-  p.give_up_at = injected < 0 ? -1 : (int)(injected & 0x7fffffff);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (d->precision == B200_PREC_FP32) B200_CUDA(launch_sample<float>(p, s));
-  else if (d->precision == B200_PREC_FP16) B200_CUDA(launch_sample<__half>(p, s));
-  else B200_CUDA(launch_sample<__nv_bfloat16>(p, s));
-  return B200_OK;
+  return at_c_entry([&]() -> int {
+    auto bad = [](const char* what) {
+      set_error(std::string("b200_op_sample: ") + what);
+      return B200_ERR_INVALID;
+    };
+    if (!d) return bad("no description");
+    if (d->rows < 0 || d->width < 1 || d->width > B200_SAMPLE_MAX_WIDTH) return bad("rows >= 0 and a width of 1 to 262144");
+    if (d->precision < B200_PREC_FP32 || d->precision > B200_PREC_BF16) return bad("unknown precision");
+    if (d->ld != 0 && d->ld < d->width) return bad("rows overlap");
+    if (d->rows > 0x7fffffff / kMaxCluster) return bad("too many rows");
+    if (d->move_ids && (!d->n_moves || d->ld_moves < 1 || d->ld_moves > 65536)) return bad("lists of moves need their lengths and a stride of 1 to 65536");
+    if (!d->move_ids && d->n_moves) return bad("lengths without lists of moves");
+    if (d->rows == 0) return B200_OK;
+    if (!d->logits || !d->u || !d->choice) return bad("logits, random numbers and choices are needed");
+    auto off = [](const void* q, uintptr_t n) { return reinterpret_cast<uintptr_t>(q) % n != 0; };
+    if (off(d->logits, d->precision == B200_PREC_FP32 ? 4 : 2) || off(d->move_ids, 2) || off(d->n_moves, 4) || off(d->temperature, 4) ||
+        off(d->top_k, 4) || off(d->top_p, 4) || off(d->min_p, 4) || off(d->u, 4) || off(d->choice, 4) || off(d->prob, 4))
+      return bad("an operand is not aligned to its type");
+    SampleParams p = {};
+    p.logits = d->logits; p.ld = d->ld ? d->ld : d->width; p.rows = d->rows; p.width = d->width;
+    p.ids = d->move_ids; p.counts = d->n_moves; p.ld_ids = d->ld_moves;
+    p.temperature = d->temperature; p.top_k = d->top_k; p.top_p = d->top_p; p.min_p = d->min_p; p.u = d->u;
+    p.choice = d->choice; p.prob = d->prob;
+    const long long injected = give_up.load(std::memory_order_relaxed);
+    p.wait_ns = injected < 0 ? 2000000000ull : 1000000ull;  // 2 s; 1 ms where one is known not to come
+    p.give_up_cta = injected < 0 ? -1 : (int)(injected >> 32);
+    p.give_up_at = injected < 0 ? -1 : (int)(injected & 0x7fffffff);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (d->precision == B200_PREC_FP32) B200_CUDA(launch_sample<float>(p, s));
+    else if (d->precision == B200_PREC_FP16) B200_CUDA(launch_sample<__half>(p, s));
+    else B200_CUDA(launch_sample<__nv_bfloat16>(p, s));
+    return B200_OK;
+  });
 }
 
 extern "C" void b200_op_sample_inject_give_up(int cta, int wait) {

@@ -48,3 +48,42 @@ def test_no_silent_cpu_fallback():
         pytest.skip("a GPU is present")
     with pytest.raises(_lib.B200Error, match="CUDA"):
         network.Network(mknet.make_net("cfg3_mini"), "precision=fp32")
+
+
+_NO_MEMORY = r"""
+#include <cstdlib>
+#include <new>
+static bool none = false;
+extern "C" void no_more_memory(int on) { none = on != 0; }
+void* operator new(std::size_t n) {
+  void* p = none ? nullptr : std::malloc(n ? n : 1);
+  if (!p) throw std::bad_alloc();
+  return p;
+}
+void operator delete(void* p) noexcept { std::free(p); }
+void operator delete(void* p, std::size_t) noexcept { std::free(p); }
+"""
+_CALLS = r"""
+import ctypes, sys
+from lc0_b200 import _lib
+lib, shim = _lib.load(), ctypes.CDLL(sys.argv[1])
+need = ctypes.c_size_t()
+sample, adapters = _lib.SampleDesc(rows=-1), _lib.AdaptersDesc(M=-1)
+shim.no_more_memory(1)
+codes = [lib.b200_op_sample(ctypes.byref(sample), None), lib.b200_op_gemm_adapters(ctypes.byref(adapters), None),
+         lib.b200_op_gemm_adapters_workspace(ctypes.byref(adapters), ctypes.byref(need))]
+shim.no_more_memory(0)
+print(codes, lib.b200_op_sample(ctypes.byref(sample), None))
+"""
+
+
+def test_operators_without_host_memory(tmp_path):
+    """An allocation that fails inside a call (the message of a refusal is one) is an error code, not an exception through the C caller."""
+    import subprocess
+    import sys
+    src, shim = tmp_path / "none.cc", tmp_path / "none.so"
+    src.write_text(_NO_MEMORY)
+    subprocess.check_call(["g++", "-shared", "-fPIC", "-O1", "-o", str(shim), str(src)])
+    r = subprocess.run([sys.executable, "-c", _CALLS, str(shim)], cwd=ROOT, env=dict(os.environ, LD_PRELOAD=str(shim)), capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-500:]
+    assert r.stdout.strip() == "%s %d" % ([_lib.ERR_NOMEM] * 3, _lib.ERR_INVALID)
