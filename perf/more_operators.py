@@ -63,7 +63,8 @@ def draw(rng):
         c = dict(op=op, type=t, n=rng.choice([32, 128, 256, 512, 1000, 1024, 1536, 1858]), k=rng.choice([64, 256, 512, 624, 1024, 1536, 2048]),
                  act=rng.choice(["none", "mish", "swish", "relu2"]), res=rng.random() < 0.4, f32=rng.random() < 0.2)
         rows = 64 * _log(rng, 1, 1024) if rng.random() < 0.6 else _log(rng, 1, 4096)
-        c["rows"] = max(1, min(rows, 65536 * 1536 * 1024 // (c["n"] * c["k"])))
+        row_bytes = 2 * c["k"] + (4 if c["f32"] else 2) * c["n"] * (2 if c["res"] else 1)
+        c["rows"] = max(1, min(rows, 65536 * 1536 * 1024 // (c["n"] * c["k"]), 460_000_000 // row_bytes))
         return c
     if op == "experts":
         c = dict(op=op, type=t, int8=rng.random() < 0.35, side=rng.choice(["up", "up", "down", "head"]),
@@ -84,7 +85,7 @@ def draw(rng):
     heads = rng.choice([4, 8, 16, 24, 32])
     c = dict(op=op, type=rng.choice(["fp16", "bf16", "fp32"]), q_heads=heads, k_heads=heads // rng.choice([1, 1, 2, 4]), depth=depth,
              rotate=rng.choice([0, depth // 2, depth, depth]), interleaved=rng.random() < 0.5, packed=rng.random() < 0.5)
-    c["rows"] = max(1, min(64 * _log(rng, 1, 1024), 65536 * 48 * 32 // ((c["q_heads"] + c["k_heads"]) * depth)) - rng.choice([0, 0, 1, 13]))
+    c["rows"] = max(1, min(64 * _log(rng, 1, 1024), 65536 * 48 * 32 // ((c["q_heads"] + c["k_heads"]) * depth * (2 if c["type"] == "fp32" else 1))) - rng.choice([0, 0, 1, 13]))
     return c
 
 
