@@ -445,6 +445,100 @@ int b200_op_sample(const b200_sample_desc* d, void* stream);
 /* Failure-injection hook for tests of that exit, process-wide: in calls from now on CTA `cta` (from 0) of each cluster behaves at its wait
  * number `wait` (from 0) as if it had run out, and all others run out after 1 ms.  A negative number: no longer. */
 void b200_op_sample_inject_give_up(int cta, int wait);
+/* ---- Operators of encoder layers in 8 bits, with experts, with normalised heads -----------------------------------------------
+ * All allocate nothing, do not synchronise and may be captured; index lists are read on the device, a captured call follows what
+ * they hold when it is replayed.  Outputs may not overlap inputs but where it says so.  Leading dimensions of 0 mean dense.  status:
+ * device int or NULL, set non-zero (and never cleared) if a bounded device-side wait gave up, the result is then undefined.
+ *
+ * b200_op_quantize_rows: 8-bit rows with a scale each: scales[m] = max_k |X[m][k]| * fp32(1 / 127) and Q[m][k] = X[m][k] / scales[m], the exact
+ *   quotient rounded to the nearest whole number (ties to even, at most 127 in size).  X [M][K] in `precision`; Q [M][K].  For activations (a scale
+ *   per token) and, with M output channels, for weights.  A row of zeros (or so small that the scale is 0): scale 0 and zeros.  A row that holds
+ *   an infinity or NaN: scale NaN and zeros, so that its products are NaN. */
+int b200_op_quantize_rows(const void* X, long long ldx, int M, int K, int precision, int8_t* Q, long long ldq, float* scales, void* stream);
+/* b200_op_gemm_int8: C[m][n] = alpha * act(x_scales[m] * w_scales[n] * sum_k X[m][k] W[n][k] + bias[n]) + res[m][n].
+ *   X [M][K] and W [N][K] 8-bit integers with a scale per row, sums in 32-bit integers (exact: K up to B200_INT8_MAX_K), `activation` as in
+ *   b200_op_gemm, C and res [M][N] of `precision`, bias and res may be NULL; res may be C itself (same leading dimension).  A row's result
+ *   does not depend on the number of rows. */
+#define B200_INT8_MAX_K 131071
+typedef struct b200_gemm_int8_desc {
+  const int8_t* X; const float* x_scales;
+  const int8_t* W; const float* w_scales;
+  const float* bias; void* C;
+  int M, N, K;
+  long long ldx, ldw, ldc;
+  int activation, precision;
+  float alpha;
+  const void* res; long long ldres;
+  int* status;
+} b200_gemm_int8_desc;
+int b200_op_gemm_int8(const b200_gemm_int8_desc* d, void* stream);
+/* b200_op_route: the router in front of expert layers.  Requests are rows of n_experts logits of `precision`, ld apart.
+ *   - ids [rows][top_k]: the experts with the largest logits, falling, equal ones by index; NaN and -infinity are never chosen (-1 and weight 0 where
+ *     nothing is left).
+ *   - weights [rows][top_k] (may be NULL): softmax over the row's logits, or, with renormalise, over the chosen ones (+infinity: 1 each before the
+ *     division, nothing beside them).
+ *   - order [rows * top_k] and offsets [n_experts + 1]: the choices r = row * top_k + j sorted by expert, equal ones by r; expert e has
+ *     order[offsets[e] .. offsets[e + 1]).  What lies from order[offsets[n_experts]] on is left as it was.
+ *   logits NULL: ids are given by the caller (entries not in [0, n_experts) have no expert) and sorted; weights has to be NULL.
+ *   workspace: b200_op_route_workspace() bytes on a 256-byte boundary, for this call alone until it has run.
+ *   n_experts 1 to B200_MAX_EXPERTS, top_k 1 to min(n_experts, B200_MAX_TOP_K); rows * top_k below 2^31. */
+#define B200_MAX_EXPERTS 256
+#define B200_MAX_TOP_K 16
+typedef struct b200_route_desc {
+  const void* logits; long long ld;
+  int rows, n_experts, top_k, precision, renormalise;
+  int* ids; float* weights; int* order; int* offsets;
+  void* workspace; size_t workspace_bytes;
+} b200_route_desc;
+int b200_op_route_workspace(const b200_route_desc* d, size_t* bytes);
+int b200_op_route(const b200_route_desc* d, void* stream);
+/* b200_op_gemm_experts: products grouped by expert with ragged sizes.  `group` consecutive rows are one request (64 in a network's body when a
+ *   position has its expert, 1 for a token or in its heads), which has top_k choices; order and offsets are b200_op_route's over the
+ *   requests.  Slot s * group + i, s < offsets[n_experts], is row i of choice r = order[s], i.e. of token (r / top_k) * group + i.
+ *     Y[slot] = act(X[.] W[e]^T + bias[e]) of the slot's expert e
+ *   - X: M tokens [M][K], or with x_by_slot M * top_k slots (what an earlier call wrote with c_by_slot).
+ *   - c_by_slot: C [M * top_k][N] is Y.  Slots behind the last expert's are left as they were.
+ *   - otherwise C [M][N] of the tokens: C[t] = res[t] + sum over t's choices j that have an expert, in their order, of
+ *     weights[(t / group) * top_k + j] * Y[.]; weights NULL: 1; res NULL: 0 (it may be C itself, with the same leading dimension).  Tokens
+ *     without any expert are left as they were.  With top_k > 1 needs ids [M / group][top_k].
+ *   - W [n_experts][N][K] (rows ldw apart, experts N * ldw), bias [n_experts][N] or NULL, `activation`, `precision` (fp16 or bf16) of X, W, C and res;
+ *     out_f32: C and res hold float.  int8: X and W are 8-bit integers with x_scales per row of X and w_scales [n_experts][N], as in b200_op_gemm_int8,
+ *     and precision may be any.
+ *   - workspace: b200_op_gemm_experts_workspace() bytes on a 256-byte boundary, for this call alone until it has run (0 bytes but where choices are summed).
+ *   Sums in fp32 (int8: exact); float results of 16-bit inputs are as exact as a plain fp32 product.  order entries outside the choices are no rows;
+ *   offsets are held to 0 <= offsets[e] <= offsets[e + 1] <= M / group * top_k.  M a multiple of group, M * top_k at most 2^30. */
+typedef struct b200_experts_desc {
+  const void* X; const void* W; const float* bias; void* C;
+  int M, N, K;
+  long long ldx, ldw, ldc;
+  int activation, precision, out_f32;
+  int int8; const float* x_scales; const float* w_scales;
+  int n_experts, top_k, group;
+  const int* ids; const int* order; const int* offsets;
+  int x_by_slot, c_by_slot;
+  const float* weights; const void* res; long long ldres;
+  int* status;
+  void* workspace; size_t workspace_bytes;
+} b200_experts_desc;
+int b200_op_gemm_experts_workspace(const b200_experts_desc* d, size_t* bytes);
+int b200_op_gemm_experts(const b200_experts_desc* d, void* stream);
+/* b200_op_qk_norm_rotate: what newer encoder layers do to queries and keys ahead of b200_op_attention, one pass over both.  For every row (token) and
+ *   head h (columns [h * depth, (h + 1) * depth)):
+ *   - norm != 0: x = x / sqrt(mean(x^2) + eps) * gamma; gamma_q, gamma_k [depth] or NULL (1).
+ *   - rotate > 0 (even, at most depth): pairs p < rotate / 2 of the first `rotate` entries, entries p and p + rotate / 2, or 2p and 2p + 1 with
+ *     `interleaved`, turn: (a, b) -> (a cos - b sin, a sin + b cos) with (cos, sin) = table[position][p][0..1], table [n_positions][rotate / 2][2].
+ *     positions [rows], or NULL: row % n_positions (the squares of a board: 64).  A row whose position is not in [0, n_positions) is not turned.
+ *   q, k in `precision`, q_heads and k_heads (0: none, k may then be NULL) heads, rows ldq and ldk apart; q_out, k_out likewise (ldq_out, ldk_out; 0:
+ *   dense, as for ldq and ldk), or the inputs themselves with the same leading dimension (in place); they may not overlap them otherwise.  Arithmetic in
+ *   fp32, one rounding at the end.  depth 1 to 256. */
+typedef struct b200_qk_norm_desc {
+  const void* q; const void* k; long long ldq, ldk;
+  void* q_out; void* k_out; long long ldq_out, ldk_out;
+  int rows, q_heads, k_heads, depth, precision;
+  int norm; float eps; const float* gamma_q; const float* gamma_k;
+  int rotate, interleaved; const float* table; int n_positions; const int* positions;
+} b200_qk_norm_desc;
+int b200_op_qk_norm_rotate(const b200_qk_norm_desc* d, void* stream);
 int b200_op_layer_norm(void* out, const void* x, const void* skip, const float* gamma,
                        const float* beta, int rows, int C, float alpha, float eps, int precision,
                        void* stream);

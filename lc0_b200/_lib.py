@@ -79,6 +79,50 @@ class SampleDesc(ctypes.Structure):
                 ("choice", ctypes.c_void_p), ("prob", ctypes.c_void_p)]
 
 
+class GemmInt8Desc(ctypes.Structure):
+    """b200_gemm_int8_desc (include/b200nn.h)."""
+    _fields_ = [("X", ctypes.c_void_p), ("x_scales", ctypes.c_void_p), ("W", ctypes.c_void_p), ("w_scales", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("C", ctypes.c_void_p),
+                ("M", ctypes.c_int), ("N", ctypes.c_int), ("K", ctypes.c_int),
+                ("ldx", ctypes.c_longlong), ("ldw", ctypes.c_longlong), ("ldc", ctypes.c_longlong),
+                ("activation", ctypes.c_int), ("precision", ctypes.c_int), ("alpha", ctypes.c_float),
+                ("res", ctypes.c_void_p), ("ldres", ctypes.c_longlong), ("status", ctypes.c_void_p)]
+
+
+class RouteDesc(ctypes.Structure):
+    """b200_route_desc (include/b200nn.h)."""
+    _fields_ = [("logits", ctypes.c_void_p), ("ld", ctypes.c_longlong),
+                ("rows", ctypes.c_int), ("n_experts", ctypes.c_int), ("top_k", ctypes.c_int), ("precision", ctypes.c_int),
+                ("renormalise", ctypes.c_int),
+                ("ids", ctypes.c_void_p), ("weights", ctypes.c_void_p), ("order", ctypes.c_void_p), ("offsets", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class ExpertsDesc(ctypes.Structure):
+    """b200_experts_desc (include/b200nn.h)."""
+    _fields_ = [("X", ctypes.c_void_p), ("W", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("C", ctypes.c_void_p),
+                ("M", ctypes.c_int), ("N", ctypes.c_int), ("K", ctypes.c_int),
+                ("ldx", ctypes.c_longlong), ("ldw", ctypes.c_longlong), ("ldc", ctypes.c_longlong),
+                ("activation", ctypes.c_int), ("precision", ctypes.c_int), ("out_f32", ctypes.c_int),
+                ("int8", ctypes.c_int), ("x_scales", ctypes.c_void_p), ("w_scales", ctypes.c_void_p),
+                ("n_experts", ctypes.c_int), ("top_k", ctypes.c_int), ("group", ctypes.c_int),
+                ("ids", ctypes.c_void_p), ("order", ctypes.c_void_p), ("offsets", ctypes.c_void_p),
+                ("x_by_slot", ctypes.c_int), ("c_by_slot", ctypes.c_int),
+                ("weights", ctypes.c_void_p), ("res", ctypes.c_void_p), ("ldres", ctypes.c_longlong),
+                ("status", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class QkNormDesc(ctypes.Structure):
+    """b200_qk_norm_desc (include/b200nn.h)."""
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("ldq", ctypes.c_longlong), ("ldk", ctypes.c_longlong),
+                ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p), ("ldq_out", ctypes.c_longlong), ("ldk_out", ctypes.c_longlong),
+                ("rows", ctypes.c_int), ("q_heads", ctypes.c_int), ("k_heads", ctypes.c_int), ("depth", ctypes.c_int),
+                ("precision", ctypes.c_int), ("norm", ctypes.c_int), ("eps", ctypes.c_float),
+                ("gamma_q", ctypes.c_void_p), ("gamma_k", ctypes.c_void_p),
+                ("rotate", ctypes.c_int), ("interleaved", ctypes.c_int), ("table", ctypes.c_void_p), ("n_positions", ctypes.c_int),
+                ("positions", ctypes.c_void_p)]
+
+
 class NetInfo(ctypes.Structure):
     _fields_ = [("input_format", ctypes.c_int), ("output_format", ctypes.c_int),
                 ("moves_left_format", ctypes.c_int), ("wdl", ctypes.c_int), ("has_mlh", ctypes.c_int),
@@ -160,6 +204,13 @@ SIGNATURES = {
     "b200_op_gemm_adapters": (_I, [ctypes.POINTER(AdaptersDesc), _P]),
     "b200_op_sample": (_I, [ctypes.POINTER(SampleDesc), _P]),
     "b200_op_sample_inject_give_up": (None, [_I, _I]),
+    "b200_op_quantize_rows": (_I, [_P, ctypes.c_longlong, _I, _I, _I, _P, ctypes.c_longlong, _P, _P]),
+    "b200_op_gemm_int8": (_I, [ctypes.POINTER(GemmInt8Desc), _P]),
+    "b200_op_route_workspace": (_I, [ctypes.POINTER(RouteDesc), ctypes.POINTER(ctypes.c_size_t)]),
+    "b200_op_route": (_I, [ctypes.POINTER(RouteDesc), _P]),
+    "b200_op_gemm_experts_workspace": (_I, [ctypes.POINTER(ExpertsDesc), ctypes.POINTER(ctypes.c_size_t)]),
+    "b200_op_gemm_experts": (_I, [ctypes.POINTER(ExpertsDesc), _P]),
+    "b200_op_qk_norm_rotate": (_I, [ctypes.POINTER(QkNormDesc), _P]),
     "b200_op_layer_norm": (_I, [_P, _P, _P, _P, _P, _I, _I, _F, _F, _I, _P]),
 }
 

@@ -202,13 +202,6 @@ cudaError_t launch_shrink_rows(const AdapterParams& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-// The second launch made dependent on the first.
-struct DependentScope {
-  bool before;
-  DependentScope() : before(t_dependent_launch) { t_dependent_launch = true; }
-  ~DependentScope() { t_dependent_launch = before; }
-};
-
 template <typename T>
 int run_adapters(const b200_adapters_desc& d, cudaStream_t s) {
   AdapterPlan plan = plan_of(d);
@@ -230,7 +223,7 @@ int run_adapters(const b200_adapters_desc& d, cudaStream_t s) {
       if (plan.piece_bytes) g.ad_pieces = p.pieces = ws + plan.h_bytes;
       if (!plan.mma || shrink_by_rows(d)) B200_CUDA(launch_shrink_rows<T>(p, s));
       else B200_CUDA(launch_adapters_shrink<T>(g, d.A, d.scales, p.H, p.pieces, d.status, s));
-      DependentScope dependent;
+      DependentLaunches dependent;
       B200_CUDA(launch_gemm_tc<T>(g, d.status, sms, s));
       return B200_OK;
     }
@@ -247,14 +240,14 @@ int run_adapters(const b200_adapters_desc& d, cudaStream_t s) {
     g.W3 = ws + plan.h_bytes;
     B200_CUDA(launch_split_weights(static_cast<const float*>(d.W), (long long)d.N * d.K, ws + plan.h_bytes, s));
     B200_CUDA(launch_shrink_rows<T>(p, s));
-    DependentScope dependent;
+    DependentLaunches dependent;
     B200_CUDA(launch_gemm_f32(g, d.status, sms, s));
   } else {
     B200_CUDA(launch_shrink_rows<T>(p, s));
-    DependentScope dependent;
+    DependentLaunches dependent;
     B200_CUDA(launch_gemm_fma<T>(g, s));
   }
-  DependentScope dependent;
+  DependentLaunches dependent;
   const int row_blocks = ceil_div(d.M, 4 * kExpandRows);
   const int vec = d.rank % 8 == 0 && aligned16(d.B);
   B200_CUDA(launch_dependent(adapters_expand_kernel<T>, dim3(ceil_div(d.N, 64), row_blocks < 65535 ? row_blocks : 65535), dim3(256), 0, s, p,

@@ -72,6 +72,11 @@ cudaError_t raise_smem_limit(int bytes) {
 
 // Whether launch_dependent() asks for the overlap (off: an ordinary launch).  Set by the host schedule per thread.
 extern thread_local bool t_dependent_launch;
+struct DependentLaunches {
+  bool before;
+  DependentLaunches() : before(t_dependent_launch) { t_dependent_launch = true; }
+  ~DependentLaunches() { t_dependent_launch = before; }
+};
 
 template <typename... KArgs, typename... Args>
 cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,

@@ -1,0 +1,299 @@
+// b200_op_gemm_int8 and b200_op_gemm_experts: entry points, the kernel for operands of any size and alignment, and the sum over a token's
+// choices.
+#include "chunk8.cuh"
+#include "grouped.cuh"
+
+namespace b200 {
+namespace {
+
+template <typename T> struct SumOf { using type = float; };
+template <> struct SumOf<int8_t> { using type = int; };
+__device__ __forceinline__ float operand(__half v) { return __half2float(v); }
+__device__ __forceinline__ float operand(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ int operand(int8_t v) { return v; }
+__device__ __forceinline__ float plus_product(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ int plus_product(int a, int b, int c) { return a * b + c; }
+
+// ---- any size and alignment -------------------------------------------------------------------------------------
+constexpr int kTile = 64, kDepth = 16;
+
+// A CTA per 64 slots of an expert and 64 columns; sums in one chain per element, k rising.
+template <typename TIn, typename TOut>
+__global__ void __launch_bounds__(256) grouped_any_kernel(const GroupedParams p) {
+  using Sum = typename SumOf<TIn>::type;
+  __shared__ Sum sx[kDepth][kTile + 1], sw[kDepth][kTile + 1];
+  __shared__ int x_row[kTile], c_row[kTile], choice_of[kTile];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16, n0 = blockIdx.x * kTile;
+  for (long long block = blockIdx.y;; block += gridDim.y) {
+    // the block's expert and first slot
+    long long left = block;
+    int e = 0, begin = 0, end = 0;
+    for (; e < p.experts; ++e) {
+      begin = expert_begin(p, e);
+      end = expert_begin(p, e + 1);
+      const int blocks = end > begin ? (end - begin + kTile - 1) / kTile : 0;
+      if (left < blocks) break;
+      left -= blocks;
+    }
+    if (e == p.experts) return;
+    const int s0 = begin + (int)left * kTile;
+    __syncthreads();
+    if (tid < kTile) {
+      SlotRows r = {-1, -1, 0};
+      if (s0 + tid < end) r = rows_of_slot(p, s0 + tid);
+      x_row[tid] = r.x; c_row[tid] = r.c; choice_of[tid] = r.choice;
+    }
+    __syncthreads();
+    Sum acc[4][4] = {};
+    const TIn* W = static_cast<const TIn*>(p.W) + (long long)e * p.N * p.ldw;
+    for (int k0 = 0; k0 < p.K; k0 += kDepth) {
+      for (int i = tid; i < kTile * kDepth; i += 256) {
+        const int r = i / kDepth, k = i % kDepth;
+        const bool in = k0 + k < p.K;
+        sx[k][r] = in && x_row[r] >= 0 ? operand(static_cast<const TIn*>(p.X)[x_row[r] * p.ldx + k0 + k]) : Sum(0);
+        sw[k][r] = in && n0 + r < p.N ? operand(W[(n0 + r) * p.ldw + k0 + k]) : Sum(0);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kDepth; ++k) {
+        Sum a[4], b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          a[i] = sx[k][ty * 4 + i];
+          b[i] = sw[k][tx + 16 * i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = plus_product(a[i], b[j], acc[i][j]);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = ty * 4 + i, c = c_row[r];
+      if (c < 0) continue;
+      const float weight = p.weights ? p.alpha * p.weights[choice_of[r]] : p.alpha;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = n0 + tx + 16 * j;
+        if (n >= p.N) continue;
+        float v = (float)acc[i][j];
+        if (p.w_scales) v *= p.x_scales[x_row[r]] * p.w_scales[e * (long long)p.N + n];
+        if (p.bias) v += p.bias[e * (long long)p.N + n];
+        v = activate<sizeof(TOut) == 2>(v, p.act) * weight;
+        if (p.res) v += to_f(static_cast<const TOut*>(p.res)[c * p.ldres + n]);
+        static_cast<TOut*>(p.C)[c * p.ldc + n] = one_of<TOut>(v);
+      }
+    }
+  }
+}
+
+template <typename TIn, typename TOut>
+cudaError_t launch_any(const GroupedParams& p, cudaStream_t s) {
+  const long long blocks = ((long long)p.slots + kTile - 1) / kTile + p.experts - 1;
+  return launch_dependent(grouped_any_kernel<TIn, TOut>, dim3(ceil_div(p.N, kTile), (unsigned)(blocks < 65535 ? blocks : 65535)), dim3(256), 0, s, p);
+}
+
+// ---- the sum over a token's choices -----------------------------------------------------------------------------
+struct CombineParams {
+  const float* Y;  // [tokens * top_k][N] by choice
+  const int* ids;
+  const void* res; long long ldres;
+  void* C; long long ldc;
+  int tokens, N, experts, top_k, group;
+};
+
+// Eight columns of a token per thread, its choices in order.
+template <typename TOut>
+__global__ void __launch_bounds__(256) combine_kernel(const CombineParams p, int vec) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int pieces = (p.N + 7) / 8;
+  const long long all = (long long)p.tokens * pieces;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
+    const int t = (int)(i / pieces), n = (int)(i % pieces) * 8, request = t / p.group, inside = t - request * p.group;
+    float v[8] = {};
+    bool any = false;
+    for (int j = 0; j < p.top_k; ++j) {
+      const int id = p.ids[(long long)request * p.top_k + j];
+      if (id < 0 || id >= p.experts) continue;
+      any = true;
+      const float* y = p.Y + (((long long)request * p.top_k + j) * p.group + inside) * p.N + n;
+      if (vec) {
+        float w[8];
+        unpack8(load8(y), w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += w[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (n + k < p.N) v[k] += y[k];
+      }
+    }
+    if (!any) continue;
+    const TOut* res = p.res ? static_cast<const TOut*>(p.res) + t * p.ldres + n : nullptr;
+    TOut* c = static_cast<TOut*>(p.C) + t * p.ldc + n;
+    if (vec) {
+      if (res) {
+        float w[8];
+        unpack8(load8(res), w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += w[k];
+      }
+      store8(c, pack8<TOut>(v));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (n + k < p.N) c[k] = one_of<TOut>(v[k] + (res ? to_f(res[k]) : 0.f));
+    }
+  }
+}
+
+template <typename TOut>
+cudaError_t launch_combine(const CombineParams& p, cudaStream_t s) {
+  auto fine = [&](const void* q, long long ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % (16 / (int)sizeof(TOut)) == 0; };
+  const int vec = p.N % 8 == 0 && fine(p.C, p.ldc) && (!p.res || fine(p.res, p.ldres));
+  const long long blocks = ((long long)p.tokens * ((p.N + 7) / 8) + 255) / 256;
+  return launch_dependent(combine_kernel<TOut>, dim3((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64)), dim3(256), 0, s, p, vec);
+}
+
+template <typename TIn, typename TOut>
+int run_grouped(const GroupedParams& p, cudaStream_t s) {
+  B200_CUDA((launch_any<TIn, TOut>(p, s)));
+  return B200_OK;
+}
+
+bool off(const void* q, uintptr_t n) { return reinterpret_cast<uintptr_t>(q) % n != 0; }
+size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+int size_of(int precision) { return precision == B200_PREC_FP32 ? 4 : 2; }
+
+// Choices are summed by a launch of their own, from fp32 rows in the workspace.
+bool sums_choices(const b200_experts_desc& d) { return !d.c_by_slot && d.top_k > 1; }
+size_t experts_bytes(const b200_experts_desc& d) { return sums_choices(d) ? round256((size_t)d.M * d.top_k * d.N * 4) : 0; }
+
+const char* check_shape(const b200_experts_desc* d) {
+  if (!d) return "no description";
+  if (d->N < 1 || d->K < 1 || d->K > (d->int8 ? B200_INT8_MAX_K : 0x7fffffff)) return "N >= 1 and K >= 1 (int8: at most 131071)";
+  if (d->n_experts < 1 || d->n_experts > B200_MAX_EXPERTS) return "n_experts 1 to 256";
+  if (d->top_k < 1 || d->top_k > B200_MAX_TOP_K) return "top_k 1 to 16";
+  if (d->group < 1 || d->M < 0 || d->M % d->group != 0) return "M is a multiple of group, which is at least 1";
+  if ((long long)d->M * d->top_k > 1 << 30) return "M * top_k of at most 2^30";
+  if ((long long)d->n_experts * d->N > 0x7fffffff) return "n_experts * N below 2^31";
+  if (d->precision < B200_PREC_FP32 || d->precision > B200_PREC_BF16) return "unknown precision";
+  if (d->precision == B200_PREC_FP32 && !d->int8) return "fp16, bf16 or int8";
+  if (d->activation < ACT_MISH || d->activation > ACT_RELU_2) return "unknown activation";
+  if ((d->ldx && d->ldx < d->K) || (d->ldw && d->ldw < d->K) || (d->ldc && d->ldc < d->N) || (d->res && d->ldres && d->ldres < d->N)) return "rows overlap";
+  if (d->c_by_slot && (d->weights || d->res)) return "weights and res are for results by token";
+  return nullptr;
+}
+
+}  // namespace
+}  // namespace b200
+
+extern "C" int b200_op_gemm_int8(const b200_gemm_int8_desc* d, void* stream) {
+  using namespace b200;
+  return at_c_entry([&]() -> int {
+    const char* wrong = nullptr;
+    if (!d) wrong = "no description";
+    else if (d->M < 0 || d->M > 1 << 30 || d->N < 1 || d->K < 1 || d->K > B200_INT8_MAX_K) wrong = "M of 0 to 2^30, N >= 1, K of 1 to 131071";
+    else if (d->precision < B200_PREC_FP32 || d->precision > B200_PREC_BF16) wrong = "unknown precision";
+    else if (d->activation < ACT_MISH || d->activation > ACT_RELU_2) wrong = "unknown activation";
+    else if ((d->ldx && d->ldx < d->K) || (d->ldw && d->ldw < d->K) || (d->ldc && d->ldc < d->N) || (d->res && d->ldres && d->ldres < d->N))
+      wrong = "rows overlap";
+    else if (d->M > 0) {
+      const uintptr_t size = size_of(d->precision);
+      if (!d->X || !d->W || !d->C || !d->x_scales || !d->w_scales) wrong = "X, W, C and both scales are needed";
+      else if (off(d->C, size) || off(d->res, size) || off(d->x_scales, 4) || off(d->w_scales, 4) || off(d->bias, 4) || off(d->status, 4))
+        wrong = "an operand is not aligned to its type";
+      else if (d->res == d->C && (d->ldres ? d->ldres : d->N) != (d->ldc ? d->ldc : d->N)) wrong = "res in place has C's leading dimension";
+    }
+    if (wrong) {
+      set_error(std::string("b200_op_gemm_int8: ") + wrong);
+      return B200_ERR_INVALID;
+    }
+    if (d->M == 0) return B200_OK;
+    GroupedParams p = {};
+    p.X = d->X; p.ldx = d->ldx ? d->ldx : d->K; p.x_rows = d->M;
+    p.W = d->W; p.ldw = d->ldw ? d->ldw : d->K;
+    p.bias = d->bias; p.x_scales = d->x_scales; p.w_scales = d->w_scales;
+    p.C = d->C; p.ldc = d->ldc ? d->ldc : d->N; p.res = d->res; p.ldres = d->ldres ? d->ldres : d->N;
+    p.alpha = d->alpha; p.slots = d->M; p.N = d->N; p.K = d->K; p.experts = 1; p.top_k = 1; p.group = 1; p.act = d->activation;
+    p.status = d->status;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    DependentLaunches dependent;
+    if (d->precision == B200_PREC_FP32) return run_grouped<int8_t, float>(p, s);
+    if (d->precision == B200_PREC_FP16) return run_grouped<int8_t, __half>(p, s);
+    return run_grouped<int8_t, __nv_bfloat16>(p, s);
+  });
+}
+
+extern "C" int b200_op_gemm_experts_workspace(const b200_experts_desc* d, size_t* bytes) {
+  using namespace b200;
+  return at_c_entry([&]() -> int {
+    const char* wrong = check_shape(d);
+    if (!wrong && !bytes) wrong = "nowhere to put the size";
+    if (wrong) {
+      set_error(std::string("b200_op_gemm_experts_workspace: ") + wrong);
+      return B200_ERR_INVALID;
+    }
+    *bytes = experts_bytes(*d);
+    return B200_OK;
+  });
+}
+
+extern "C" int b200_op_gemm_experts(const b200_experts_desc* d, void* stream) {
+  using namespace b200;
+  return at_c_entry([&]() -> int {
+    const char* wrong = check_shape(d);
+    if (!wrong && d->M > 0) {
+      const uintptr_t in = d->int8 ? 1 : size_of(d->precision), out = d->out_f32 ? 4 : size_of(d->precision);
+      if (!d->X || !d->W || !d->C || !d->order || !d->offsets) wrong = "X, W, C, order and offsets are needed";
+      else if (d->int8 && (!d->x_scales || !d->w_scales)) wrong = "int8 needs both scales";
+      else if (sums_choices(*d) && !d->ids) wrong = "the sum over choices needs ids";
+      else if (off(d->X, in) || off(d->W, in) || off(d->C, out) || off(d->res, out) || off(d->bias, 4) || off(d->x_scales, 4) || off(d->w_scales, 4) ||
+               off(d->ids, 4) || off(d->order, 4) || off(d->offsets, 4) || off(d->weights, 4) || off(d->status, 4))
+        wrong = "an operand is not aligned to its type";
+      else if (d->res == d->C && (d->ldres ? d->ldres : d->N) != (d->ldc ? d->ldc : d->N)) wrong = "res in place has C's leading dimension";
+      else if (experts_bytes(*d) && (!d->workspace || off(d->workspace, 256) || d->workspace_bytes < experts_bytes(*d)))
+        wrong = "the workspace is missing, too small or not on a 256-byte boundary";
+    }
+    if (wrong) {
+      set_error(std::string("b200_op_gemm_experts: ") + wrong);
+      return B200_ERR_INVALID;
+    }
+    if (d->M == 0) return B200_OK;
+    const bool sums = sums_choices(*d), f32 = d->out_f32 || d->precision == B200_PREC_FP32;
+    GroupedParams p = {};
+    p.X = d->X; p.ldx = d->ldx ? d->ldx : d->K; p.x_rows = d->x_by_slot ? d->M * d->top_k : d->M;
+    p.W = d->W; p.ldw = d->ldw ? d->ldw : d->K; p.bias = d->bias;
+    if (d->int8) { p.x_scales = d->x_scales; p.w_scales = d->w_scales; }
+    p.C = sums ? d->workspace : d->C; p.ldc = !sums && d->ldc ? d->ldc : d->N;
+    if (!sums) { p.res = d->res; p.ldres = d->ldres ? d->ldres : d->N; }
+    p.alpha = 1.f; p.weights = d->weights; p.order = d->order; p.offsets = d->offsets;
+    p.slots = d->M * d->top_k; p.N = d->N; p.K = d->K; p.experts = d->n_experts; p.top_k = d->top_k; p.group = d->group; p.act = d->activation;
+    p.x_by_slot = d->x_by_slot; p.c_by_slot = d->c_by_slot; p.by_choice = sums;
+    p.status = d->status;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    DependentLaunches dependent;
+    int rc = B200_OK;
+    const bool wide = f32 || sums;
+    if (d->int8) {
+      rc = wide ? run_grouped<int8_t, float>(p, s) : d->precision == B200_PREC_FP16 ? run_grouped<int8_t, __half>(p, s) : run_grouped<int8_t, __nv_bfloat16>(p, s);
+    } else if (d->precision == B200_PREC_FP16) {
+      rc = wide ? run_grouped<__half, float>(p, s) : run_grouped<__half, __half>(p, s);
+    } else {
+      rc = wide ? run_grouped<__nv_bfloat16, float>(p, s) : run_grouped<__nv_bfloat16, __nv_bfloat16>(p, s);
+    }
+    if (rc != B200_OK || !sums) return rc;
+    CombineParams c = {};
+    c.Y = static_cast<const float*>(d->workspace); c.ids = d->ids; c.res = d->res; c.ldres = d->ldres ? d->ldres : d->N;
+    c.C = d->C; c.ldc = d->ldc ? d->ldc : d->N; c.tokens = d->M; c.N = d->N; c.experts = d->n_experts; c.top_k = d->top_k; c.group = d->group;
+    if (f32) B200_CUDA(launch_combine<float>(c, s));
+    else if (d->precision == B200_PREC_FP16) B200_CUDA(launch_combine<__half>(c, s));
+    else B200_CUDA(launch_combine<__nv_bfloat16>(c, s));
+    return B200_OK;
+  });
+}

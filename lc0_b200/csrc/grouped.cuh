@@ -1,0 +1,51 @@
+// Products grouped by expert, and those of 8-bit integers, which have one group: what their kernels share.
+#pragma once
+#include "kernels.cuh"
+
+namespace b200 {
+
+// v[slot][n] = act(scales * (X[x_row(slot)] . W[e]^T) + bias[e][n]) with the slot's expert e; see b200_op_gemm_experts and b200_op_gemm_int8.
+// The output is alpha * weight * v + res, stored by token, by slot, or by choice (`sums`, fp32, which combine_kernel adds up).
+struct GroupedParams {
+  const void* X; long long ldx; int x_rows;
+  const void* W; long long ldw;
+  const float* bias; const float* x_scales; const float* w_scales;
+  void* C; long long ldc;
+  const void* res; long long ldres;
+  float alpha;
+  const float* weights;
+  const int* order; const int* offsets;  // null: one group, all slots in order
+  int slots;                             // rows of choices there may be (M * top_k)
+  int N, K, experts, top_k, group, act;
+  int x_by_slot, c_by_slot, by_choice;
+  int* status;
+};
+
+// The rows of a slot.  x: of X; c: of C (and res); choice: in `weights`.  c < 0: no row.
+struct SlotRows {
+  int x, c, choice;
+};
+__device__ __forceinline__ SlotRows rows_of_slot(const GroupedParams& p, int slot) {
+  SlotRows r;
+  if (!p.order) {
+    r.x = r.c = slot;
+    r.choice = 0;
+    return r;
+  }
+  const int s = p.group == 1 ? slot : slot / p.group, i = p.group == 1 ? 0 : slot - s * p.group;
+  const int choice = __ldg(p.order + s);
+  if (choice < 0 || choice >= p.slots / p.group) return {-1, -1, 0};
+  const int token = (p.top_k == 1 ? choice : choice / p.top_k) * p.group + i;
+  r.x = p.x_by_slot ? slot : token;
+  r.c = p.c_by_slot ? slot : p.by_choice ? choice * p.group + i : token;
+  r.choice = choice;
+  return r;
+}
+// offsets[e] in slots, held within what there is.
+__device__ __forceinline__ int expert_begin(const GroupedParams& p, int e) {
+  if (!p.offsets) return e == 0 ? 0 : p.slots;
+  const int most = p.slots / p.group, at = __ldg(p.offsets + e);
+  return (at < 0 ? 0 : at < most ? at : most) * p.group;
+}
+
+}  // namespace b200
