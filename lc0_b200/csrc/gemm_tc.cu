@@ -2057,6 +2057,25 @@ cudaError_t tma_encode_2d(const void* ptr, long long ld, long long rows, int col
   return cudaSuccess;
 }
 
+cudaError_t tma_encode_rows(const void* ptr, long long ld, long long rows, int cols, int box_rows, int prec, void* out) {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  if (!g_encode) return cudaErrorNotReady;
+  const int size = prec == 3 ? 1 : 2;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * size};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = g_encode(reinterpret_cast<CUtensorMap*>(out),
+                        prec == 3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : prec == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                        const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with CUresult " + std::to_string((int)r));
+    return cudaErrorInvalidValue;
+  }
+  return cudaSuccess;
+}
+
 cudaError_t gemm_f32_map(const float* ptr, long long ld, int rows, int cols, bool board, CUtensorMap* out) {
   std::lock_guard<std::mutex> lock(g_mutex);
   if (!g_encode) return cudaErrorNotReady;

@@ -160,9 +160,23 @@ cudaError_t launch_combine(const CombineParams& p, cudaStream_t s) {
   return launch_dependent(combine_kernel<TOut>, dim3((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64)), dim3(256), 0, s, p, vec);
 }
 
+// Rows of X and W that TMA can read.
+template <typename TIn> bool tma_readable(const GroupedParams& p) {
+  const int per = 16 / (int)sizeof(TIn);
+  return p.K % per == 0 && p.ldx % per == 0 && p.ldw % per == 0 && reinterpret_cast<uintptr_t>(p.X) % 16 == 0 && reinterpret_cast<uintptr_t>(p.W) % 16 == 0;
+}
+
 template <typename TIn, typename TOut>
-int run_grouped(const GroupedParams& p, cudaStream_t s) {
-  B200_CUDA((launch_any<TIn, TOut>(p, s)));
+int run_grouped(const GroupedParams& p, bool exact_sums, cudaStream_t s) {
+  if (!tma_readable<TIn>(p) || exact_sums) {
+    B200_CUDA((launch_any<TIn, TOut>(p, s)));
+    return B200_OK;
+  }
+  int dev = 0, sms = 0;
+  B200_CUDA(gemm_tc_init());
+  B200_CUDA(cudaGetDevice(&dev));
+  B200_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  B200_CUDA((launch_grouped_pair<TIn, TOut>(p, sms, s)));
   return B200_OK;
 }
 
@@ -224,9 +238,9 @@ extern "C" int b200_op_gemm_int8(const b200_gemm_int8_desc* d, void* stream) {
     p.status = d->status;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     DependentLaunches dependent;
-    if (d->precision == B200_PREC_FP32) return run_grouped<int8_t, float>(p, s);
-    if (d->precision == B200_PREC_FP16) return run_grouped<int8_t, __half>(p, s);
-    return run_grouped<int8_t, __nv_bfloat16>(p, s);
+    if (d->precision == B200_PREC_FP32) return run_grouped<int8_t, float>(p, false, s);
+    if (d->precision == B200_PREC_FP16) return run_grouped<int8_t, __half>(p, false, s);
+    return run_grouped<int8_t, __nv_bfloat16>(p, false, s);
   });
 }
 
@@ -281,11 +295,11 @@ extern "C" int b200_op_gemm_experts(const b200_experts_desc* d, void* stream) {
     int rc = B200_OK;
     const bool wide = f32 || sums;
     if (d->int8) {
-      rc = wide ? run_grouped<int8_t, float>(p, s) : d->precision == B200_PREC_FP16 ? run_grouped<int8_t, __half>(p, s) : run_grouped<int8_t, __nv_bfloat16>(p, s);
+      rc = wide ? run_grouped<int8_t, float>(p, false, s) : d->precision == B200_PREC_FP16 ? run_grouped<int8_t, __half>(p, false, s) : run_grouped<int8_t, __nv_bfloat16>(p, false, s);
     } else if (d->precision == B200_PREC_FP16) {
-      rc = wide ? run_grouped<__half, float>(p, s) : run_grouped<__half, __half>(p, s);
+      rc = wide ? run_grouped<__half, float>(p, f32, s) : run_grouped<__half, __half>(p, false, s);
     } else {
-      rc = wide ? run_grouped<__nv_bfloat16, float>(p, s) : run_grouped<__nv_bfloat16, __nv_bfloat16>(p, s);
+      rc = wide ? run_grouped<__nv_bfloat16, float>(p, f32, s) : run_grouped<__nv_bfloat16, __nv_bfloat16>(p, false, s);
     }
     if (rc != B200_OK || !sums) return rc;
     CombineParams c = {};

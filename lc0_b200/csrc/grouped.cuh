@@ -48,4 +48,7 @@ __device__ __forceinline__ int expert_begin(const GroupedParams& p, int e) {
   return (at < 0 ? 0 : at < most ? at : most) * p.group;
 }
 
+// Many rows (grouped_pair.cu): operands that TMA can read.
+template <typename TIn, typename TOut> cudaError_t launch_grouped_pair(const GroupedParams& p, int sm_count, cudaStream_t s);
+
 }  // namespace b200

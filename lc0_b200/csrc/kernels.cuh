@@ -131,6 +131,9 @@ cudaError_t gemm_tc_init();  // resolves the driver entry point used to encode T
 cudaError_t tma_encode_2d(const void* ptr, long long ld, long long rows, int cols, int box_cols, int box_rows,
                           int swizzle_bytes, int prec, void* out);
 
+// The same over rows of 128-byte pieces (64 16-bit entries, or 128 8-bit integers with prec 3), box of one piece x box_rows, 128-byte swizzle.
+cudaError_t tma_encode_rows(const void* ptr, long long ld, long long rows, int cols, int box_rows, int prec, void* out);
+
 // fp32 products and 3x3 convolutions on tensor cores (gemm_f32.cu), with W cut into pieces [3][...] ahead of time.
 cudaError_t launch_split_weights(const float* w, long long count, void* planes, cudaStream_t s);
 bool gemm_f32_supported(const GemmParams& p);
