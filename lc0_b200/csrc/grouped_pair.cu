@@ -2,7 +2,8 @@
 //
 // A persistent grid of pairs walks the tiles of all experts (256 slots of one expert each; how many an expert has is read on the device).  Per
 // k-block of 128 bytes each CTA fetches its 128 rows of X and half of the tile's rows of W:
-//   warp 0      TMA producer.  Rows that lie in order come as one box; those that the order names by gather4, four rows per lane.
+//   warp 0      TMA producer of W, and of X where its rows lie in order
+//   warps 2, 3  gather4 of X's rows that the order names, 64 rows each
 //   warp 1      tcgen05.mma issuer (even CTA), kind::f16 or kind::i8, two accumulators in tensor memory
 //   warps 4-11  epilogue: two groups of four warps, 128 bytes of each of a warp's 32 rows at a time: tensor memory -> scales, bias, activation,
 //               weight, residual -> the warp's own staging buffer -> whole 128-byte pieces of the rows.  Rows behind the expert's last are not
@@ -38,10 +39,10 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uin
   }
 }
 // Four rows of a matrix, 128 bytes of each, one below the other; counted on a barrier of either CTA of the pair.
-__device__ __forceinline__ void tma_gather4_pair(uint32_t dst, const CUtensorMap* map, int x, const int (&row)[4], uint32_t bar) {
+__device__ __forceinline__ void tma_gather4_pair(uint32_t dst, const CUtensorMap* map, int x, const int4 row, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row.x), "r"(row.y), "r"(row.z), "r"(row.w), "r"(bar)
       : "memory");
 }
 
@@ -52,8 +53,8 @@ template <int BN> struct GroupedPairCfg {
   static constexpr int kTmemCols = 2 * BN;
   static constexpr int kStagingBytes = 8 * 32 * 128;
   static constexpr int kVecBytes = 8 * 128 * 4;                    // per epilogue warp: bias and scale of 64 columns
-  static constexpr int kListBytes = 2 * (B200_MAX_EXPERTS + 1) * 4;  // first tile and first slot of each expert
-  static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + kVecBytes + kListBytes + 256 + 1024;
+  static constexpr int kListBytes = (2 * (B200_MAX_EXPERTS + 1) * 4 + 15) / 16 * 16;  // first tile and first slot of each expert
+  static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + kVecBytes + kListBytes + BM * 4 + 256 + 1024;
 };
 
 // A tile of the walk: its expert, the first slot and column.
@@ -93,7 +94,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   float* vectors = reinterpret_cast<float*>(staging + Cfg::kStagingBytes);
   int* first = reinterpret_cast<int*>(staging + Cfg::kStagingBytes + Cfg::kVecBytes);
   int* begin = first + B200_MAX_EXPERTS + 1;
-  uint8_t* bar_mem = reinterpret_cast<uint8_t*>(first) + Cfg::kListBytes;
+  int* gathered = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(first) + Cfg::kListBytes);  // [128] rows of X of this CTA's half tile
+  uint8_t* bar_mem = reinterpret_cast<uint8_t*>(gathered + BM);
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(bar_mem);  // [S]  waited on by the even CTA only
   uint64_t* empty_bar = full_bar + S;                          // [S]  per CTA
   uint64_t* tfull_bar = empty_bar + S;                         // [2]  per CTA
@@ -163,38 +165,24 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   int s0, end, n0;
 
   if (warp == 0) {
-    // ---------------- TMA producer (both CTAs) ----------------
-    int s = 0;
-    uint32_t ph = 0;
-    bool ok = true;
-    int row[4] = {0, 0, 0, 0};
-    for (int t = pair; t < tiles && ok; t += pairs) {
-      walk.at(t, BN, s0, end, n0);
-      s0 += (int)rank * BM;
-      if constexpr (kGather) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int slot = s0 + 4 * lane + i, x = slot < end ? rows_of_slot(p, slot).x : 0;
-          row[i] = x < 0 ? 0 : x;  // whatever lies there: its results are not stored
-        }
-      }
-      const int w_row = walk.e * p.N + n0 + (int)rank * (min(BN, (p.N - n0 + 31) & ~31) / 2);
-      for (int kb = 0; kb < k_blocks; ++kb) {
-        if (lane == 0) ok = mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 1);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) break;
-        const uint32_t fb_local = smem_u32(&full_bar[s]);
-        const uint32_t fb = mapa(fb_local, 0), sa = smem_u32(smem + s * Cfg::kStageBytes);
-        if (elect_one()) {
+    // ---------------- TMA producer (both CTAs): W, and X where its rows lie in order ----------------
+    if (elect_one()) {
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        walk.at(t, BN, s0, end, n0);
+        s0 += (int)rank * BM;
+        const int w_row = walk.e * p.N + n0 + (int)rank * (min(BN, (p.N - n0 + 31) & ~31) / 2);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 1)) { ok = false; break; }
+          const uint32_t fb_local = smem_u32(&full_bar[s]);
+          const uint32_t fb = mapa(fb_local, 0), sa = smem_u32(smem + s * Cfg::kStageBytes);
           if (rank == 0) mbar_expect_tx(fb_local, 2 * Cfg::kStageBytes);
           if constexpr (!kGather) tma_load_2d_pair(sa, &map_x, kb * Operand<TIn>::k, s0, fb);
           tma_load_2d_pair(sa + BM * 128, &map_w, kb * Operand<TIn>::k, w_row, fb);
+          if (++s == S) { s = 0; ph ^= 1; }
         }
-        if constexpr (kGather) {
-          __syncwarp();
-          tma_gather4_pair(sa + lane * 512, &map_x, kb * Operand<TIn>::k, row, fb);
-        }
-        if (++s == S) { s = 0; ph ^= 1; }
       }
     }
   } else if (warp == 1) {
@@ -223,7 +211,37 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         if (ok) tcgen05_commit_both(smem_u32(&tfull_bar[acc]));
       }
     }
-  } else if (warp >= 4) {
+  } else if (warp < 4) {
+    // ---------------- gather (both CTAs): half of the CTA's rows of X each ----------------
+    if constexpr (kGather) {
+      int* rows = gathered + (warp - 2) * 64;
+      uint32_t done = 0;  // k-blocks before this tile's
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs, done += k_blocks) {
+        walk.at(t, BN, s0, end, n0);
+        s0 += (int)rank * BM + (warp - 2) * 64;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int slot = s0 + 32 * i + lane, x = slot < end ? rows_of_slot(p, slot).x : 0;
+          rows[32 * i + lane] = x < 0 ? 0 : x;  // whatever lies there: its results are not stored
+        }
+        __syncwarp();
+        if (elect_one()) {
+          int s = (int)(done % S);
+          uint32_t ph = (done / S) & 1;
+          for (int kb = 0; kb < k_blocks; ++kb) {
+            if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 5)) { ok = false; break; }
+            const uint32_t fb = mapa(smem_u32(&full_bar[s]), 0), sa = smem_u32(smem + s * Cfg::kStageBytes) + (warp - 2) * 64 * 128;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) tma_gather4_pair(sa + i * 512, &map_x, kb * Operand<TIn>::k, reinterpret_cast<const int4*>(rows)[i], fb);
+            if (++s == S) { s = 0; ph ^= 1; }
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+      }
+    }
+  } else {
     // ---------------- epilogue ----------------
     const int quarter = warp & 3, group = (warp - 4) >> 2;
     uint8_t* mine_bytes = staging + (warp - 4) * 4096;
