@@ -168,7 +168,7 @@ template <typename TIn> bool tma_readable(const GroupedParams& p) {
 
 template <typename TIn, typename TOut>
 int run_grouped(const GroupedParams& p, bool exact_sums, cudaStream_t s) {
-  if (!tma_readable<TIn>(p) || exact_sums) {
+  if (!tma_readable<TIn>(p)) {
     B200_CUDA((launch_any<TIn, TOut>(p, s)));
     return B200_OK;
   }
@@ -176,7 +176,9 @@ int run_grouped(const GroupedParams& p, bool exact_sums, cudaStream_t s) {
   B200_CUDA(gemm_tc_init());
   B200_CUDA(cudaGetDevice(&dev));
   B200_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  B200_CUDA((launch_grouped_pair<TIn, TOut>(p, sms, s)));
+  const int used = p.experts < p.slots ? p.experts : p.slots;
+  if (exact_sums || p.slots / used <= 64) B200_CUDA((launch_grouped_rows<TIn, TOut>(p, exact_sums, sms, s)));
+  else B200_CUDA((launch_grouped_pair<TIn, TOut>(p, sms, s)));
   return B200_OK;
 }
 

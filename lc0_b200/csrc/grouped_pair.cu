@@ -10,21 +10,10 @@
 //               stored, which a TMA store of the tile could not leave out.
 // Every wait is bounded by wall-clock time like those of gemm_tc.cu.
 #include "chunk8.cuh"
-#include "grouped.cuh"
-#include "tcgen05.cuh"
+#include "grouped_tc.cuh"
 
 namespace b200 {
 namespace {
-
-template <typename T> struct Operand {
-  static constexpr int prec = TypeTag<T>::prec, k = 64;
-  static constexpr uint32_t idesc = (1u << 4) | (FmtCode<T>::v << 7) | (FmtCode<T>::v << 10);
-};
-// D format s32 (bits 4-5 = 2), A and B signed (bits 7-9, 10-12 = 1)
-template <> struct Operand<int8_t> {
-  static constexpr int prec = 3, k = 128;
-  static constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10);
-};
 
 template <typename T>
 __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -56,31 +45,6 @@ template <int BN> struct GroupedPairCfg {
   static constexpr int kListBytes = (2 * (B200_MAX_EXPERTS + 1) * 4 + 15) / 16 * 16;  // first tile and first slot of each expert
   static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + kVecBytes + kListBytes + BM * 4 + 256 + 1024;
 };
-
-// A tile of the walk: its expert, the first slot and column.
-struct TileWalk {
-  const int* first;  // [experts + 1] row tiles ahead of each expert's
-  const int* begin;  // [experts + 1] slots
-  int experts, n_tiles, e = 0;
-  __device__ __forceinline__ int total() const { return first[experts] * n_tiles; }
-  // t may only grow
-  __device__ __forceinline__ void at(int t, int bn, int& s0, int& end, int& n0) {
-    const int mt = t / n_tiles;
-    while (first[e + 1] <= mt) ++e;
-    s0 = begin[e] + (mt - first[e]) * (2 * BM);
-    end = begin[e + 1];
-    n0 = (t - mt * n_tiles) * bn;
-  }
-};
-
-template <typename TOut> __device__ __forceinline__ void activate32(float (&v)[32], int act) {
-  if constexpr (sizeof(TOut) == 2) {
-    apply_activation(v, act);
-  } else if (act != ACT_NONE) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = activate<false>(v[j], act);
-  }
-}
 
 template <typename TIn, typename TOut, int BN, bool kGather>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg<BN>::kThreads, 1)
@@ -130,37 +94,13 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   grid_dependency_wait();
-  // row tiles ahead of each expert's
-  int mine = 0, upto = 0;
-  if (threadIdx.x < 256) {
-    const int e = threadIdx.x;
-    if (e < p.experts) {
-      const int b = expert_begin(p, e), n = expert_begin(p, e + 1) - b;
-      begin[e] = b;
-      if (e == p.experts - 1) begin[p.experts] = b + max(n, 0);
-      mine = n > 0 ? (n + 2 * BM - 1) / (2 * BM) : 0;
-    }
-    upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int n = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += n;
-    }
-    if (lane == 31) scan[warp] = upto;
-  }
   tcgen05_fence_before();
-  __syncthreads();
-  if (threadIdx.x < 256) {
-    for (int w = 0; w < warp; ++w) upto += scan[w];
-    if (threadIdx.x < (unsigned)p.experts) first[threadIdx.x + 1] = upto;
-    if (threadIdx.x == 0) first[0] = 0;
-  }
-  __syncthreads();
+  list_tiles<2 * BM>(p, first, begin, scan);
   cluster_sync_all();  // the peer's barriers are initialised before anything arrives on them
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   grid_launch_dependents();  // not ahead of the tensor memory: a dependent that took it would hold it while it waits for this kernel
-  TileWalk walk{first, begin, p.experts, n_tiles};
+  TileWalk<2 * BM> walk{first, begin, p.experts, n_tiles};
   const int tiles = walk.total();
   int s0, end, n0;
 
@@ -412,8 +352,6 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)Cfg::kTmemCols) : "memory");
   }
 }
-
-bool aligned16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; }
 
 template <typename TIn, typename TOut, int BN, bool kGather>
 cudaError_t launch_tiles(const GroupedParams& p, int sm_count, cudaStream_t s) {
