@@ -24,32 +24,53 @@ template <typename T> __device__ __forceinline__ uint32_t largest8(const Chunk<T
   return max(size_bits(f.x), size_bits(f.y));
 }
 
-// x / s to the nearest whole number as the exact quotient has it: the sign of x - (r +- 1/2) s, which one fma gives without a rounding that
-// could change it, says on which side of a tie x lies.
-__device__ __noinline__ int exact_q(float x, float s) {
-  if (s < 1e-30f) return (int)fmin(fmax(rint((double)x / (double)s), -127.0), 127.0);  // the reciprocal and the fma may leave fp32's range
-  float r = rintf(x / s);
-  const float up = fmaf(-(r + 0.5f), s, x), down = fmaf(-(r - 0.5f), s, x);
-  const bool odd = ((int)r & 1) != 0;
-  if (up > 0.f || (up == 0.f && odd)) r += 1.f;
-  else if (down < 0.f || (down == 0.f && odd)) r -= 1.f;
-  return (int)fminf(fmaxf(r, -127.f), 127.f);
-}
+// x / s where the reciprocal of s, or what the steps below need, may leave fp32's range.
+__device__ __noinline__ uint32_t tiny_q(float x, float s) { return (uint32_t)(int)fmin(fmax(rint((double)x / (double)s), -127.0), 127.0); }
 
-// Adding 1.5 2^23 rounds to a whole number and leaves it in the low byte.  The product with the reciprocal is off by 2e-5 at most: chunks
-// with a quotient that close to a tie are done again exactly.
+// x / s to the nearest whole number, in the low byte.  Adding 1.5 2^23 rounds the product with the reciprocal, which is off by 1e-5 at most, to r
+// or, beside a tie, to its neighbour.  e = x - r s is exact there (a multiple of half an ulp of s below s), so comparing it with s / 2 says which:
+// beyond it the neighbour is nearer, and at a tie the even one of the two is taken.  bf16 rows meet ties often, by the eight bits of their entries: with
+// these steps for chunks that have one alone, most warps took both ways (65536x1536 127 us).
+__device__ __forceinline__ uint32_t exact_q(float x, float s, float inv) {
+  const float t = fmaf(x, inv, 12582912.f);
+  uint32_t b = __float_as_uint(t);
+  const float e = fmaf(12582912.f - t, s, x);
+  const float limit = __uint_as_float(__float_as_uint(0.5f * s) + (~b & 1u));  // an even r keeps the tie
+  if (fabsf(e) >= limit) b += (uint32_t)((__float_as_int(e) >> 31) | 1);
+  return b;
+}
+// Two at a time where the arithmetic comes in pairs.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t nearer(uint32_t b, float e, uint32_t half) {
+  const float limit = __uint_as_float(half + (~b & 1u));
+  if (fabsf(e) >= limit) b += (uint32_t)((__float_as_int(e) >> 31) | 1);
+  return b;
+}
 __device__ __forceinline__ uint2 quantize8(const float (&v)[8], float s, float inv) {
   uint32_t b[8];
-  float far = 0.f;
+  const uint64_t inv2 = two(inv, inv), s2 = two(s, s), magic = two(12582912.f, 12582912.f), minus = two(-1.f, -1.f);
+  const uint32_t half = __float_as_uint(0.5f * s);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = fmaf(v[i], inv, 12582912.f);
-    b[i] = __float_as_uint(t);
-    far = fmaxf(far, fabsf(fmaf(v[i], inv, 12582912.f - t)));
+  for (int i = 0; i < 8; i += 2) {
+    const uint64_t x2 = two(v[i], v[i + 1]), t2 = fma2(x2, inv2, magic), e2 = fma2(fma2(t2, minus, magic), s2, x2);
+    float e0, e1;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(b[i]), "=r"(b[i + 1]) : "l"(t2));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(e0), "=f"(e1) : "l"(e2));
+    b[i] = nearer(b[i], e0, half);
+    b[i + 1] = nearer(b[i + 1], e1, half);
   }
-  if (far > 0.4999f) {
+  if (inv == 0.f) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = (uint32_t)exact_q(v[i], s);
+    for (int i = 0; i < 8; ++i) b[i] = tiny_q(v[i], s);
   }
   uint2 q;
   q.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
@@ -59,64 +80,97 @@ __device__ __forceinline__ uint2 quantize8(const float (&v)[8], float s, float i
 
 struct RowScale {
   float s, inv;
-  bool zero;   // all entries become 0
-  bool exact;  // the reciprocal is not usable
+  bool zero;  // all entries become 0
 };
 __device__ __forceinline__ RowScale scale_of(uint32_t largest) {
   RowScale r;
   r.s = __fmul_rn(__uint_as_float(largest), 1.f / 127.f);
   if (largest >= 0x7f800000u) r.s = __uint_as_float(0x7fffffffu);
   r.zero = !(r.s > 0.f);
-  r.exact = r.s < 1e-30f;
-  r.inv = r.zero || r.exact ? 0.f : 1.f / r.s;
+  r.inv = r.zero || r.s < 1e-30f ? 0.f : 1.f / r.s;
   return r;
 }
 
-// A warp per row, which stays in registers (kPer chunks of eight entries per lane) where it fits, and is read again where it does not.
-template <typename T, int kPer>
-__global__ void __launch_bounds__(32 * kWarps) quantize_rows_kernel(const T* X, long long ldx, int M, int K, int8_t* Q, long long ldq, float* scales) {
+template <typename T> __device__ __forceinline__ Chunk<T> load8_once(const T* p) {  // read once: leaves L2 ahead of what is written
+  Chunk<T> c;
+#pragma unroll
+  for (int i = 0; i < Chunk<T>::kLoads; ++i) c.raw[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  return c;
+}
+
+// A row in the registers of kThreads threads, kPer chunks of eight entries each; the next row is on its way meanwhile.
+//   Many rows: a warp each, as many as fit, each walking over its rows (us, a warp for one row and the next CTA behind it / now: 65536x1536 bf16
+//   69 / 60, 65536x1024 fp32 62 / 53: 5.0 and 6.3 TB/s of 6.55).
+//   Few rows: four warps each, so that a thread has one or two chunks (64x1024 1.2 us in a chain of launches).
+template <typename T, int kPer, int kThreads>
+__global__ void __launch_bounds__(128) quantize_rows_kernel(const T* X, long long ldx, int M, int K, int8_t* Q, long long ldq, float* scales) {
+  __shared__ uint32_t of_warp[4];
   grid_launch_dependents();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31, chunks = K / 8;
-  for (long long m = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); m < M; m += (long long)gridDim.x * kWarps) {
-    const T* x = X + m * ldx;
-    Chunk<T> held[kPer > 0 ? kPer : 1];
+  const int at = threadIdx.x % kThreads, chunks = K / 8;
+  const long long step = (long long)gridDim.x * (128 / kThreads);
+  long long m = (long long)blockIdx.x * (128 / kThreads) + threadIdx.x / kThreads;
+  Chunk<T> next[kPer];
+  auto fetch = [&](long long row) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (row < M && at + kThreads * i < chunks) next[i] = load8_once(X + row * ldx + 8 * (at + kThreads * i));
+  };
+  fetch(m);
+  for (; m < M; m += step) {
+    Chunk<T> held[kPer];
     uint32_t largest = 0;
-    if constexpr (kPer > 0) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (lane + 32 * i < chunks) held[i] = load8(x + 8 * (lane + 32 * i));
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (lane + 32 * i < chunks) largest = max(largest, largest8(held[i]));
-    } else {
-#pragma unroll 4
-      for (int c = lane; c < chunks; c += 32) largest = max(largest, largest8(load8(x + 8 * c)));
+    for (int i = 0; i < kPer; ++i) {
+      held[i] = next[i];
+      if (at + kThreads * i < chunks) largest = max(largest, largest8(held[i]));
     }
-    const RowScale r = scale_of(__reduce_max_sync(0xffffffffu, largest));
-    if (lane == 0) scales[m] = r.s;
-    auto put = [&](const Chunk<T>& c, int at) {
+    fetch(m + step);
+    largest = __reduce_max_sync(0xffffffffu, largest);
+    if constexpr (kThreads > 32) {
+      if (threadIdx.x % 32 == 0) of_warp[threadIdx.x / 32] = largest;
+      __syncthreads();
+      largest = max(max(of_warp[0], of_warp[1]), max(of_warp[2], of_warp[3]));
+      __syncthreads();
+    }
+    const RowScale r = scale_of(largest);
+    if (at == 0) scales[m] = r.s;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int c = at + kThreads * i;
+      if (c >= chunks) continue;
       float v[8];
-      unpack8(c, v);
-      uint2 q = make_uint2(0u, 0u);
-      if (r.exact && !r.zero) {
-        int8_t b[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) b[i] = (int8_t)exact_q(v[i], r.s);
-        q = make_uint2((uint8_t)b[0] | (uint8_t)b[1] << 8 | (uint8_t)b[2] << 16 | (uint32_t)(uint8_t)b[3] << 24,
-                       (uint8_t)b[4] | (uint8_t)b[5] << 8 | (uint8_t)b[6] << 16 | (uint32_t)(uint8_t)b[7] << 24);
-      } else if (!r.zero) {
-        q = quantize8(v, r.s, r.inv);
-      }
-      *reinterpret_cast<uint2*>(Q + m * ldq + 8 * at) = q;
-    };
-    if constexpr (kPer > 0) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (lane + 32 * i < chunks) put(held[i], lane + 32 * i);
-    } else {
+      unpack8(held[i], v);
+      *reinterpret_cast<uint2*>(Q + m * ldq + 8 * c) = r.zero ? make_uint2(0u, 0u) : quantize8(v, r.s, r.inv);
+    }
+  }
+}
+
+// Rows too long for that: a CTA reads each twice.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_long_rows_kernel(const T* X, long long ldx, int M, int K, int8_t* Q, long long ldq, float* scales) {
+  __shared__ uint32_t of_warp[8];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int chunks = K / 8;
+  for (long long m = blockIdx.x; m < M; m += gridDim.x) {
+    const T* x = X + m * ldx;
+    uint32_t largest = 0;
 #pragma unroll 4
-      for (int c = lane; c < chunks; c += 32) put(load8(x + 8 * c), c);
+    for (int c = threadIdx.x; c < chunks; c += 256) largest = max(largest, largest8(load8(x + 8 * c)));
+    largest = __reduce_max_sync(0xffffffffu, largest);
+    if (threadIdx.x % 32 == 0) of_warp[threadIdx.x / 32] = largest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) largest = max(largest, of_warp[w]);
+    __syncthreads();
+    const RowScale r = scale_of(largest);
+    if (threadIdx.x == 0) scales[m] = r.s;
+#pragma unroll 2
+    for (int c = threadIdx.x; c < chunks; c += 256) {
+      float v[8];
+      unpack8(load8_once(x + 8 * c), v);
+      *reinterpret_cast<uint2*>(Q + m * ldq + 8 * c) = r.zero ? make_uint2(0u, 0u) : quantize8(v, r.s, r.inv);
     }
   }
 }
@@ -132,25 +186,50 @@ __global__ void __launch_bounds__(32 * kWarps) quantize_rows_any_kernel(const T*
     for (int k = lane; k < K; k += 32) largest = max(largest, size_bits(to_f(X[m * ldx + k])));
     const RowScale r = scale_of(__reduce_max_sync(0xffffffffu, largest));
     if (lane == 0) scales[m] = r.s;
-    for (int k = lane; k < K; k += 32) Q[m * ldq + k] = r.zero ? (int8_t)0 : (int8_t)exact_q(to_f(X[m * ldx + k]), r.s);
+    for (int k = lane; k < K; k += 32) {
+      const float v = to_f(X[m * ldx + k]);
+      Q[m * ldq + k] = r.zero ? (int8_t)0 : (int8_t)(r.inv == 0.f ? tiny_q(v, r.s) : exact_q(v, r.s, r.inv));
+    }
   }
+}
+
+template <typename T, int kPer, int kThreads>
+cudaError_t launch_rows(const T* x, long long ldx, int M, int K, int8_t* Q, long long ldq, float* scales, cudaStream_t s) {
+  auto kernel = quantize_rows_kernel<T, kPer, kThreads>;
+  const long long blocks = ((long long)M + 128 / kThreads - 1) / (128 / kThreads);
+  int per_sm = 0, dev = 0, sms = 0;
+  cudaError_t e = cudaSuccess;
+  if (kThreads == 32) {
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess || (e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess ||
+        (e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, 128, 0)) != cudaSuccess)
+      return e;
+  }
+  const long long most = kThreads == 32 ? (long long)sms * per_sm : 0x7fffffff;
+  return launch_dependent(kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(128), 0, s, x, ldx, M, K, Q, ldq, scales);
 }
 
 template <typename T>
 cudaError_t launch_quantize(const void* X, long long ldx, int M, int K, int8_t* Q, long long ldq, float* scales, cudaStream_t s) {
   const T* x = static_cast<const T*>(X);
-  const long long blocks = ((long long)M + kWarps - 1) / kWarps;
-  const dim3 grid((unsigned)(blocks < 0x7fffffff ? blocks : 0x7fffffff)), block(32 * kWarps);
+  DependentLaunches dependent;
   const bool vec = K % 8 == 0 && ldx % (16 / (int)sizeof(T)) == 0 && ldq % 8 == 0 && reinterpret_cast<uintptr_t>(X) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(Q) % 8 == 0;
-  auto kernel = !vec         ? quantize_rows_any_kernel<T>
-                : K <= 256   ? quantize_rows_kernel<T, 1>
-                : K <= 512   ? quantize_rows_kernel<T, 2>
-                : K <= 1024  ? quantize_rows_kernel<T, 4>
-                : K <= 2048  ? quantize_rows_kernel<T, 8>
-                             : quantize_rows_kernel<T, 0>;
-  DependentLaunches dependent;
-  return launch_dependent(kernel, grid, block, 0, s, x, ldx, M, K, Q, ldq, scales);
+  if (!vec)
+    return launch_dependent(quantize_rows_any_kernel<T>, dim3((unsigned)(((long long)M + kWarps - 1) / kWarps)), dim3(32 * kWarps), 0, s, x, ldx, M, K, Q, ldq,
+                            scales);
+  const int chunks = K / 8;
+  if (M <= 2048 && chunks > 32) {
+    if (chunks <= 128) return launch_rows<T, 1, 128>(x, ldx, M, K, Q, ldq, scales, s);
+    if (chunks <= 256) return launch_rows<T, 2, 128>(x, ldx, M, K, Q, ldq, scales, s);
+    if (chunks <= 512) return launch_rows<T, 4, 128>(x, ldx, M, K, Q, ldq, scales, s);
+  }
+  if (chunks <= 32) return launch_rows<T, 1, 32>(x, ldx, M, K, Q, ldq, scales, s);
+  if (chunks <= 64) return launch_rows<T, 2, 32>(x, ldx, M, K, Q, ldq, scales, s);
+  if (chunks <= 128) return launch_rows<T, 4, 32>(x, ldx, M, K, Q, ldq, scales, s);
+  if (chunks <= 192) return launch_rows<T, 6, 32>(x, ldx, M, K, Q, ldq, scales, s);
+  if (chunks <= 256) return launch_rows<T, 8, 32>(x, ldx, M, K, Q, ldq, scales, s);
+  if (chunks <= 512) return launch_rows<T, 4, 128>(x, ldx, M, K, Q, ldq, scales, s);
+  return launch_dependent(quantize_long_rows_kernel<T>, dim3((unsigned)(M < 65536 ? M : 65536)), dim3(256), 0, s, x, ldx, M, K, Q, ldq, scales);
 }
 
 }  // namespace
