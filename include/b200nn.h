@@ -504,7 +504,8 @@ int b200_op_route(const b200_route_desc* d, void* stream);
  *   - W [n_experts][N][K] (rows ldw apart, experts N * ldw), bias [n_experts][N] or NULL, `activation`, `precision` (fp16 or bf16) of X, W, C and res;
  *     out_f32: C and res hold float.  int8: X and W are 8-bit integers with x_scales per row of X and w_scales [n_experts][N], as in b200_op_gemm_int8,
  *     and precision may be any.
- *   - workspace: b200_op_gemm_experts_workspace() bytes on a 256-byte boundary, for this call alone until it has run (0 bytes but where choices are summed).
+ *   - workspace: b200_op_gemm_experts_workspace() bytes on a 256-byte boundary, for this call alone until it has run (0 for some
+ *     sizes, and may then be NULL).
  *   Sums in fp32 (int8: exact); float results of 16-bit inputs are as exact as a plain fp32 product.  order entries outside the choices are no rows;
  *   offsets are held to 0 <= offsets[e] <= offsets[e + 1] <= M / group * top_k.  M a multiple of group, M * top_k at most 2^30. */
 typedef struct b200_experts_desc {

@@ -160,15 +160,34 @@ cudaError_t launch_combine(const CombineParams& p, cudaStream_t s) {
   return launch_dependent(combine_kernel<TOut>, dim3((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64)), dim3(256), 0, s, p, vec);
 }
 
-// Rows of X and W that TMA can read.
-template <typename TIn> bool tma_readable(const GroupedParams& p) {
-  const int per = 16 / (int)sizeof(TIn);
-  return p.K % per == 0 && p.ldx % per == 0 && p.ldw % per == 0 && reinterpret_cast<uintptr_t>(p.X) % 16 == 0 && reinterpret_cast<uintptr_t>(p.W) % 16 == 0;
+// ---- rows in the order of their slots ---------------------------------------------------------------------------
+// The pair kernel reads X by boxes of 128 rows, so rows that the order names are copied into their order first, once for all tiles of
+// columns, which then find them in L2.  Fetched in place by TMA's gather4, 33 cycles for four rows and anew for each tile of columns, the
+// product takes half as long again: us, 32768 slots x 1024 to 1536 columns, Mish: 161, now NOW; int8, 18000 slots: 71, now NOW8.  (By cp.async into the
+// swizzled tiles 325: the proxy fence ahead of each hand-over waits for all copies in flight.)
+__global__ void __launch_bounds__(256) spread_rows_kernel(const GroupedParams p, uint8_t* to, int row_bytes, int size) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, pieces = row_bytes / 16;
+  const int end = expert_begin(p, p.experts);
+  for (long long slot = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); slot < end; slot += (long long)gridDim.x * 8) {
+    const int x = rows_of_slot(p, (int)slot).x;
+    if (x < 0) continue;
+    const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.X) + x * p.ldx * size);
+    uint4* at = reinterpret_cast<uint4*>(to + slot * row_bytes);
+#pragma unroll 4
+    for (int i = lane; i < pieces; i += 32) at[i] = from[i];
+  }
 }
 
+// Rows of X and W that TMA can read.
+bool tma_rows(int K, long long ldx, long long ldw, int size) { return K * (long long)size % 16 == 0 && ldx * size % 16 == 0 && ldw * size % 16 == 0; }
+// The pair kernel's 256 slots pay from half a tile per expert on.
+bool many_rows(int slots, int experts) { return slots / (experts < slots ? experts : slots) > 64; }
+
 template <typename TIn, typename TOut>
-int run_grouped(const GroupedParams& p, bool exact_sums, cudaStream_t s) {
-  if (!tma_readable<TIn>(p)) {
+int run_grouped(GroupedParams p, bool exact_sums, void* spread, cudaStream_t s) {
+  if (!tma_rows(p.K, p.ldx, p.ldw, sizeof(TIn)) || reinterpret_cast<uintptr_t>(p.X) % 16 != 0 || reinterpret_cast<uintptr_t>(p.W) % 16 != 0) {
     B200_CUDA((launch_any<TIn, TOut>(p, s)));
     return B200_OK;
   }
@@ -176,9 +195,18 @@ int run_grouped(const GroupedParams& p, bool exact_sums, cudaStream_t s) {
   B200_CUDA(gemm_tc_init());
   B200_CUDA(cudaGetDevice(&dev));
   B200_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  const int used = p.experts < p.slots ? p.experts : p.slots;
-  if (exact_sums || p.slots / used <= 64) B200_CUDA((launch_grouped_rows<TIn, TOut>(p, exact_sums, sms, s)));
-  else B200_CUDA((launch_grouped_pair<TIn, TOut>(p, sms, s)));
+  if (exact_sums || !many_rows(p.slots, p.experts)) {
+    B200_CUDA((launch_grouped_rows<TIn, TOut>(p, exact_sums, sms, s)));
+    return B200_OK;
+  }
+  if (p.order && !p.x_by_slot) {
+    const long long blocks = ((long long)p.slots + 7) / 8;
+    B200_CUDA(launch_dependent(spread_rows_kernel, dim3((unsigned)(blocks < sms * 8 ? blocks : sms * 8)), dim3(256), 0, s, p, static_cast<uint8_t*>(spread),
+                               p.K * (int)sizeof(TIn), (int)sizeof(TIn)));
+    p.X = spread;
+    p.ldx = p.K;
+  }
+  B200_CUDA((launch_grouped_pair<TIn, TOut>(p, sms, s)));
   return B200_OK;
 }
 
@@ -188,7 +216,15 @@ int size_of(int precision) { return precision == B200_PREC_FP32 ? 4 : 2; }
 
 // Choices are summed by a launch of their own, from fp32 rows in the workspace.
 bool sums_choices(const b200_experts_desc& d) { return !d.c_by_slot && d.top_k > 1; }
-size_t experts_bytes(const b200_experts_desc& d) { return sums_choices(d) ? round256((size_t)d.M * d.top_k * d.N * 4) : 0; }
+size_t sums_bytes(const b200_experts_desc& d) { return sums_choices(d) ? round256((size_t)d.M * d.top_k * d.N * 4) : 0; }
+// X in the order of the slots.
+size_t spread_bytes(const b200_experts_desc& d) {
+  const int size = d.int8 ? 1 : 2;
+  const bool spread = !d.x_by_slot && !(d.out_f32 && !d.int8) && d.M > 0 && many_rows(d.M * d.top_k, d.n_experts) &&
+                      tma_rows(d.K, d.ldx ? d.ldx : d.K, d.ldw ? d.ldw : d.K, size);
+  return spread ? round256((size_t)d.M * d.top_k * d.K * size) : 0;
+}
+size_t experts_bytes(const b200_experts_desc& d) { return sums_bytes(d) + spread_bytes(d); }
 
 const char* check_shape(const b200_experts_desc* d) {
   if (!d) return "no description";
@@ -240,9 +276,9 @@ extern "C" int b200_op_gemm_int8(const b200_gemm_int8_desc* d, void* stream) {
     p.status = d->status;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     DependentLaunches dependent;
-    if (d->precision == B200_PREC_FP32) return run_grouped<int8_t, float>(p, false, s);
-    if (d->precision == B200_PREC_FP16) return run_grouped<int8_t, __half>(p, false, s);
-    return run_grouped<int8_t, __nv_bfloat16>(p, false, s);
+    if (d->precision == B200_PREC_FP32) return run_grouped<int8_t, float>(p, false, nullptr, s);
+    if (d->precision == B200_PREC_FP16) return run_grouped<int8_t, __half>(p, false, nullptr, s);
+    return run_grouped<int8_t, __nv_bfloat16>(p, false, nullptr, s);
   });
 }
 
@@ -296,12 +332,15 @@ extern "C" int b200_op_gemm_experts(const b200_experts_desc* d, void* stream) {
     DependentLaunches dependent;
     int rc = B200_OK;
     const bool wide = f32 || sums;
+    void* spread = static_cast<char*>(d->workspace) + sums_bytes(*d);
     if (d->int8) {
-      rc = wide ? run_grouped<int8_t, float>(p, false, s) : d->precision == B200_PREC_FP16 ? run_grouped<int8_t, __half>(p, false, s) : run_grouped<int8_t, __nv_bfloat16>(p, false, s);
+      rc = wide                              ? run_grouped<int8_t, float>(p, false, spread, s)
+           : d->precision == B200_PREC_FP16 ? run_grouped<int8_t, __half>(p, false, spread, s)
+                                             : run_grouped<int8_t, __nv_bfloat16>(p, false, spread, s);
     } else if (d->precision == B200_PREC_FP16) {
-      rc = wide ? run_grouped<__half, float>(p, f32, s) : run_grouped<__half, __half>(p, false, s);
+      rc = wide ? run_grouped<__half, float>(p, f32, spread, s) : run_grouped<__half, __half>(p, false, spread, s);
     } else {
-      rc = wide ? run_grouped<__nv_bfloat16, float>(p, f32, s) : run_grouped<__nv_bfloat16, __nv_bfloat16>(p, false, s);
+      rc = wide ? run_grouped<__nv_bfloat16, float>(p, f32, spread, s) : run_grouped<__nv_bfloat16, __nv_bfloat16>(p, false, spread, s);
     }
     if (rc != B200_OK || !sums) return rc;
     CombineParams c = {};

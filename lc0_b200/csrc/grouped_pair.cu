@@ -2,8 +2,7 @@
 //
 // A persistent grid of pairs walks the tiles of all experts (256 slots of one expert each; how many an expert has is read on the device).  Per
 // k-block of 128 bytes each CTA fetches its 128 rows of X and half of the tile's rows of W:
-//   warp 0      TMA producer of W, and of X where its rows lie in order
-//   warps 2, 3  gather4 of X's rows that the order names, 64 rows each
+//   warp 0      TMA producer
 //   warp 1      tcgen05.mma issuer (even CTA), kind::f16 or kind::i8, two accumulators in tensor memory
 //   warps 4-11  epilogue: two groups of four warps, 128 bytes of each of a warp's 32 rows at a time: tensor memory -> scales, bias, activation,
 //               weight, residual -> the warp's own staging buffer -> whole 128-byte pieces of the rows.  Rows behind the expert's last are not
@@ -27,42 +26,42 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uin
     tcgen05_mma_f16_pair(d, a, b, idesc, accumulate);
   }
 }
-// Four rows of a matrix, 128 bytes of each, one below the other; counted on a barrier of either CTA of the pair.
-__device__ __forceinline__ void tma_gather4_pair(uint32_t dst, const CUtensorMap* map, int x, const int4 row, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row.x), "r"(row.y), "r"(row.z), "r"(row.w), "r"(bar)
-      : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {  // zeros behind `bytes`
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 template <int BN> struct GroupedPairCfg {
   static constexpr int kStageBytes = (BM + BN / 2) * 128;
-  static constexpr int kStages = BN == 256 ? 5 : 6;
+  static constexpr int kMaxStages = BN == 256 ? 5 : 6;
   static constexpr int kThreads = 384;
   static constexpr int kTmemCols = 2 * BN;
   static constexpr int kStagingBytes = 8 * 32 * 128;
   static constexpr int kVecBytes = 8 * 128 * 4;                    // per epilogue warp: bias and scale of 64 columns
   static constexpr int kListBytes = (2 * (B200_MAX_EXPERTS + 1) * 4 + 15) / 16 * 16;  // first tile and first slot of each expert
-  static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + kVecBytes + kListBytes + BM * 4 + 256 + 1024;
+  // With a residual the epilogue warps have two staging buffers each, which the 32 KB of a pipeline stage make room for.
+  static constexpr int stages(bool res) { return kMaxStages - res; }
+  static constexpr int smem_bytes(bool res) {
+    return stages(res) * kStageBytes + (1 + res) * kStagingBytes + kVecBytes + kListBytes + 256 + 1024;
+  }
 };
 
-template <typename TIn, typename TOut, int BN, bool kGather>
+template <typename TIn, typename TOut, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg<BN>::kThreads, 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const GroupedParams p, int vec) {
   using Cfg = GroupedPairCfg<BN>;
-  constexpr int S = Cfg::kStages;
+  const int S = Cfg::kMaxStages - (p.res ? 1 : 0);
   constexpr int kCols = 128 / (int)sizeof(TOut);  // columns of a 128-byte piece of an output row
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = smem + S * Cfg::kStageBytes;
-  float* vectors = reinterpret_cast<float*>(staging + Cfg::kStagingBytes);
-  int* first = reinterpret_cast<int*>(staging + Cfg::kStagingBytes + Cfg::kVecBytes);
+  float* vectors = reinterpret_cast<float*>(staging + (p.res ? 2 : 1) * Cfg::kStagingBytes);
+  int* first = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(vectors) + Cfg::kVecBytes);
   int* begin = first + B200_MAX_EXPERTS + 1;
-  int* gathered = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(first) + Cfg::kListBytes);  // [128] rows of X of this CTA's half tile
-  uint8_t* bar_mem = reinterpret_cast<uint8_t*>(gathered + BM);
+  uint8_t* bar_mem = reinterpret_cast<uint8_t*>(first) + Cfg::kListBytes;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(bar_mem);  // [S]  waited on by the even CTA only
-  uint64_t* empty_bar = full_bar + S;                          // [S]  per CTA
-  uint64_t* tfull_bar = empty_bar + S;                         // [2]  per CTA
+  uint64_t* empty_bar = full_bar + Cfg::kMaxStages;                          // [S]  per CTA
+  uint64_t* tfull_bar = empty_bar + Cfg::kMaxStages;                         // [2]  per CTA
   uint64_t* tempty_bar = tfull_bar + 2;                        // [2]  even CTA: one arrival per epilogue warp of both CTAs
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -119,7 +118,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           const uint32_t fb_local = smem_u32(&full_bar[s]);
           const uint32_t fb = mapa(fb_local, 0), sa = smem_u32(smem + s * Cfg::kStageBytes);
           if (rank == 0) mbar_expect_tx(fb_local, 2 * Cfg::kStageBytes);
-          if constexpr (!kGather) tma_load_2d_pair(sa, &map_x, kb * Operand<TIn>::k, s0, fb);
+          tma_load_2d_pair(sa, &map_x, kb * Operand<TIn>::k, s0, fb);
           tma_load_2d_pair(sa + BM * 128, &map_w, kb * Operand<TIn>::k, w_row, fb);
           if (++s == S) { s = 0; ph ^= 1; }
         }
@@ -151,191 +150,190 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         if (ok) tcgen05_commit_both(smem_u32(&tfull_bar[acc]));
       }
     }
-  } else if (warp < 4) {
-    // ---------------- gather (both CTAs): half of the CTA's rows of X each ----------------
-    if constexpr (kGather) {
-      int* rows = gathered + (warp - 2) * 64;
-      uint32_t done = 0;  // k-blocks before this tile's
-      bool ok = true;
-      for (int t = pair; t < tiles && ok; t += pairs, done += k_blocks) {
-        walk.at(t, BN, s0, end, n0);
-        s0 += (int)rank * BM + (warp - 2) * 64;
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int slot = s0 + 32 * i + lane, x = slot < end ? rows_of_slot(p, slot).x : 0;
-          rows[32 * i + lane] = x < 0 ? 0 : x;  // whatever lies there: its results are not stored
-        }
-        __syncwarp();
-        if (elect_one()) {
-          int s = (int)(done % S);
-          uint32_t ph = (done / S) & 1;
-          for (int kb = 0; kb < k_blocks; ++kb) {
-            if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 5)) { ok = false; break; }
-            const uint32_t fb = mapa(smem_u32(&full_bar[s]), 0), sa = smem_u32(smem + s * Cfg::kStageBytes) + (warp - 2) * 64 * 128;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) tma_gather4_pair(sa + i * 512, &map_x, kb * Operand<TIn>::k, reinterpret_cast<const int4*>(rows)[i], fb);
-            if (++s == S) { s = 0; ph ^= 1; }
-          }
-        }
-        ok = __all_sync(0xffffffffu, ok);
-      }
-    }
-  } else {
+  } else if (warp >= 4) {
     // ---------------- epilogue ----------------
-    const int quarter = warp & 3, group = (warp - 4) >> 2;
-    uint8_t* mine_bytes = staging + (warp - 4) * 4096;
-    float* vec_b = vectors + (warp - 4) * 128;
-    float* vec_w = vec_b + 64;
-    uint32_t tile_it = 0;
+    // A tile is pieces of 128 bytes of each of the warp's rows: 64 or 32 columns, in slabs of 64 that the two groups take in turn.  The residual
+    // of the piece after this one is copied to the warp's other staging buffer meanwhile (65536x1024x1536 int8, us: 151 with loads at the
+    // start of each piece, AHEAD; 80 without a residual).
+    constexpr int kPieces = BN / 2 / kCols, kPer = 16 / (int)sizeof(TOut);  // entries of 16 bytes
+    const int quarter = warp & 3, group = (warp - 4) >> 2, sub = lane >> 3, part = lane & 7;
     const TOut* res = static_cast<const TOut*>(p.res);
     TOut* C = static_cast<TOut*>(p.C);
-    for (int t = pair; t < tiles; t += pairs, ++tile_it) {
-      const uint32_t acc = tile_it & 1, aph = (tile_it >> 1) & 1;
+    uint8_t* buffers = staging + (warp - 4) * 4096 * (res ? 2 : 1);
+    float* vec_b = vectors + (warp - 4) * 128;
+    float* vec_w = vec_b + 64;
+    const bool scaled = p.weights != nullptr || p.alpha != 1.f;
+    auto offset = [&](int i) { return kCols == 64 ? group * 64 + i * 128 : group * 64 + (i >> 1) * 128 + (i & 1) * 32; };  // of piece i in the tile
+    auto at = [&](uint8_t* buffer, int row, int q) { return buffer + row * 128 + ((q ^ (row & 7)) << 4); };                 // 16 bytes, swizzled
+    auto copy_res = [&](uint8_t* buffer, int c_row, int n) {  // the residual's piece that begins at column n
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const int c = __shfl_sync(0xffffffffu, c_row, it * 4 + sub), col = n + part * kPer;
+        if (c >= 0 && col < p.N) cp_async16(smem_u32(at(buffer, it * 4 + sub, part)), res + c * p.ldres + col, 16);
+      }
+    };
+    float b0 = 0.f, b1 = 0.f, w0 = 1.f, w1 = 1.f;  // bias and scale of columns lane and 32 + lane of the next slab
+    auto fetch_vectors = [&](long long wb, int n) {
+      b0 = p.bias && n + lane < p.N ? __ldg(p.bias + wb + n + lane) : 0.f;
+      b1 = p.bias && n + 32 + lane < p.N ? __ldg(p.bias + wb + n + 32 + lane) : 0.f;
+      if (sizeof(TIn) == 1) {
+        w0 = n + lane < p.N ? __ldg(p.w_scales + wb + n + lane) : 0.f;
+        w1 = n + 32 + lane < p.N ? __ldg(p.w_scales + wb + n + 32 + lane) : 0.f;
+      }
+    };
+    struct Tile {
+      SlotRows r;
+      float sx, weight;
+      int n0;
+      long long wb;
+    };
+    auto tile_of = [&](int t) {
+      Tile x = {{-1, -1, 0}, 1.f, p.alpha, 0, 0};
+      if (t >= tiles) return x;
       walk.at(t, BN, s0, end, n0);
       const int slot = s0 + (int)rank * BM + quarter * 32 + lane;
-      SlotRows r = {-1, -1, 0};
-      if (slot < end) r = rows_of_slot(p, slot);
-      float sx = 1.f, weight = p.alpha;
-      if (r.c >= 0) {
-        if (sizeof(TIn) == 1) sx = p.x_scales[r.x];
-        if (p.weights) weight *= p.weights[r.choice];
+      if (slot < end) x.r = rows_of_slot(p, slot);
+      if (x.r.c >= 0) {
+        if (sizeof(TIn) == 1) x.sx = p.x_scales[x.r.x];
+        if (p.weights) x.weight *= p.weights[x.r.choice];
       }
-      const bool scaled = p.weights != nullptr || p.alpha != 1.f;
-      const bool any = __any_sync(0xffffffffu, r.c >= 0);
-      const long long wb = (long long)walk.e * p.N;
-      float b0, b1, w0 = 1.f, w1 = 1.f;  // bias and scale of columns lane and 32 + lane of a slab, fetched one slab ahead
-      auto fetch = [&](int c0) {
-        const int a = n0 + c0 + lane, b = a + 32;
-        b0 = p.bias && a < p.N ? __ldg(p.bias + wb + a) : 0.f;
-        b1 = p.bias && b < p.N ? __ldg(p.bias + wb + b) : 0.f;
-        if (sizeof(TIn) == 1) {
-          w0 = a < p.N ? __ldg(p.w_scales + wb + a) : 0.f;
-          w1 = b < p.N ? __ldg(p.w_scales + wb + b) : 0.f;
-        }
-      };
-      fetch(group * 64);
+      x.n0 = n0;
+      x.wb = (long long)walk.e * p.N;
+      return x;
+    };
+    uint32_t tile_it = 0;
+    int buf = 0;
+    bool copied = false;  // the residual of the next piece is in, or on its way to, its buffer
+    Tile next = tile_of(pair);
+    for (int t = pair; t < tiles; t += pairs, ++tile_it) {
+      const uint32_t acc = tile_it & 1, aph = (tile_it >> 1) & 1;
+      const Tile x = next;
+      fetch_vectors(x.wb, x.n0 + offset(0));
+      next = tile_of(t + pairs);
+      const bool any = __any_sync(0xffffffffu, x.r.c >= 0), any_next = __any_sync(0xffffffffu, next.r.c >= 0);
+      if (res && vec && any && !copied && x.n0 + offset(0) < p.N) {
+        copy_res(buffers + buf * 4096, x.r.c, x.n0 + offset(0));
+        cp_async_commit();
+      }
+      copied = false;
       if (!mbar_wait(smem_u32(&tfull_bar[acc]), aph, abort_flag, 4)) break;
       tcgen05_fence_after();
       const uint32_t trow = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN;
 #pragma unroll 1
-      for (int c0 = group * 64; c0 < BN && n0 + c0 < p.N && any; c0 += 128) {
-        vec_b[lane] = b0;
-        vec_b[32 + lane] = b1;
-        if (sizeof(TIn) == 1) {
-          vec_w[lane] = w0;
-          vec_w[32 + lane] = w1;
+      for (int i = 0; i < kPieces && any; ++i) {
+        const int n = x.n0 + offset(i), in_slab = kCols == 64 ? 0 : (i & 1) * 32;
+        if (n >= p.N) break;
+        uint8_t* buffer = buffers + buf * 4096;
+        if (in_slab == 0) {
+          vec_b[lane] = b0;
+          vec_b[32 + lane] = b1;
+          if (sizeof(TIn) == 1) {
+            vec_w[lane] = w0;
+            vec_w[32 + lane] = w1;
+          }
+          if (offset(i) + 128 < BN) fetch_vectors(x.wb, n + 128);
         }
-        __syncwarp();
-        if (c0 + 128 < BN) fetch(c0 + 128);
-#pragma unroll 1
-        for (int half = 0; half < 64; half += kCols) {  // pieces of 128 bytes: one of 64 columns, or two of 32
-          const int n = n0 + c0 + half;
-          if (n >= p.N) break;
-          if (res) {
-            if (vec) {
-              uint4 piece[8];
-#pragma unroll
-              for (int it = 0; it < 8; ++it) {
-                const int c = __shfl_sync(0xffffffffu, r.c, it * 4 + (lane >> 3)), col = n + (lane & 7) * (kCols / 8);
-                piece[it] = make_uint4(0u, 0u, 0u, 0u);
-                if (c >= 0 && col < p.N) piece[it] = *reinterpret_cast<const uint4*>(res + c * p.ldres + col);
-              }
-#pragma unroll
-              for (int it = 0; it < 8; ++it) {
-                const int rr = it * 4 + (lane >> 3);
-                *reinterpret_cast<uint4*>(mine_bytes + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4)) = piece[it];
-              }
-            } else {
-#pragma unroll 1
-              for (int rr = 0; rr < 32; ++rr) {
-                const int c = __shfl_sync(0xffffffffu, r.c, rr);
-                for (int j = lane; j < kCols; j += 32)
-                  if (c >= 0 && n + j < p.N)
-                    reinterpret_cast<TOut*>(mine_bytes + rr * 128 + (((j / (kCols / 8)) ^ (rr & 7)) << 4))[j % (kCols / 8)] = res[c * p.ldres + n + j];
-              }
-            }
-            __syncwarp();
-          }
-#pragma unroll
-          for (int q = 0; q < kCols; q += 32) {
-            uint32_t a[32];
-            tmem_ld32(trow + c0 + half + q, a);
-            tmem_ld_wait();
-            float v[32];
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 b = *reinterpret_cast<const float4*>(vec_b + half + q + j);
-              if constexpr (sizeof(TIn) == 1) {
-                const float4 w = *reinterpret_cast<const float4*>(vec_w + half + q + j);
-                v[j] = fmaf((float)(int)a[j], sx * w.x, b.x);
-                v[j + 1] = fmaf((float)(int)a[j + 1], sx * w.y, b.y);
-                v[j + 2] = fmaf((float)(int)a[j + 2], sx * w.z, b.z);
-                v[j + 3] = fmaf((float)(int)a[j + 3], sx * w.w, b.w);
-              } else {
-                v[j] = __uint_as_float(a[j]) + b.x;
-                v[j + 1] = __uint_as_float(a[j + 1]) + b.y;
-                v[j + 2] = __uint_as_float(a[j + 2]) + b.z;
-                v[j + 3] = __uint_as_float(a[j + 3]) + b.w;
-              }
-            }
-            activate32<TOut>(v, p.act);
-            if (scaled) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] *= weight;
-            }
-            constexpr int kPer = 16 / (int)sizeof(TOut);  // entries of a 16-byte piece
-#pragma unroll
-            for (int j = 0; j < 32; j += kPer) {
-              uint4* at = reinterpret_cast<uint4*>(mine_bytes + lane * 128 + ((((q + j) / kPer) ^ (lane & 7)) << 4));
-              uint4 out;
-              uint32_t* o = &out.x;
-              if (res) {
-                const uint4 have = *at;
-                const uint32_t* h = &have.x;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  if constexpr (sizeof(TOut) == 2) {
-                    const float2 f = pair_f<TOut>(h[i]);
-                    v[j + 2 * i] += f.x;
-                    v[j + 2 * i + 1] += f.y;
-                  } else {
-                    v[j + i] += __uint_as_float(h[i]);
-                  }
-                }
-              }
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                if constexpr (sizeof(TOut) == 2) o[i] = two_of<TOut>(v[j + 2 * i], v[j + 2 * i + 1]);
-                else o[i] = __float_as_uint(v[j + i]);
-              }
-              *at = out;
-            }
-          }
-          __syncwarp();
+        if (res) {
           if (vec) {
-#pragma unroll
-            for (int it = 0; it < 8; ++it) {
-              const int rr = it * 4 + (lane >> 3), c = __shfl_sync(0xffffffffu, r.c, rr), col = n + (lane & 7) * (kCols / 8);
-              const uint4 piece = *reinterpret_cast<const uint4*>(mine_bytes + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
-              if (c >= 0 && col < p.N) *reinterpret_cast<uint4*>(C + c * p.ldc + col) = piece;
-            }
+            uint8_t* other = buffers + (buf ^ 1) * 4096;
+            const bool here = i + 1 < kPieces && x.n0 + offset(i + 1) < p.N;
+            if (here) copy_res(other, x.r.c, x.n0 + offset(i + 1));
+            else if (any_next && next.n0 + offset(0) < p.N) copy_res(other, next.r.c, next.n0 + offset(0)), copied = true;
+            cp_async_commit();
+            cp_async_wait<1>();
+            buf ^= 1;
           } else {
 #pragma unroll 1
             for (int rr = 0; rr < 32; ++rr) {
-              const int c = __shfl_sync(0xffffffffu, r.c, rr);
+              const int c = __shfl_sync(0xffffffffu, x.r.c, rr);
               for (int j = lane; j < kCols; j += 32)
-                if (c >= 0 && n + j < p.N)
-                  C[c * p.ldc + n + j] = reinterpret_cast<const TOut*>(mine_bytes + rr * 128 + (((j / (kCols / 8)) ^ (rr & 7)) << 4))[j % (kCols / 8)];
+                if (c >= 0 && n + j < p.N) reinterpret_cast<TOut*>(at(buffer, rr, j / kPer))[j % kPer] = res[c * p.ldres + n + j];
             }
           }
-          __syncwarp();
         }
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < kCols; q += 32) {
+          uint32_t a[32];
+          tmem_ld32(trow + offset(i) + q, a);
+          tmem_ld_wait();
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(vec_b + in_slab + q + j);
+            if constexpr (sizeof(TIn) == 1) {
+              const float4 w = *reinterpret_cast<const float4*>(vec_w + in_slab + q + j);
+              v[j] = fmaf((float)(int)a[j], x.sx * w.x, b.x);
+              v[j + 1] = fmaf((float)(int)a[j + 1], x.sx * w.y, b.y);
+              v[j + 2] = fmaf((float)(int)a[j + 2], x.sx * w.z, b.z);
+              v[j + 3] = fmaf((float)(int)a[j + 3], x.sx * w.w, b.w);
+            } else {
+              v[j] = __uint_as_float(a[j]) + b.x;
+              v[j + 1] = __uint_as_float(a[j + 1]) + b.y;
+              v[j + 2] = __uint_as_float(a[j + 2]) + b.z;
+              v[j + 3] = __uint_as_float(a[j + 3]) + b.w;
+            }
+          }
+          if (n + q + 32 > p.N) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (n + q + j >= p.N) v[j] = 0.f;
+          }
+          activate32<TOut>(v, p.act);
+          if (scaled) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] *= x.weight;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += kPer) {
+            uint4* place = reinterpret_cast<uint4*>(at(buffer, lane, (q + j) / kPer));
+            uint4 out;
+            uint32_t* o = &out.x;
+            if (res) {
+              const uint4 have = *place;
+              const uint32_t* h = &have.x;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if constexpr (sizeof(TOut) == 2) {
+                  const float2 f = pair_f<TOut>(h[k]);
+                  v[j + 2 * k] += f.x;
+                  v[j + 2 * k + 1] += f.y;
+                } else {
+                  v[j + k] += __uint_as_float(h[k]);
+                }
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if constexpr (sizeof(TOut) == 2) o[k] = two_of<TOut>(v[j + 2 * k], v[j + 2 * k + 1]);
+              else o[k] = __float_as_uint(v[j + k]);
+            }
+            *place = out;
+          }
+        }
+        __syncwarp();
+        if (vec) {
+#pragma unroll
+          for (int it = 0; it < 8; ++it) {
+            const int c = __shfl_sync(0xffffffffu, x.r.c, it * 4 + sub), col = n + part * kPer;
+            const uint4 out = *reinterpret_cast<const uint4*>(at(buffer, it * 4 + sub, part));
+            if (c >= 0 && col < p.N) *reinterpret_cast<uint4*>(C + c * p.ldc + col) = out;
+          }
+        } else {
+#pragma unroll 1
+          for (int rr = 0; rr < 32; ++rr) {
+            const int c = __shfl_sync(0xffffffffu, x.r.c, rr);
+            for (int j = lane; j < kCols; j += 32)
+              if (c >= 0 && n + j < p.N) C[c * p.ldc + n + j] = reinterpret_cast<const TOut*>(at(buffer, rr, j / kPer))[j % kPer];
+          }
+        }
+        __syncwarp();
       }
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(mapa(smem_u32(&tempty_bar[acc]), 0));
     }
+    cp_async_wait<0>();
   }
 
   __syncwarp();
@@ -353,29 +351,27 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   }
 }
 
-template <typename TIn, typename TOut, int BN, bool kGather>
+template <typename TIn, typename TOut, int BN>
 cudaError_t launch_tiles(const GroupedParams& p, int sm_count, cudaStream_t s) {
   using Cfg = GroupedPairCfg<BN>;
   CUtensorMap mx, mw;
-  cudaError_t e = tma_encode_rows(p.X, p.ldx, p.x_rows, p.K, kGather ? 1 : BM, Operand<TIn>::prec, &mx);
+  cudaError_t e = tma_encode_rows(p.X, p.ldx, p.slots, p.K, BM, Operand<TIn>::prec, &mx);
   if (e == cudaSuccess) e = tma_encode_rows(p.W, p.ldw, (long long)p.experts * p.N, p.K, BN / 2, Operand<TIn>::prec, &mw);
-  if (e == cudaSuccess) e = raise_smem_limit<grouped_pair_kernel<TIn, TOut, BN, kGather>>(Cfg::kSmemBytes);
+  if (e == cudaSuccess) e = raise_smem_limit<grouped_pair_kernel<TIn, TOut, BN>>(Cfg::smem_bytes(false) > Cfg::smem_bytes(true) ? Cfg::smem_bytes(false) : Cfg::smem_bytes(true));
   if (e != cudaSuccess) return e;
   const int per = 16 / (int)sizeof(TOut);
   const int vec = p.N % per == 0 && p.ldc % per == 0 && aligned16(p.C) && (!p.res || (p.ldres % per == 0 && aligned16(p.res)));
   const long long row_tiles = ((long long)p.slots + 2 * BM - 1) / (2 * BM) + (p.experts < p.slots ? p.experts : p.slots) - 1;
   const long long tiles = row_tiles * ceil_div(p.N, BN);
   const int pairs = (int)(tiles < sm_count / 2 ? tiles : sm_count / 2);
-  return launch_dependent(grouped_pair_kernel<TIn, TOut, BN, kGather>, dim3(2 * pairs), dim3(Cfg::kThreads), Cfg::kSmemBytes, s, mx, mw, p, vec);
+  return launch_dependent(grouped_pair_kernel<TIn, TOut, BN>, dim3(2 * pairs), dim3(Cfg::kThreads), Cfg::smem_bytes(p.res != nullptr), s, mx, mw, p, vec);
 }
 
 }  // namespace
 
 template <typename TIn, typename TOut>
 cudaError_t launch_grouped_pair(const GroupedParams& p, int sm_count, cudaStream_t s) {
-  const bool gather = p.order && !p.x_by_slot;
-  if (p.N <= 128) return gather ? launch_tiles<TIn, TOut, 128, true>(p, sm_count, s) : launch_tiles<TIn, TOut, 128, false>(p, sm_count, s);
-  return gather ? launch_tiles<TIn, TOut, 256, true>(p, sm_count, s) : launch_tiles<TIn, TOut, 256, false>(p, sm_count, s);
+  return p.N <= 128 ? launch_tiles<TIn, TOut, 128>(p, sm_count, s) : launch_tiles<TIn, TOut, 256>(p, sm_count, s);
 }
 #define INSTANCE(TIn, TOut) template cudaError_t launch_grouped_pair<TIn, TOut>(const GroupedParams&, int, cudaStream_t)
 INSTANCE(__half, __half);

@@ -238,20 +238,16 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           if (half * 32 + j < rows) part[(half * 32 + j) * 128 + column] = sum[j];
         continue;
       }
-      float v[32];
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = scaled_sum<TIn>(sum[j], sizeof(TIn) == 1 ? __shfl_sync(0xffffffffu, sx, j) : 1.f, sw, bias);
-      activate32<TOut>(v, p.act);
-      const bool scaled = p.weights != nullptr || p.alpha != 1.f;
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
         if (half * 32 + j >= rows) break;
         const int c = __shfl_sync(0xffffffffu, r.c, j);
         const float w = __shfl_sync(0xffffffffu, weight, j);
-        if (scaled) v[j] *= w;
+        float v = scaled_sum<TIn>(sum[j], sizeof(TIn) == 1 ? __shfl_sync(0xffffffffu, sx, j) : 1.f, sw, bias);
+        v = activate_lane<TOut>(n < p.N ? v : 0.f, p.act) * w;
         if (c >= 0 && n < p.N) {
-          if (p.res) v[j] += to_f(static_cast<const TOut*>(p.res)[c * p.ldres + n]);
-          static_cast<TOut*>(p.C)[c * p.ldc + n] = one_of<TOut>(v[j]);
+          if (p.res) v += to_f(static_cast<const TOut*>(p.res)[c * p.ldres + n]);
+          static_cast<TOut*>(p.C)[c * p.ldc + n] = one_of<TOut>(v);
         }
       }
     }
@@ -286,13 +282,14 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 #pragma unroll
       for (int k = 0; k < 8; ++k) from[k] = k < ks ? ld_cluster(at, k) : 0u;
       const SlotRows r = rows_of_slot(p, s0 + m);
-      if (r.c < 0 || n >= p.N) continue;
+      if (r.c < 0) continue;
       uint32_t sum = from[0];
 #pragma unroll
       for (int k = 1; k < 8; ++k)
         if (k < ks) sum = plus<TIn>(sum, from[k]);
       float v = scaled_sum<TIn>(sum, sizeof(TIn) == 1 ? p.x_scales[r.x] : 1.f, sw, bias);
-      v = activate<sizeof(TOut) == 2>(v, p.act) * (p.weights ? p.alpha * p.weights[r.choice] : p.alpha);
+      v = activate_lane<TOut>(n < p.N ? v : 0.f, p.act) * (p.weights ? p.alpha * p.weights[r.choice] : p.alpha);
+      if (n >= p.N) continue;
       if (p.res) v += to_f(static_cast<const TOut*>(p.res)[r.c * p.ldres + n]);
       static_cast<TOut*>(p.C)[r.c * p.ldc + n] = one_of<TOut>(v);
     }

@@ -62,9 +62,50 @@ template <int kRows> struct TileWalk {
   }
 };
 
+// v e / (e + 1) with e = exp(v), and v n / (n + 2) with n = e (e + 2): four at a time share one reciprocal.  exp is held to exp(10) (Mish) and
+// exp(20), beyond which the quotient is 1 to 2^-27, so that the four denominators' product stays finite.  An epilogue of 65536x1024 columns
+// with a reciprocal each spent 121 us where one without an activation took 80.
+template <bool kMish> __device__ __forceinline__ void gate4(float* v) {
+  float n[4], d[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float e = __expf(fminf(v[i], kMish ? 10.f : 20.f));
+    n[i] = kMish ? e * (e + 2.f) : e;
+    d[i] = n[i] + (kMish ? 2.f : 1.f);
+  }
+  const float d01 = d[0] * d[1], d23 = d[2] * d[3], r = __fdividef(1.f, d01 * d23), r01 = r * d23, r23 = r * d01;
+  v[0] *= n[0] * (r01 * d[1]);  // (a row's columns share it, whose number does not depend on the batch)
+  v[1] *= n[1] * (r01 * d[0]);
+  v[2] *= n[2] * (r23 * d[3]);
+  v[3] *= n[3] * (r23 * d[2]);
+}
+
+// The same with the four columns in neighbouring lanes: the same products, so the same bits.
+template <bool kMish> __device__ __forceinline__ float gate_lane(float v) {
+  const float e = __expf(fminf(v, kMish ? 10.f : 20.f)), n = kMish ? e * (e + 2.f) : e, d = n + (kMish ? 2.f : 1.f);
+  const float other = __shfl_xor_sync(0xffffffffu, d, 1), both = d * other, far = __shfl_xor_sync(0xffffffffu, both, 2);
+  return v * (n * (__fdividef(1.f, both * far) * far * other));
+}
+
+// By all lanes of a warp, four neighbours having columns 4i .. 4i + 3 of one row (0 behind the last column).
+template <typename TOut> __device__ __forceinline__ float activate_lane(float v, int act) {
+  if (sizeof(TOut) == 2 && act == ACT_MISH) return gate_lane<true>(v);
+  if (sizeof(TOut) == 2 && act == ACT_SWISH) return gate_lane<false>(v);
+  return activate<sizeof(TOut) == 2>(v, act);
+}
+
+// 32 columns of a row, the first a multiple of 4 and 0 behind the last column.
 template <typename TOut> __device__ __forceinline__ void activate32(float (&v)[32], int act) {
   if constexpr (sizeof(TOut) == 2) {
-    apply_activation(v, act);
+    if (act == ACT_MISH) {
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) gate4<true>(v + j);
+    } else if (act == ACT_SWISH) {
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) gate4<false>(v + j);
+    } else {
+      apply_activation(v, act);
+    }
   } else if (act != ACT_NONE) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = activate<false>(v[j], act);

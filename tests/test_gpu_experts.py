@@ -433,12 +433,12 @@ def test_an_encoder_layer(lib, n):
                               order=ptr(r.order), offsets=ptr(r.offsets), c_by_slot=1, status=ptr(status))
         down = _lib.ExpertsDesc(X=ptr(mid), W=ptr(w2), bias=ptr(b2), C=ptr(out), M=T, N=C, K=F, activation=oracle.ACT_NONE, precision=1, n_experts=E, top_k=top_k,
                                 group=group, ids=ptr(r.ids), order=ptr(r.order), offsets=ptr(r.offsets), x_by_slot=1, weights=ptr(r.weights), res=ptr(y), status=ptr(status))
-        work = workspace(lib.b200_op_gemm_experts_workspace, down)
+        work = [workspace(lib.b200_op_gemm_experts_workspace, d) for d in (up, down)]
         st.wait_stream(torch.cuda.current_stream())
         for d in (up, down):
             _lib.check(lib.b200_op_gemm_experts(ctypes.byref(d), s))
         torch.cuda.synchronize()
-        assert status.item() == 0 and work is not None
+        assert status.item() == 0 and all((w[-64:] == 255).all() for w in work)
         # step by step in 64 bits, each from the values that the step before it left
         def near(got, want, steps):
             # fp16: half a step of the result, and `steps` of the values on the way
