@@ -4,8 +4,8 @@
 // k-block of 128 bytes each CTA fetches its 128 rows of X and half of the tile's rows of W:
 //   warp 0      TMA producer
 //   warp 1      tcgen05.mma issuer (even CTA), kind::f16 or kind::i8, two accumulators in tensor memory
-//   warps 4-11  epilogue: two groups of four warps, 128 bytes of each of a warp's 32 rows at a time: tensor memory -> scales, bias, activation,
-//               weight, residual -> the warp's own staging buffer -> whole 128-byte pieces of the rows.  Rows behind the expert's last are not
+//   warps 4-19  epilogue: four groups of four warps, 64 bytes of each of a warp's 32 rows at a time: tensor memory -> scales, bias, activation,
+//               weight, residual -> the warp's own staging buffer -> whole 64-byte pieces of the rows.  Rows behind the expert's last are not
 //               stored, which a TMA store of the tile could not leave out.
 // Every wait is bounded by wall-clock time like those of gemm_tc.cu.
 #include "chunk8.cuh"
@@ -34,10 +34,10 @@ template <int kLeft> __device__ __forceinline__ void cp_async_wait() { asm volat
 template <int BN> struct GroupedPairCfg {
   static constexpr int kStageBytes = (BM + BN / 2) * 128;
   static constexpr int kMaxStages = BN == 256 ? 5 : 6;
-  static constexpr int kThreads = 384;
+  static constexpr int kThreads = 640;
   static constexpr int kTmemCols = 2 * BN;
-  static constexpr int kStagingBytes = 8 * 32 * 128;
-  static constexpr int kVecBytes = 8 * 128 * 4;                    // per epilogue warp: bias and scale of 64 columns
+  static constexpr int kStagingBytes = 16 * 32 * 64;  // per epilogue warp: 64 bytes of its 32 rows
+  static constexpr int kVecBytes = 16 * 128 * 4;      // ... and bias and scale of up to 64 columns
   static constexpr int kListBytes = (2 * (B200_MAX_EXPERTS + 1) * 4 + 15) / 16 * 16;  // first tile and first slot of each expert
   // With a residual the epilogue warps have two staging buffers each, which the 32 KB of a pipeline stage make room for.
   static constexpr int stages(bool res) { return kMaxStages - res; }
@@ -51,7 +51,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg<BN>::
 grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const GroupedParams p, int vec) {
   using Cfg = GroupedPairCfg<BN>;
   const int S = Cfg::kMaxStages - (p.res ? 1 : 0);
-  constexpr int kCols = 128 / (int)sizeof(TOut);  // columns of a 128-byte piece of an output row
+  constexpr int kCols = 64 / (int)sizeof(TOut);  // columns of a 64-byte piece of an output row
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = smem + S * Cfg::kStageBytes;
@@ -83,7 +83,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&tfull_bar[i]), 1);
-      mbar_init(smem_u32(&tempty_bar[i]), 16);
+      mbar_init(smem_u32(&tempty_bar[i]), 32);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -152,39 +152,39 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     }
   } else if (warp >= 4) {
     // ---------------- epilogue ----------------
-    // A tile is pieces of 128 bytes of each of the warp's rows: 64 or 32 columns, in slabs of 64 that the two groups take in turn.  The residual
-    // of the piece after this one is copied to the warp's other staging buffer meanwhile (65536x1024x1536 int8, us: 151 with loads at the
-    // start of each piece, AHEAD; 80 without a residual).
-    constexpr int kPieces = BN / 2 / kCols, kPer = 16 / (int)sizeof(TOut);  // entries of 16 bytes
-    const int quarter = warp & 3, group = (warp - 4) >> 2, sub = lane >> 3, part = lane & 7;
+    // Four groups of four warps, a quarter of the columns each, in pieces of 64 bytes of each of the warp's rows.  The residual of the piece
+    // after this one is copied to the warp's other staging buffer meanwhile (65536x1024x1536 int8, us: 151 with loads at the start of each
+    // piece, 97 ahead of it; 80 without a residual).  EIGHT
+    constexpr int kSlab = BN / 4, kPieces = kSlab / kCols, kPer = 16 / (int)sizeof(TOut);  // kPer: entries of 16 bytes
+    const int quarter = warp & 3, group = (warp - 4) >> 2, sub = lane >> 2, part = lane & 3;
     const TOut* res = static_cast<const TOut*>(p.res);
     TOut* C = static_cast<TOut*>(p.C);
-    uint8_t* buffers = staging + (warp - 4) * 4096 * (res ? 2 : 1);
+    uint8_t* buffers = staging + (warp - 4) * 2048 * (res ? 2 : 1);
     float* vec_b = vectors + (warp - 4) * 128;
     float* vec_w = vec_b + 64;
     const bool scaled = p.weights != nullptr || p.alpha != 1.f;
-    auto offset = [&](int i) { return kCols == 64 ? group * 64 + i * 128 : group * 64 + (i >> 1) * 128 + (i & 1) * 32; };  // of piece i in the tile
-    auto at = [&](uint8_t* buffer, int row, int q) { return buffer + row * 128 + ((q ^ (row & 7)) << 4); };                 // 16 bytes, swizzled
+    auto at = [&](uint8_t* buffer, int row, int q) { return buffer + row * 64 + ((q ^ ((row >> 1) & 3)) << 4); };  // 16 bytes, swizzled
     auto copy_res = [&](uint8_t* buffer, int c_row, int n) {  // the residual's piece that begins at column n
 #pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const int c = __shfl_sync(0xffffffffu, c_row, it * 4 + sub), col = n + part * kPer;
-        if (c >= 0 && col < p.N) cp_async16(smem_u32(at(buffer, it * 4 + sub, part)), res + c * p.ldres + col, 16);
+      for (int it = 0; it < 4; ++it) {
+        const int c = __shfl_sync(0xffffffffu, c_row, it * 8 + sub), col = n + part * kPer;
+        if (c >= 0 && col < p.N) cp_async16(smem_u32(at(buffer, it * 8 + sub, part)), res + c * p.ldres + col, 16);
       }
     };
-    float b0 = 0.f, b1 = 0.f, w0 = 1.f, w1 = 1.f;  // bias and scale of columns lane and 32 + lane of the next slab
+    float b0 = 0.f, b1 = 0.f, w0 = 1.f, w1 = 1.f;  // bias and scale of columns lane and 32 + lane of the next tile's slab
     auto fetch_vectors = [&](long long wb, int n) {
-      b0 = p.bias && n + lane < p.N ? __ldg(p.bias + wb + n + lane) : 0.f;
-      b1 = p.bias && n + 32 + lane < p.N ? __ldg(p.bias + wb + n + 32 + lane) : 0.f;
+      const bool first = n + lane < p.N, second = kSlab > 32 && n + 32 + lane < p.N;
+      b0 = p.bias && first ? __ldg(p.bias + wb + n + lane) : 0.f;
+      b1 = p.bias && second ? __ldg(p.bias + wb + n + 32 + lane) : 0.f;
       if (sizeof(TIn) == 1) {
-        w0 = n + lane < p.N ? __ldg(p.w_scales + wb + n + lane) : 0.f;
-        w1 = n + 32 + lane < p.N ? __ldg(p.w_scales + wb + n + 32 + lane) : 0.f;
+        w0 = first ? __ldg(p.w_scales + wb + n + lane) : 0.f;
+        w1 = second ? __ldg(p.w_scales + wb + n + 32 + lane) : 0.f;
       }
     };
     struct Tile {
       SlotRows r;
       float sx, weight;
-      int n0;
+      int n;  // the first column of the group's slab
       long long wb;
     };
     auto tile_of = [&](int t) {
@@ -197,7 +197,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         if (sizeof(TIn) == 1) x.sx = p.x_scales[x.r.x];
         if (p.weights) x.weight *= p.weights[x.r.choice];
       }
-      x.n0 = n0;
+      x.n = n0 + group * kSlab;
       x.wb = (long long)walk.e * p.N;
       return x;
     };
@@ -205,40 +205,39 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     int buf = 0;
     bool copied = false;  // the residual of the next piece is in, or on its way to, its buffer
     Tile next = tile_of(pair);
+    fetch_vectors(next.wb, next.n);
     for (int t = pair; t < tiles; t += pairs, ++tile_it) {
       const uint32_t acc = tile_it & 1, aph = (tile_it >> 1) & 1;
       const Tile x = next;
-      fetch_vectors(x.wb, x.n0 + offset(0));
+      const bool any = __any_sync(0xffffffffu, x.r.c >= 0) && x.n < p.N;
+      vec_b[lane] = b0;
+      vec_b[32 + lane] = b1;
+      if (sizeof(TIn) == 1) {
+        vec_w[lane] = w0;
+        vec_w[32 + lane] = w1;
+      }
       next = tile_of(t + pairs);
-      const bool any = __any_sync(0xffffffffu, x.r.c >= 0), any_next = __any_sync(0xffffffffu, next.r.c >= 0);
-      if (res && vec && any && !copied && x.n0 + offset(0) < p.N) {
-        copy_res(buffers + buf * 4096, x.r.c, x.n0 + offset(0));
+      fetch_vectors(next.wb, next.n);
+      const bool any_next = __any_sync(0xffffffffu, next.r.c >= 0) && next.n < p.N;
+      if (res && vec && any && !copied) {
+        copy_res(buffers + buf * 2048, x.r.c, x.n);
         cp_async_commit();
       }
       copied = false;
       if (!mbar_wait(smem_u32(&tfull_bar[acc]), aph, abort_flag, 4)) break;
       tcgen05_fence_after();
-      const uint32_t trow = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN;
+      const uint32_t trow = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN + group * kSlab;
 #pragma unroll 1
       for (int i = 0; i < kPieces && any; ++i) {
-        const int n = x.n0 + offset(i), in_slab = kCols == 64 ? 0 : (i & 1) * 32;
+        const int n = x.n + i * kCols;
         if (n >= p.N) break;
-        uint8_t* buffer = buffers + buf * 4096;
-        if (in_slab == 0) {
-          vec_b[lane] = b0;
-          vec_b[32 + lane] = b1;
-          if (sizeof(TIn) == 1) {
-            vec_w[lane] = w0;
-            vec_w[32 + lane] = w1;
-          }
-          if (offset(i) + 128 < BN) fetch_vectors(x.wb, n + 128);
-        }
+        uint8_t* buffer = buffers + buf * 2048;
         if (res) {
           if (vec) {
-            uint8_t* other = buffers + (buf ^ 1) * 4096;
-            const bool here = i + 1 < kPieces && x.n0 + offset(i + 1) < p.N;
-            if (here) copy_res(other, x.r.c, x.n0 + offset(i + 1));
-            else if (any_next && next.n0 + offset(0) < p.N) copy_res(other, next.r.c, next.n0 + offset(0)), copied = true;
+            uint8_t* other = buffers + (buf ^ 1) * 2048;
+            const bool here = i + 1 < kPieces && n + kCols < p.N;
+            if (here) copy_res(other, x.r.c, n + kCols);
+            else if (any_next) copy_res(other, next.r.c, next.n), copied = true;
             cp_async_commit();
             cp_async_wait<1>();
             buf ^= 1;
@@ -246,23 +245,22 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 #pragma unroll 1
             for (int rr = 0; rr < 32; ++rr) {
               const int c = __shfl_sync(0xffffffffu, x.r.c, rr);
-              for (int j = lane; j < kCols; j += 32)
-                if (c >= 0 && n + j < p.N) reinterpret_cast<TOut*>(at(buffer, rr, j / kPer))[j % kPer] = res[c * p.ldres + n + j];
+              if (c >= 0 && lane < kCols && n + lane < p.N) reinterpret_cast<TOut*>(at(buffer, rr, lane / kPer))[lane % kPer] = res[c * p.ldres + n + lane];
             }
           }
         }
         __syncwarp();
 #pragma unroll
-        for (int q = 0; q < kCols; q += 32) {
-          uint32_t a[32];
-          tmem_ld32(trow + offset(i) + q, a);
+        for (int q = 0; q < kCols; q += 16) {
+          uint32_t a[16];
+          tmem_ld16(trow + i * kCols + q, a);
           tmem_ld_wait();
-          float v[32];
+          float v[16];
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 b = *reinterpret_cast<const float4*>(vec_b + in_slab + q + j);
+          for (int j = 0; j < 16; j += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(vec_b + i * kCols + q + j);
             if constexpr (sizeof(TIn) == 1) {
-              const float4 w = *reinterpret_cast<const float4*>(vec_w + in_slab + q + j);
+              const float4 w = *reinterpret_cast<const float4*>(vec_w + i * kCols + q + j);
               v[j] = fmaf((float)(int)a[j], x.sx * w.x, b.x);
               v[j + 1] = fmaf((float)(int)a[j + 1], x.sx * w.y, b.y);
               v[j + 2] = fmaf((float)(int)a[j + 2], x.sx * w.z, b.z);
@@ -274,18 +272,18 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
               v[j + 3] = __uint_as_float(a[j + 3]) + b.w;
             }
           }
-          if (n + q + 32 > p.N) {
+          if (n + q + 16 > p.N) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
+            for (int j = 0; j < 16; ++j)
               if (n + q + j >= p.N) v[j] = 0.f;
           }
-          activate32<TOut>(v, p.act);
+          activate_columns<TOut>(v, p.act);
           if (scaled) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= x.weight;
+            for (int j = 0; j < 16; ++j) v[j] *= x.weight;
           }
 #pragma unroll
-          for (int j = 0; j < 32; j += kPer) {
+          for (int j = 0; j < 16; j += kPer) {
             uint4* place = reinterpret_cast<uint4*>(at(buffer, lane, (q + j) / kPer));
             uint4 out;
             uint32_t* o = &out.x;
@@ -314,17 +312,16 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         __syncwarp();
         if (vec) {
 #pragma unroll
-          for (int it = 0; it < 8; ++it) {
-            const int c = __shfl_sync(0xffffffffu, x.r.c, it * 4 + sub), col = n + part * kPer;
-            const uint4 out = *reinterpret_cast<const uint4*>(at(buffer, it * 4 + sub, part));
+          for (int it = 0; it < 4; ++it) {
+            const int c = __shfl_sync(0xffffffffu, x.r.c, it * 8 + sub), col = n + part * kPer;
+            const uint4 out = *reinterpret_cast<const uint4*>(at(buffer, it * 8 + sub, part));
             if (c >= 0 && col < p.N) *reinterpret_cast<uint4*>(C + c * p.ldc + col) = out;
           }
         } else {
 #pragma unroll 1
           for (int rr = 0; rr < 32; ++rr) {
             const int c = __shfl_sync(0xffffffffu, x.r.c, rr);
-            for (int j = lane; j < kCols; j += 32)
-              if (c >= 0 && n + j < p.N) C[c * p.ldc + n + j] = reinterpret_cast<const TOut*>(at(buffer, rr, j / kPer))[j % kPer];
+            if (c >= 0 && lane < kCols && n + lane < p.N) C[c * p.ldc + n + lane] = reinterpret_cast<const TOut*>(at(buffer, rr, lane / kPer))[lane % kPer];
           }
         }
         __syncwarp();

@@ -94,21 +94,21 @@ template <typename TOut> __device__ __forceinline__ float activate_lane(float v,
   return activate<sizeof(TOut) == 2>(v, act);
 }
 
-// 32 columns of a row, the first a multiple of 4 and 0 behind the last column.
-template <typename TOut> __device__ __forceinline__ void activate32(float (&v)[32], int act) {
+// Columns of a row, the first a multiple of 4 and 0 behind the last column.
+template <typename TOut, int kN> __device__ __forceinline__ void activate_columns(float (&v)[kN], int act) {
   if constexpr (sizeof(TOut) == 2) {
     if (act == ACT_MISH) {
 #pragma unroll
-      for (int j = 0; j < 32; j += 4) gate4<true>(v + j);
+      for (int j = 0; j < kN; j += 4) gate4<true>(v + j);
     } else if (act == ACT_SWISH) {
 #pragma unroll
-      for (int j = 0; j < 32; j += 4) gate4<false>(v + j);
+      for (int j = 0; j < kN; j += 4) gate4<false>(v + j);
     } else {
       apply_activation(v, act);
     }
   } else if (act != ACT_NONE) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = activate<false>(v[j], act);
+    for (int j = 0; j < kN; ++j) v[j] = activate<false>(v[j], act);
   }
 }
 
