@@ -184,6 +184,8 @@ __global__ void __launch_bounds__(256) spread_rows_kernel(const GroupedParams p,
 bool tma_rows(int K, long long ldx, long long ldw, int size) { return K * (long long)size % 16 == 0 && ldx * size % 16 == 0 && ldw * size % 16 == 0; }
 // The pair kernel's 256 slots pay from half a tile per expert on.
 bool many_rows(int slots, int experts) { return slots / (experts < slots ? experts : slots) > 64; }
+// Beyond 16 rows per expert the other kernel, too, is ahead with rows in order, although the copy is a launch more.
+bool spreads(int slots, int experts) { return slots / (experts < slots ? experts : slots) > 16; }
 
 template <typename TIn, typename TOut>
 int run_grouped(GroupedParams p, bool exact_sums, void* spread, cudaStream_t s) {
@@ -195,18 +197,17 @@ int run_grouped(GroupedParams p, bool exact_sums, void* spread, cudaStream_t s) 
   B200_CUDA(gemm_tc_init());
   B200_CUDA(cudaGetDevice(&dev));
   B200_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  if (exact_sums || !many_rows(p.slots, p.experts)) {
-    B200_CUDA((launch_grouped_rows<TIn, TOut>(p, exact_sums, sms, s)));
-    return B200_OK;
-  }
-  if (p.order && !p.x_by_slot) {
+  const bool pairs = !exact_sums && many_rows(p.slots, p.experts), in_place = !p.order || p.x_by_slot || (!pairs && !spreads(p.slots, p.experts));
+  if (!in_place) {
     const long long blocks = ((long long)p.slots + 7) / 8;
     B200_CUDA(launch_dependent(spread_rows_kernel, dim3((unsigned)(blocks < sms * 8 ? blocks : sms * 8)), dim3(256), 0, s, p, static_cast<uint8_t*>(spread),
                                p.K * (int)sizeof(TIn), (int)sizeof(TIn)));
     p.X = spread;
     p.ldx = p.K;
   }
-  B200_CUDA((launch_grouped_pair<TIn, TOut>(p, sms, s)));
+  const bool in_order = !p.order || p.x_by_slot || !in_place;
+  if (pairs) B200_CUDA((launch_grouped_pair<TIn, TOut>(p, sms, s)));
+  else B200_CUDA((launch_grouped_rows<TIn, TOut>(p, in_order, exact_sums, sms, s)));
   return B200_OK;
 }
 
@@ -220,7 +221,7 @@ size_t sums_bytes(const b200_experts_desc& d) { return sums_choices(d) ? round25
 // X in the order of the slots.
 size_t spread_bytes(const b200_experts_desc& d) {
   const int size = d.int8 ? 1 : 2;
-  const bool spread = !d.x_by_slot && !(d.out_f32 && !d.int8) && d.M > 0 && many_rows(d.M * d.top_k, d.n_experts) &&
+  const bool spread = !d.x_by_slot && d.M > 0 && spreads(d.M * d.top_k, d.n_experts) &&
                       tma_rows(d.K, d.ldx ? d.ldx : d.K, d.ldw ? d.ldw : d.K, size);
   return spread ? round256((size_t)d.M * d.top_k * d.K * size) : 0;
 }

@@ -51,7 +51,7 @@ __device__ __forceinline__ int expert_begin(const GroupedParams& p, int e) {
 // Many rows (grouped_pair.cu): operands that TMA can read, X [slots][K] in the order of the slots.
 template <typename TIn, typename TOut> cudaError_t launch_grouped_pair(const GroupedParams& p, int sm_count, cudaStream_t s);
 
-// Few rows per expert (grouped_rows.cu): operands that TMA can read.  rounded: fp32 results of 16-bit operands as exact as a plain fp32 product.
-template <typename TIn, typename TOut> cudaError_t launch_grouped_rows(const GroupedParams& p, bool rounded, int sm_count, cudaStream_t s);
+// Few rows per expert (grouped_rows.cu): operands that TMA can read.  in_order: X is [slots][K] in the order of the slots.  rounded: fp32 results of 16-bit operands as exact as a plain fp32 product.
+template <typename TIn, typename TOut> cudaError_t launch_grouped_rows(const GroupedParams& p, bool in_order, bool rounded, int sm_count, cudaStream_t s);
 
 }  // namespace b200

@@ -224,7 +224,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         cp_async_commit();
       }
       copied = false;
-      if (!mbar_wait(smem_u32(&tfull_bar[acc]), aph, abort_flag, 4)) break;
+      if (!mbar_wait_warp(smem_u32(&tfull_bar[acc]), aph, abort_flag, 4)) break;
       tcgen05_fence_after();
       const uint32_t trow = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN + group * kSlab;
 #pragma unroll 1

@@ -8,11 +8,13 @@
 //   warp 1      tcgen05.mma issuer, kind::f16 or kind::i8
 //   warp 2      gather4 of X's rows that the order names
 //   warps 4-11  epilogue: four warps per half of the slots
-// With fewer tiles than SMs the k-blocks of a tile are cut over the CTAs of a cluster (`ks`), which add their sums from one another's
-// shared memory, in the order of their ranks, each a part of the slots.
+// With fewer tiles than SMs the k-blocks of a tile are cut over the CTAs of a cluster (`ks`), which send their sums of each CTA's part of the slots
+// to its shared memory, where they are added in the order of the ranks.
 // The tensor core truncates its sums, the more the longer they are; results of 16 bits hide it.  For fp32 results of 16-bit operands (kRounded)
 // the accumulators leave tensor memory after every k-block and are added in registers, rounded to nearest.
 // Every wait is bounded by wall-clock time like those of gemm_tc.cu; the cluster barriers are reached by all threads whatever happened before.
+#include <type_traits>
+
 #include "grouped_tc.cuh"
 
 namespace b200 {
@@ -22,9 +24,13 @@ constexpr int kRows = 64;  // slots of a tile
 constexpr int kStageBytes = (BM + kRows) * 128;
 constexpr int kMaxStages = 8;
 constexpr int kThreads = 384;
-constexpr int kTmemCols = 2 * kRows;
+constexpr int kAccs = 4;  // accumulators
+constexpr int kTmemCols = kAccs * kRows;
 constexpr int kListBytes = (2 * (B200_MAX_EXPERTS + 1) * 4 + 15) / 16 * 16;
-constexpr int smem_bytes(int stages) { return stages * kStageBytes + kListBytes + kRows * 4 + 256 + 1024; }
+// ks > 1: 32 KB for the sums that the CTAs of the cluster send to one another
+constexpr int kMaxSplitStages = 6;
+constexpr int kPartBytes = 8 * 128 * 8 * 4;
+constexpr int smem_bytes(int stages, bool split) { return stages * kStageBytes + (split ? kPartBytes : 0) + kListBytes + kRows * 4 + 256 + 1024; }
 
 template <typename T>
 __device__ __forceinline__ void mma_one(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -44,11 +50,11 @@ __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row.x), "r"(row.y), "r"(row.z), "r"(row.w), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr, uint32_t rank) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(mapa(addr, rank)) : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster4(uint32_t addr, uint32_t rank, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mapa(addr, rank)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// Slots that each CTA of a cluster finishes: whole fours.
+__device__ __forceinline__ int slots_each(int rows, int log_ks) { return (((rows + (1 << log_ks) - 1) >> log_ks) + 3) & ~3; }
 
 // A sum in tensor memory's type with its scales and bias.
 template <typename TIn> __device__ __forceinline__ float scaled_sum(uint32_t sum, float sx, float sw, float bias) {
@@ -60,25 +66,27 @@ template <typename TIn> __device__ __forceinline__ uint32_t plus(uint32_t a, uin
 
 template <typename TIn, typename TOut, bool kGather, bool kRounded>
 __global__ void __launch_bounds__(kThreads, 1)
-grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const GroupedParams p, int stages, int ks) {
+grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const GroupedParams p, int stages, int log_ks) {
+  const int ks = 1 << log_ks;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  int* first = reinterpret_cast<int*>(smem + stages * kStageBytes);
+  uint32_t* part = reinterpret_cast<uint32_t*>(smem + stages * kStageBytes);  // ks > 1: [ks][slots_each / 4][128][4] sums of this CTA's slots from each CTA
+  int* first = reinterpret_cast<int*>(smem + stages * kStageBytes + (ks > 1 ? kPartBytes : 0));
   int* begin = first + B200_MAX_EXPERTS + 1;
   int* gathered = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(first) + kListBytes);  // [64] rows of X
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(gathered + kRows);  // [stages]
   uint64_t* empty_bar = full_bar + kMaxStages;                          // [stages]
-  uint64_t* tfull_bar = empty_bar + kMaxStages;                         // [2]
-  uint64_t* tempty_bar = tfull_bar + 2;                                 // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
+  uint64_t* tfull_bar = empty_bar + kMaxStages;                         // [kAccs]
+  uint64_t* tempty_bar = tfull_bar + kAccs;                             // [kAccs]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + kAccs);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* scan = reinterpret_cast<int*>(tmem_slot + 2);  // [8]
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const uint32_t rank = ks > 1 ? cluster_ctarank() : 0;
-  const int unit = blockIdx.x / ks, units = gridDim.x / ks;
+  const int unit = blockIdx.x >> log_ks, units = gridDim.x >> log_ks;
   const int n_tiles = (p.N + BM - 1) / BM, k_blocks = (p.K + Operand<TIn>::k - 1) / Operand<TIn>::k;
-  const int kb0 = k_blocks * (int)rank / ks, kb1 = k_blocks * ((int)rank + 1) / ks;
+  const int kb0 = k_blocks * (int)rank >> log_ks, kb1 = k_blocks * ((int)rank + 1) >> log_ks;
 
   if (threadIdx.x == 64) {
     tma_prefetch_map(&map_x);
@@ -89,7 +97,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       mbar_init(smem_u32(&full_bar[i]), 1);
       mbar_init(smem_u32(&empty_bar[i]), 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kAccs; ++i) {
       mbar_init(smem_u32(&tfull_bar[i]), 1);
       mbar_init(smem_u32(&tempty_bar[i]), 8);
     }
@@ -100,6 +108,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)kTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (ks > 1) cluster_arrive();  // waited for ahead of the first store to another CTA: that it runs
   grid_dependency_wait();
   tcgen05_fence_before();
   list_tiles<kRows>(p, first, begin, scan);
@@ -141,9 +150,9 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         uint32_t d = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (kRounded || kb == kb0) {
-            if (!mbar_wait(smem_u32(&tempty_bar[it & 1]), ((it >> 1) & 1) ^ 1, abort_flag, 2)) { ok = false; break; }
+            if (!mbar_wait(smem_u32(&tempty_bar[it % kAccs]), ((it / kAccs) & 1) ^ 1, abort_flag, 2)) { ok = false; break; }
             tcgen05_fence_after();
-            d = tmem_base + (it & 1) * kRows;
+            d = tmem_base + (it % kAccs) * kRows;
           }
           if (!mbar_wait(smem_u32(&full_bar[s]), ph, abort_flag, 3)) { ok = false; break; }
           tcgen05_fence_after();
@@ -153,7 +162,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
           for (int k = 0; k < 4; ++k) mma_one<TIn>(d, adesc + 2 * k, bdesc + 2 * k, idesc, ((!kRounded && kb > kb0) || k > 0) ? 1u : 0u);
           tcgen05_commit(smem_u32(&empty_bar[s]));
           if (kRounded || kb + 1 == kb1) {
-            tcgen05_commit(smem_u32(&tfull_bar[it & 1]));
+            tcgen05_commit(smem_u32(&tfull_bar[it % kAccs]));
             ++it;
           }
           if (++s == stages) { s = 0; ph ^= 1; }
@@ -192,63 +201,91 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   }
   // ---------------- epilogue ----------------
   const int quarter = warp & 3, half = warp >= 8 ? 1 : 0, column = quarter * 32 + lane;
-  uint32_t* part = reinterpret_cast<uint32_t*>(smem);  // [64][128] sums of this CTA, once its stages are used up (ks > 1: one tile)
-  int rows = 0;
+  const TOut* res = static_cast<const TOut*>(p.res);
+  TOut* C = static_cast<TOut*>(p.C);
+  const bool scaled = p.weights != nullptr || p.alpha != 1.f;
+  int rows = 0, n = 0;
+  bool met = false;  // this thread has waited for the cluster's start
+  float bias = 0.f, sw = 1.f, sx = 1.f, weight = p.alpha;  // of this thread's column, of the warp's slot `lane`
+  SlotRows r = {-1, -1, 0};
+  // Scales, activation and residual of kN slots of this warp's, the first `j0`, and their rows written; by all lanes.
+  auto finish = [&](auto sum_of, int j0, int count, auto kN) {
+    float v[kN.value], x[kN.value];
+    int c[kN.value];
+#pragma unroll
+    for (int j = 0; j < kN.value; ++j) {
+      c[j] = __shfl_sync(0xffffffffu, r.c, j0 + j);
+      v[j] = scaled_sum<TIn>(sum_of(j), sizeof(TIn) == 1 ? __shfl_sync(0xffffffffu, sx, j0 + j) : 1.f, sw, bias);
+      if (n >= p.N) v[j] = 0.f;
+      x[j] = res && j < count && c[j] >= 0 && n < p.N ? to_f(res[c[j] * p.ldres + n]) : 0.f;
+    }
+    activate_lanes<TOut>(v, p.act);
+#pragma unroll
+    for (int j = 0; j < kN.value; ++j) {
+      if (scaled) v[j] *= __shfl_sync(0xffffffffu, weight, j0 + j);
+      if (j < count && c[j] >= 0 && n < p.N) C[c[j] * p.ldc + n] = one_of<TOut>(res ? v[j] + x[j] : v[j]);
+    }
+  };
   if (warp >= 4) {
     uint32_t it = 0;
     for (int t = unit; t < tiles; t += units) {
       walk.at(t, BM, s0, end, n0);
       rows = min(kRows, end - s0);
-      const int n = n0 + column, slot = s0 + half * 32 + lane;
-      const bool mine = half * 32 < rows;  // the same in the whole warp
-      float bias = 0.f, sw = 1.f, sx = 1.f, weight = p.alpha;
-      SlotRows r = {-1, -1, 0};
-      if (ks == 1) {
-        if (n < p.N) {
-          if (p.bias) bias = __ldg(p.bias + (long long)walk.e * p.N + n);
-          if (sizeof(TIn) == 1) sw = __ldg(p.w_scales + (long long)walk.e * p.N + n);
-        }
-        if (slot < end) r = rows_of_slot(p, slot);
-        if (r.c >= 0) {
-          if (sizeof(TIn) == 1) sx = p.x_scales[r.x];
-          if (p.weights) weight *= p.weights[r.choice];
-        }
+      n = n0 + column;
+      // ks > 1: the slots that this CTA finishes; else all 64
+      const int slot = s0 + (ks > 1 ? (int)rank * slots_each(rows, log_ks) + lane : half * 32 + lane);
+      bias = n < p.N && p.bias ? __ldg(p.bias + (long long)walk.e * p.N + n) : 0.f;
+      if (sizeof(TIn) == 1) sw = n < p.N ? __ldg(p.w_scales + (long long)walk.e * p.N + n) : 0.f;
+      r = {-1, -1, 0};
+      sx = 1.f;
+      weight = p.alpha;
+      if (slot < end) r = rows_of_slot(p, slot);
+      if (r.c >= 0) {
+        if (sizeof(TIn) == 1) sx = p.x_scales[r.x];
+        if (p.weights) weight *= p.weights[r.choice];
       }
+      const bool mine = half * 32 < rows;  // the same in the whole warp
       uint32_t sum[32];
       bool ok = true;
       for (int kb = kb0; kb < kb1; kb = kRounded ? kb + 1 : kb1, ++it) {
-        if (!mbar_wait(smem_u32(&tfull_bar[it & 1]), (it >> 1) & 1, abort_flag, 4)) { ok = false; break; }
+        ok = mbar_wait_warp(smem_u32(&tfull_bar[it % kAccs]), (it / kAccs) & 1, abort_flag, 4);
+        if (!ok) break;
         tcgen05_fence_after();
         if (mine) {
           uint32_t a[32];
-          tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (it & 1) * kRows + half * 32, a);
+          tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (it % kAccs) * kRows + half * 32, a);
           tmem_ld_wait();
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[it % kAccs]));
 #pragma unroll
           for (int j = 0; j < 32; ++j) sum[j] = kRounded && kb > kb0 ? plus<TIn>(sum[j], a[j]) : a[j];
+        } else if (lane == 0) {
+          mbar_arrive(smem_u32(&tempty_bar[it % kAccs]));
         }
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[it & 1]));
       }
       if (!ok) break;
-      if (!mine) continue;
-      if (ks > 1) {
+      if (ks > 1) {  // (one tile)
+        cluster_wait();
+        met = true;
+        const int each = slots_each(rows, log_ks);
+        int k = 0, k0 = 0;  // the CTA whose slots they are, its first
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (half * 32 + j < rows) part[(half * 32 + j) * 128 + column] = sum[j];
-        continue;
-      }
-#pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        if (half * 32 + j >= rows) break;
-        const int c = __shfl_sync(0xffffffffu, r.c, j);
-        const float w = __shfl_sync(0xffffffffu, weight, j);
-        float v = scaled_sum<TIn>(sum[j], sizeof(TIn) == 1 ? __shfl_sync(0xffffffffu, sx, j) : 1.f, sw, bias);
-        v = activate_lane<TOut>(n < p.N ? v : 0.f, p.act) * w;
-        if (c >= 0 && n < p.N) {
-          if (p.res) v += to_f(static_cast<const TOut*>(p.res)[c * p.ldres + n]);
-          static_cast<TOut*>(p.C)[c * p.ldc + n] = one_of<TOut>(v);
+        for (int j = 0; j < 32; j += 4) {
+          const int m = half * 32 + j;
+          if (m >= rows) break;
+          for (; m >= k0 + each; ++k) k0 += each;
+          st_cluster4(smem_u32(part + (((int)rank * each + m - k0) * 128 + column * 4)), k, sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
         }
+        break;
+      }
+      if (!mine) continue;
+      const int count = min(rows - half * 32, 32);
+#pragma unroll 1
+      for (int j0 = 0; j0 < count; j0 += 8) {  // one copy of the code, whose fetching took longer than its running
+        finish([&](int j) { return sum[j]; }, j0, count - j0, std::integral_constant<int, 8>());
+#pragma unroll
+        for (int j = 0; j < 24; ++j) sum[j] = sum[j + 8];
       }
     }
   }
@@ -266,58 +303,44 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)kTmemCols) : "memory");
   }
   if (ks == 1) return;
-  cluster_sync_all();  // the sums of all CTAs are in their shared memory
+  if (!met) cluster_wait();
+  cluster_sync_all();  // all sums have arrived
   if (warp >= 4 && unit < tiles) {
-    const int n = n0 + column;
-    float bias = 0.f, sw = 1.f;
-    if (n < p.N) {
-      if (p.bias) bias = __ldg(p.bias + (long long)walk.e * p.N + n);
-      if (sizeof(TIn) == 1) sw = __ldg(p.w_scales + (long long)walk.e * p.N + n);
-    }
-    const int m0 = rows * (int)rank / ks, m1 = rows * ((int)rank + 1) / ks;
-#pragma unroll 2
-    for (int m = m0 + half; m < m1; m += 2) {
-      const uint32_t at = smem_u32(part + m * 128 + column);
-      uint32_t from[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) from[k] = k < ks ? ld_cluster(at, k) : 0u;
-      const SlotRows r = rows_of_slot(p, s0 + m);
-      if (r.c < 0) continue;
-      uint32_t sum = from[0];
-#pragma unroll
-      for (int k = 1; k < 8; ++k)
-        if (k < ks) sum = plus<TIn>(sum, from[k]);
-      float v = scaled_sum<TIn>(sum, sizeof(TIn) == 1 ? p.x_scales[r.x] : 1.f, sw, bias);
-      v = activate_lane<TOut>(n < p.N ? v : 0.f, p.act) * (p.weights ? p.alpha * p.weights[r.choice] : p.alpha);
-      if (n >= p.N) continue;
-      if (p.res) v += to_f(static_cast<const TOut*>(p.res)[r.c * p.ldres + n]);
-      static_cast<TOut*>(p.C)[r.c * p.ldc + n] = one_of<TOut>(v);
+    const int each = slots_each(rows, log_ks), count = min(each, rows - (int)rank * each);
+    for (int j0 = half * 4; j0 < count; j0 += 8) {  // four slots of a warp at a time
+      const uint4* from = reinterpret_cast<const uint4*>(part) + j0 * 32 + column;
+      uint4 four = *from;
+      for (int k = 1; k < ks; ++k) {
+        const uint4 more = from[k * 32 * each];
+        four = make_uint4(plus<TIn>(four.x, more.x), plus<TIn>(four.y, more.y), plus<TIn>(four.z, more.z), plus<TIn>(four.w, more.w));
+      }
+      finish([&](int j) { return j == 0 ? four.x : j == 1 ? four.y : j == 2 ? four.z : four.w; }, j0, count - j0, std::integral_constant<int, 4>());
     }
   }
-  cluster_sync_all();  // no CTA leaves while another may read its sums
 }
 
 template <typename TIn, typename TOut, bool kGather, bool kRounded>
 cudaError_t launch_rows(const GroupedParams& p, int sm_count, cudaStream_t s) {
   CUtensorMap mx, mw;
-  cudaError_t e = tma_encode_rows(p.X, p.ldx, p.x_rows, p.K, kGather ? 1 : kRows, Operand<TIn>::prec, &mx);
+  cudaError_t e = tma_encode_rows(p.X, p.ldx, kGather ? p.x_rows : p.slots, p.K, kGather ? 1 : kRows, Operand<TIn>::prec, &mx);
   if (e == cudaSuccess) e = tma_encode_rows(p.W, p.ldw, (long long)p.experts * p.N, p.K, BM, Operand<TIn>::prec, &mw);
-  if (e == cudaSuccess) e = raise_smem_limit<grouped_rows_kernel<TIn, TOut, kGather, kRounded>>(smem_bytes(kMaxStages));
+  if (e == cudaSuccess) e = raise_smem_limit<grouped_rows_kernel<TIn, TOut, kGather, kRounded>>(smem_bytes(kMaxStages, false) > smem_bytes(kMaxSplitStages, true) ? smem_bytes(kMaxStages, false) : smem_bytes(kMaxSplitStages, true));
   if (e != cudaSuccess) return e;
   const int n_tiles = ceil_div(p.N, BM), k_blocks = ceil_div(p.K, Operand<TIn>::k);
   const int used = p.experts < p.slots ? p.experts : p.slots;
-  const long long most = ((long long)p.slots + kRows - 1) / kRows + used - 1;  // row tiles there can be
-  // Row tiles to expect: one per expert, or what the slots fill.  A tile is cut over as many CTAs as leave each of them an SM.
-  const long long expected = ((long long)p.slots / kRows > used ? (long long)p.slots / kRows : used) * n_tiles;
+  const long long full = ((long long)p.slots + kRows - 1) / kRows, most = full + used - 1;  // row tiles: all full, and as many as there can be
+  // A tile is cut over as many CTAs as leave each of them an SM of its own, going by one row tile per expert, or what the slots fill.  Clusters
+  // of eight do not all find eight free SMs of a GPC: sixteen of them took two turns (128x1024x1024 int8 11.8 us, by four CTAs KS4).
+  const long long expected = (full > used ? full : used) * n_tiles;
   int ks = 1;
-  while (ks < 8 && expected * ks * 2 <= sm_count && 2 * ks <= k_blocks) ks *= 2;
+  while (ks < 8 && expected * ks * 2 <= (ks == 4 ? 120 : ks == 2 ? 128 : sm_count) && 2 * ks <= k_blocks) ks *= 2;
   const long long tiles = most * n_tiles;
-  const int per_cta = ceil_div(k_blocks, ks);
-  const int stages = ks > 1 && per_cta < kMaxStages ? (per_cta < 2 ? 2 : per_cta) : kMaxStages;
+  const int per_cta = ceil_div(k_blocks, ks), room = ks > 1 ? kMaxSplitStages : kMaxStages;
+  const int stages = per_cta < room && ks > 1 ? (per_cta < 2 ? 2 : per_cta) : room;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(ks > 1 ? tiles * ks : tiles < sm_count ? tiles : sm_count));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem_bytes(stages);
+  cfg.dynamicSmemBytes = smem_bytes(stages, ks > 1);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -327,20 +350,20 @@ cudaError_t launch_rows(const GroupedParams& p, int sm_count, cudaStream_t s) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = ks > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, grouped_rows_kernel<TIn, TOut, kGather, kRounded>, mx, mw, p, stages, ks);
+  return cudaLaunchKernelEx(&cfg, grouped_rows_kernel<TIn, TOut, kGather, kRounded>, mx, mw, p, stages, ks == 8 ? 3 : ks / 2);
 }
 
 }  // namespace
 
 template <typename TIn, typename TOut>
-cudaError_t launch_grouped_rows(const GroupedParams& p, bool rounded, int sm_count, cudaStream_t s) {
-  const bool gather = p.order && !p.x_by_slot;
+cudaError_t launch_grouped_rows(const GroupedParams& p, bool in_order, bool rounded, int sm_count, cudaStream_t s) {
+  const bool gather = !in_order;
   if constexpr (sizeof(TIn) == 2 && sizeof(TOut) == 4) {
     if (rounded) return gather ? launch_rows<TIn, TOut, true, true>(p, sm_count, s) : launch_rows<TIn, TOut, false, true>(p, sm_count, s);
   }
   return gather ? launch_rows<TIn, TOut, true, false>(p, sm_count, s) : launch_rows<TIn, TOut, false, false>(p, sm_count, s);
 }
-#define INSTANCE(TIn, TOut) template cudaError_t launch_grouped_rows<TIn, TOut>(const GroupedParams&, bool, int, cudaStream_t)
+#define INSTANCE(TIn, TOut) template cudaError_t launch_grouped_rows<TIn, TOut>(const GroupedParams&, bool, bool, int, cudaStream_t)
 INSTANCE(__half, __half);
 INSTANCE(__half, float);
 INSTANCE(__nv_bfloat16, __nv_bfloat16);

@@ -18,6 +18,11 @@ template <> struct Operand<int8_t> {
 };
 
 
+// A wait whose answer is the same in the whole warp.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code));
+}
+
 // Row tiles of kRows slots ahead of each expert's, and the experts' first slots; by all threads of a CTA of at least 256.
 template <int kRows>
 __device__ __forceinline__ void list_tiles(const GroupedParams& p, int* first, int* begin, int* scan) {
@@ -87,11 +92,18 @@ template <bool kMish> __device__ __forceinline__ float gate_lane(float v) {
   return v * (n * (__fdividef(1.f, both * far) * far * other));
 }
 
-// By all lanes of a warp, four neighbours having columns 4i .. 4i + 3 of one row (0 behind the last column).
-template <typename TOut> __device__ __forceinline__ float activate_lane(float v, int act) {
-  if (sizeof(TOut) == 2 && act == ACT_MISH) return gate_lane<true>(v);
-  if (sizeof(TOut) == 2 && act == ACT_SWISH) return gate_lane<false>(v);
-  return activate<sizeof(TOut) == 2>(v, act);
+// By all lanes of a warp, four neighbours having columns 4i .. 4i + 3 of each of kN rows (0 behind the last column).
+template <typename TOut, int kN> __device__ __forceinline__ void activate_lanes(float (&v)[kN], int act) {
+  if (sizeof(TOut) == 2 && act == ACT_MISH) {
+#pragma unroll
+    for (int j = 0; j < kN; ++j) v[j] = gate_lane<true>(v[j]);
+  } else if (sizeof(TOut) == 2 && act == ACT_SWISH) {
+#pragma unroll
+    for (int j = 0; j < kN; ++j) v[j] = gate_lane<false>(v[j]);
+  } else if (act != ACT_NONE) {
+#pragma unroll
+    for (int j = 0; j < kN; ++j) v[j] = activate<sizeof(TOut) == 2>(v[j], act);
+  }
 }
 
 // Columns of a row, the first a multiple of 4 and 0 behind the last column.
