@@ -21,54 +21,79 @@ __device__ __forceinline__ int position_of(const QkParams& p, int row) {
   return at >= 0 && at < p.n_positions ? at : -1;
 }
 
-// kLanes lanes hold one head, eight entries each, a warp 32 / kLanes heads at a time and kIter times as many of one row: gamma and the row's
-// angles stay in registers over all of them, and that many loads are on their way together.
+// Eight floats, with 16-byte loads where their address allows.
+__device__ __forceinline__ void load_eight(const float* from, bool aligned, float (&v)[8]) {
+  if (aligned) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(from)), b = __ldg(reinterpret_cast<const float4*>(from) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __ldg(from + i);
+  }
+}
+
+// kLanes lanes hold one head, eight entries each, a warp 32 / kLanes heads of the queries or of the keys at a time and kIter times as many of one
+// row: gamma and the row's angles stay in registers over all of them, and that many loads are on their way together.
+// Bound by memory: COUNTED
 template <typename T, int kLanes, int kIter>
-__global__ void __launch_bounds__(128) qk_norm_rotate_kernel(const QkParams p, int blocks_per_row) {
+__global__ void __launch_bounds__(128) qk_norm_rotate_kernel(const QkParams p, int q_units, int units) {
   grid_launch_dependents();
   grid_dependency_wait();
   constexpr int kHeads = 32 / kLanes;
   const int lane = threadIdx.x & 31, c = lane % kLanes, sub = lane / kLanes;
-  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int row = (int)(unit / blocks_per_row), h0 = (int)(unit % blocks_per_row) * (kHeads * kIter) + sub;
+  const long long all = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int row = (int)(all / units), unit = (int)(all - (long long)row * units), k = unit >= q_units;
   if (row >= p.rows) return;
+  const int heads = k ? p.heads - p.heads_q : p.heads_q, h0 = (k ? unit - q_units : unit) * (kHeads * kIter) + sub;
   const bool inside = 8 * c < p.depth;
+  const T* in = static_cast<const T*>(p.in[k]) + row * p.ld_in[k] + 8 * c;
   Chunk<T> raw[kIter];
 #pragma unroll
   for (int i = 0; i < kIter; ++i) {
-    const int h = h0 + i * kHeads, k = h >= p.heads_q;
-    if (inside && h < p.heads) raw[i] = load8(static_cast<const T*>(p.in[k]) + row * p.ld_in[k] + (long long)(k ? h - p.heads_q : h) * p.depth + 8 * c);
+    const int h = h0 + i * kHeads;
+    if (inside && h < heads) raw[i] = load8(in + h * p.depth);
 #pragma unroll
     for (int j = 0; j < Chunk<T>::kLoads; ++j)
-      if (!(inside && h < p.heads)) raw[i].raw[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (!(inside && h < heads)) raw[i].raw[j] = make_uint4(0u, 0u, 0u, 0u);
   }
+  float gamma[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) gamma[j] = 1.f;
+  if (p.norm && p.gamma[k] && inside) load_eight(p.gamma[k] + 8 * c, (reinterpret_cast<uintptr_t>(p.gamma[k]) & 15) == 0, gamma);
   const int at = position_of(p, row);
   const bool turned = at >= 0 && 8 * c < p.rotate;
-  float cs[8], sn[8];  // with interleaved pairs the first four alone
+  const bool second = !p.interleaved && 8 * c >= p.rotate / 2;  // of the halves
+  float cs[8], sn[8];                                           // with interleaved pairs the first four alone
   int partner = lane;
   if (turned) {
-    const float2* angles = p.table + (long long)at * (p.rotate / 2);
-    if (p.interleaved) {
+    const float* angles = reinterpret_cast<const float*>(p.table + (long long)at * (p.rotate / 2) + (p.interleaved ? 4 * c : second ? 8 * c - p.rotate / 2 : 8 * c));
+    const bool aligned = (reinterpret_cast<uintptr_t>(angles) & 15) == 0;
+    float a[8];
+    load_eight(angles, aligned, a);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      cs[i] = a[2 * i];
+      sn[i] = a[2 * i + 1];
+    }
+    if (!p.interleaved) {
+      load_eight(angles + 8, aligned, a);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 a = __ldg(angles + 4 * c + i);
-        cs[i] = a.x;
-        sn[i] = a.y;
+        cs[4 + i] = a[2 * i];
+        sn[4 + i] = a[2 * i + 1];
       }
-    } else {
-      const int first = 8 * c < p.rotate / 2 ? 8 * c : 8 * c - p.rotate / 2;
-      partner = 8 * c < p.rotate / 2 ? lane + p.rotate / 16 : lane - p.rotate / 16;
+      partner = second ? lane - p.rotate / 16 : lane + p.rotate / 16;
+      if (!second) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 a = __ldg(angles + first + i);
-        cs[i] = a.x;
-        sn[i] = 8 * c < p.rotate / 2 ? -a.y : a.y;
+        for (int i = 0; i < 8; ++i) sn[i] = -sn[i];
       }
     }
   }
+  const float inv_depth = 1.f / (float)p.depth;
+  T* out = static_cast<T*>(p.out[k]) + row * p.ld_out[k] + 8 * c;
 #pragma unroll
   for (int i = 0; i < kIter; ++i) {
-    const int h = h0 + i * kHeads, k = h >= p.heads_q;
+    const int h = h0 + i * kHeads;
     float v[8];
     unpack8(raw[i], v);
     if (p.norm) {
@@ -77,10 +102,9 @@ __global__ void __launch_bounds__(128) qk_norm_rotate_kernel(const QkParams p, i
       for (int j = 0; j < 8; ++j) sum = fmaf(v[j], v[j], sum);
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float r = 1.f / sqrtf(sum / (float)p.depth + p.eps);
-      const float* gamma = p.gamma[k];
+      const float r = rsqrtf(fmaf(sum, inv_depth, p.eps));  // (off by two steps at most)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= gamma && inside ? r * __ldg(gamma + 8 * c + j) : r;
+      for (int j = 0; j < 8; ++j) v[j] *= r * gamma[j];
     }
     if (p.rotate) {
       if (p.interleaved) {
@@ -102,8 +126,7 @@ __global__ void __launch_bounds__(128) qk_norm_rotate_kernel(const QkParams p, i
         }
       }
     }
-    if (inside && h < p.heads)
-      store8(static_cast<T*>(p.out[k]) + row * p.ld_out[k] + (long long)(k ? h - p.heads_q : h) * p.depth + 8 * c, pack8<T>(v));
+    if (inside && h < heads) store8(out + h * p.depth, pack8<T>(v));
   }
 }
 
@@ -153,18 +176,19 @@ __global__ void __launch_bounds__(128) qk_norm_rotate_any_kernel(const QkParams 
 template <typename T, int kLanes>
 cudaError_t launch_lanes(const QkParams& p, cudaStream_t s) {
   constexpr int kHeads = 32 / kLanes;
-  // As many heads per warp as leave warps for every SM: one row's heads in one or two turns of up to four loads.
-  const int steps = (p.heads + kHeads - 1) / kHeads;
+  // As many heads per warp as leave warps for every SM: the iterations with the fewest empty places, the most of equal ones.
+  const int q_steps = (p.heads_q + kHeads - 1) / kHeads, k_steps = (p.heads - p.heads_q + kHeads - 1) / kHeads;
+  auto units_of = [&](int i) { return (q_steps + i - 1) / i + (k_steps + i - 1) / i; };
   int iter = 1;
   for (int i = 2; i <= 4; ++i)
-    if ((long long)p.rows * ((steps + i - 1) / i) >= 148 * 16 && (steps + i - 1) / i * i <= (steps + iter - 1) / iter * iter) iter = i;
-  const int per_row = (steps + iter - 1) / iter;
-  const long long blocks = ((long long)p.rows * per_row + 3) / 4;
+    if ((long long)p.rows * units_of(i) >= 148 * 16 && units_of(i) * i <= units_of(iter) * iter) iter = i;
+  const int q_units = (q_steps + iter - 1) / iter, units = units_of(iter);
+  const long long blocks = ((long long)p.rows * units + 3) / 4;
   auto kernel = iter == 1 ? qk_norm_rotate_kernel<T, kLanes, 1>
                 : iter == 2 ? qk_norm_rotate_kernel<T, kLanes, 2>
                 : iter == 3 ? qk_norm_rotate_kernel<T, kLanes, 3>
                             : qk_norm_rotate_kernel<T, kLanes, 4>;
-  return launch_dependent(kernel, dim3((unsigned)blocks), dim3(128), 0, s, p, per_row);
+  return launch_dependent(kernel, dim3((unsigned)blocks), dim3(128), 0, s, p, q_units, units);
 }
 
 template <typename T>

@@ -1,21 +1,25 @@
 // The router in front of expert layers: every row's largest logits, their weights, and the choices sorted by expert (a counting sort that
-// keeps equal ones in order).
-//   1. route_choose_kernel: a CTA per block of rows chooses and counts its choices by expert.
-//   2. route_order_kernel: the counts of all blocks give each block its first place among an expert's choices; it places its own.
+// keeps equal ones in order).  A CTA has a block of rows: it chooses, counts its choices by expert, learns how many of each expert lie
+// ahead of its own, and places them.
+//   Few rows: the CTAs of one cluster, which write their counts to one another's shared memory (route_cluster_kernel, one launch).
+//   Many: route_choose_kernel leaves the counts in the workspace, route_order_kernel reads all of them.
 #include "chunk8.cuh"
 #include "kernels.cuh"
 
 namespace b200 {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kMaxBlocks = 296;  // two per SM
+constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kMaxBlocks = 148;    // a CTA takes an SM's registers
+constexpr int kMaxCluster = 8;
+constexpr int kClusterChoices = 8192;  // of a CTA of the cluster, kept in shared memory
 
 struct RouteParams {
   const void* logits; long long ld;
   int rows, experts, top_k, renormalise;
   int* ids; float* weights; int* order; int* offsets;
-  int* counts;  // [blocks][experts]
+  int* counts;  // [blocks][stride]
+  int stride;   // experts rounded up to whole fours
   int rows_per_block, blocks;
 };
 
@@ -29,7 +33,7 @@ __device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float
 // kLanes lanes have a row, eight entries each (entry 8 * lane + i), so that a row's logits are one load per lane and all of a warp's shuffles
 // serve 32 / kLanes rows.
 template <typename T, int kLanes>
-__device__ __forceinline__ void choose_row(const RouteParams& p, int row, int lane, bool vec, int* counts) {
+__device__ __forceinline__ void choose_row(const RouteParams& p, int row, int first, int lane, bool vec, int* counts, int* kept) {
   const int c = lane % kLanes, e0 = 8 * c;
   const bool live = row < p.rows;
   float v[8];
@@ -103,8 +107,93 @@ __device__ __forceinline__ void choose_row(const RouteParams& p, int row, int la
     if (j >= p.top_k) continue;
     const long long r = (long long)row * p.top_k + j;
     p.ids[r] = id[q];
+    if (kept) kept[(row - first) * p.top_k + j] = id[q];
     if (p.weights) p.weights[r] = total > 0.f ? weight[q] / total : 0.f;
     if (id[q] >= 0) atomicAdd(counts + id[q], 1);
+  }
+}
+
+// All rows of a block; kLanes 0: the ids are given.  `kept` (may be nullptr) gets the block's choices.
+template <typename T, int kLanes>
+__device__ __forceinline__ void choose_block(const RouteParams& p, int first, int end, bool vec, int* counts, int* kept) {
+  for (int e = threadIdx.x; e < p.stride; e += kThreads) counts[e] = 0;
+  __syncthreads();
+  if constexpr (kLanes > 0) {
+    const int lane = threadIdx.x & 31;
+    for (int row0 = first; row0 < end; row0 += kThreads / kLanes) {
+      const int row = row0 + (int)threadIdx.x / kLanes;
+      choose_row<T, kLanes>(p, row < end ? row : p.rows, first, lane, vec, counts, kept);
+    }
+  } else {
+    const long long from = (long long)first * p.top_k;
+    const int n = (end - first) * p.top_k;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const int id = p.ids[from + i];
+      if (kept) kept[i] = id;
+      if (id >= 0 && id < p.experts) atomicAdd(counts + id, 1);
+    }
+  }
+  __syncthreads();
+}
+
+struct PlaceMemory {
+  int of_warp[kWarps][B200_MAX_EXPERTS];  // an expert's choices of each warp, then the place of the warp's next one
+  int total[B200_MAX_EXPERTS], before[B200_MAX_EXPERTS];  // choices of an expert: in all blocks, in the blocks ahead of this one
+  int scan[8];
+};
+// Places this block's choices, given total and before.
+__device__ __forceinline__ void place_block(const RouteParams& p, int first, int end, bool first_block, const int* kept, PlaceMemory& m) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = threadIdx.x;
+  const long long from = (long long)first * p.top_k;
+  const int n = (end - first) * p.top_k, per_warp = ((n + kWarps - 1) / kWarps + 31) & ~31;
+  const int w0 = warp * per_warp, w1 = min(w0 + per_warp, n);
+  auto id_of = [&](int i) {
+    const int id = i < w1 ? (kept ? kept[i] : p.ids[from + i]) : -1;
+    return id >= 0 && id < p.experts ? id : -1;
+  };
+  for (int i = threadIdx.x; i < kWarps * B200_MAX_EXPERTS; i += kThreads) (&m.of_warp[0][0])[i] = 0;
+  __syncthreads();
+  for (int i = w0 + lane; i < w1; i += 32) {
+    const int id = id_of(i);
+    if (id >= 0) atomicAdd(&m.of_warp[warp][id], 1);
+  }
+  int upto = 0;
+  if (e < 256) {
+    upto = e < p.experts ? m.total[e] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int k = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += k;
+    }
+    if (lane == 31) m.scan[warp] = upto;
+  }
+  __syncthreads();
+  if (e < p.experts) {
+    for (int w = 0; w < warp; ++w) upto += m.scan[w];
+    const int begin = upto - m.total[e];
+    if (first_block) {
+      p.offsets[e] = begin;
+      if (e == p.experts - 1) p.offsets[p.experts] = upto;
+    }
+    int at = begin + m.before[e];
+#pragma unroll 8
+    for (int w = 0; w < kWarps; ++w) {
+      const int k = m.of_warp[w][e];
+      m.of_warp[w][e] = at;
+      at += k;
+    }
+  }
+  __syncthreads();
+  for (int i0 = w0; i0 < w1; i0 += 32) {
+    const int id = id_of(i0 + lane);
+    const uint32_t same = __match_any_sync(0xffffffffu, id);
+    const int rank = __popc(same & ((1u << lane) - 1u)), at = id >= 0 ? m.of_warp[warp][id] : 0;
+    __syncwarp();
+    if (id >= 0) {
+      p.order[at + rank] = (int)(from + i0 + lane);
+      if (rank == 0) m.of_warp[warp][id] = at + __popc(same);
+    }
+    __syncwarp();
   }
 }
 
@@ -112,101 +201,75 @@ template <typename T, int kLanes>
 __global__ void __launch_bounds__(kThreads) route_choose_kernel(const RouteParams p, bool vec) {
   __shared__ int counts[B200_MAX_EXPERTS];
   grid_launch_dependents();
-  for (int e = threadIdx.x; e < p.experts; e += kThreads) counts[e] = 0;
-  __syncthreads();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31, first = blockIdx.x * p.rows_per_block;
-  const int end = min(first + p.rows_per_block, p.rows);
-  for (int row0 = first; row0 < end; row0 += kThreads / kLanes) {
-    const int row = row0 + (int)threadIdx.x / kLanes;
-    choose_row<T, kLanes>(p, row < end ? row : p.rows, lane, vec, counts);
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < p.experts; e += kThreads) p.counts[blockIdx.x * p.experts + e] = counts[e];
+  const int first = blockIdx.x * p.rows_per_block;
+  choose_block<T, kLanes>(p, first, min(first + p.rows_per_block, p.rows), vec, counts, nullptr);
+  for (int e = threadIdx.x; e < p.stride; e += kThreads) p.counts[blockIdx.x * p.stride + e] = counts[e];
 }
 
-// Given ids: counts alone.
-__global__ void __launch_bounds__(kThreads) route_count_kernel(const RouteParams p) {
-  __shared__ int counts[B200_MAX_EXPERTS];
-  grid_launch_dependents();
-  for (int e = threadIdx.x; e < p.experts; e += kThreads) counts[e] = 0;
-  __syncthreads();
-  grid_dependency_wait();
-  const long long first = (long long)blockIdx.x * p.rows_per_block * p.top_k;
-  const long long end = min(first + (long long)p.rows_per_block * p.top_k, (long long)p.rows * p.top_k);
-  for (long long r = first + threadIdx.x; r < end; r += kThreads) {
-    const int id = p.ids[r];
-    if (id >= 0 && id < p.experts) atomicAdd(counts + id, 1);
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < p.experts; e += kThreads) p.counts[blockIdx.x * p.experts + e] = counts[e];
-}
-
+// Four experts' counts per load, all loads of a thread on their way together.
 __global__ void __launch_bounds__(kThreads) route_order_kernel(const RouteParams p) {
-  __shared__ int of_warp[kWarps][B200_MAX_EXPERTS];  // an expert's choices of each warp, then the place of the warp's next one
-  __shared__ int scan[kWarps];
+  __shared__ PlaceMemory m;
   grid_launch_dependents();
-  for (int i = threadIdx.x; i < kWarps * B200_MAX_EXPERTS; i += kThreads) (&of_warp[0][0])[i] = 0;
+  for (int e = threadIdx.x; e < B200_MAX_EXPERTS; e += kThreads) m.total[e] = m.before[e] = 0;
   __syncthreads();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = threadIdx.x;
-  // place of this block's first choice of expert e
-  int total = 0, before = 0;
-  if (e < p.experts) {
-#pragma unroll 8
-    for (int b = 0; b < p.blocks; ++b) {
-      const int n = p.counts[b * p.experts + e];
-      total += n;
-      before += b < (int)blockIdx.x ? n : 0;
+  const int fours = p.stride / 4, groups = kThreads / fours, q = threadIdx.x % fours, g = threadIdx.x / fours;
+  if (g < groups) {
+    int4 total = make_int4(0, 0, 0, 0), before = total;
+#pragma unroll 10
+    for (int b = g; b < p.blocks; b += groups) {
+      const int4 n = reinterpret_cast<const int4*>(p.counts)[b * fours + q];
+      total = make_int4(total.x + n.x, total.y + n.y, total.z + n.z, total.w + n.w);
+      if (b < (int)blockIdx.x) before = make_int4(before.x + n.x, before.y + n.y, before.z + n.z, before.w + n.w);
     }
-  }
-  int upto = total;
+    const int t[4] = {total.x, total.y, total.z, total.w}, u[4] = {before.x, before.y, before.z, before.w};
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int n = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += n;
-  }
-  if (lane == 31) scan[warp] = upto;
-  // this block's choices by warp
-  const long long first = (long long)blockIdx.x * p.rows_per_block * p.top_k;
-  const long long end = min(first + (long long)p.rows_per_block * p.top_k, (long long)p.rows * p.top_k);
-  const long long per_warp = (end - first + kWarps - 1) / kWarps;
-  const long long w0 = first + warp * per_warp, w1 = min(w0 + per_warp, end);
-  for (long long r = w0 + lane; r < w1; r += 32) {
-    const int id = p.ids[r];
-    if (id >= 0 && id < p.experts) atomicAdd(&of_warp[warp][id], 1);
-  }
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) upto += scan[w];
-  if (e < p.experts) {
-    int at = upto - total + before;
-    if (blockIdx.x == 0) {
-      p.offsets[e] = upto - total;
-      if (e == p.experts - 1) p.offsets[p.experts] = upto;
-    }
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const int n = of_warp[w][e];
-      of_warp[w][e] = at;
-      at += n;
+    for (int i = 0; i < 4; ++i) {
+      if (t[i]) atomicAdd(m.total + 4 * q + i, t[i]);
+      if (u[i]) atomicAdd(m.before + 4 * q + i, u[i]);
     }
   }
   __syncthreads();
-  for (long long r0 = w0; r0 < w1; r0 += 32) {
-    const long long r = r0 + lane;
-    int id = r < w1 ? p.ids[r] : -1;
-    if (id >= p.experts) id = -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, id);
-    const int rank = __popc(same & ((1u << lane) - 1u));
-    const int at = id >= 0 ? of_warp[warp][id] : 0;
-    __syncwarp();
-    if (id >= 0) {
-      p.order[at + rank] = (int)r;
-      if (rank == 0) of_warp[warp][id] = at + __popc(same);
-    }
-    __syncwarp();
-  }
+  const int first = blockIdx.x * p.rows_per_block;
+  place_block(p, first, min(first + p.rows_per_block, p.rows), blockIdx.x == 0, nullptr, m);
 }
+
+// All of it by one cluster.
+template <typename T, int kLanes>
+__global__ void __launch_bounds__(kThreads) route_cluster_kernel(const RouteParams p, bool vec) {
+  extern __shared__ int smem[];
+  PlaceMemory& m = *reinterpret_cast<PlaceMemory*>(smem);
+  int* all = smem + sizeof(PlaceMemory) / 4;              // [8][256] counts of each CTA
+  int* counts = all + kMaxCluster * B200_MAX_EXPERTS;     // [256]
+  int* kept = counts + B200_MAX_EXPERTS;                  // [kClusterChoices]
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int first = blockIdx.x * p.rows_per_block, end = max(first, min(first + p.rows_per_block, p.rows));
+  choose_block<T, kLanes>(p, first, end, vec, counts, kept);
+  if (p.blocks > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");  // all run
+    for (int i = threadIdx.x; i < p.blocks * p.stride; i += kThreads) {
+      const int cta = i / p.stride, e = i - cta * p.stride;
+      uint32_t to;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(all + blockIdx.x * B200_MAX_EXPERTS + e)), "r"(cta));
+      asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(counts[e]) : "memory");
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  for (int e = threadIdx.x; e < p.experts; e += kThreads) {
+    int total = p.blocks > 1 ? 0 : counts[e], before = 0;
+    for (int b = 0; p.blocks > 1 && b < p.blocks; ++b) {
+      if (b == (int)blockIdx.x) before = total;
+      total += all[b * B200_MAX_EXPERTS + e];
+    }
+    m.total[e] = total;
+    m.before[e] = before;
+  }
+  __syncthreads();
+  place_block(p, first, end, blockIdx.x == 0, kept, m);
+}
+constexpr int kClusterBytes = (int)sizeof(PlaceMemory) + 4 * (kMaxCluster * B200_MAX_EXPERTS + B200_MAX_EXPERTS + kClusterChoices);
 
 int lanes_of(int experts) {
   int l = 1;
@@ -214,27 +277,57 @@ int lanes_of(int experts) {
   return l;
 }
 
-// Blocks of rows: enough for every SM to have some, none without a full pass of its threads.
-void plan_blocks(RouteParams& p) {
-  const int pass = kThreads / lanes_of(p.experts);
+// Rows to a block: whole passes of its threads.  A cluster where its eight CTAs have few passes (KMEASURED).
+bool plan_blocks(RouteParams& p, int lanes) {
+  const int pass = kThreads / lanes;
   const long long passes = ((long long)p.rows + pass - 1) / pass;
-  const long long blocks = passes < kMaxBlocks ? passes : kMaxBlocks;
-  const long long per = (passes + blocks - 1) / blocks;
+  const long long few = (passes + kMaxCluster - 1) / kMaxCluster;
+  const bool cluster = few <= 2 && few * pass * p.top_k <= kClusterChoices;
+  const long long most = cluster ? kMaxCluster : kMaxBlocks, per = (passes + most - 1) / most;
   p.rows_per_block = (int)(per * pass);
   p.blocks = (int)((p.rows + per * pass - 1) / (per * pass));
+  p.stride = (p.experts + 3) & ~3;
+  return cluster;
 }
 
-template <typename T>
-cudaError_t launch_choose(const RouteParams& p, cudaStream_t s) {
+template <typename T, int kLanes>
+cudaError_t launch_route(RouteParams p, cudaStream_t s) {
   const bool vec = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.ld % (16 / (int)sizeof(T)) == 0;
-  const int lanes = lanes_of(p.experts);
-  auto kernel = lanes == 1 ? route_choose_kernel<T, 1>
-                : lanes == 2 ? route_choose_kernel<T, 2>
-                : lanes == 4 ? route_choose_kernel<T, 4>
-                : lanes == 8 ? route_choose_kernel<T, 8>
-                : lanes == 16 ? route_choose_kernel<T, 16>
-                              : route_choose_kernel<T, 32>;
-  return launch_dependent(kernel, dim3(p.blocks), dim3(kThreads), 0, s, p, vec);
+  cudaError_t e;
+  if (plan_blocks(p, kLanes ? kLanes : 1)) {
+    auto kernel = route_cluster_kernel<T, kLanes>;
+    if ((e = raise_smem_limit<route_cluster_kernel<T, kLanes>>(kClusterBytes)) != cudaSuccess) return e;
+    int size = 1;
+    while (size < p.blocks) size *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kClusterBytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = size;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    p.blocks = size;
+    return cudaLaunchKernelEx(&cfg, kernel, p, vec);
+  }
+  if ((e = launch_dependent(route_choose_kernel<T, kLanes>, dim3(p.blocks), dim3(kThreads), 0, s, p, vec)) != cudaSuccess) return e;
+  return launch_dependent(route_order_kernel, dim3(p.blocks), dim3(kThreads), 0, s, p);
+}
+template <typename T>
+cudaError_t launch_lanes(const RouteParams& p, cudaStream_t s) {
+  switch (lanes_of(p.experts)) {
+    case 1: return launch_route<T, 1>(p, s);
+    case 2: return launch_route<T, 2>(p, s);
+    case 4: return launch_route<T, 4>(p, s);
+    case 8: return launch_route<T, 8>(p, s);
+    case 16: return launch_route<T, 16>(p, s);
+    default: return launch_route<T, 32>(p, s);
+  }
 }
 
 __global__ void route_none_kernel(int* offsets, int n) {
@@ -253,7 +346,7 @@ const char* check_shape(const b200_route_desc* d) {
   return nullptr;
 }
 size_t route_bytes(const b200_route_desc& d) {
-  return ((size_t)kMaxBlocks * d.n_experts * 4 + 255) & ~size_t(255);
+  return ((size_t)kMaxBlocks * ((d.n_experts + 3) / 4 * 4) * 4 + 255) & ~size_t(255);
 }
 
 }  // namespace
@@ -302,12 +395,10 @@ extern "C" int b200_op_route(const b200_route_desc* d, void* stream) {
     p.rows = d->rows; p.experts = d->n_experts; p.top_k = d->top_k; p.renormalise = d->renormalise;
     p.ids = d->ids; p.weights = d->weights; p.order = d->order; p.offsets = d->offsets;
     p.counts = static_cast<int*>(d->workspace);
-    plan_blocks(p);
-    if (!d->logits) B200_CUDA(launch_dependent(route_count_kernel, dim3(p.blocks), dim3(kThreads), 0, s, p));
-    else if (d->precision == B200_PREC_FP32) B200_CUDA(launch_choose<float>(p, s));
-    else if (d->precision == B200_PREC_FP16) B200_CUDA(launch_choose<__half>(p, s));
-    else B200_CUDA(launch_choose<__nv_bfloat16>(p, s));
-    B200_CUDA(launch_dependent(route_order_kernel, dim3(p.blocks), dim3(kThreads), 0, s, p));
+    if (!d->logits) B200_CUDA((launch_route<float, 0>(p, s)));
+    else if (d->precision == B200_PREC_FP32) B200_CUDA(launch_lanes<float>(p, s));
+    else if (d->precision == B200_PREC_FP16) B200_CUDA(launch_lanes<__half>(p, s));
+    else B200_CUDA(launch_lanes<__nv_bfloat16>(p, s));
     return B200_OK;
   });
 }
