@@ -106,48 +106,66 @@ struct CombineParams {
   int tokens, N, experts, top_k, group;
 };
 
-// Eight columns of a token per thread, its choices in order.
+// A warp per token and 512 columns: two pieces of eight columns per lane, whose rows of all choices are on their way together; the choices are
+// added in order.
 template <typename TOut>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p, int vec) {
   grid_launch_dependents();
   grid_dependency_wait();
-  const int pieces = (p.N + 7) / 8;
-  const long long all = (long long)p.tokens * pieces;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
-    const int t = (int)(i / pieces), n = (int)(i % pieces) * 8, request = t / p.group, inside = t - request * p.group;
-    float v[8] = {};
-    bool any = false;
-    for (int j = 0; j < p.top_k; ++j) {
-      const int id = p.ids[(long long)request * p.top_k + j];
-      if (id < 0 || id >= p.experts) continue;
-      any = true;
-      const float* y = p.Y + (((long long)request * p.top_k + j) * p.group + inside) * p.N + n;
-      if (vec) {
-        float w[8];
-        unpack8(load8(y), w);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] += w[k];
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (n + k < p.N) v[k] += y[k];
-      }
-    }
-    if (!any) continue;
-    const TOut* res = p.res ? static_cast<const TOut*>(p.res) + t * p.ldres + n : nullptr;
-    TOut* c = static_cast<TOut*>(p.C) + t * p.ldc + n;
+  const int lane = threadIdx.x & 31, parts = (p.N + 511) / 512;
+  const long long all = (long long)p.tokens * parts;
+  for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < all; i += (long long)gridDim.x * 8) {
+    const int t = (int)(i / parts), n0 = (int)(i - (long long)t * parts) * 512 + lane * 8, request = t / p.group, inside = t - request * p.group;
+    const TOut* res = p.res ? static_cast<const TOut*>(p.res) + t * p.ldres : nullptr;
+    TOut* c = static_cast<TOut*>(p.C) + t * p.ldc;
     if (vec) {
-      if (res) {
-        float w[8];
-        unpack8(load8(res), w);
+      Chunk<TOut> more[2];
+      float v[2][8] = {};
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] += w[k];
+      for (int h = 0; h < 2; ++h)
+        if (res && n0 + 256 * h < p.N) more[h] = load8(res + n0 + 256 * h);
+      bool any = false;
+#pragma unroll 2
+      for (int j = 0; j < p.top_k; ++j) {
+        const int id = __ldg(p.ids + (long long)request * p.top_k + j);
+        if (id < 0 || id >= p.experts) continue;
+        any = true;
+        const float* y = p.Y + (((long long)request * p.top_k + j) * p.group + inside) * p.N + n0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (n0 + 256 * h >= p.N) continue;
+          const float4 a = __ldcs(reinterpret_cast<const float4*>(y + 256 * h)), b = __ldcs(reinterpret_cast<const float4*>(y + 256 * h) + 1);
+          v[h][0] += a.x; v[h][1] += a.y; v[h][2] += a.z; v[h][3] += a.w;
+          v[h][4] += b.x; v[h][5] += b.y; v[h][6] += b.z; v[h][7] += b.w;
+        }
       }
-      store8(c, pack8<TOut>(v));
-    } else {
+      if (!any) continue;
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (n + k < p.N) c[k] = one_of<TOut>(v[k] + (res ? to_f(res[k]) : 0.f));
+      for (int h = 0; h < 2; ++h) {
+        if (n0 + 256 * h >= p.N) continue;
+        if (res) {
+          float w[8];
+          unpack8(more[h], w);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[h][k] += w[k];
+        }
+        store8(c + n0 + 256 * h, pack8<TOut>(v[h]));
+      }
+    } else {
+      bool any = false;
+      for (int j = 0; j < p.top_k; ++j) {
+        const int id = p.ids[(long long)request * p.top_k + j];
+        any |= id >= 0 && id < p.experts;
+      }
+      if (!any) continue;
+      for (int n = n0 - 7 * lane; n < min(n0 - 8 * lane + 512, p.N); n += 32) {  // column by column
+        float v = 0.f;
+        for (int j = 0; j < p.top_k; ++j) {
+          const int id = p.ids[(long long)request * p.top_k + j];
+          if (id >= 0 && id < p.experts) v += p.Y[(((long long)request * p.top_k + j) * p.group + inside) * p.N + n];
+        }
+        c[n] = one_of<TOut>(res ? v + to_f(res[n]) : v);
+      }
     }
   }
 }
@@ -156,7 +174,7 @@ template <typename TOut>
 cudaError_t launch_combine(const CombineParams& p, cudaStream_t s) {
   auto fine = [&](const void* q, long long ld) { return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld % (16 / (int)sizeof(TOut)) == 0; };
   const int vec = p.N % 8 == 0 && fine(p.C, p.ldc) && (!p.res || fine(p.res, p.ldres));
-  const long long blocks = ((long long)p.tokens * ((p.N + 7) / 8) + 255) / 256;
+  const long long blocks = ((long long)p.tokens * ((p.N + 511) / 512) + 7) / 8;
   return launch_dependent(combine_kernel<TOut>, dim3((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64)), dim3(256), 0, s, p, vec);
 }
 
@@ -170,13 +188,27 @@ __global__ void __launch_bounds__(256) spread_rows_kernel(const GroupedParams p,
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, pieces = row_bytes / 16;
   const int end = expert_begin(p, p.experts);
-  for (long long slot = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); slot < end; slot += (long long)gridDim.x * 8) {
-    const int x = rows_of_slot(p, (int)slot).x;
-    if (x < 0) continue;
-    const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.X) + x * p.ldx * size);
+  // two rows per warp at a time
+  for (long long slot = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * 2; slot < end; slot += (long long)gridDim.x * 16) {
+    const uint4* from[2];
+    bool there[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int x = slot + k < end ? rows_of_slot(p, (int)slot + k).x : -1;
+      there[k] = x >= 0;
+      from[k] = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.X) + (x < 0 ? 0 : x) * p.ldx * size);
+    }
     uint4* at = reinterpret_cast<uint4*>(to + slot * row_bytes);
-#pragma unroll 4
-    for (int i = lane; i < pieces; i += 32) at[i] = from[i];
+#pragma unroll 2
+    for (int i = lane; i < pieces; i += 32) {
+      uint4 v[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (there[k]) v[k] = from[k][i];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (there[k]) at[k * pieces + i] = v[k];
+    }
   }
 }
 
@@ -199,7 +231,7 @@ int run_grouped(GroupedParams p, bool exact_sums, void* spread, cudaStream_t s) 
   B200_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   const bool pairs = !exact_sums && many_rows(p.slots, p.experts), in_place = !p.order || p.x_by_slot || (!pairs && !spreads(p.slots, p.experts));
   if (!in_place) {
-    const long long blocks = ((long long)p.slots + 7) / 8;
+    const long long blocks = ((long long)p.slots + 15) / 16;
     B200_CUDA(launch_dependent(spread_rows_kernel, dim3((unsigned)(blocks < sms * 8 ? blocks : sms * 8)), dim3(256), 0, s, p, static_cast<uint8_t*>(spread),
                                p.K * (int)sizeof(TIn), (int)sizeof(TIn)));
     p.X = spread;

@@ -9,10 +9,10 @@
 namespace b200 {
 namespace {
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kThreads = 1024, kClusterThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxBlocks = 148;    // a CTA takes an SM's registers
 constexpr int kMaxCluster = 8;
-constexpr int kClusterChoices = 8192;  // of a CTA of the cluster, kept in shared memory
+constexpr int kClusterChoices = 4096;  // of a CTA of the cluster, kept in shared memory
 
 struct RouteParams {
   const void* logits; long long ld;
@@ -23,17 +23,42 @@ struct RouteParams {
   int rows_per_block, blocks;
 };
 
-// A logit as a whole number of the same order; 0 for what is never chosen.
+// A logit (not NaN) as a whole number of the same order; those below kLeast are minus infinity, which is never chosen.
+constexpr uint32_t kLeast = 0x00800000u;
 __device__ __forceinline__ uint32_t key_of(float v) {
   const uint32_t u = __float_as_uint(v + 0.f);  // -0 is 0
-  return v > -INFINITY ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0u;
+  return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
+// A logit and its expert as one whole number, larger for the one to be chosen first: equal logits by falling 255 - expert.  16-bit logits leave the
+// last 13 bits of a float's key free, which hold the expert.
+template <typename T> struct Choice {
+  using type = uint32_t;
+  static __device__ __forceinline__ type of(float v, int e) { return (key_of(v) & ~0x1fffu) | (uint32_t)(255 - e); }
+  static __device__ __forceinline__ bool some(type c) { return c >= kLeast; }
+  static __device__ __forceinline__ float logit(type c) { return logit_of(c & 0x80000000u ? c & ~0x1fffu : c | 0x1fffu); }
+};
+template <> struct Choice<float> {
+  using type = unsigned long long;
+  static __device__ __forceinline__ type of(float v, int e) { return (type)key_of(v) << 32 | (uint32_t)(255 - e); }
+  static __device__ __forceinline__ bool some(type c) { return (uint32_t)(c >> 32) >= kLeast; }
+  static __device__ __forceinline__ float logit(type c) { return logit_of((uint32_t)(c >> 32)); }
+};
+template <typename C> __device__ __forceinline__ C larger(C a, C b) { return a > b ? a : b; }
+template <typename C> __device__ __forceinline__ void order_two(C& a, C& b) {
+  const C most = larger(a, b);
+  b = a > b ? b : a;
+  a = most;
+}
+
 // kLanes lanes have a row, eight entries each (entry 8 * lane + i), so that a row's logits are one load per lane and all of a warp's shuffles
-// serve 32 / kLanes rows.
+// serve 32 / kLanes rows.  16-bit logits: each lane sorts its eight (19 exchanges of two instructions) and offers the first of what it has left.
+// fp32, whose choices are 64 bits wide: the largest of the eight is looked for anew, which costs the same from there on.  Bound by
+// instructions (COUNTED).
 template <typename T, int kLanes>
 __device__ __forceinline__ void choose_row(const RouteParams& p, int row, int first, int lane, bool vec, int* counts, int* kept) {
+  using Ch = Choice<T>;
   const int c = lane % kLanes, e0 = 8 * c;
   const bool live = row < p.rows;
   float v[8];
@@ -49,56 +74,71 @@ __device__ __forceinline__ void choose_row(const RouteParams& p, int row, int fi
         if (e0 + i < p.experts) v[i] = to_f(x[i]);
     }
   }
-  uint32_t key[8];
+  typename Ch::type mine[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) key[i] = key_of(v[i]);
-  constexpr int kKeep = (B200_MAX_TOP_K + kLanes - 1) / kLanes;
-  float top = 0.f, total = 0.f, weight[kKeep];  // lane c of the row keeps the choices c, c + kLanes, ...
-  int id[kKeep];
-#pragma unroll
-  for (int q = 0; q < kKeep; ++q) {
-    weight[q] = 0.f;
-    id[q] = -1;
+  for (int i = 0; i < 8; ++i) {
+    v[i] = fmaxf(v[i], -INFINITY);  // NaN becomes minus infinity
+    mine[i] = Ch::of(v[i], e0 + i);
   }
+  constexpr bool kSorted = sizeof(T) == 2;
+  if constexpr (kSorted) {  // odd-even merging
+#pragma unroll
+    for (int size = 1; size < 8; size *= 2)
+#pragma unroll
+      for (int gap = size; gap > 0; gap /= 2)
+#pragma unroll
+        for (int i = gap % size; i + gap < 8; i += 2 * gap)
+#pragma unroll
+          for (int k = 0; k < gap; ++k)
+            if (i + k + gap < 8 && (i + k) / (2 * size) == (i + k + gap) / (2 * size)) order_two(mine[i + k], mine[i + k + gap]);
+  }
+  constexpr int kMost = 8 * kLanes < B200_MAX_TOP_K ? 8 * kLanes : B200_MAX_TOP_K, kKeep = (kMost + kLanes - 1) / kLanes;
+  typename Ch::type keep[kKeep], head = 0;  // lane c of the row keeps the choices c, c + kLanes, ...
+#pragma unroll
+  for (int q = 0; q < kKeep; ++q) keep[q] = 0;
   for (int j = 0; j < p.top_k; ++j) {
-    uint32_t best = 0;
-    int at = 0;
+    typename Ch::type best = mine[0];
+    if constexpr (!kSorted) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (key[i] > best) {
-        best = key[i];
-        at = e0 + i;
-      }
-#pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) {
-      const uint32_t b = __shfl_xor_sync(0xffffffffu, best, o);
-      const int a = __shfl_xor_sync(0xffffffffu, at, o);
-      if (b > best || (b == best && a < at)) {
-        best = b;
-        at = a;
-      }
+      for (int i = 1; i < 8; ++i) best = larger(best, mine[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (at == e0 + i) key[i] = 0;
-    const float l = logit_of(best);
-    if (j == 0) {
-      top = l;
-      if (!p.renormalise) {
+    for (int o = kLanes / 2; o > 0; o >>= 1) best = larger(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if constexpr (kSorted) {
+      const bool pop = mine[0] == best;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) total += v[i] == top ? 1.f : (v[i] > -INFINITY && top < INFINITY ? expf(v[i] - top) : 0.f);
+      for (int i = 0; i < 7; ++i) mine[i] = pop ? mine[i + 1] : mine[i];
+      if (pop) mine[7] = 0;
+    } else {
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-      }
+      for (int i = 0; i < 8; ++i) mine[i] = mine[i] == best ? 0 : mine[i];
     }
-    const float w = best == 0 ? 0.f : l == top ? 1.f : top < INFINITY ? expf(l - top) : 0.f;
-    if (p.renormalise) total += w;
+    if (j == 0) head = best;
 #pragma unroll
     for (int q = 0; q < kKeep; ++q)
-      if (q * kLanes + c == j) {
-        weight[q] = w;
-        id[q] = best ? at : -1;
-      }
+      if (q * kLanes + c == j) keep[q] = best;
+  }
+  const float top = Ch::some(head) ? Ch::logit(head) : 0.f;
+  // (sums may take the quick exponential: a term e^x is off by (|x| 2^-24.5 + 2^-22) e^x)
+  float total = 0.f, weight[kKeep];
+  if (p.weights) {
+#pragma unroll
+    for (int q = 0; q < kKeep; ++q) {
+      const float l = Ch::logit(keep[q]);
+      weight[q] = !Ch::some(keep[q]) ? 0.f : l == top ? 1.f : top < INFINITY ? expf(l - top) : 0.f;
+    }
+    if (p.renormalise) {
+#pragma unroll
+      for (int q = 0; q < kKeep; ++q) total += weight[q];
+    } else if (top < INFINITY) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) total += __expf(v[i] - top);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) total += v[i] == top ? 1.f : 0.f;
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   }
   if (!live) return;
 #pragma unroll
@@ -106,28 +146,30 @@ __device__ __forceinline__ void choose_row(const RouteParams& p, int row, int fi
     const int j = q * kLanes + c;
     if (j >= p.top_k) continue;
     const long long r = (long long)row * p.top_k + j;
-    p.ids[r] = id[q];
-    if (kept) kept[(row - first) * p.top_k + j] = id[q];
-    if (p.weights) p.weights[r] = total > 0.f ? weight[q] / total : 0.f;
-    if (id[q] >= 0) atomicAdd(counts + id[q], 1);
+    const int id = Ch::some(keep[q]) ? 255 - (int)(keep[q] & 0xffu) : -1;
+    p.ids[r] = id;
+    if (kept) kept[(row - first) * p.top_k + j] = id;
+    if (p.weights) p.weights[r] = id >= 0 ? weight[q] / total : 0.f;
+    if (id >= 0) atomicAdd(counts + id, 1);
   }
 }
 
 // All rows of a block; kLanes 0: the ids are given.  `kept` (may be nullptr) gets the block's choices.
 template <typename T, int kLanes>
 __device__ __forceinline__ void choose_block(const RouteParams& p, int first, int end, bool vec, int* counts, int* kept) {
-  for (int e = threadIdx.x; e < p.stride; e += kThreads) counts[e] = 0;
+  const int threads = blockDim.x;
+  for (int e = threadIdx.x; e < p.stride; e += threads) counts[e] = 0;
   __syncthreads();
   if constexpr (kLanes > 0) {
     const int lane = threadIdx.x & 31;
-    for (int row0 = first; row0 < end; row0 += kThreads / kLanes) {
+    for (int row0 = first; row0 < end; row0 += threads / kLanes) {
       const int row = row0 + (int)threadIdx.x / kLanes;
       choose_row<T, kLanes>(p, row < end ? row : p.rows, first, lane, vec, counts, kept);
     }
   } else {
     const long long from = (long long)first * p.top_k;
     const int n = (end - first) * p.top_k;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+    for (int i = threadIdx.x; i < n; i += threads) {
       const int id = p.ids[from + i];
       if (kept) kept[i] = id;
       if (id >= 0 && id < p.experts) atomicAdd(counts + id, 1);
@@ -136,13 +178,13 @@ __device__ __forceinline__ void choose_block(const RouteParams& p, int first, in
   __syncthreads();
 }
 
-struct PlaceMemory {
+template <int kWarps> struct PlaceMemory {
   int of_warp[kWarps][B200_MAX_EXPERTS];  // an expert's choices of each warp, then the place of the warp's next one
   int total[B200_MAX_EXPERTS], before[B200_MAX_EXPERTS];  // choices of an expert: in all blocks, in the blocks ahead of this one
   int scan[8];
 };
 // Places this block's choices, given total and before.
-__device__ __forceinline__ void place_block(const RouteParams& p, int first, int end, bool first_block, const int* kept, PlaceMemory& m) {
+template <int kWarps> __device__ __forceinline__ void place_block(const RouteParams& p, int first, int end, bool first_block, const int* kept, PlaceMemory<kWarps>& m) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = threadIdx.x;
   const long long from = (long long)first * p.top_k;
   const int n = (end - first) * p.top_k, per_warp = ((n + kWarps - 1) / kWarps + 31) & ~31;
@@ -151,7 +193,8 @@ __device__ __forceinline__ void place_block(const RouteParams& p, int first, int
     const int id = i < w1 ? (kept ? kept[i] : p.ids[from + i]) : -1;
     return id >= 0 && id < p.experts ? id : -1;
   };
-  for (int i = threadIdx.x; i < kWarps * B200_MAX_EXPERTS; i += kThreads) (&m.of_warp[0][0])[i] = 0;
+  for (int w = 0; w < kWarps; ++w)
+    if (threadIdx.x < (unsigned)p.experts) m.of_warp[w][threadIdx.x] = 0;
   __syncthreads();
   for (int i = w0 + lane; i < w1; i += 32) {
     const int id = id_of(i);
@@ -209,7 +252,7 @@ __global__ void __launch_bounds__(kThreads) route_choose_kernel(const RouteParam
 
 // Four experts' counts per load, all loads of a thread on their way together.
 __global__ void __launch_bounds__(kThreads) route_order_kernel(const RouteParams p) {
-  __shared__ PlaceMemory m;
+  __shared__ PlaceMemory<kWarps> m;
   grid_launch_dependents();
   for (int e = threadIdx.x; e < B200_MAX_EXPERTS; e += kThreads) m.total[e] = m.before[e] = 0;
   __syncthreads();
@@ -237,39 +280,36 @@ __global__ void __launch_bounds__(kThreads) route_order_kernel(const RouteParams
 
 // All of it by one cluster.
 template <typename T, int kLanes>
-__global__ void __launch_bounds__(kThreads) route_cluster_kernel(const RouteParams p, bool vec) {
-  extern __shared__ int smem[];
-  PlaceMemory& m = *reinterpret_cast<PlaceMemory*>(smem);
-  int* all = smem + sizeof(PlaceMemory) / 4;              // [8][256] counts of each CTA
-  int* counts = all + kMaxCluster * B200_MAX_EXPERTS;     // [256]
-  int* kept = counts + B200_MAX_EXPERTS;                  // [kClusterChoices]
+__global__ void __launch_bounds__(kClusterThreads) route_cluster_kernel(const RouteParams p, bool vec) {
+  __shared__ PlaceMemory<kClusterThreads / 32> m;
+  __shared__ int all[kMaxCluster][B200_MAX_EXPERTS];  // counts of each CTA
+  __shared__ int counts[B200_MAX_EXPERTS];
+  __shared__ int kept[kClusterChoices];
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   grid_launch_dependents();
   grid_dependency_wait();
-  const int first = blockIdx.x * p.rows_per_block, end = max(first, min(first + p.rows_per_block, p.rows));
+  const int first = min(blockIdx.x * p.rows_per_block, p.rows), end = min(first + p.rows_per_block, p.rows);
   choose_block<T, kLanes>(p, first, end, vec, counts, kept);
-  if (p.blocks > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");  // all run
-    for (int i = threadIdx.x; i < p.blocks * p.stride; i += kThreads) {
-      const int cta = i / p.stride, e = i - cta * p.stride;
-      uint32_t to;
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(all + blockIdx.x * B200_MAX_EXPERTS + e)), "r"(cta));
-      asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(counts[e]) : "memory");
-    }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs run
+  for (int i = threadIdx.x; i < p.blocks * p.stride; i += kClusterThreads) {
+    const int cta = i / p.stride, e = i - cta * p.stride;
+    uint32_t to;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(&all[blockIdx.x][e])), "r"(cta));
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(counts[e]) : "memory");
   }
-  for (int e = threadIdx.x; e < p.experts; e += kThreads) {
-    int total = p.blocks > 1 ? 0 : counts[e], before = 0;
-    for (int b = 0; p.blocks > 1 && b < p.blocks; ++b) {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (threadIdx.x < (unsigned)p.experts) {
+    int total = 0, before = 0;
+    for (int b = 0; b < p.blocks; ++b) {
       if (b == (int)blockIdx.x) before = total;
-      total += all[b * B200_MAX_EXPERTS + e];
+      total += all[b][threadIdx.x];
     }
-    m.total[e] = total;
-    m.before[e] = before;
+    m.total[threadIdx.x] = total;
+    m.before[threadIdx.x] = before;
   }
   __syncthreads();
   place_block(p, first, end, blockIdx.x == 0, kept, m);
 }
-constexpr int kClusterBytes = (int)sizeof(PlaceMemory) + 4 * (kMaxCluster * B200_MAX_EXPERTS + B200_MAX_EXPERTS + kClusterChoices);
 
 int lanes_of(int experts) {
   int l = 1;
@@ -279,10 +319,9 @@ int lanes_of(int experts) {
 
 // Rows to a block: whole passes of its threads.  A cluster where its eight CTAs have few passes (KMEASURED).
 bool plan_blocks(RouteParams& p, int lanes) {
-  const int pass = kThreads / lanes;
-  const long long passes = ((long long)p.rows + pass - 1) / pass;
-  const long long few = (passes + kMaxCluster - 1) / kMaxCluster;
-  const bool cluster = few <= 2 && few * pass * p.top_k <= kClusterChoices;
+  const long long small = kClusterThreads / lanes, few = (p.rows + kMaxCluster * small - 1) / (kMaxCluster * small);
+  const bool cluster = few <= 2 && few * small * p.top_k <= kClusterChoices;
+  const long long pass = cluster ? small : kThreads / lanes, passes = (p.rows + pass - 1) / pass;
   const long long most = cluster ? kMaxCluster : kMaxBlocks, per = (passes + most - 1) / most;
   p.rows_per_block = (int)(per * pass);
   p.blocks = (int)((p.rows + per * pass - 1) / (per * pass));
@@ -295,14 +334,11 @@ cudaError_t launch_route(RouteParams p, cudaStream_t s) {
   const bool vec = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.ld % (16 / (int)sizeof(T)) == 0;
   cudaError_t e;
   if (plan_blocks(p, kLanes ? kLanes : 1)) {
-    auto kernel = route_cluster_kernel<T, kLanes>;
-    if ((e = raise_smem_limit<route_cluster_kernel<T, kLanes>>(kClusterBytes)) != cudaSuccess) return e;
     int size = 1;
     while (size < p.blocks) size *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(size);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kClusterBytes;
+    cfg.blockDim = dim3(kClusterThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -313,7 +349,7 @@ cudaError_t launch_route(RouteParams p, cudaStream_t s) {
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     p.blocks = size;
-    return cudaLaunchKernelEx(&cfg, kernel, p, vec);
+    return cudaLaunchKernelEx(&cfg, route_cluster_kernel<T, kLanes>, static_cast<const RouteParams&>(p), vec);
   }
   if ((e = launch_dependent(route_choose_kernel<T, kLanes>, dim3(p.blocks), dim3(kThreads), 0, s, p, vec)) != cudaSuccess) return e;
   return launch_dependent(route_order_kernel, dim3(p.blocks), dim3(kThreads), 0, s, p);
