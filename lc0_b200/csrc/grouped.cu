@@ -188,34 +188,24 @@ __global__ void __launch_bounds__(256) spread_rows_kernel(const GroupedParams p,
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, pieces = row_bytes / 16;
   const int end = expert_begin(p, p.experts);
-  // two rows per warp at a time
-  for (long long slot = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * 2; slot < end; slot += (long long)gridDim.x * 16) {
-    const uint4* from[2];
-    bool there[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int x = slot + k < end ? rows_of_slot(p, (int)slot + k).x : -1;
-      there[k] = x >= 0;
-      from[k] = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.X) + (x < 0 ? 0 : x) * p.ldx * size);
-    }
+  for (long long slot = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); slot < end; slot += (long long)gridDim.x * 8) {
+    const int x = rows_of_slot(p, (int)slot).x;
+    if (x < 0) continue;
+    const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.X) + x * p.ldx * size);
     uint4* at = reinterpret_cast<uint4*>(to + slot * row_bytes);
-#pragma unroll 2
-    for (int i = lane; i < pieces; i += 32) {
-      uint4 v[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (there[k]) v[k] = from[k][i];
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (there[k]) at[k * pieces + i] = v[k];
-    }
+#pragma unroll 4
+    for (int i = lane; i < pieces; i += 32) at[i] = from[i];
   }
 }
 
 // Rows of X and W that TMA can read.
 bool tma_rows(int K, long long ldx, long long ldw, int size) { return K * (long long)size % 16 == 0 && ldx * size % 16 == 0 && ldw * size % 16 == 0; }
-// The pair kernel's 256 slots pay from half a tile per expert on.
-bool many_rows(int slots, int experts) { return slots / (experts < slots ? experts : slots) > 64; }
+// The pair kernel's 256 slots pay from a quarter of a tile per expert on, and where the other kernel's tiles of 64 slots x 128 columns are more than
+// half of the SMs (K and N 1024, int8, us, pair kernel / the other: MIDDLE).
+bool many_rows(const GroupedParams& p, int sms) {
+  const int used = p.experts < p.slots ? p.experts : p.slots;
+  return p.slots / used > 64 && ((long long)p.slots / 64 + used / 2) * ceil_div(p.N, 128) > sms / 2;
+}
 // Beyond 16 rows per expert the other kernel, too, is ahead with rows in order, although the copy is a launch more.
 bool spreads(int slots, int experts) { return slots / (experts < slots ? experts : slots) > 16; }
 
@@ -229,9 +219,9 @@ int run_grouped(GroupedParams p, bool exact_sums, void* spread, cudaStream_t s) 
   B200_CUDA(gemm_tc_init());
   B200_CUDA(cudaGetDevice(&dev));
   B200_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  const bool pairs = !exact_sums && many_rows(p.slots, p.experts), in_place = !p.order || p.x_by_slot || (!pairs && !spreads(p.slots, p.experts));
+  const bool pairs = !exact_sums && many_rows(p, sms), in_place = !p.order || p.x_by_slot || (!pairs && !spreads(p.slots, p.experts));
   if (!in_place) {
-    const long long blocks = ((long long)p.slots + 15) / 16;
+    const long long blocks = ((long long)p.slots + 7) / 8;
     B200_CUDA(launch_dependent(spread_rows_kernel, dim3((unsigned)(blocks < sms * 8 ? blocks : sms * 8)), dim3(256), 0, s, p, static_cast<uint8_t*>(spread),
                                p.K * (int)sizeof(TIn), (int)sizeof(TIn)));
     p.X = spread;

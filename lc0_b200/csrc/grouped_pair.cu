@@ -99,9 +99,15 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   grid_launch_dependents();  // not ahead of the tensor memory: a dependent that took it would hold it while it waits for this kernel
-  TileWalk<2 * BM> walk{first, begin, p.experts, n_tiles};
-  const int tiles = walk.total();
-  int s0, end, n0;
+  TileWalk<2 * BM, BN> walk{first, begin, p.experts, n_tiles};
+  int tiles = walk.whole();
+  const int last = tiles % pairs;
+  if (BN == 256 && 2 * last <= pairs) {  // a last wave that at most half of the pairs have a tile of: half a tile each (TAIL)
+    walk.split = tiles - last;
+    tiles += last;
+  }
+  // columns that the MMA computes: the tile's, or what is left of N rounded up to 32
+  auto columns = [&]() { return max(32, min(walk.width, (p.N - walk.n0 + 31) & ~31)); };
 
   if (warp == 0) {
     // ---------------- TMA producer (both CTAs): W, and X where its rows lie in order ----------------
@@ -110,15 +116,14 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       uint32_t ph = 0;
       bool ok = true;
       for (int t = pair; t < tiles && ok; t += pairs) {
-        walk.at(t, BN, s0, end, n0);
-        s0 += (int)rank * BM;
-        const int w_row = walk.e * p.N + n0 + (int)rank * (min(BN, (p.N - n0 + 31) & ~31) / 2);
+        walk.at(t);
+        const int x_row = walk.s0 + (int)rank * BM, w_row = walk.e * p.N + walk.n0 + (int)rank * (columns() / 2);
         for (int kb = 0; kb < k_blocks; ++kb) {
           if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 1)) { ok = false; break; }
           const uint32_t fb_local = smem_u32(&full_bar[s]);
           const uint32_t fb = mapa(fb_local, 0), sa = smem_u32(smem + s * Cfg::kStageBytes);
           if (rank == 0) mbar_expect_tx(fb_local, 2 * Cfg::kStageBytes);
-          tma_load_2d_pair(sa, &map_x, kb * Operand<TIn>::k, s0, fb);
+          tma_load_2d_pair(sa, &map_x, kb * Operand<TIn>::k, x_row, fb);
           tma_load_2d_pair(sa + BM * 128, &map_w, kb * Operand<TIn>::k, w_row, fb);
           if (++s == S) { s = 0; ph ^= 1; }
         }
@@ -131,8 +136,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       uint32_t ph = 0, tile_it = 0;
       bool ok = true;
       for (int t = pair; t < tiles && ok; t += pairs, ++tile_it) {
-        const int left = p.N - (t % n_tiles) * BN;
-        const uint32_t idesc = Operand<TIn>::idesc | ((uint32_t)((2 * BM) >> 4) << 24) | ((uint32_t)(min(BN, (left + 31) & ~31) >> 3) << 17);
+        walk.at(t);
+        const uint32_t idesc = Operand<TIn>::idesc | ((uint32_t)((2 * BM) >> 4) << 24) | ((uint32_t)(columns() >> 3) << 17);
         const uint32_t acc = tile_it & 1, aph = (tile_it >> 1) & 1;
         if (!mbar_wait(smem_u32(&tempty_bar[acc]), aph ^ 1, abort_flag, 2)) break;
         tcgen05_fence_after();
@@ -190,14 +195,14 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     auto tile_of = [&](int t) {
       Tile x = {{-1, -1, 0}, 1.f, p.alpha, 0, 0};
       if (t >= tiles) return x;
-      walk.at(t, BN, s0, end, n0);
-      const int slot = s0 + (int)rank * BM + quarter * 32 + lane;
-      if (slot < end) x.r = rows_of_slot(p, slot);
+      walk.at(t);
+      const int slot = walk.s0 + (int)rank * BM + quarter * 32 + lane;
+      if (slot < walk.end) x.r = rows_of_slot(p, slot);
       if (x.r.c >= 0) {
         if (sizeof(TIn) == 1) x.sx = p.x_scales[x.r.x];
         if (p.weights) x.weight *= p.weights[x.r.choice];
       }
-      x.n = n0 + group * kSlab;
+      x.n = group * kSlab < walk.width ? walk.n0 + group * kSlab : p.N;  // (half a tile is two groups')
       x.wb = (long long)walk.e * p.N;
       return x;
     };
@@ -368,7 +373,9 @@ cudaError_t launch_tiles(const GroupedParams& p, int sm_count, cudaStream_t s) {
 
 template <typename TIn, typename TOut>
 cudaError_t launch_grouped_pair(const GroupedParams& p, int sm_count, cudaStream_t s) {
-  return p.N <= 128 ? launch_tiles<TIn, TOut, 128>(p, sm_count, s) : launch_tiles<TIn, TOut, 256>(p, sm_count, s);
+  // Narrow tiles where whole ones leave half of the pairs without any (2048x1024x1024 int8, us: NARROW).
+  const long long row_tiles = ((long long)p.slots + 2 * BM - 1) / (2 * BM) + ((p.experts < p.slots ? p.experts : p.slots) - 1) / 2;
+  return p.N <= 128 || 4 * row_tiles * ceil_div(p.N, 256) <= sm_count ? launch_tiles<TIn, TOut, 128>(p, sm_count, s) : launch_tiles<TIn, TOut, 256>(p, sm_count, s);
 }
 #define INSTANCE(TIn, TOut) template cudaError_t launch_grouped_pair<TIn, TOut>(const GroupedParams&, int, cudaStream_t)
 INSTANCE(__half, __half);

@@ -115,9 +115,9 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   grid_launch_dependents();  // not ahead of the tensor memory: a dependent that took it would hold it while it waits for this kernel
-  TileWalk<kRows> walk{first, begin, p.experts, n_tiles};
-  const int tiles = walk.total();
-  int s0 = 0, end = 0, n0 = 0;
+  TileWalk<kRows, BM> walk{first, begin, p.experts, n_tiles};
+  const int tiles = walk.whole();
+  const int &s0 = walk.s0, &end = walk.end, &n0 = walk.n0;
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
@@ -126,7 +126,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       uint32_t ph = 0;
       bool ok = true;
       for (int t = unit; t < tiles && ok; t += units) {
-        walk.at(t, BM, s0, end, n0);
+        walk.at(t);
         const int x_bytes = kGather ? (min(kRows, end - s0) + 3) / 4 * 512 : kRows * 128;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 1)) { ok = false; break; }
@@ -145,7 +145,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       uint32_t ph = 0, it = 0;  // it: accumulators filled
       bool ok = true;
       for (int t = unit; t < tiles && ok; t += units) {
-        walk.at(t, BM, s0, end, n0);
+        walk.at(t);
         const uint32_t idesc = Operand<TIn>::idesc | ((uint32_t)(BM >> 4) << 24) | ((uint32_t)(((min(kRows, end - s0) + 15) & ~15) >> 3) << 17);
         uint32_t d = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
@@ -175,7 +175,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       uint32_t done = 0;  // k-blocks before this tile's
       bool ok = true;
       for (int t = unit; t < tiles && ok; t += units, done += kb1 - kb0) {
-        walk.at(t, BM, s0, end, n0);
+        walk.at(t);
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -229,7 +229,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   if (warp >= 4) {
     uint32_t it = 0;
     for (int t = unit; t < tiles; t += units) {
-      walk.at(t, BM, s0, end, n0);
+      walk.at(t);
       rows = min(kRows, end - s0);
       n = n0 + column;
       // ks > 1: the slots that this CTA finishes; else all 64

@@ -51,19 +51,26 @@ __device__ __forceinline__ void list_tiles(const GroupedParams& p, int* first, i
   __syncthreads();
 }
 
-// A tile of the walk: its expert, the first slot and column.
-template <int kRows> struct TileWalk {
+// The tiles in the order they are computed: row tile by row tile, its column tiles of kCols.  Those from `split` on count twice, as a left and a right
+// half.
+template <int kRows, int kCols> struct TileWalk {
   const int* first;  // [experts + 1] row tiles ahead of each expert's
   const int* begin;  // [experts + 1] slots
-  int experts, n_tiles, e = 0;
-  __device__ __forceinline__ int total() const { return first[experts] * n_tiles; }
-  // t may only grow
-  __device__ __forceinline__ void at(int t, int bn, int& s0, int& end, int& n0) {
+  int experts, n_tiles, split = 0x7fffffff;
+  int e = 0, s0 = 0, end = 0, n0 = 0, width = kCols;  // of the tile last asked for: its expert, slots from s0 on below `end`, columns
+  __device__ __forceinline__ int whole() const { return first[experts] * n_tiles; }
+  __device__ __forceinline__ void at(int t) {  // t may only grow
+    int right = 0;
+    if (t >= split) {
+      right = (t - split) & 1;
+      t = split + ((t - split) >> 1);
+      width = kCols / 2;
+    }
     const int mt = t / n_tiles;
     while (first[e + 1] <= mt) ++e;
     s0 = begin[e] + (mt - first[e]) * kRows;
     end = begin[e + 1];
-    n0 = (t - mt * n_tiles) * bn;
+    n0 = (t - mt * n_tiles) * kCols + right * (kCols / 2);
   }
 };
 
