@@ -2076,6 +2076,25 @@ cudaError_t tma_encode_rows(const void* ptr, long long ld, long long rows, int c
   return cudaSuccess;
 }
 
+cudaError_t tma_encode_out(void* ptr, long long ld, long long rows, int cols, int prec, void* out) {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  if (!g_encode) return cudaErrorNotReady;
+  const int size = prec == 0 ? 4 : 2;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * size};
+  cuuint32_t box[2] = {(cuuint32_t)(64 / size), 32};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = g_encode(reinterpret_cast<CUtensorMap*>(out),
+                        prec == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : prec == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dims,
+                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with CUresult " + std::to_string((int)r));
+    return cudaErrorInvalidValue;
+  }
+  return cudaSuccess;
+}
+
 cudaError_t gemm_f32_map(const float* ptr, long long ld, int rows, int cols, bool board, CUtensorMap* out) {
   std::lock_guard<std::mutex> lock(g_mutex);
   if (!g_encode) return cudaErrorNotReady;

@@ -43,6 +43,7 @@ __global__ void __launch_bounds__(256) grouped_any_kernel(const GroupedParams p)
     if (tid < kTile) {
       SlotRows r = {-1, -1, 0};
       if (s0 + tid < end) r = rows_of_slot(p, s0 + tid);
+      if (n0 == 0) keep_place(p, r, s0 + tid);
       x_row[tid] = r.x; c_row[tid] = r.c; choice_of[tid] = r.choice;
     }
     __syncthreads();
@@ -99,12 +100,20 @@ cudaError_t launch_any(const GroupedParams& p, cudaStream_t s) {
 
 // ---- the sum over a token's choices -----------------------------------------------------------------------------
 struct CombineParams {
-  const float* Y;  // [tokens * top_k][N] by choice
+  const float* Y;    // [tokens * top_k][N] by slot
+  const int* place;  // of each choice, in requests
   const int* ids;
   const void* res; long long ldres;
   void* C; long long ldc;
   int tokens, N, experts, top_k, group;
 };
+
+// The place of a request's choice, -1 where it has no expert (or order does not name it, which is the caller's to rule out).
+__device__ __forceinline__ int place_of(const CombineParams& p, int request, int j) {
+  const long long choice = (long long)request * p.top_k + j;
+  const int id = __ldg(p.ids + choice), at = __ldg(p.place + choice);
+  return id >= 0 && id < p.experts && at >= 0 && at < p.tokens / p.group * p.top_k ? at : -1;
+}
 
 // A warp per token and 512 columns: two pieces of eight columns per lane, whose rows of all choices are on their way together; the choices are
 // added in order.
@@ -127,10 +136,10 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p, int
       bool any = false;
 #pragma unroll 2
       for (int j = 0; j < p.top_k; ++j) {
-        const int id = __ldg(p.ids + (long long)request * p.top_k + j);
-        if (id < 0 || id >= p.experts) continue;
+        const int at = place_of(p, request, j);
+        if (at < 0) continue;
         any = true;
-        const float* y = p.Y + (((long long)request * p.top_k + j) * p.group + inside) * p.N + n0;
+        const float* y = p.Y + ((long long)at * p.group + inside) * p.N + n0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (n0 + 256 * h >= p.N) continue;
@@ -153,16 +162,13 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p, int
       }
     } else {
       bool any = false;
-      for (int j = 0; j < p.top_k; ++j) {
-        const int id = p.ids[(long long)request * p.top_k + j];
-        any |= id >= 0 && id < p.experts;
-      }
+      for (int j = 0; j < p.top_k; ++j) any |= place_of(p, request, j) >= 0;
       if (!any) continue;
       for (int n = n0 - 7 * lane; n < min(n0 - 8 * lane + 512, p.N); n += 32) {  // column by column
         float v = 0.f;
         for (int j = 0; j < p.top_k; ++j) {
-          const int id = p.ids[(long long)request * p.top_k + j];
-          if (id >= 0 && id < p.experts) v += p.Y[(((long long)request * p.top_k + j) * p.group + inside) * p.N + n];
+          const int at = place_of(p, request, j);
+          if (at >= 0) v += p.Y[((long long)at * p.group + inside) * p.N + n];
         }
         c[n] = one_of<TOut>(res ? v + to_f(res[n]) : v);
       }
@@ -239,7 +245,8 @@ int size_of(int precision) { return precision == B200_PREC_FP32 ? 4 : 2; }
 
 // Choices are summed by a launch of their own, from fp32 rows in the workspace.
 bool sums_choices(const b200_experts_desc& d) { return !d.c_by_slot && d.top_k > 1; }
-size_t sums_bytes(const b200_experts_desc& d) { return sums_choices(d) ? round256((size_t)d.M * d.top_k * d.N * 4) : 0; }
+size_t place_bytes(const b200_experts_desc& d) { return round256((size_t)(d.M / d.group) * d.top_k * 4); }
+size_t sums_bytes(const b200_experts_desc& d) { return sums_choices(d) ? round256((size_t)d.M * d.top_k * d.N * 4) + place_bytes(d) : 0; }
 // X in the order of the slots.
 size_t spread_bytes(const b200_experts_desc& d) {
   const int size = d.int8 ? 1 : 2;
@@ -349,7 +356,8 @@ extern "C" int b200_op_gemm_experts(const b200_experts_desc* d, void* stream) {
     if (!sums) { p.res = d->res; p.ldres = d->ldres ? d->ldres : d->N; }
     p.alpha = 1.f; p.weights = d->weights; p.order = d->order; p.offsets = d->offsets;
     p.slots = d->M * d->top_k; p.N = d->N; p.K = d->K; p.experts = d->n_experts; p.top_k = d->top_k; p.group = d->group; p.act = d->activation;
-    p.x_by_slot = d->x_by_slot; p.c_by_slot = d->c_by_slot; p.by_choice = sums;
+    p.x_by_slot = d->x_by_slot; p.c_by_slot = d->c_by_slot || sums;
+    if (sums) p.place = reinterpret_cast<int*>(static_cast<char*>(d->workspace) + sums_bytes(*d) - place_bytes(*d));
     p.status = d->status;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     DependentLaunches dependent;
@@ -367,7 +375,7 @@ extern "C" int b200_op_gemm_experts(const b200_experts_desc* d, void* stream) {
     }
     if (rc != B200_OK || !sums) return rc;
     CombineParams c = {};
-    c.Y = static_cast<const float*>(d->workspace); c.ids = d->ids; c.res = d->res; c.ldres = d->ldres ? d->ldres : d->N;
+    c.Y = static_cast<const float*>(d->workspace); c.place = p.place; c.ids = d->ids; c.res = d->res; c.ldres = d->ldres ? d->ldres : d->N;
     c.C = d->C; c.ldc = d->ldc ? d->ldc : d->N; c.tokens = d->M; c.N = d->N; c.experts = d->n_experts; c.top_k = d->top_k; c.group = d->group;
     if (f32) B200_CUDA(launch_combine<float>(c, s));
     else if (d->precision == B200_PREC_FP16) B200_CUDA(launch_combine<__half>(c, s));

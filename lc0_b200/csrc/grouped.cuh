@@ -5,7 +5,8 @@
 namespace b200 {
 
 // v[slot][n] = act(scales * (X[x_row(slot)] . W[e]^T) + bias[e][n]) with the slot's expert e; see b200_op_gemm_experts and b200_op_gemm_int8.
-// The output is alpha * weight * v + res, stored by token, by slot, or by choice (`sums`, fp32, which combine_kernel adds up).
+// The output is alpha * weight * v + res, stored by token or by slot.  Where a token's choices are summed they are stored by slot in fp32, and
+// `place` learns the slot of each choice for combine_kernel.
 struct GroupedParams {
   const void* X; long long ldx; int x_rows;
   const void* W; long long ldw;
@@ -17,7 +18,8 @@ struct GroupedParams {
   const int* order; const int* offsets;  // null: one group, all slots in order
   int slots;                             // rows of choices there may be (M * top_k)
   int N, K, experts, top_k, group, act;
-  int x_by_slot, c_by_slot, by_choice;
+  int x_by_slot, c_by_slot;
+  int* place;  // [choices] or nullptr
   int* status;
 };
 
@@ -37,9 +39,13 @@ __device__ __forceinline__ SlotRows rows_of_slot(const GroupedParams& p, int slo
   if (choice < 0 || choice >= p.slots / p.group) return {-1, -1, 0};
   const int token = (p.top_k == 1 ? choice : choice / p.top_k) * p.group + i;
   r.x = p.x_by_slot ? slot : token;
-  r.c = p.c_by_slot ? slot : p.by_choice ? choice * p.group + i : token;
+  r.c = p.c_by_slot ? slot : token;
   r.choice = choice;
   return r;
+}
+// Kept by whichever thread has the slot's rows in hand for the first column.
+__device__ __forceinline__ void keep_place(const GroupedParams& p, const SlotRows& r, int slot) {
+  if (p.place && r.c >= 0) p.place[r.choice] = slot / p.group;
 }
 // offsets[e] in slots, held within what there is.
 __device__ __forceinline__ int expert_begin(const GroupedParams& p, int e) {

@@ -5,8 +5,9 @@
 //   warp 0      TMA producer
 //   warp 1      tcgen05.mma issuer (even CTA), kind::f16 or kind::i8, two accumulators in tensor memory
 //   warps 4-19  epilogue: four groups of four warps, 64 bytes of each of a warp's 32 rows at a time: tensor memory -> scales, bias, activation,
-//               weight, residual -> the warp's own staging buffer -> whole 64-byte pieces of the rows.  Rows behind the expert's last are not
-//               stored, which a TMA store of the tile could not leave out.
+//               weight, residual -> the warp's own staging buffer -> a TMA store where the 32 rows lie in order and are all this expert's, else
+//               64-byte pieces of those rows that are.  The epilogue is bound by the wavefronts of shared memory that it shares with
+//               the operands; a TMA store spares it those of reading the buffer and of writing line by line (STORES).
 // Every wait is bounded by wall-clock time like those of gemm_tc.cu.
 #include "chunk8.cuh"
 #include "grouped_tc.cuh"
@@ -48,7 +49,8 @@ template <int BN> struct GroupedPairCfg {
 
 template <typename TIn, typename TOut, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg<BN>::kThreads, 1)
-grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const GroupedParams p, int vec) {
+grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_c,
+                    const GroupedParams p, int vec, int boxes) {
   using Cfg = GroupedPairCfg<BN>;
   const int S = Cfg::kMaxStages - (p.res ? 1 : 0);
   constexpr int kCols = 64 / (int)sizeof(TOut);  // columns of a 64-byte piece of an output row
@@ -75,6 +77,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   if (threadIdx.x == 64) {
     tma_prefetch_map(&map_x);
     tma_prefetch_map(&map_w);
+    if (boxes) tma_prefetch_map(&map_c);
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
@@ -189,20 +192,23 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     struct Tile {
       SlotRows r;
       float sx, weight;
-      int n;  // the first column of the group's slab
+      int n;     // the first column of the group's slab
+      int row0;  // the first of the warp's slots
       long long wb;
     };
     auto tile_of = [&](int t) {
-      Tile x = {{-1, -1, 0}, 1.f, p.alpha, 0, 0};
+      Tile x = {{-1, -1, 0}, 1.f, p.alpha, 0, 0, 0};
       if (t >= tiles) return x;
       walk.at(t);
       const int slot = walk.s0 + (int)rank * BM + quarter * 32 + lane;
       if (slot < walk.end) x.r = rows_of_slot(p, slot);
+      if (walk.n0 == 0 && group == 0) keep_place(p, x.r, slot);
       if (x.r.c >= 0) {
         if (sizeof(TIn) == 1) x.sx = p.x_scales[x.r.x];
         if (p.weights) x.weight *= p.weights[x.r.choice];
       }
       x.n = group * kSlab < walk.width ? walk.n0 + group * kSlab : p.N;  // (half a tile is two groups')
+      x.row0 = slot - lane;
       x.wb = (long long)walk.e * p.N;
       return x;
     };
@@ -215,6 +221,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       const uint32_t acc = tile_it & 1, aph = (tile_it >> 1) & 1;
       const Tile x = next;
       const bool any = __any_sync(0xffffffffu, x.r.c >= 0) && x.n < p.N;
+      const bool box = boxes && __all_sync(0xffffffffu, x.r.c >= 0);  // the warp's rows are 32 in order, all of them this expert's
       vec_b[lane] = b0;
       vec_b[32 + lane] = b1;
       if (sizeof(TIn) == 1) {
@@ -240,6 +247,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         if (res) {
           if (vec) {
             uint8_t* other = buffers + (buf ^ 1) * 2048;
+            if (lane == 0) tma_store_wait_read0();  // (of the piece before this one)
+            __syncwarp();
             const bool here = i + 1 < kPieces && n + kCols < p.N;
             if (here) copy_res(other, x.r.c, n + kCols);
             else if (any_next) copy_res(other, next.r.c, next.n), copied = true;
@@ -287,6 +296,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] *= x.weight;
           }
+          if (q == 0 && !res) {
+            if (lane == 0) tma_store_wait_read0();  // the piece before this one has left the buffer
+            __syncwarp();
+          }
 #pragma unroll
           for (int j = 0; j < 16; j += kPer) {
             uint4* place = reinterpret_cast<uint4*>(at(buffer, lane, (q + j) / kPer));
@@ -314,8 +327,14 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             *place = out;
           }
         }
+        if (box) fence_async_smem();
         __syncwarp();
-        if (vec) {
+        if (box) {
+          if (lane == 0) {
+            tma_store_2d(&map_c, n, x.row0, smem_u32(buffer));
+            tma_store_commit();
+          }
+        } else if (vec) {
 #pragma unroll
           for (int it = 0; it < 4; ++it) {
             const int c = __shfl_sync(0xffffffffu, x.r.c, it * 8 + sub), col = n + part * kPer;
@@ -336,6 +355,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       if (lane == 0) mbar_arrive_cluster(mapa(smem_u32(&tempty_bar[acc]), 0));
     }
     cp_async_wait<0>();
+    if (lane == 0) tma_store_wait_all0();
   }
 
   __syncwarp();
@@ -356,17 +376,19 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 template <typename TIn, typename TOut, int BN>
 cudaError_t launch_tiles(const GroupedParams& p, int sm_count, cudaStream_t s) {
   using Cfg = GroupedPairCfg<BN>;
-  CUtensorMap mx, mw;
+  CUtensorMap mx, mw, mc = {};
   cudaError_t e = tma_encode_rows(p.X, p.ldx, p.slots, p.K, BM, Operand<TIn>::prec, &mx);
   if (e == cudaSuccess) e = tma_encode_rows(p.W, p.ldw, (long long)p.experts * p.N, p.K, BN / 2, Operand<TIn>::prec, &mw);
   if (e == cudaSuccess) e = raise_smem_limit<grouped_pair_kernel<TIn, TOut, BN>>(Cfg::smem_bytes(false) > Cfg::smem_bytes(true) ? Cfg::smem_bytes(false) : Cfg::smem_bytes(true));
   if (e != cudaSuccess) return e;
   const int per = 16 / (int)sizeof(TOut);
   const int vec = p.N % per == 0 && p.ldc % per == 0 && aligned16(p.C) && (!p.res || (p.ldres % per == 0 && aligned16(p.res)));
+  const int boxes = vec && (!p.order || p.c_by_slot);  // rows of C in the order of the slots
+  if (boxes && (e = tma_encode_out(p.C, p.ldc, p.slots, p.N, TypeTag<TOut>::prec, &mc)) != cudaSuccess) return e;
   const long long row_tiles = ((long long)p.slots + 2 * BM - 1) / (2 * BM) + (p.experts < p.slots ? p.experts : p.slots) - 1;
   const long long tiles = row_tiles * ceil_div(p.N, BN);
   const int pairs = (int)(tiles < sm_count / 2 ? tiles : sm_count / 2);
-  return launch_dependent(grouped_pair_kernel<TIn, TOut, BN>, dim3(2 * pairs), dim3(Cfg::kThreads), Cfg::smem_bytes(p.res != nullptr), s, mx, mw, p, vec);
+  return launch_dependent(grouped_pair_kernel<TIn, TOut, BN>, dim3(2 * pairs), dim3(Cfg::kThreads), Cfg::smem_bytes(p.res != nullptr), s, mx, mw, mc, p, vec, boxes);
 }
 
 }  // namespace

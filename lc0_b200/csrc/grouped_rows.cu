@@ -240,6 +240,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       sx = 1.f;
       weight = p.alpha;
       if (slot < end) r = rows_of_slot(p, slot);
+      if (n0 == 0 && quarter == 0) keep_place(p, r, slot);
       if (r.c >= 0) {
         if (sizeof(TIn) == 1) sx = p.x_scales[r.x];
         if (p.weights) weight *= p.weights[r.choice];

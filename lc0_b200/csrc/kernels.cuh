@@ -134,6 +134,9 @@ cudaError_t tma_encode_2d(const void* ptr, long long ld, long long rows, int col
 // The same over rows of 128-byte pieces (64 16-bit entries, or 128 8-bit integers with prec 3), box of one piece x box_rows, 128-byte swizzle.
 cudaError_t tma_encode_rows(const void* ptr, long long ld, long long rows, int cols, int box_rows, int prec, void* out);
 
+// For stores: rows of fp32 (prec 0) or 16-bit entries, box of 64 bytes x 32 rows, 64-byte swizzle.
+cudaError_t tma_encode_out(void* ptr, long long ld, long long rows, int cols, int prec, void* out);
+
 // fp32 products and 3x3 convolutions on tensor cores (gemm_f32.cu), with W cut into pieces [3][...] ahead of time.
 cudaError_t launch_split_weights(const float* w, long long count, void* planes, cudaStream_t s);
 bool gemm_f32_supported(const GemmParams& p);
