@@ -286,27 +286,26 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
               v[j + 3] = __uint_as_float(a[j + 3]) + b.w;
             }
           }
-          if (n + q + 16 > p.N) {
+          if ((p.N & 3) != 0 && n + q + 16 > p.N) {  // (each branch here is one: as predicated instructions they cost what they do either way)
+            asm volatile("");
 #pragma unroll
             for (int j = 0; j < 16; ++j)
               if (n + q + j >= p.N) v[j] = 0.f;
           }
-          activate_columns<TOut>(v, p.act);
+          if (p.act != ACT_NONE) {
+            asm volatile("");
+            activate_columns<TOut>(v, p.act);
+          }
           if (scaled) {
+            asm volatile("");
 #pragma unroll
             for (int j = 0; j < 16; ++j) v[j] *= x.weight;
           }
-          if (q == 0 && !res) {
-            if (lane == 0) tma_store_wait_read0();  // the piece before this one has left the buffer
-            __syncwarp();
-          }
+          if (res) {
+            asm volatile("");
 #pragma unroll
-          for (int j = 0; j < 16; j += kPer) {
-            uint4* place = reinterpret_cast<uint4*>(at(buffer, lane, (q + j) / kPer));
-            uint4 out;
-            uint32_t* o = &out.x;
-            if (res) {
-              const uint4 have = *place;
+            for (int j = 0; j < 16; j += kPer) {
+              const uint4 have = *reinterpret_cast<const uint4*>(at(buffer, lane, (q + j) / kPer));
               const uint32_t* h = &have.x;
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
@@ -319,12 +318,20 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                 }
               }
             }
+          } else if (q == 0) {
+            if (lane == 0) tma_store_wait_read0();  // the piece before this one has left the buffer
+            __syncwarp();
+          }
+#pragma unroll
+          for (int j = 0; j < 16; j += kPer) {
+            uint4 out;
+            uint32_t* o = &out.x;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               if constexpr (sizeof(TOut) == 2) o[k] = two_of<TOut>(v[j + 2 * k], v[j + 2 * k + 1]);
               else o[k] = __float_as_uint(v[j + k]);
             }
-            *place = out;
+            *reinterpret_cast<uint4*>(at(buffer, lane, (q + j) / kPer)) = out;
           }
         }
         if (box) fence_async_smem();
