@@ -102,13 +102,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   grid_launch_dependents();  // not ahead of the tensor memory: a dependent that took it would hold it while it waits for this kernel
-  TileWalk<2 * BM, BN> walk{first, begin, p.experts, n_tiles};
-  int tiles = walk.whole();
-  const int last = tiles % pairs;
-  if (BN == 256 && 2 * last <= pairs) {  // a last wave that at most half of the pairs have a tile of: half a tile each (TAIL)
-    walk.split = tiles - last;
-    tiles += last;
-  }
+  TileWalk<2 * BM, BN> walk(first, begin, p.experts, n_tiles, pair, pairs, BN == 256 ? pairs : 0);
   // columns that the MMA computes: the tile's, or what is left of N rounded up to 32
   auto columns = [&]() { return max(32, min(walk.width, (p.N - walk.n0 + 31) & ~31)); };
 
@@ -118,8 +112,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int t = pair; t < tiles && ok; t += pairs) {
-        walk.at(t);
+      for (; walk.valid() && ok; walk.next()) {
         const int x_row = walk.s0 + (int)rank * BM, w_row = walk.e * p.N + walk.n0 + (int)rank * (columns() / 2);
         for (int kb = 0; kb < k_blocks; ++kb) {
           if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 1)) { ok = false; break; }
@@ -138,8 +131,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       int s = 0;
       uint32_t ph = 0, tile_it = 0;
       bool ok = true;
-      for (int t = pair; t < tiles && ok; t += pairs, ++tile_it) {
-        walk.at(t);
+      for (; walk.valid() && ok; walk.next(), ++tile_it) {
         const uint32_t idesc = Operand<TIn>::idesc | ((uint32_t)((2 * BM) >> 4) << 24) | ((uint32_t)(columns() >> 3) << 17);
         const uint32_t acc = tile_it & 1, aph = (tile_it >> 1) & 1;
         if (!mbar_wait(smem_u32(&tempty_bar[acc]), aph ^ 1, abort_flag, 2)) break;
@@ -180,7 +172,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       }
     };
     float b0 = 0.f, b1 = 0.f, w0 = 1.f, w1 = 1.f;  // bias and scale of columns lane and 32 + lane of the next tile's slab
-    auto fetch_vectors = [&](long long wb, int n) {
+    auto fetch_vectors = [&](int wb, int n) {
       const bool first = n + lane < p.N, second = kSlab > 32 && n + 32 + lane < p.N;
       b0 = p.bias && first ? __ldg(p.bias + wb + n + lane) : 0.f;
       b1 = p.bias && second ? __ldg(p.bias + wb + n + 32 + lane) : 0.f;
@@ -194,12 +186,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       float sx, weight;
       int n;     // the first column of the group's slab
       int row0;  // the first of the warp's slots
-      long long wb;
+      int wb;    // where the expert's vectors begin
     };
-    auto tile_of = [&](int t) {
-      Tile x = {{-1, -1, 0}, 1.f, p.alpha, 0, 0, 0};
-      if (t >= tiles) return x;
-      walk.at(t);
+    auto tile_at_hand = [&]() {
+      Tile x = {{-1, -1, 0}, 1.f, p.alpha, p.N, 0, 0};
+      if (!walk.valid()) return x;
       const int slot = walk.s0 + (int)rank * BM + quarter * 32 + lane;
       if (slot < walk.end) x.r = rows_of_slot(p, slot);
       if (walk.n0 == 0 && group == 0) keep_place(p, x.r, slot);
@@ -209,15 +200,16 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       }
       x.n = group * kSlab < walk.width ? walk.n0 + group * kSlab : p.N;  // (half a tile is two groups')
       x.row0 = slot - lane;
-      x.wb = (long long)walk.e * p.N;
+      x.wb = walk.e * p.N;
       return x;
     };
     uint32_t tile_it = 0;
     int buf = 0;
     bool copied = false;  // the residual of the next piece is in, or on its way to, its buffer
-    Tile next = tile_of(pair);
+    bool more = walk.valid();
+    Tile next = tile_at_hand();
     fetch_vectors(next.wb, next.n);
-    for (int t = pair; t < tiles; t += pairs, ++tile_it) {
+    for (; more; ++tile_it) {
       const uint32_t acc = tile_it & 1, aph = (tile_it >> 1) & 1;
       const Tile x = next;
       const bool any = __any_sync(0xffffffffu, x.r.c >= 0) && x.n < p.N;
@@ -228,7 +220,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         vec_w[lane] = w0;
         vec_w[32 + lane] = w1;
       }
-      next = tile_of(t + pairs);
+      walk.next();
+      more = walk.valid();
+      next = tile_at_hand();
       fetch_vectors(next.wb, next.n);
       const bool any_next = __any_sync(0xffffffffu, next.r.c >= 0) && next.n < p.N;
       if (res && vec && any && !copied) {

@@ -115,8 +115,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   grid_launch_dependents();  // not ahead of the tensor memory: a dependent that took it would hold it while it waits for this kernel
-  TileWalk<kRows, BM> walk{first, begin, p.experts, n_tiles};
-  const int tiles = walk.whole();
+  TileWalk<kRows, BM> walk(first, begin, p.experts, n_tiles, unit, units, 0);
   const int &s0 = walk.s0, &end = walk.end, &n0 = walk.n0;
 
   if (warp == 0) {
@@ -125,8 +124,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
-      for (int t = unit; t < tiles && ok; t += units) {
-        walk.at(t);
+      for (; walk.valid() && ok; walk.next()) {
         const int x_bytes = kGather ? (min(kRows, end - s0) + 3) / 4 * 512 : kRows * 128;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 1)) { ok = false; break; }
@@ -144,8 +142,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       int s = 0;
       uint32_t ph = 0, it = 0;  // it: accumulators filled
       bool ok = true;
-      for (int t = unit; t < tiles && ok; t += units) {
-        walk.at(t);
+      for (; walk.valid() && ok; walk.next()) {
         const uint32_t idesc = Operand<TIn>::idesc | ((uint32_t)(BM >> 4) << 24) | ((uint32_t)(((min(kRows, end - s0) + 15) & ~15) >> 3) << 17);
         uint32_t d = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
@@ -174,8 +171,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     if constexpr (kGather) {
       uint32_t done = 0;  // k-blocks before this tile's
       bool ok = true;
-      for (int t = unit; t < tiles && ok; t += units, done += kb1 - kb0) {
-        walk.at(t);
+      for (; walk.valid() && ok; walk.next(), done += kb1 - kb0) {
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -228,8 +224,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   };
   if (warp >= 4) {
     uint32_t it = 0;
-    for (int t = unit; t < tiles; t += units) {
-      walk.at(t);
+    for (; walk.valid(); walk.next()) {
       rows = min(kRows, end - s0);
       n = n0 + column;
       // ks > 1: the slots that this CTA finishes; else all 64
@@ -306,7 +301,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   if (ks == 1) return;
   if (!met) cluster_wait();
   cluster_sync_all();  // all sums have arrived
-  if (warp >= 4 && unit < tiles) {
+  if (warp >= 4 && rows > 0) {
     const int each = slots_each(rows, log_ks), count = min(each, rows - (int)rank * each);
     for (int j0 = half * 4; j0 < count; j0 += 8) {  // four slots of a warp at a time
       const uint4* from = reinterpret_cast<const uint4*>(part) + j0 * 32 + column;

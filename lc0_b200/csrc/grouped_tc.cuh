@@ -51,52 +51,102 @@ __device__ __forceinline__ void list_tiles(const GroupedParams& p, int* first, i
   __syncthreads();
 }
 
-// The tiles in the order they are computed: row tile by row tile, its column tiles of kCols.  Those from `split` on count twice, as a left and a right
-// half.
+// The tiles in the order they are computed, row tile by row tile, every `step`th of them.  Those from `split` on count twice, as a left and a right half of
+// their kCols columns.
 template <int kRows, int kCols> struct TileWalk {
   const int* first;  // [experts + 1] row tiles ahead of each expert's
   const int* begin;  // [experts + 1] slots
-  int experts, n_tiles, split = 0x7fffffff;
-  int e = 0, s0 = 0, end = 0, n0 = 0, width = kCols;  // of the tile last asked for: its expert, slots from s0 on below `end`, columns
-  __device__ __forceinline__ int whole() const { return first[experts] * n_tiles; }
-  __device__ __forceinline__ void at(int t) {  // t may only grow
-    int right = 0;
-    if (t >= split) {
-      right = (t - split) & 1;
-      t = split + ((t - split) >> 1);
+  int n_tiles, step, split, tiles;
+  int t, e = 0, s0 = 0, end = 0, n0 = 0, width = kCols;  // the tile at hand: its expert, slots from s0 on below `end`, columns
+  int mt, nt;
+  // split_pairs: a last round that at most half of these have a tile of is computed in half tiles; 0: never.
+  __device__ __forceinline__ TileWalk(const int* first_, const int* begin_, int experts, int n_tiles_, int start, int step_, int split_pairs)
+      : first(first_), begin(begin_), n_tiles(n_tiles_), step(step_), t(start) {
+    const int whole = first[experts] * n_tiles, last = split_pairs > 0 ? whole % split_pairs : 0;
+    const bool halves = split_pairs > 0 && 2 * last <= split_pairs;
+    split = halves ? whole - last : 0x7fffffff;
+    tiles = halves ? whole + last : whole;
+    mt = t / n_tiles;
+    nt = t - mt * n_tiles;
+    locate();
+  }
+  __device__ __forceinline__ bool valid() const { return t < tiles; }
+  __device__ __forceinline__ void next() {
+    t += step;
+    nt += step % n_tiles;
+    mt += step / n_tiles;
+    if (nt >= n_tiles) {
+      nt -= n_tiles;
+      ++mt;
+    }
+    locate();
+  }
+  __device__ __forceinline__ void locate() {
+    if (t >= tiles) return;
+    if (t < split) {
+      n0 = nt * kCols;
+    } else {
+      const int whole = split + ((t - split) >> 1);
+      mt = whole / n_tiles;
+      n0 = (whole - mt * n_tiles) * kCols + ((t - split) & 1) * (kCols / 2);
       width = kCols / 2;
     }
-    const int mt = t / n_tiles;
     while (first[e + 1] <= mt) ++e;
     s0 = begin[e] + (mt - first[e]) * kRows;
     end = begin[e + 1];
-    n0 = (t - mt * n_tiles) * kCols + right * (kCols / 2);
   }
 };
 
 // v e / (e + 1) with e = exp(v), and v n / (n + 2) with n = e (e + 2): four at a time share one reciprocal.  exp is held to exp(10) (Mish) and
-// exp(20), beyond which the quotient is 1 to 2^-27, so that the four denominators' product stays finite.  An epilogue of 65536x1024 columns
-// with a reciprocal each spent 121 us where one without an activation took 80.
+// exp(20), beyond which the quotient is 1 to 2^-27, so that the four denominators' product stays finite; arithmetic in pairs.  us, 65536x1536x1024
+// int8 with Mish: a reciprocal each, one by one MISHA, now MISHB; without an activation 88.
+__device__ __forceinline__ float exp2_quick(float x) {  // results below 2^-126 are 0, which nothing of these formulas shows
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_quick(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+struct Two {
+  uint64_t v;
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void parts(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+  return a;
+}
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.v) : "l"(b.v));
+  return a;
+}
+constexpr float kLog2e = 1.44269504f;
 template <bool kMish> __device__ __forceinline__ void gate4(float* v) {
-  float n[4], d[4];
+  constexpr float kMost = kMish ? 10.f : 20.f;
+  float d[4];
+  Two n[2] = {Two(0.f, 0.f), Two(0.f, 0.f)};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float e = __expf(fminf(v[i], kMish ? 10.f : 20.f));
-    n[i] = kMish ? e * (e + 2.f) : e;
-    d[i] = n[i] + (kMish ? 2.f : 1.f);
+  for (int i = 0; i < 2; ++i) {
+    float a, b;
+    (Two(fminf(v[2 * i], kMost), fminf(v[2 * i + 1], kMost)) * Two(kLog2e, kLog2e)).parts(a, b);
+    const Two e(exp2_quick(a), exp2_quick(b));
+    n[i] = kMish ? e * (e + Two(2.f, 2.f)) : e;
+    (n[i] + (kMish ? Two(2.f, 2.f) : Two(1.f, 1.f))).parts(d[2 * i], d[2 * i + 1]);
   }
-  const float d01 = d[0] * d[1], d23 = d[2] * d[3], r = __fdividef(1.f, d01 * d23), r01 = r * d23, r23 = r * d01;
-  v[0] *= n[0] * (r01 * d[1]);  // (a row's columns share it, whose number does not depend on the batch)
-  v[1] *= n[1] * (r01 * d[0]);
-  v[2] *= n[2] * (r23 * d[3]);
-  v[3] *= n[3] * (r23 * d[2]);
+  const float d01 = d[0] * d[1], d23 = d[2] * d[3], r = reciprocal_quick(d01 * d23), r01 = r * d23, r23 = r * d01;
+  // (a row's columns share it, whose number does not depend on the batch)
+  (Two(v[0], v[1]) * (n[0] * (Two(r01, r01) * Two(d[1], d[0])))).parts(v[0], v[1]);
+  (Two(v[2], v[3]) * (n[1] * (Two(r23, r23) * Two(d[3], d[2])))).parts(v[2], v[3]);
 }
 
 // The same with the four columns in neighbouring lanes: the same products, so the same bits.
 template <bool kMish> __device__ __forceinline__ float gate_lane(float v) {
-  const float e = __expf(fminf(v, kMish ? 10.f : 20.f)), n = kMish ? e * (e + 2.f) : e, d = n + (kMish ? 2.f : 1.f);
+  const float e = exp2_quick(fminf(v, kMish ? 10.f : 20.f) * kLog2e), n = kMish ? __fmul_rn(e, __fadd_rn(e, 2.f)) : e, d = __fadd_rn(n, kMish ? 2.f : 1.f);
   const float other = __shfl_xor_sync(0xffffffffu, d, 1), both = d * other, far = __shfl_xor_sync(0xffffffffu, both, 2);
-  return v * (n * (__fdividef(1.f, both * far) * far * other));
+  return v * (n * (reciprocal_quick(both * far) * far * other));
 }
 
 // By all lanes of a warp, four neighbours having columns 4i .. 4i + 3 of each of kN rows (0 behind the last column).
