@@ -448,7 +448,7 @@ void b200_op_sample_inject_give_up(int cta, int wait);
 /* ---- Operators of encoder layers in 8 bits, with experts, with normalised heads -----------------------------------------------
  * All allocate nothing, do not synchronise and may be captured; index lists are read on the device, a captured call follows what
  * they hold when it is replayed.  Outputs may not overlap inputs but where it says so.  Leading dimensions of 0 mean dense.  status:
- * device int or NULL, set non-zero (and never cleared) if a bounded device-side wait gave up, the result is then undefined.
+ * device int or NULL, set non-zero (and never cleared) if a bounded device-side wait gave up, the result is then undefined.  fp16 results saturate.
  *
  * b200_op_quantize_rows: 8-bit rows with a scale each: scales[m] = max_k |X[m][k]| * fp32(1 / 127) and Q[m][k] = X[m][k] / scales[m], the exact
  *   quotient rounded to the nearest whole number (ties to even, at most 127 in size).  X [M][K] in `precision`; Q [M][K].  For activations (a scale
@@ -481,7 +481,7 @@ int b200_op_gemm_int8(const b200_gemm_int8_desc* d, void* stream);
  *     order[offsets[e] .. offsets[e + 1]).  What lies from order[offsets[n_experts]] on is left as it was.
  *   logits NULL: ids are given by the caller (entries not in [0, n_experts) have no expert) and sorted; weights has to be NULL.
  *   workspace: b200_op_route_workspace() bytes on a 256-byte boundary, for this call alone until it has run.
- *   n_experts 1 to B200_MAX_EXPERTS, top_k 1 to min(n_experts, B200_MAX_TOP_K); rows * top_k below 2^31. */
+ *   n_experts 1 to B200_MAX_EXPERTS, top_k 1 to min(n_experts, B200_MAX_TOP_K) (ids given: to B200_MAX_TOP_K); rows * top_k at most 2^30. */
 #define B200_MAX_EXPERTS 256
 #define B200_MAX_TOP_K 16
 typedef struct b200_route_desc {

@@ -88,6 +88,9 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
   const int n_tiles = (p.N + BM - 1) / BM, k_blocks = (p.K + Operand<TIn>::k - 1) / Operand<TIn>::k;
   const int kb0 = k_blocks * (int)rank >> log_ks, kb1 = k_blocks * ((int)rank + 1) >> log_ks;
 
+  // Waited for ahead of the first store to another CTA: that it runs.  Not behind the tensor memory, which a CTA then holds for no longer than its own
+  // products take: clusters that each wait for what another holds would wait for ever.
+  if (ks > 1) cluster_arrive();
   if (threadIdx.x == 64) {
     tma_prefetch_map(&map_x);
     tma_prefetch_map(&map_w);
@@ -108,7 +111,6 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)kTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (ks > 1) cluster_arrive();  // waited for ahead of the first store to another CTA: that it runs
   grid_dependency_wait();
   tcgen05_fence_before();
   list_tiles<kRows>(p, first, begin, scan);

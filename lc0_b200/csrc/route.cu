@@ -376,7 +376,7 @@ const char* check_shape(const b200_route_desc* d) {
   if (!d) return "no description";
   if (d->n_experts < 1 || d->n_experts > B200_MAX_EXPERTS) return "n_experts 1 to 256";
   if (d->top_k < 1 || d->top_k > B200_MAX_TOP_K || (d->top_k > d->n_experts && d->logits)) return "top_k 1 to 16 and at most n_experts";
-  if (d->rows < 0 || (long long)d->rows * d->top_k > 0x7fffffffll) return "rows * top_k of 0 to 2^31 - 1";
+  if (d->rows < 0 || (long long)d->rows * d->top_k > 1 << 30) return "rows * top_k of 0 to 2^30";
   if (d->precision < B200_PREC_FP32 || d->precision > B200_PREC_BF16) return "unknown precision";
   if (d->ld && d->ld < d->n_experts) return "rows overlap";
   return nullptr;

@@ -288,6 +288,44 @@ def test_residual_in_place_and_no_weights(lib, prec, requests, N, top_k):
 
 
 @gpu
+@pytest.mark.parametrize("requests", [20, 700])
+def test_weights_beyond_32_bits(lib, requests):
+    """The last expert's weights lie more than 2^32 behind the first's."""
+    e, N, K = 70, 8192, 8192
+    c = Experts(lib, "head", requests, N, 64, 1, 1, 1, 1, int8=True, ids=torch.zeros(requests, 1))
+    w = torch.zeros(e, N, K, dtype=torch.int8, device="cuda")
+    w[-1].random_(-127, 128)
+    x = torch.randint(-127, 128, (requests, K), device="cuda").to(torch.int8)
+    sw, bias = torch.ones(e, N, device="cuda"), torch.zeros(e, N, device="cuda")
+    sw[-1], bias[-1] = c.sw[0] / 10, c.bias[0]
+    offsets = torch.zeros(e + 1, dtype=torch.int32, device="cuda")
+    offsets[-1] = requests
+    c.d.X, c.d.W, c.d.ldx, c.d.ldw, c.d.K, c.d.n_experts = x.data_ptr(), w.data_ptr(), K, K, K, e
+    c.d.w_scales, c.d.bias, c.d.offsets = sw.data_ptr(), bias.data_ptr(), offsets.data_ptr()
+    work = workspace(lib.b200_op_gemm_experts_workspace, c.d)
+    c.run()
+    c.x, c.w, c.sw, c.bias, c.K = x, w[-1], sw[-1:], bias[-1:], K
+    c.check()
+    assert (work[-64:] == 255).all()
+
+
+@gpu
+@pytest.mark.parametrize("requests,N,K,experts,top_k", [(3000, 512, 256, 4, 2), (300, 264, 128, 4, 2), (70, 136, 64, 40, 1)])
+def test_calls_at_once(lib, requests, N, K, experts, top_k):
+    """The same product on four streams at once, a workspace and outputs each, again and again."""
+    calls = [Experts(lib, "down", requests, N, K, experts, top_k, 1, 1 + i % 2, seed=i, res=True) for i in range(4)]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for c, st in zip(calls, streams):
+            _lib.check(lib.b200_op_gemm_experts(ctypes.byref(c.d), st.cuda_stream))
+    torch.cuda.synchronize()
+    for c in calls:
+        assert c.status.item() == 0
+        c.check()
+
+
+@gpu
 @pytest.mark.parametrize("int8", [False, True])
 def test_what_is_not_finite_stays_in_its_rows(lib, int8):
     """Another expert's weights and another request's rows, NaN or infinite, reach nobody else."""

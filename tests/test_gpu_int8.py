@@ -216,6 +216,26 @@ def test_rows_do_not_depend_on_their_number(lib):
 
 
 @gpu
+def test_offsets_beyond_32_bits(lib):
+    """Rows whose entries, and whose bytes, lie more than 2^32 behind the first."""
+    M, N, K = 600000, 4096, 32
+    p = Product(lib, 64, N, K, 1, res=False)
+    x, out = torch.zeros(M, K, dtype=torch.int8, device="cuda"), torch.empty(M, N, dtype=torch.float16, device="cuda")
+    sx = torch.ones(M, device="cuda")
+    x[-64:], sx[-64:] = p.x, p.sx
+    p.d.X, p.d.x_scales, p.d.C, p.d.M = x.data_ptr(), sx.data_ptr(), out.data_ptr(), M
+    p.run()
+    p.out = out[-64:]
+    p.check()
+    del out
+    wide = torch.empty(33000, 131072 // 2, dtype=torch.float16, device="cuda")
+    wide[-1].normal_()
+    wide[:-1] = 1
+    q, s = quantize(lib, wide)
+    assert torch.equal(q[-1:], quantized(wide[-1:])[0]) and torch.equal(s[-1:], quantized(wide[-1:])[1]) and (q[-2] == 127).all()
+
+
+@gpu
 def test_scales_that_are_not_numbers_stay_in_their_row_and_column(lib):
     for M in (64, 900):
         p = Product(lib, M, 300, 256, 1, res=False)

@@ -140,6 +140,20 @@ def test_zeros_and_what_is_not_finite(lib, depth, interleaved):
 
 
 @gpu
+def test_offsets_beyond_32_bits(lib):
+    rows = 560000
+    q = torch.ones(rows, 4096, dtype=torch.float16, device="cuda")
+    q[-64:].normal_()
+    c = Call(lib, 64, 32, 0, 128, 1, 128)
+    c.q_in = q[-64:].clone()
+    out = torch.empty_like(q)
+    c.d.q, c.d.q_out, c.d.ldq, c.d.ldq_out, c.d.rows = q.data_ptr(), out.data_ptr(), 4096, 4096, rows
+    c.run()
+    c.q, c.qo = q[-64:], out[-64:]
+    c.check()
+
+
+@gpu
 def test_captured_and_on_a_stream(lib):
     c = Call(lib, 640, 12, 12, 32, 1, 32)
     st = torch.cuda.Stream()
