@@ -28,16 +28,18 @@ template <typename T> __device__ __forceinline__ uint32_t largest8(const Chunk<T
 __device__ __noinline__ uint32_t tiny_q(float x, float s) { return (uint32_t)(int)fmin(fmax(rint((double)x / (double)s), -127.0), 127.0); }
 
 // x / s to the nearest whole number, in the low byte.  Adding 1.5 2^23 rounds the product with the reciprocal, which is off by 1e-5 at most, to r
-// or, beside a tie, to its neighbour.  e = x - r s is exact there (a multiple of half an ulp of s below s), so comparing it with s / 2 says which:
-// beyond it the neighbour is nearer, and at a tie the even one of the two is taken.  bf16 rows meet ties often, by the eight bits of their entries: with
-// these steps for chunks that have one alone, most warps took both ways (65536x1536 127 us).
+// or, beside a tie, to its neighbour.  e = x - r s is exact (r s and x are multiples of half an ulp of s or more, and beside a tie e is about s / 2), so
+// r + e / s is the quotient, and a second fma rounds r + e (1 / s): off by |e| 2^-24 < ulp(s) / 2 with the reciprocal's rounding, while what is
+// no tie is at least ulp(s) / 2 away from one.  Ties proper, |e| = s / 2, are told by comparing and go to the even of the two.
+// us at 65536x1536 bf16: remainders only for chunks beside a tie, which bf16's eight bits bring about in most 127; remainders compared with s / 2
+// entry by entry 60; now 51 (6.0 TB/s).
+__device__ __forceinline__ uint32_t nearer(uint32_t b, float e, float half) {  // b: r in its low byte
+  const float limit = __uint_as_float(__float_as_uint(half) + (~b & 1u));      // an even r keeps the tie
+  return fabsf(e) >= limit ? b + (uint32_t)((__float_as_int(e) >> 31) | 1) : b;
+}
 __device__ __forceinline__ uint32_t exact_q(float x, float s, float inv) {
   const float t = fmaf(x, inv, 12582912.f);
-  uint32_t b = __float_as_uint(t);
-  const float e = fmaf(12582912.f - t, s, x);
-  const float limit = __uint_as_float(__float_as_uint(0.5f * s) + (~b & 1u));  // an even r keeps the tie
-  if (fabsf(e) >= limit) b += (uint32_t)((__float_as_int(e) >> 31) | 1);
-  return b;
+  return nearer(__float_as_uint(t), fmaf(12582912.f - t, s, x), 0.5f * s);
 }
 // Two at a time where the arithmetic comes in pairs.
 __device__ __forceinline__ uint64_t two(float a, float b) {
@@ -50,27 +52,23 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-__device__ __forceinline__ uint32_t nearer(uint32_t b, float e, uint32_t half) {
-  const float limit = __uint_as_float(half + (~b & 1u));
-  if (fabsf(e) >= limit) b += (uint32_t)((__float_as_int(e) >> 31) | 1);
-  return b;
-}
 __device__ __forceinline__ uint2 quantize8(const float (&v)[8], float s, float inv) {
   uint32_t b[8];
   const uint64_t inv2 = two(inv, inv), s2 = two(s, s), magic = two(12582912.f, 12582912.f), minus = two(-1.f, -1.f);
-  const uint32_t half = __float_as_uint(0.5f * s);
+  const float half = 0.5f * s;
+  bool tie = inv == 0.f;  // (no usable reciprocal)
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
-    const uint64_t x2 = two(v[i], v[i + 1]), t2 = fma2(x2, inv2, magic), e2 = fma2(fma2(t2, minus, magic), s2, x2);
+    const uint64_t x2 = two(v[i], v[i + 1]), t2 = fma2(x2, inv2, magic), e2 = fma2(fma2(t2, minus, magic), s2, x2), u2 = fma2(e2, inv2, t2);
     float e0, e1;
-    asm("mov.b64 {%0, %1}, %2;" : "=r"(b[i]), "=r"(b[i + 1]) : "l"(t2));
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(b[i]), "=r"(b[i + 1]) : "l"(u2));
     asm("mov.b64 {%0, %1}, %2;" : "=f"(e0), "=f"(e1) : "l"(e2));
-    b[i] = nearer(b[i], e0, half);
-    b[i + 1] = nearer(b[i + 1], e1, half);
+    tie = tie || fabsf(e0) == half || fabsf(e1) == half;
   }
-  if (inv == 0.f) {
+  if (tie) {
+    asm volatile("");
 #pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = tiny_q(v[i], s);
+    for (int i = 0; i < 8; ++i) b[i] = inv == 0.f ? tiny_q(v[i], s) : exact_q(v[i], s, inv);
   }
   uint2 q;
   q.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
@@ -100,7 +98,7 @@ template <typename T> __device__ __forceinline__ Chunk<T> load8_once(const T* p)
 
 // A row in the registers of kThreads threads, kPer chunks of eight entries each; the next row is on its way meanwhile.
 //   Many rows: a warp each, as many as fit, each walking over its rows (us, a warp for one row and the next CTA behind it / now: 65536x1536 bf16
-//   69 / 60, 65536x1024 fp32 62 / 53: 5.0 and 6.3 TB/s of 6.55).
+//   57 / 51, 65536x1024 fp32 62 / 53: 6.0 and 6.3 TB/s of 6.55).
 //   Few rows: four warps each, so that a thread has one or two chunks (64x1024 1.2 us in a chain of launches).
 template <typename T, int kPer, int kThreads>
 __global__ void __launch_bounds__(128) quantize_rows_kernel(const T* X, long long ldx, int M, int K, int8_t* Q, long long ldq, float* scales) {
