@@ -187,8 +187,8 @@ cudaError_t launch_combine(const CombineParams& p, cudaStream_t s) {
 // ---- rows in the order of their slots ---------------------------------------------------------------------------
 // The pair kernel reads X by boxes of 128 rows, so rows that the order names are copied into their order first, once for all tiles of
 // columns, which then find them in L2.  Fetched in place by TMA's gather4, 33 cycles for four rows and anew for each tile of columns, the
-// product takes half as long again: us, 32768 slots x 1024 to 1536 columns, Mish: 161, now NOW; int8, 18000 slots: 71, now NOW8.  (By cp.async into the
-// swizzled tiles 325: the proxy fence ahead of each hand-over waits for all copies in flight.)
+// product takes half as long again (us, 32768 slots x 1024 to 1536 columns: 136, in order with the copy 102; by cp.async into the swizzled
+// tiles 318, as the proxy fence ahead of each hand-over waits for all copies in flight).
 __global__ void __launch_bounds__(256) spread_rows_kernel(const GroupedParams p, uint8_t* to, int row_bytes, int size) {
   grid_launch_dependents();
   grid_dependency_wait();
@@ -207,12 +207,14 @@ __global__ void __launch_bounds__(256) spread_rows_kernel(const GroupedParams p,
 // Rows of X and W that TMA can read.
 bool tma_rows(int K, long long ldx, long long ldw, int size) { return K * (long long)size % 16 == 0 && ldx * size % 16 == 0 && ldw * size % 16 == 0; }
 // The pair kernel's 256 slots pay from a quarter of a tile per expert on, and where the other kernel's tiles of 64 slots x 128 columns are more than
-// half of the SMs (K and N 1024, int8, us, pair kernel / the other: MIDDLE).
+// half of the SMs (K and N 1024, int8, us, pair kernel / the other: 128 rows 6.9 / 5.8, 256 6.9 / 6.1, 512 7.0 / 7.4, 1024 7.2 / 8.0, 2048
+// 7.5 / 12.5; 768 rows over 8 experts to 1536 columns 14.6 / 16.6).
 bool many_rows(const GroupedParams& p, int sms) {
   const int used = p.experts < p.slots ? p.experts : p.slots;
   return p.slots / used > 64 && ((long long)p.slots / 64 + used / 2) * ceil_div(p.N, 128) > sms / 2;
 }
-// Beyond 16 rows per expert the other kernel, too, is ahead with rows in order, although the copy is a launch more.
+// Beyond 16 rows per expert the other kernel, too, is ahead with rows in order, although the copy is a launch more (333 rows over 12 experts to 1858
+// columns 25.1 in place, 20.2).
 bool spreads(int slots, int experts) { return slots / (experts < slots ? experts : slots) > 16; }
 
 template <typename TIn, typename TOut>
@@ -258,7 +260,7 @@ size_t experts_bytes(const b200_experts_desc& d) { return sums_bytes(d) + spread
 
 const char* check_shape(const b200_experts_desc* d) {
   if (!d) return "no description";
-  if (d->N < 1 || d->K < 1 || d->K > (d->int8 ? B200_INT8_MAX_K : 0x7fffffff)) return "N >= 1 and K >= 1 (int8: at most 131071)";
+  if (d->N < 1 || d->K < 1 || d->K > B200_INT8_MAX_K) return "N >= 1 and K of 1 to 131071";
   if (d->n_experts < 1 || d->n_experts > B200_MAX_EXPERTS) return "n_experts 1 to 256";
   if (d->top_k < 1 || d->top_k > B200_MAX_TOP_K) return "top_k 1 to 16";
   if (d->group < 1 || d->M < 0 || d->M % d->group != 0) return "M is a multiple of group, which is at least 1";

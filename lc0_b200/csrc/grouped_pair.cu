@@ -7,7 +7,10 @@
 //   warps 4-19  epilogue: four groups of four warps, 64 bytes of each of a warp's 32 rows at a time: tensor memory -> scales, bias, activation,
 //               weight, residual -> the warp's own staging buffer -> a TMA store where the 32 rows lie in order and are all this expert's, else
 //               64-byte pieces of those rows that are.  The epilogue is bound by the wavefronts of shared memory that it shares with
-//               the operands; a TMA store spares it those of reading the buffer and of writing line by line (STORES).
+//               the operands, and by instructions; a TMA store spares it those of reading the buffer and of writing line by line
+//               (65536x1536x1024 int8, us: 104 without, 94 with).
+// us and what they are of 1.65 PFLOP/s (int8: of twice that), on the device: 32768 slots over 16 experts, 1024x1536 columns by slot 90, 69 %;
+// 65536x1536x1024 int8 88, 71 %; without an epilogue 81 and 62.
 // Every wait is bounded by wall-clock time like those of gemm_tc.cu.
 #include "chunk8.cuh"
 #include "grouped_tc.cuh"
@@ -27,11 +30,12 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uin
     tcgen05_mma_f16_pair(d, a, b, idesc, accumulate);
   }
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {  // zeros behind `bytes`
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+
 template <int BN> struct GroupedPairCfg {
   static constexpr int kStageBytes = (BM + BN / 2) * 128;
   static constexpr int kMaxStages = BN == 256 ? 5 : 6;
@@ -154,7 +158,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     // ---------------- epilogue ----------------
     // Four groups of four warps, a quarter of the columns each, in pieces of 64 bytes of each of the warp's rows.  The residual of the piece
     // after this one is copied to the warp's other staging buffer meanwhile (65536x1024x1536 int8, us: 151 with loads at the start of each
-    // piece, 97 ahead of it; 80 without a residual).  EIGHT
+    // piece, 97 ahead of it; 80 without a residual).  Eight
+    // warps with pieces of 128 bytes had too little to do while they waited: 18000 slots of int8 with Mish 71, now 58; without an activation 102, 105.
     constexpr int kSlab = BN / 4, kPieces = kSlab / kCols, kPer = 16 / (int)sizeof(TOut);  // kPer: entries of 16 bytes
     const int quarter = warp & 3, group = (warp - 4) >> 2, sub = lane >> 2, part = lane & 3;
     const TOut* res = static_cast<const TOut*>(p.res);
@@ -168,7 +173,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
         const int c = __shfl_sync(0xffffffffu, c_row, it * 8 + sub), col = n + part * kPer;
-        if (c >= 0 && col < p.N) cp_async16(smem_u32(at(buffer, it * 8 + sub, part)), res + c * p.ldres + col, 16);
+        if (c >= 0 && col < p.N) cp_async16(smem_u32(at(buffer, it * 8 + sub, part)), res + c * p.ldres + col);
       }
     };
     float b0 = 0.f, b1 = 0.f, w0 = 1.f, w1 = 1.f;  // bias and scale of columns lane and 32 + lane of the next tile's slab
@@ -378,9 +383,10 @@ template <typename TIn, typename TOut, int BN>
 cudaError_t launch_tiles(const GroupedParams& p, int sm_count, cudaStream_t s) {
   using Cfg = GroupedPairCfg<BN>;
   CUtensorMap mx, mw, mc = {};
+  constexpr int kMostBytes = Cfg::smem_bytes(false) > Cfg::smem_bytes(true) ? Cfg::smem_bytes(false) : Cfg::smem_bytes(true);
   cudaError_t e = tma_encode_rows(p.X, p.ldx, p.slots, p.K, BM, Operand<TIn>::prec, &mx);
   if (e == cudaSuccess) e = tma_encode_rows(p.W, p.ldw, (long long)p.experts * p.N, p.K, BN / 2, Operand<TIn>::prec, &mw);
-  if (e == cudaSuccess) e = raise_smem_limit<grouped_pair_kernel<TIn, TOut, BN>>(Cfg::smem_bytes(false) > Cfg::smem_bytes(true) ? Cfg::smem_bytes(false) : Cfg::smem_bytes(true));
+  if (e == cudaSuccess) e = raise_smem_limit<grouped_pair_kernel<TIn, TOut, BN>>(kMostBytes);
   if (e != cudaSuccess) return e;
   const int per = 16 / (int)sizeof(TOut);
   const int vec = p.N % per == 0 && p.ldc % per == 0 && aligned16(p.C) && (!p.res || (p.ldres % per == 0 && aligned16(p.res)));
@@ -396,7 +402,7 @@ cudaError_t launch_tiles(const GroupedParams& p, int sm_count, cudaStream_t s) {
 
 template <typename TIn, typename TOut>
 cudaError_t launch_grouped_pair(const GroupedParams& p, int sm_count, cudaStream_t s) {
-  // Narrow tiles where whole ones leave half of the pairs without any (2048x1024x1024 int8, us: NARROW).
+  // Narrow tiles where whole ones leave half of the pairs without any (2048x1024x1024 int8, us: 9.6 with wide ones, 7.5).
   const long long row_tiles = ((long long)p.slots + 2 * BM - 1) / (2 * BM) + ((p.experts < p.slots ? p.experts : p.slots) - 1) / 2;
   return p.N <= 128 || 4 * row_tiles * ceil_div(p.N, 256) <= sm_count ? launch_tiles<TIn, TOut, 128>(p, sm_count, s) : launch_tiles<TIn, TOut, 256>(p, sm_count, s);
 }

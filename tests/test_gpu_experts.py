@@ -544,7 +544,7 @@ def test_products_refusals(lib):
     assert lib.b200_op_gemm_experts_workspace(None, ctypes.byref(need)) == _lib.ERR_INVALID
     assert lib.b200_op_gemm_experts_workspace(ctypes.byref(_lib.ExpertsDesc(**good)), None) == _lib.ERR_INVALID
     assert call(M=0) == _lib.OK
-    for kw in (dict(M=-64), dict(N=0), dict(K=0), dict(int8=1, x_scales=256, w_scales=256, K=131072), dict(n_experts=0), dict(n_experts=257), dict(top_k=0), dict(top_k=17),
+    for kw in (dict(M=-64), dict(N=0), dict(K=0), dict(K=131072), dict(int8=1, x_scales=256, w_scales=256, K=131072), dict(n_experts=0), dict(n_experts=257), dict(top_k=0), dict(top_k=17),
                dict(group=0), dict(group=48), dict(M=2 ** 30), dict(N=2 ** 30), dict(precision=0), dict(precision=3), dict(activation=0), dict(activation=9), dict(ldx=63),
                dict(ldw=63), dict(ldc=7), dict(res=256, ldres=7), dict(c_by_slot=1, weights=256), dict(c_by_slot=1, res=256), dict(X=None), dict(W=None), dict(C=None),
                dict(order=None), dict(offsets=None), dict(ids=None), dict(int8=1), dict(int8=1, x_scales=256), dict(X=257), dict(W=257), dict(C=257), dict(C=258, out_f32=1),
