@@ -127,7 +127,7 @@ def test_route_without_rows(lib):
 
 # ---- products ---------------------------------------------------------------------------------------------------
 class Experts:
-    """side: up (tokens to slots), down (slots to tokens) or head (tokens to tokens)."""
+    """side: up (tokens to slots), down (slots to tokens), head (tokens to tokens) or slots (slots to slots)."""
 
     def __init__(self, lib, side, requests, N, K, experts, top_k=1, group=1, prec=1, int8=False, f32=False, act=oracle.ACT_NONE, bias=True, weights=None, res=False,
                  ids=None, pads=(0, 0, 0), shift=0, seed=0, in_place=False):
@@ -141,8 +141,8 @@ class Experts:
             ids = (rnd(requests, experts) + 1.5 * rnd(experts)).topk(top_k, dim=1).indices
             ids = torch.where(torch.rand(requests, top_k, device="cuda", generator=g) < 0.1, -1, ids)
         self.ids = torch.as_tensor(ids, dtype=torch.int32, device="cuda").reshape(requests, top_k).contiguous()
-        self.by_slot = side == "up"
-        n_x = M * top_k if side == "down" else M
+        self.by_slot, self.from_slots = side in ("up", "slots"), side in ("down", "slots")
+        n_x = M * top_k if self.from_slots else M
         self.x = rows(n_x, K, pads[0], whole(n_x, K) if int8 else rnd(n_x, K).to(t), 99 if int8 else NAN, shift)
         w = whole(experts * N, K) if int8 else (rnd(experts * N, K) * K ** -0.5).to(t)
         self.w = rows(experts * N, K, pads[1], w, 99 if int8 else NAN, shift)
@@ -155,7 +155,7 @@ class Experts:
         if in_place:
             self.out.copy_(self.res)
         self.in_place = in_place
-        self.weights = torch.rand(requests, top_k, device="cuda", generator=g) if (side != "up" if weights is None else weights) else None
+        self.weights = torch.rand(requests, top_k, device="cuda", generator=g) if (not self.by_slot if weights is None else weights) else None
         key = torch.where((self.ids < 0) | (self.ids >= experts), experts, self.ids.long()).reshape(-1)
         self.order = torch.argsort(key, stable=True).int()
         self.offsets = torch.cat([key.new_zeros(1), torch.bincount(key, minlength=experts + 1)[:experts].cumsum(0)]).int()
@@ -166,7 +166,7 @@ class Experts:
         self.d = _lib.ExpertsDesc(X=p(self.x), W=p(self.w), bias=p(self.bias), C=p(self.out), M=M, N=N, K=K, ldx=self.x.stride(0), ldw=self.w.stride(0),
                                   ldc=self.out.stride(0), activation=act, precision=prec, out_f32=int(f32), int8=int(int8), x_scales=p(self.sx) if int8 else None,
                                   w_scales=p(self.sw) if int8 else None, n_experts=experts, top_k=top_k, group=group, ids=p(self.ids), order=p(self.order),
-                                  offsets=p(self.offsets), x_by_slot=int(side == "down"), c_by_slot=int(self.by_slot), weights=p(self.weights),
+                                  offsets=p(self.offsets), x_by_slot=int(self.from_slots), c_by_slot=int(self.by_slot), weights=p(self.weights),
                                   res=p(self.out if in_place else self.res), ldres=self.out.stride(0), status=p(self.status))
         self.work = workspace(lib.b200_op_gemm_experts_workspace, self.d)
 
@@ -193,7 +193,7 @@ class Experts:
             choice = order[at[e]:at[e + 1]]
             slot = torch.arange(at[e] * self.group, at[e + 1] * self.group, device="cuda")
             token = ((choice // self.top_k)[:, None] * self.group + inside).view(-1)
-            src = slot if self.side == "down" else token
+            src = slot if self.from_slots else token
             x, w = self.x[src].double(), self.w[e * self.N:(e + 1) * self.N].double()
             if self.int8:
                 y = (x @ w.T) * (self.sx[src].double()[:, None] * self.sw[e].double())
@@ -307,6 +307,13 @@ def test_weights_beyond_32_bits(lib, requests):
     c.x, c.w, c.sw, c.bias, c.K = x, w[-1], sw[-1:], bias[-1:], K
     c.check()
     assert (work[-64:] == 255).all()
+
+
+@gpu
+@pytest.mark.parametrize("requests,N,K,experts,top_k,group", [(50, 264, 128, 6, 2, 1), (2000, 512, 320, 4, 2, 1), (40, 300, 192, 3, 1, 64), (9, 70, 33, 3, 2, 1)])
+@pytest.mark.parametrize("int8", [False, True])
+def test_from_slots_to_slots(lib, requests, N, K, experts, top_k, group, int8):
+    Experts(lib, "slots", requests, N, K, experts, top_k, group, 2, int8, act=oracle.ACT_SWISH).run().check()
 
 
 @gpu

@@ -162,7 +162,7 @@ class Product:
 
 SHAPES = [(1, 1, 1), (1, 8, 16), (2, 130, 45), (31, 64, 64), (64, 1024, 1024), (65, 96, 64), (37, 1858, 2048), (128, 128, 128), (129, 257, 144), (200, 264, 136),
           (256, 256, 512), (300, 1000, 624), (513, 520, 320), (1000, 32, 256), (1536, 1536, 1024), (4096, 768, 256), (20000, 512, 128), (16384, 1024, 1536),
-          (333, 1858, 1024), (70000, 16, 32)]
+          (333, 1858, 1024), (70000, 16, 32), (300, 1, 64), (60, 3, 128), (5000, 5, 64), (2000, 129, 64), (6000, 385, 256)]
 
 
 @gpu
