@@ -185,10 +185,11 @@ cudaError_t launch_combine(const CombineParams& p, cudaStream_t s) {
 }
 
 // ---- rows in the order of their slots ---------------------------------------------------------------------------
-// The pair kernel reads X by boxes of 128 rows, so rows that the order names are copied into their order first, once for all tiles of
-// columns, which then find them in L2.  Fetched in place by TMA's gather4, 33 cycles for four rows and anew for each tile of columns, the
-// product takes half as long again (us, 32768 slots x 1024 to 1536 columns: 136, in order with the copy 102; by cp.async into the swizzled
-// tiles 318, as the proxy fence ahead of each hand-over waits for all copies in flight).
+// The pair kernel reads X by boxes of 128 rows, or of 64 where requests are whole 64 rows (1344 rows over 8 experts 13.1 us, copied 18.1); other
+// rows that the order names are copied into their order first, once for all tiles of columns, which then find them in L2.
+// Fetched in place by TMA's gather4, 33 cycles for four rows and anew for each tile of columns, the product takes half as long again (us, 32768
+// slots x 1024 to 1536 columns: 136, in order with the copy 102; by cp.async into the swizzled tiles 318, as the proxy fence ahead of each
+// hand-over waits for all copies in flight).
 __global__ void __launch_bounds__(256) spread_rows_kernel(const GroupedParams p, uint8_t* to, int row_bytes, int size) {
   grid_launch_dependents();
   grid_dependency_wait();
@@ -208,7 +209,8 @@ __global__ void __launch_bounds__(256) spread_rows_kernel(const GroupedParams p,
 bool tma_rows(int K, long long ldx, long long ldw, int size) { return K * (long long)size % 16 == 0 && ldx * size % 16 == 0 && ldw * size % 16 == 0; }
 // The pair kernel's 256 slots pay from a quarter of a tile per expert on, and where the other kernel's tiles of 64 slots x 128 columns are more than
 // half of the SMs (K and N 1024, int8, us, pair kernel / the other: 128 rows 6.9 / 5.8, 256 6.9 / 6.1, 512 7.0 / 7.4, 1024 7.2 / 8.0, 2048
-// 7.5 / 12.5; 768 rows over 8 experts to 1536 columns 14.6 / 16.6).
+// 7.5 / 12.5; 768 rows over 8 experts to 1536 columns, copied into
+// order, 14.6 / 16.6).
 bool many_rows(const GroupedParams& p, int sms) {
   const int used = p.experts < p.slots ? p.experts : p.slots;
   return p.slots / used > 64 && ((long long)p.slots / 64 + used / 2) * ceil_div(p.N, 128) > sms / 2;
@@ -227,7 +229,9 @@ int run_grouped(GroupedParams p, bool exact_sums, void* spread, cudaStream_t s) 
   B200_CUDA(gemm_tc_init());
   B200_CUDA(cudaGetDevice(&dev));
   B200_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  const bool pairs = !exact_sums && many_rows(p, sms), in_place = !p.order || p.x_by_slot || (!pairs && !spreads(p.slots, p.experts));
+  p.x_by_blocks = p.order && !p.x_by_slot && p.group % 64 == 0;
+  const bool pairs = !exact_sums && many_rows(p, sms), in_order_already = !p.order || p.x_by_slot || p.x_by_blocks;
+  const bool in_place = in_order_already || (!pairs && !spreads(p.slots, p.experts));
   if (!in_place) {
     const long long blocks = ((long long)p.slots + 7) / 8;
     B200_CUDA(launch_dependent(spread_rows_kernel, dim3((unsigned)(blocks < sms * 8 ? blocks : sms * 8)), dim3(256), 0, s, p, static_cast<uint8_t*>(spread),
@@ -235,7 +239,7 @@ int run_grouped(GroupedParams p, bool exact_sums, void* spread, cudaStream_t s) 
     p.X = spread;
     p.ldx = p.K;
   }
-  const bool in_order = !p.order || p.x_by_slot || !in_place;
+  const bool in_order = in_order_already || !in_place;
   if (pairs) B200_CUDA((launch_grouped_pair<TIn, TOut>(p, sms, s)));
   else B200_CUDA((launch_grouped_rows<TIn, TOut>(p, in_order, exact_sums, sms, s)));
   return B200_OK;
@@ -252,7 +256,7 @@ size_t sums_bytes(const b200_experts_desc& d) { return sums_choices(d) ? round25
 // X in the order of the slots.
 size_t spread_bytes(const b200_experts_desc& d) {
   const int size = d.int8 ? 1 : 2;
-  const bool spread = !d.x_by_slot && d.M > 0 && spreads(d.M * d.top_k, d.n_experts) &&
+  const bool spread = !d.x_by_slot && d.group % 64 != 0 && d.M > 0 && spreads(d.M * d.top_k, d.n_experts) &&
                       tma_rows(d.K, d.ldx ? d.ldx : d.K, d.ldw ? d.ldw : d.K, size);
   return spread ? round256((size_t)d.M * d.top_k * d.K * size) : 0;
 }

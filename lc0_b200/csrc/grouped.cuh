@@ -19,6 +19,7 @@ struct GroupedParams {
   int slots;                             // rows of choices there may be (M * top_k)
   int N, K, experts, top_k, group, act;
   int x_by_slot, c_by_slot;
+  int x_by_blocks;  // tensor-core kernels: X in the tokens' order, requests of whole 64 rows, which are fetched where they lie
   int* place;  // [choices] or nullptr
   int* status;
 };
@@ -47,6 +48,11 @@ __device__ __forceinline__ SlotRows rows_of_slot(const GroupedParams& p, int slo
 __device__ __forceinline__ void keep_place(const GroupedParams& p, const SlotRows& r, int slot) {
   if (p.place && r.c >= 0) p.place[r.choice] = slot / p.group;
 }
+// The first row of X of the 64 slots from `slot` on, a multiple of 64 behind the expert's first (x_by_blocks).
+__device__ __forceinline__ int row_of_block(const GroupedParams& p, int slot, int end) {
+  const int x = slot < end ? rows_of_slot(p, slot).x : 0;
+  return x < 0 ? 0 : x;  // whatever lies there: its results are not stored
+}
 // offsets[e] in slots, held within what there is.
 __device__ __forceinline__ int expert_begin(const GroupedParams& p, int e) {
   if (!p.offsets) return e == 0 ? 0 : p.slots;
@@ -54,10 +60,10 @@ __device__ __forceinline__ int expert_begin(const GroupedParams& p, int e) {
   return (at < 0 ? 0 : at < most ? at : most) * p.group;
 }
 
-// Many rows (grouped_pair.cu): operands that TMA can read, X [slots][K] in the order of the slots.
+// Many rows (grouped_pair.cu): operands that TMA can read, X [slots][K] in the order of the slots, or x_by_blocks.
 template <typename TIn, typename TOut> cudaError_t launch_grouped_pair(const GroupedParams& p, int sm_count, cudaStream_t s);
 
-// Few rows per expert (grouped_rows.cu): operands that TMA can read.  in_order: X is [slots][K] in the order of the slots.  rounded: fp32 results of 16-bit operands as exact as a plain fp32 product.
+// Few rows per expert (grouped_rows.cu): operands that TMA can read.  in_order: X is [slots][K] in the order of the slots, or x_by_blocks.  rounded: fp32 results of 16-bit operands as exact as a plain fp32 product.
 template <typename TIn, typename TOut> cudaError_t launch_grouped_rows(const GroupedParams& p, bool in_order, bool rounded, int sm_count, cudaStream_t s);
 
 }  // namespace b200

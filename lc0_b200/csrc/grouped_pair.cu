@@ -2,7 +2,7 @@
 //
 // A persistent grid of pairs walks the tiles of all experts (256 slots of one expert each; how many an expert has is read on the device).  Per
 // k-block of 128 bytes each CTA fetches its 128 rows of X and half of the tile's rows of W:
-//   warp 0      TMA producer
+//   warp 0      TMA producer; requests of whole 64 rows are fetched where they lie, two boxes for one
 //   warp 1      tcgen05.mma issuer (even CTA), kind::f16 or kind::i8, two accumulators in tensor memory
 //   warps 4-19  epilogue: four groups of four warps, 64 bytes of each of a warp's 32 rows at a time: tensor memory -> scales, bias, activation,
 //               weight, residual -> the warp's own staging buffer -> a TMA store where the 32 rows lie in order and are all this expert's, else
@@ -117,13 +117,16 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       uint32_t ph = 0;
       bool ok = true;
       for (; walk.valid() && ok; walk.next()) {
-        const int x_row = walk.s0 + (int)rank * BM, w_row = walk.e * p.N + walk.n0 + (int)rank * (columns() / 2);
+        const int x0 = walk.s0 + (int)rank * BM;
+        const int x_row = p.x_by_blocks ? row_of_block(p, x0, walk.end) : x0, x_next = p.x_by_blocks ? row_of_block(p, x0 + 64, walk.end) : 0;
+        const int w_row = walk.e * p.N + walk.n0 + (int)rank * (columns() / 2);
         for (int kb = 0; kb < k_blocks; ++kb) {
           if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 1)) { ok = false; break; }
           const uint32_t fb_local = smem_u32(&full_bar[s]);
           const uint32_t fb = mapa(fb_local, 0), sa = smem_u32(smem + s * Cfg::kStageBytes);
           if (rank == 0) mbar_expect_tx(fb_local, 2 * Cfg::kStageBytes);
           tma_load_2d_pair(sa, &map_x, kb * Operand<TIn>::k, x_row, fb);
+          if (p.x_by_blocks) tma_load_2d_pair(sa + 64 * 128, &map_x, kb * Operand<TIn>::k, x_next, fb);
           tma_load_2d_pair(sa + BM * 128, &map_w, kb * Operand<TIn>::k, w_row, fb);
           if (++s == S) { s = 0; ph ^= 1; }
         }
@@ -384,7 +387,7 @@ cudaError_t launch_tiles(const GroupedParams& p, int sm_count, cudaStream_t s) {
   using Cfg = GroupedPairCfg<BN>;
   CUtensorMap mx, mw, mc = {};
   constexpr int kMostBytes = Cfg::smem_bytes(false) > Cfg::smem_bytes(true) ? Cfg::smem_bytes(false) : Cfg::smem_bytes(true);
-  cudaError_t e = tma_encode_rows(p.X, p.ldx, p.slots, p.K, BM, Operand<TIn>::prec, &mx);
+  cudaError_t e = tma_encode_rows(p.X, p.ldx, p.x_by_blocks ? p.x_rows : p.slots, p.K, p.x_by_blocks ? 64 : BM, Operand<TIn>::prec, &mx);
   if (e == cudaSuccess) e = tma_encode_rows(p.W, p.ldw, (long long)p.experts * p.N, p.K, BN / 2, Operand<TIn>::prec, &mw);
   if (e == cudaSuccess) e = raise_smem_limit<grouped_pair_kernel<TIn, TOut, BN>>(kMostBytes);
   if (e != cudaSuccess) return e;

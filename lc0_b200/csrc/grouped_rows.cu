@@ -127,13 +127,14 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       uint32_t ph = 0;
       bool ok = true;
       for (; walk.valid() && ok; walk.next()) {
+        const int x_row = p.x_by_blocks ? row_of_block(p, s0, end) : s0;
         const int x_bytes = kGather ? (min(kRows, end - s0) + 3) / 4 * 512 : kRows * 128;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, 1)) { ok = false; break; }
           const uint32_t fb = smem_u32(&full_bar[s]), sa = smem_u32(smem + s * kStageBytes);
           mbar_expect_tx(fb, BM * 128 + x_bytes);
           tma_load_2d(sa, &map_w, kb * Operand<TIn>::k, walk.e * p.N + n0, fb);
-          if constexpr (!kGather) tma_load_2d(sa + BM * 128, &map_x, kb * Operand<TIn>::k, s0, fb);
+          if constexpr (!kGather) tma_load_2d(sa + BM * 128, &map_x, kb * Operand<TIn>::k, x_row, fb);
           if (++s == stages) { s = 0; ph ^= 1; }
         }
       }
@@ -320,7 +321,7 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 template <typename TIn, typename TOut, bool kGather, bool kRounded>
 cudaError_t launch_rows(const GroupedParams& p, int sm_count, cudaStream_t s) {
   CUtensorMap mx, mw;
-  cudaError_t e = tma_encode_rows(p.X, p.ldx, kGather ? p.x_rows : p.slots, p.K, kGather ? 1 : kRows, Operand<TIn>::prec, &mx);
+  cudaError_t e = tma_encode_rows(p.X, p.ldx, kGather || p.x_by_blocks ? p.x_rows : p.slots, p.K, kGather ? 1 : kRows, Operand<TIn>::prec, &mx);
   if (e == cudaSuccess) e = tma_encode_rows(p.W, p.ldw, (long long)p.experts * p.N, p.K, BM, Operand<TIn>::prec, &mw);
   if (e == cudaSuccess) e = raise_smem_limit<grouped_rows_kernel<TIn, TOut, kGather, kRounded>>(smem_bytes(kMaxStages, false) > smem_bytes(kMaxSplitStages, true) ? smem_bytes(kMaxStages, false) : smem_bytes(kMaxSplitStages, true));
   if (e != cudaSuccess) return e;
