@@ -33,6 +33,9 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uin
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 
@@ -173,14 +176,22 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     const bool scaled = p.weights != nullptr || p.alpha != 1.f;
     auto at = [&](uint8_t* buffer, int row, int q) { return buffer + row * 64 + ((q ^ ((row >> 1) & 3)) << 4); };  // 16 bytes, swizzled
     // Rows that are no whole 16 bytes but whole words leave by two rows of 16 words at a time (16384x1858x512 int8, fp16
-    // results, us: 70 entry by entry, 45; fp32 124, 62).
+    // results, us: 70 entry by entry, 45; with a residual, copied ahead like the others, 231, 67; fp32 124, 61).
     constexpr int kWord = 4 / (int)sizeof(TOut);
     auto word_at = [&](uint8_t* buffer, int row) { return reinterpret_cast<uint32_t*>(at(buffer, row, (lane & 15) >> 2) + (lane & 3) * 4); };
     auto copy_res = [&](uint8_t* buffer, int c_row, int n) {  // the residual's piece that begins at column n
+      if (vec == 2) {
 #pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        const int c = __shfl_sync(0xffffffffu, c_row, it * 8 + sub), col = n + part * kPer;
-        if (c >= 0 && col < p.N) cp_async16(smem_u32(at(buffer, it * 8 + sub, part)), res + c * p.ldres + col);
+        for (int it = 0; it < 4; ++it) {
+          const int c = __shfl_sync(0xffffffffu, c_row, it * 8 + sub), col = n + part * kPer;
+          if (c >= 0 && col < p.N) cp_async16(smem_u32(at(buffer, it * 8 + sub, part)), res + c * p.ldres + col);
+        }
+      } else {
+#pragma unroll 4
+        for (int rr = lane >> 4; rr < 32; rr += 2) {
+          const int c = __shfl_sync(0xffffffffu, c_row, rr), col = n + (lane & 15) * kWord;
+          if (c >= 0 && col < p.N) cp_async4(smem_u32(word_at(buffer, rr)), res + c * p.ldres + col);
+        }
       }
     };
     float b0 = 0.f, b1 = 0.f, w0 = 1.f, w1 = 1.f;  // bias and scale of columns lane and 32 + lane of the next tile's slab
@@ -237,7 +248,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       next = tile_at_hand();
       fetch_vectors(next.wb, next.n);
       const bool any_next = __any_sync(0xffffffffu, next.r.c >= 0) && next.n < p.N;
-      if (res && vec == 2 && any && !copied) {
+      if (res && vec && any && !copied) {
         copy_res(buffers + buf * 2048, x.r.c, x.n);
         cp_async_commit();
       }
@@ -251,7 +262,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         if (n >= p.N) break;
         uint8_t* buffer = buffers + buf * 2048;
         if (res) {
-          if (vec == 2) {
+          if (vec) {
             uint8_t* other = buffers + (buf ^ 1) * 2048;
             if (lane == 0) tma_store_wait_read0();  // (of the piece before this one)
             __syncwarp();
@@ -261,12 +272,6 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             cp_async_commit();
             cp_async_wait<1>();
             buf ^= 1;
-          } else if (vec == 1) {
-#pragma unroll 8
-            for (int rr = lane >> 4; rr < 32; rr += 2) {
-              const int c = __shfl_sync(0xffffffffu, x.r.c, rr), col = n + (lane & 15) * kWord;
-              if (c >= 0 && col < p.N) *word_at(buffer, rr) = *reinterpret_cast<const uint32_t*>(res + c * p.ldres + col);
-            }
           } else {
 #pragma unroll 1
             for (int rr = 0; rr < 32; ++rr) {
