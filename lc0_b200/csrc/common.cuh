@@ -47,8 +47,9 @@ template <typename F> int at_c_entry(F&& f) noexcept {
 // kernel calls grid_dependency_wait() in every thread that touches global memory, before it reads anything a kernel may
 // have written and before it writes at all: the call returns when the kernels before it have completed and their writes
 // are visible.  What may be read ahead of it are loaded weights alone: parameter vectors (bias, LayerNorm and gate
-// parameters, column sums) and, where GemmParams::w_const says so, the matrix W.  Every launch waits in some thread, so a kernel
-// is over only when those before it are.  grid_launch_dependents() lets the kernel after it be made resident; it promises
+// parameters, column sums) and, where GemmParams::w_const says so, the matrix W.  __ldg is for those alone: it promises that its data stays as it is
+// from the kernel's start on, and nothing holds it behind the wait; lists, places and scales that another operator makes are read by plain loads.  Every
+// launch waits in some thread, so a kernel is over only when those before it are.  grid_launch_dependents() lets the kernel after it be made resident; it promises
 // nothing about data and may come before this kernel's own wait.  Both are no-ops in a kernel that was launched the
 // ordinary way.
 #ifdef __CUDACC__

@@ -111,7 +111,7 @@ struct CombineParams {
 // The place of a request's choice, -1 where it has no expert (or order does not name it, which is the caller's to rule out).
 __device__ __forceinline__ int place_of(const CombineParams& p, int request, int j) {
   const long long choice = (long long)request * p.top_k + j;
-  const int id = __ldg(p.ids + choice), at = __ldg(p.place + choice);
+  const int id = p.ids[choice], at = p.place[choice];
   return id >= 0 && id < p.experts && at >= 0 && at < p.tokens / p.group * p.top_k ? at : -1;
 }
 

@@ -36,7 +36,7 @@ __device__ __forceinline__ SlotRows rows_of_slot(const GroupedParams& p, int slo
     return r;
   }
   const int s = p.group == 1 ? slot : slot / p.group, i = p.group == 1 ? 0 : slot - s * p.group;
-  const int choice = __ldg(p.order + s);
+  const int choice = p.order[s];
   if (choice < 0 || choice >= p.slots / p.group) return {-1, -1, 0};
   const int token = (p.top_k == 1 ? choice : choice / p.top_k) * p.group + i;
   r.x = p.x_by_slot ? slot : token;
@@ -56,7 +56,7 @@ __device__ __forceinline__ int row_of_block(const GroupedParams& p, int slot, in
 // offsets[e] in slots, held within what there is.
 __device__ __forceinline__ int expert_begin(const GroupedParams& p, int e) {
   if (!p.offsets) return e == 0 ? 0 : p.slots;
-  const int most = p.slots / p.group, at = __ldg(p.offsets + e);
+  const int most = p.slots / p.group, at = p.offsets[e];
   return (at < 0 ? 0 : at < most ? at : most) * p.group;
 }
 

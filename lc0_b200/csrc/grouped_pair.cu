@@ -197,11 +197,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     float b0 = 0.f, b1 = 0.f, w0 = 1.f, w1 = 1.f;  // bias and scale of columns lane and 32 + lane of the next tile's slab
     auto fetch_vectors = [&](int wb, int n) {
       const bool first = n + lane < p.N, second = kSlab > 32 && n + 32 + lane < p.N;
-      b0 = p.bias && first ? __ldg(p.bias + wb + n + lane) : 0.f;
-      b1 = p.bias && second ? __ldg(p.bias + wb + n + 32 + lane) : 0.f;
+      b0 = p.bias && first ? p.bias[wb + n + lane] : 0.f;
+      b1 = p.bias && second ? p.bias[wb + n + 32 + lane] : 0.f;
       if (sizeof(TIn) == 1) {
-        w0 = first ? __ldg(p.w_scales + wb + n + lane) : 0.f;
-        w1 = second ? __ldg(p.w_scales + wb + n + 32 + lane) : 0.f;
+        w0 = first ? p.w_scales[wb + n + lane] : 0.f;
+        w1 = second ? p.w_scales[wb + n + 32 + lane] : 0.f;
       }
     };
     struct Tile {

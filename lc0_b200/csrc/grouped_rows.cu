@@ -232,8 +232,8 @@ grouped_rows_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
       n = n0 + column;
       // ks > 1: the slots that this CTA finishes; else all 64
       const int slot = s0 + (ks > 1 ? (int)rank * slots_each(rows, log_ks) + lane : half * 32 + lane);
-      bias = n < p.N && p.bias ? __ldg(p.bias + (long long)walk.e * p.N + n) : 0.f;
-      if (sizeof(TIn) == 1) sw = n < p.N ? __ldg(p.w_scales + (long long)walk.e * p.N + n) : 0.f;
+      bias = n < p.N && p.bias ? p.bias[(long long)walk.e * p.N + n] : 0.f;
+      if (sizeof(TIn) == 1) sw = n < p.N ? p.w_scales[(long long)walk.e * p.N + n] : 0.f;
       r = {-1, -1, 0};
       sx = 1.f;
       weight = p.alpha;

@@ -24,11 +24,11 @@ __device__ __forceinline__ int position_of(const QkParams& p, int row) {
 // Eight floats, with 16-byte loads where their address allows.
 __device__ __forceinline__ void load_eight(const float* from, bool aligned, float (&v)[8]) {
   if (aligned) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(from)), b = __ldg(reinterpret_cast<const float4*>(from) + 1);
+    const float4 a = reinterpret_cast<const float4*>(from)[0], b = reinterpret_cast<const float4*>(from)[1];
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __ldg(from + i);
+    for (int i = 0; i < 8; ++i) v[i] = from[i];
   }
 }
 
