@@ -507,7 +507,8 @@ int b200_op_route(const b200_route_desc* d, void* stream);
  *   - workspace: b200_op_gemm_experts_workspace() bytes on a 256-byte boundary, for this call alone until it has run (0 for some
  *     sizes, and may then be NULL).
  *   Sums in fp32 (int8: exact); float results of 16-bit inputs are as exact as a plain fp32 product.  order entries outside the choices are no rows;
- *   offsets are held to 0 <= offsets[e] <= offsets[e + 1] <= M / group * top_k.  M a multiple of group, M * top_k at most 2^30, K at
+ *   offsets are held to 0 <= offsets[e] <= offsets[e + 1] <= M / group * top_k (an entry below one ahead of it counts as that one).  Where choices are
+ *   summed, a choice that ids give an expert and order and offsets no slot leaves its token's result undefined.  M a multiple of group, M * top_k at most 2^30, K at
  *   most B200_INT8_MAX_K. */
 typedef struct b200_experts_desc {
   const void* X; const void* W; const float* bias; void* C;

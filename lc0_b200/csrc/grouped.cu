@@ -29,11 +29,11 @@ __global__ void __launch_bounds__(256) grouped_any_kernel(const GroupedParams p)
   for (long long block = blockIdx.y;; block += gridDim.y) {
     // the block's expert and first slot
     long long left = block;
-    int e = 0, begin = 0, end = 0;
+    int e = 0, begin = 0, end = expert_begin(p, 0);
     for (; e < p.experts; ++e) {
-      begin = expert_begin(p, e);
-      end = expert_begin(p, e + 1);
-      const int blocks = end > begin ? (end - begin + kTile - 1) / kTile : 0;
+      begin = end;
+      end = max(begin, expert_begin(p, e + 1));
+      const int blocks = (end - begin + kTile - 1) / kTile;
       if (left < blocks) break;
       left -= blocks;
     }
@@ -194,7 +194,9 @@ __global__ void __launch_bounds__(256) spread_rows_kernel(const GroupedParams p,
   grid_launch_dependents();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, pieces = row_bytes / 16;
-  const int end = expert_begin(p, p.experts);
+  int end = 0;
+  for (int e = lane; e <= p.experts; e += 32) end = max(end, expert_begin(p, e));
+  end = __reduce_max_sync(0xffffffffu, end);
   for (long long slot = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); slot < end; slot += (long long)gridDim.x * 8) {
     const int x = rows_of_slot(p, (int)slot).x;
     if (x < 0) continue;

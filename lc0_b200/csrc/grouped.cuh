@@ -53,7 +53,7 @@ __device__ __forceinline__ int row_of_block(const GroupedParams& p, int slot, in
   const int x = slot < end ? rows_of_slot(p, slot).x : 0;
   return x < 0 ? 0 : x;  // whatever lies there: its results are not stored
 }
-// offsets[e] in slots, held within what there is.
+// offsets[e] in slots, held within what there is.  (An entry below one ahead of it counts as that one; it is the callers that see to it.)
 __device__ __forceinline__ int expert_begin(const GroupedParams& p, int e) {
   if (!p.offsets) return e == 0 ? 0 : p.slots;
   const int most = p.slots / p.group, at = p.offsets[e];

@@ -27,22 +27,32 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
 template <int kRows>
 __device__ __forceinline__ void list_tiles(const GroupedParams& p, int* first, int* begin, int* scan) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = threadIdx.x;
-  int upto = 0;
-  if (e < 256) {
-    if (e < p.experts) {
-      const int b = expert_begin(p, e), n = expert_begin(p, e + 1) - b;
-      begin[e] = b;
-      if (e == p.experts - 1) begin[p.experts] = b + max(n, 0);
-      upto = n > 0 ? (n + kRows - 1) / kRows : 0;
-    }
+  int b = 0, n = 0, upto = 0;
+  if (e < p.experts) {
+    b = expert_begin(p, e);
+    n = expert_begin(p, e + 1) - b;
+  }
+  auto list = [&]() {
+    if (e >= 256) return;
+    if (e < p.experts) begin[e] = b;
+    if (e == p.experts - 1) begin[p.experts] = b + n;
+    upto = (n + kRows - 1) / kRows;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int n = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += n;
+      const int ahead = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += ahead;
     }
     if (lane == 31) scan[warp] = upto;
+  };
+  list();
+  if (__syncthreads_or(n < 0)) {  // falling offsets: an entry counts as the largest ahead of it, so that no slot has two experts
+    if (e < p.experts) {
+      for (int i = 0; i < e; ++i) b = max(b, expert_begin(p, i));
+      n = max(expert_begin(p, e + 1) - b, 0);
+    }
+    list();
+    __syncthreads();
   }
-  __syncthreads();
   if (e < 256) {
     for (int w = 0; w < warp; ++w) upto += scan[w];
     if (e < p.experts) first[e + 1] = upto;

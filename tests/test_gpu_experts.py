@@ -590,3 +590,19 @@ def test_without_host_memory(tmp_path):
     r = subprocess.run([sys.executable, "-c", _CALLS, str(shim)], cwd=ROOT, env=dict(os.environ, LD_PRELOAD=str(shim)), capture_output=True, text=True)
     assert r.returncode == 0, r.stderr[-500:]
     assert r.stdout.strip() == "%s %d" % ([_lib.ERR_NOMEM] * 7, _lib.ERR_INVALID)
+
+
+@gpu
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("side,requests,N,K,top_k,group", [("head", 40, 136, 512, 1, 1), ("up", 300, 264, 128, 1, 1), ("head", 3000, 512, 256, 1, 1), ("down", 300, 136, 256, 2, 1),
+                                                           ("down", 3000, 256, 128, 2, 1), ("up", 30, 264, 256, 1, 64), ("head", 60, 50, 45, 1, 1)])
+def test_falling_offsets(lib, side, requests, N, K, top_k, group, int8):
+    """An offset below one ahead of it counts as that one: every slot has one expert, whatever lies behind the fall."""
+    S = requests * top_k
+    for bad in ([0, S, 0, S, 0, S, 0], [0, 10, 5, 20, 2 ** 31 - 1, -7, S], [0, 0, S // 2, 3, S // 2 + 3, 1, S]):
+        c = Experts(lib, side, requests, N, K, 6, top_k, group, 1, int8, ids=torch.arange(S).view(requests, top_k) % 6, res=side == "down")
+        at = torch.tensor(bad, device="cuda")
+        given = at.int()
+        c.offsets = at.clamp(0, S).cummax(0).values.int()
+        c.d.offsets = given.data_ptr()
+        c.run().check()
