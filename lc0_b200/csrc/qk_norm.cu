@@ -103,7 +103,8 @@ __global__ void __launch_bounds__(128) qk_norm_rotate_kernel(const QkParams p, i
       for (int j = 0; j < 8; ++j) sum = fmaf(v[j], v[j], sum);
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const float r = rsqrtf(fmaf(sum, inv_depth, p.eps));  // (off by two steps at most)
+      // fp32 results: rounded to nearest, as in the kernel below; rsqrtf, off by two steps, does not show in 16 bits.
+      const float mean = fmaf(sum, inv_depth, p.eps), r = sizeof(T) == 4 ? __frsqrt_rn(mean) : rsqrtf(mean);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] *= r * gamma[j];
     }
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(128) qk_norm_rotate_any_kernel(const QkParams 
     v[i] = e < p.depth ? to_f(x[e]) : 0.f;
     sum = fmaf(v[i], v[i], sum);
   }
-  const float r = p.norm ? 1.f / sqrtf(warp_sum(sum) / (float)p.depth + p.eps) : 1.f;
+  const float r = p.norm ? __frsqrt_rn(warp_sum(sum) / (float)p.depth + p.eps) : 1.f;
   auto scaled = [&](float u, int e) { return p.norm ? u * (gamma ? r * gamma[e] : r) : u; };
 #pragma unroll
   for (int i = 0; i < 8; ++i) {

@@ -140,6 +140,22 @@ def test_zeros_and_what_is_not_finite(lib, depth, interleaved):
 
 
 @gpu
+@pytest.mark.parametrize("depth", [8, 16, 64])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_float_heads_by_operations_rounded_to_nearest(lib, depth, shift):
+    """Entries of one size a < 2^9: the sum of squares (18 bits and 6 more), its mean and that one's root a are exact, 1 / a and a (1 / a) are
+    rounded to nearest.  a (1 / a) lies within 2^-24 of 1, so the result is 1 or its neighbour below."""
+    a = torch.arange(256, 512, device="cuda").float()[:, None, None]
+    c = Call(lib, 256, 2, 1, depth, 0, gamma=False, eps=0.0, shift=shift)
+    for v, heads in ((c.q, 2), (c.k, 1)):
+        v.copy_((a * (1 - 2 * torch.randint(0, 2, (256, heads, depth), device="cuda"))).view(256, -1))
+    c.run()
+    for out, v in ((c.qo, c.q), (c.ko, c.k)):
+        size = out * v.sign()
+        assert ((size == 1) | (size == 1 - 2.0 ** -24)).all()
+
+
+@gpu
 def test_offsets_beyond_32_bits(lib):
     rows = 560000
     q = torch.ones(rows, 4096, dtype=torch.float16, device="cuda")
