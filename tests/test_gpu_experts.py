@@ -106,6 +106,39 @@ def test_route_ties_and_what_is_no_number(lib, e, renormalise):
 
 
 @gpu
+@pytest.mark.parametrize("rows", [300, 20000])
+@pytest.mark.parametrize("experts", [32, 64, 128, 256])
+def test_float_weights_are_of_rounded_exponentials(lib, rows, experts):
+    """fp32 logits: the softmax's denominator takes expf, off by two steps at most as CUDA documents it, so one of five numbers around the rounded
+    exponential.  One logit of 0 beside equal ones x: eight of a lane are added in order, then the lanes in pairs, so with each of the five the weight
+    1 / sum is one number."""
+    f = np.float32
+    x = np.random.default_rng(experts).uniform(-7, -0.5, rows).astype(f)
+    l = np.repeat(x[:, None], experts, axis=1)
+    first = np.arange(rows) % experts
+    l[np.arange(rows), first] = 0
+    r = Route(lib, torch.from_numpy(l).cuda(), 1).run()
+    r.check()
+    best = np.exp(x.astype(np.float64)).astype(f)
+    sums = []
+    for step in range(-2, 3):
+        e = (best.view(np.int32) + np.int32(step)).view(f)
+        terms = np.repeat(e[:, None], experts, axis=1)
+        terms[np.arange(rows), first] = 1
+        lanes = terms.reshape(rows, experts // 8, 8)
+        total = np.zeros((rows, experts // 8), f)
+        for i in range(8):
+            total = total + lanes[:, :, i]
+        while total.shape[1] > 1:
+            half = total.shape[1] // 2
+            total = total[:, :half] + total[:, half:]
+        sums.append(f(1) / total[:, 0])
+    assert total.dtype == f
+    got = r.weights.cpu().numpy()[:, 0]
+    assert (got <= np.maximum.reduce(sums)).all() and (got >= np.minimum.reduce(sums)).all()
+
+
+@gpu
 @pytest.mark.parametrize("n,e,top_k", [(1, 1, 1), (24, 8, 1), (333, 12, 1), (70000, 256, 3), (5000, 1, 2), (100, 5, 16)])
 def test_route_of_given_ids(lib, n, e, top_k):
     ids = torch.randint(-2, e + 2, (n, top_k), dtype=torch.int32, device="cuda")
