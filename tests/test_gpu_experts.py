@@ -639,3 +639,89 @@ def test_falling_offsets(lib, side, requests, N, K, top_k, group, int8):
         c.offsets = at.clamp(0, S).cummax(0).values.int()
         c.d.offsets = given.data_ptr()
         c.run().check()
+
+
+@gpu
+@pytest.mark.parametrize("prec", [0, 1, 2])
+@pytest.mark.parametrize("act", [oracle.ACT_NONE, oracle.ACT_MISH, oracle.ACT_SELU])
+@pytest.mark.parametrize("top_k", [1, 2])
+def test_int8_rows_do_not_depend_on_their_number(lib, prec, act, top_k):
+    """The same bits by gathers, from rows in order, and by CTA pairs, with weights and a residual."""
+    made = lambda: Experts(lib, "head", 3000, 264, 512, 6, top_k, 1, prec, True, act=act, res=True, seed=5)
+    whole = made().run()
+    whole.check()
+    for n in (1, 40, 300):
+        part = made()
+        part.requests = part.M = part.d.M = n
+        key = torch.where(part.ids[:n] < 0, 6, part.ids[:n].long()).reshape(-1)
+        part.order = torch.argsort(key, stable=True).int()
+        part.offsets = torch.cat([key.new_zeros(1), torch.bincount(key, minlength=7)[:6].cumsum(0)]).int()
+        part.d.order, part.d.offsets = part.order.data_ptr(), part.offsets.data_ptr()
+        part.run()
+        assert torch.equal(part.out[:n], whole.out[:n]) and (part.out[n:] == 55).all()
+
+
+@gpu
+@pytest.mark.parametrize("side", ["head", "down", "slots"])
+@pytest.mark.parametrize("requests,N,experts,top_k", [(1, 1858, 6, 1), (40, 264, 6, 1), (40, 264, 6, 2), (96, 1858, 12, 1), (333, 1858, 6, 1), (2500, 256, 6, 2)])
+@pytest.mark.parametrize("prec", [1, 2])
+def test_float_results_are_as_exact_as_a_chain_in_fp32(lib, side, requests, N, experts, top_k, prec):
+    """In the root mean square, by gathers, from rows in order, with K cut over a cluster, with choices summed.  Products of two 16-bit numbers are exact
+    in fp32; a chain of 1024 rounded sums is off by about 9 2^-24 of the result's size, sums of 64 truncated at every 16 and added rounded by 2 2^-24,
+    sums truncated all the way by 28 2^-24."""
+    K = 1024
+    ids = (torch.arange(requests)[:, None] + torch.arange(top_k) * 2) % experts
+    c = Experts(lib, side, requests, N, K, experts, top_k, 1, prec, f32=True, weights=False, ids=ids, seed=9).run()
+    c.check()
+    want, _, written = c.want()
+    chain, at = torch.zeros_like(c.out), c.offsets.tolist()
+    for e in range(experts):
+        choice, slot = c.order[at[e]:at[e + 1]].long(), torch.arange(at[e], at[e + 1], device="cuda")
+        x, w = c.x[slot if c.from_slots else choice // top_k].float(), c.w[e * N:(e + 1) * N].float()
+        y = torch.zeros(len(slot), N, device="cuda")
+        for k in range(K):
+            y += x[:, k, None] * w[:, k]
+        chain.index_add_(0, slot if c.by_slot else choice // top_k, y + c.bias[e])
+    rms = lambda v: (v.double() - want)[written].square().mean().sqrt().item()
+    assert rms(c.out) <= 1.5 * rms(chain) + 2.0 ** -26
+
+
+@gpu
+@pytest.mark.parametrize("act", [oracle.ACT_MISH, oracle.ACT_SWISH])
+@pytest.mark.parametrize("requests", [60, 900, 6000])
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("worst", [NAN, INF, -INF])
+def test_columns_that_share_a_reciprocal_keep_apart(lib, act, requests, int8, worst):
+    c = Experts(lib, "head", requests, 264, 256, 4, 1, 1, 2, int8, act=act, weights=False, ids=torch.arange(requests)[:, None] % 4)
+    clean, columns, theirs = c.bias.clone(), [5, 130, 263], torch.arange(requests, device="cuda") % 4 == 2
+    c.bias[2, columns] = worst
+    c.run()
+    for col in columns:
+        assert (c.out[theirs, col] == INF).all() if worst == INF else c.out[theirs, col].isnan().all()
+    same = Experts(lib, "head", requests, 264, 256, 4, 1, 1, 2, int8, act=act, weights=False, ids=torch.arange(requests)[:, None] % 4).run()
+    c.bias = clean
+    for col in columns:
+        c.out[theirs, col] = same.out[theirs, col]
+    c.check()
+
+
+@gpu
+@pytest.mark.parametrize("pads", [(16, 32, 8), (0, 0, 2), (8, 0, 1), (0, 16, 0)])
+@pytest.mark.parametrize("side,top_k", [("up", 2), ("down", 1), ("down", 2), ("head", 1), ("slots", 1)])
+@pytest.mark.parametrize("N", [264, 1858])
+@pytest.mark.parametrize("prec,int8", [(1, False), (2, False), (2, True), (0, True)])
+def test_strides_of_many_rows(lib, pads, side, top_k, N, prec, int8):
+    """CTA pairs: padded rows of each operand; results and residuals by whole 16 bytes, by words and by entries."""
+    res = side in ("down", "head")
+    pads = (2 * pads[0], *pads[1:]) if int8 else pads
+    Experts(lib, side, 6000, N, 192, 5, top_k, 1, prec, int8, pads=pads, res=res, in_place=res and N == 264).run().check()
+
+
+@gpu
+@pytest.mark.parametrize("side", ["up", "down", "head"])
+@pytest.mark.parametrize("group", [128, 192])
+@pytest.mark.parametrize("requests,N", [(2, 136), (40, 520)])
+@pytest.mark.parametrize("int8", [False, True])
+def test_requests_of_several_whole_64_rows(lib, side, group, requests, N, int8):
+    Experts(lib, side, requests, N, 256, 3, 1, group, 1, int8, res=side != "up").run().check()
+    Experts(lib, side, requests, N, 192, 3, 2, group, 2, int8, res=side != "up").run().check()

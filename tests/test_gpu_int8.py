@@ -113,6 +113,26 @@ def test_quantize_rows_at_the_ends(lib, prec, k):
     assert s[6:9].isnan().all() and not q[6:9].any() and s[0] == 0
 
 
+@gpu
+@pytest.mark.parametrize("k", [768, 765])
+def test_quotients_a_step_from_a_tie(lib, k):
+    """fp32 rows whose scales lie at both ends of a binade and anywhere in it, of many sizes, with entries at (r + 1/2) s rounded and one step to
+    either side: what the remainder alone decides."""
+    ends = [1.0, 1 + 2.0 ** -23, 1 + 3 * 2.0 ** -23, 1.5, 2 - 2.0 ** -22, 2 - 2.0 ** -23]
+    some = (1 + torch.rand(58, dtype=torch.float64, generator=torch.Generator().manual_seed(k))).tolist()
+    most = torch.tensor([127 * s * 2.0 ** e for s in ends + some for e in (-110, -97, -20, 0, 3, 60, 119)], dtype=torch.float64, device="cuda").float()
+    scale = most * torch.tensor(1 / 127, device="cuda")
+    tie = ((torch.arange(-127, 127, device="cuda") + 0.5).double() * scale.double()[:, None]).float()
+    inf = torch.full_like(tie, INF)
+    x = torch.cat([tie, torch.nextafter(tie, inf), torch.nextafter(tie, -inf)], dim=1)
+    x = torch.cat([x, torch.zeros(len(most), 6, device="cuda")], dim=1)[:, :k].contiguous()
+    x[:, k - 1] = most
+    assert (x.abs().amax(dim=1) == most).all()
+    q, s = quantize(lib, x)
+    want_q, want_s = quantized(x)
+    assert torch.equal(s, want_s) and torch.equal(q, want_q)
+
+
 class Product:
     def __init__(self, lib, M, N, K, prec, act=oracle.ACT_NONE, bias=True, res=True, alpha=1.0, pads=(0, 0, 0), shift=0, seed=0, in_place=False):
         g = torch.Generator(device="cuda").manual_seed(seed + M + 3 * N + 7 * K)
@@ -213,6 +233,54 @@ def test_rows_do_not_depend_on_their_number(lib):
         part.d.M = m
         part.run()
         assert torch.equal(part.out[:m], whole.out[:m]) and not part.out[m:].any()  # rows behind the last are left as they were
+
+
+@gpu
+@pytest.mark.parametrize("act", [oracle.ACT_NONE, oracle.ACT_MISH, oracle.ACT_SWISH, oracle.ACT_RELU_2, oracle.ACT_SELU])
+@pytest.mark.parametrize("prec", [0, 1, 2])
+def test_rows_do_not_depend_on_their_number_whatever_follows(lib, act, prec):
+    """The same bits from each kernel with alpha, bias and residual: a cluster per tile, a tile per CTA, CTA pairs with narrow and with wide tiles."""
+    made = lambda: Product(lib, 6000, 520, 1024, prec, act=act, alpha=-0.7, seed=2)
+    whole = made().run()
+    whole.check()
+    for m in (1, 64, 500, 3000):
+        part = made()
+        part.d.M = m
+        part.run()
+        assert torch.equal(part.out[:m], whole.out[:m]) and not part.out[m:].any()
+
+
+@gpu
+@pytest.mark.parametrize("pads", [(16, 32, 8), (0, 0, 2), (48, 0, 1), (0, 16, 0)])
+@pytest.mark.parametrize("M,N,K", [(3000, 520, 256), (6000, 520, 336), (3000, 1858, 144), (6000, 1857, 128)])
+@pytest.mark.parametrize("prec", [0, 1, 2])
+def test_strides_of_many_rows(lib, pads, M, N, K, prec):
+    """CTA pairs: padded rows of each operand; results and residuals by whole 16 bytes, by words and by entries, in narrow and in wide tiles."""
+    act = oracle.ACT_MISH if pads[2] == 2 else oracle.ACT_NONE
+    Product(lib, M, N, K, prec, pads=pads, act=act).run().check()
+    Product(lib, M, N, K, prec, pads=pads, in_place=True).run().check()
+    Product(lib, M, N, K, prec, pads=pads, res=False, alpha=0.5).run().check()
+
+
+@gpu
+@pytest.mark.parametrize("act", [oracle.ACT_MISH, oracle.ACT_SWISH])
+@pytest.mark.parametrize("M", [64, 500, 3000])
+@pytest.mark.parametrize("prec", [1, 2])
+@pytest.mark.parametrize("worst", [NAN, INF, -INF])
+def test_columns_that_share_a_reciprocal_keep_apart(lib, act, M, prec, worst):
+    """Four columns of a row share the activation's reciprocal; one that is not finite reaches none of the others."""
+    p = Product(lib, M, 300, 256, prec, act=act, res=False)
+    clean = p.bias.clone()
+    p.bias[7], p.bias[12], p.bias[298] = worst, worst, worst
+    p.run()
+    bad = [7, 12, 298]
+    if worst != INF:
+        assert p.out[:, bad].isnan().all()
+    else:
+        assert (p.out[:, bad] == (65504 if prec == 1 else INF)).all()
+    p.out[:, bad] = Product(lib, M, 300, 256, prec, act=act, res=False).run().out[:, bad]
+    p.bias = clean
+    p.check()
 
 
 @gpu
