@@ -210,12 +210,12 @@ __global__ void __launch_bounds__(256) spread_rows_kernel(const GroupedParams p,
 // Rows of X and W that TMA can read.
 bool tma_rows(int K, long long ldx, long long ldw, int size) { return K * (long long)size % 16 == 0 && ldx * size % 16 == 0 && ldw * size % 16 == 0; }
 // The pair kernel's 256 slots pay from a quarter of a tile per expert on, and where the other kernel's tiles of 64 slots x 128 columns are more than
-// half of the SMs (K and N 1024, int8, us, pair kernel / the other: 128 rows 6.9 / 5.8, 256 6.9 / 6.1, 512 7.0 / 7.4, 1024 7.2 / 8.0, 2048
-// 7.5 / 12.5; 768 rows over 8 experts to 1536 columns, copied into
-// order, 14.6 / 16.6).
+// a quarter of the SMs (us, pair kernel / the other; int8, K 1024, to 1024 columns: 256 rows, 32 tiles, 7.0 / 6.3, 320 rows, 40 tiles, 7.0 / 7.3,
+// 512 rows 7.1 / 7.7, 1024 rows 7.2 / 8.2; K 1536, to 512 columns: 512 rows, 32 tiles, 7.6 / 6.5, 768 rows, 48 tiles, 7.7 / 7.8; 16 bits: 300 rows over 4
+// experts, copied into order, to 1024 columns, 48 tiles, 11.1 / 12.4, eight positions over 4 experts to 768 columns, 60 tiles, 9.5 / 10.0).
 bool many_rows(const GroupedParams& p, int sms) {
   const int used = p.experts < p.slots ? p.experts : p.slots;
-  return p.slots / used > 64 && ((long long)p.slots / 64 + used / 2) * ceil_div(p.N, 128) > sms / 2;
+  return p.slots / used > 64 && ((long long)p.slots / 64 + used / 2) * ceil_div(p.N, 128) > sms / 4;
 }
 // Beyond 16 rows per expert the other kernel, too, is ahead with rows in order, although the copy is a launch more (333 rows over 12 experts to 1858
 // columns 25.1 in place, 20.2).
