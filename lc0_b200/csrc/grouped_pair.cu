@@ -6,11 +6,14 @@
 //   warp 1      tcgen05.mma issuer (even CTA), kind::f16 or kind::i8, two accumulators in tensor memory
 //   warps 4-19  epilogue: four groups of four warps, 64 bytes of each of a warp's 32 rows at a time: tensor memory -> scales, bias, activation,
 //               weight, residual -> the warp's own staging buffer -> a TMA store where the 32 rows lie in order and are all this expert's, else
-//               64-byte pieces of those rows that are.  The epilogue is bound by the wavefronts of shared memory that it shares with
-//               the operands, and by instructions; a TMA store spares it those of reading the buffer and of writing line by line
+//               64-byte pieces of those rows that are.  A TMA store spares it reading the buffer and writing line by line
 //               (65536x1536x1024 int8, us: 104 without, 94 with).
 // us and what they are of 1.65 PFLOP/s (int8: of twice that), on the device: 32768 slots over 16 experts, 1024x1536 columns by slot 90, 69 %;
-// 65536x1536x1024 int8 88, 71 %; without an epilogue 81 and 62.
+// 65536x1536x1024 int8 86 - 88, 71 %; without an epilogue 81 and 62.
+// No unit is full: the epilogue is bound by latency, four warps per scheduler that wait for each 16 columns of tensor memory and for their residual
+// before they compute.  Counters, % of the tensor pipe, of the issue slots, of shared memory's wavefronts (the epilogue's and the operands'):
+// 65536x1024x1536 int8 65, 38, 41 + 33; with a residual 50, 41, 36 + 25; 18000 slots of int8 over 16 experts, 1536x1024, 38, 37, 34 + 20; with
+// Mish 29, 41, 25 + 15.
 // Every wait is bounded by wall-clock time like those of gemm_tc.cu.
 #include "chunk8.cuh"
 #include "grouped_tc.cuh"

@@ -329,7 +329,8 @@ cudaError_t launch_rows(const GroupedParams& p, int sm_count, cudaStream_t s) {
   const int used = p.experts < p.slots ? p.experts : p.slots;
   const long long full = ((long long)p.slots + kRows - 1) / kRows, most = full + used - 1;  // row tiles: all full, and as many as there can be
   // A tile is cut over as many CTAs as leave each of them an SM of its own, going by one row tile per expert, or what the slots fill.  Clusters
-  // of eight do not all find eight free SMs of a GPC: sixteen of them took two turns (128x1024x1024 int8 11.8 us, by four CTAs 5.3).
+  // of eight do not all find eight free SMs of a GPC: sixteen of them took two turns (128x1024x1024 int8 11.8 us, by four CTAs 5.3), so fifteen at
+  // most; of four, 32 at most (64 rows, K 1024, us by four CTAs / by two: 32 tiles 6.3, 33 tiles 6.4 / 7.5, 34 tiles 11.6 / 7.5).
   const long long expected = (full > used ? full : used) * n_tiles;
   int ks = 1;
   while (ks < 8 && expected * ks * 2 <= (ks == 4 ? 120 : ks == 2 ? 128 : sm_count) && 2 * ks <= k_blocks) ks *= 2;

@@ -110,7 +110,9 @@ template <int kRows, int kCols> struct TileWalk {
 // v e / (e + 1) with e = exp(v), and v n / (n + 2) with n = e (e + 2): four at a time share one reciprocal.  exp is held to exp(10) (Mish) and
 // exp(20), beyond which the quotient is 1 to 2^-27, so that the four denominators' product stays finite; arithmetic in pairs.  us, 65536x1536x1024
 // int8 with Mish: a reciprocal each, one by one 133, now 120; without an activation 88.
-__device__ __forceinline__ float exp2_quick(float x) {  // results below 2^-126 are 0, which nothing of these formulas shows
+// (Results below 2^-126 are 0, and with them Mish and Swish of less than -87, which are up to 1e-36 in size: what bf16 could hold, and the quick Swish of
+// the other products, whose denominator passes 2^126 there, does not give either.)
+__device__ __forceinline__ float exp2_quick(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;

@@ -99,7 +99,9 @@ template <typename T> __device__ __forceinline__ Chunk<T> load8_once(const T* p)
 // A row in the registers of kThreads threads, kPer chunks of eight entries each; the next row is on its way meanwhile.
 //   Many rows: a warp each, as many as fit, each walking over its rows (us, a warp for one row and the next CTA behind it / now: 65536x1536 bf16
 //   57 / 51, 65536x1024 fp32 62 / 53: 6.0 and 6.3 TB/s of 6.55).
-//   Few rows: four warps each, so that a thread has one or two chunks (64x1024 1.2 us in a chain of launches).
+//   Up to 2048 rows: four warps each, so that a thread has one or two chunks (bf16 in a chain of launches, us, four warps / one: 64x1024 1.2 / 1.8,
+//   1024x1024 2.2 / 2.7, 2048x1024 3.3 / 3.4, 2560x1024 3.6 / 3.5, 4096x1024 4.8 / 3.9; rows of 2048 entries turn later, 4096 of them 6.3 / 7.6, rows
+//   of 512 earlier, 1024 of them 2.0 / 1.9).
 template <typename T, int kPer, int kThreads>
 __global__ void __launch_bounds__(128) quantize_rows_kernel(const T* X, long long ldx, int M, int K, int8_t* Q, long long ldq, float* scales) {
   __shared__ uint32_t of_warp[4];
